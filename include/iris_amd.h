@@ -390,6 +390,152 @@ int iris_p2p_bench_launch(int32_t op, int32_t dtype, void* buffer, void* result,
                           int32_t cur_rank, int32_t peer_rank, int32_t num_ranks, const uint64_t* heap_bases,
                           int32_t block_size, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* The attention block of one rank: its heads, between the shard of the       */
+/* query / key / value projection and the output projection's K-shard.        */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Bits that these launchers' kernels OR into *status (may be NULL), for what only the device can see.
+ * BAD_INDEX: a position outside the angle table (the rotated elements are NaN), a slot outside the cache (nothing is
+ * written), or a page outside the cache in a table entry that is read (the output rows are NaN).
+ * NO_PAGES: a request did not get its pages (the ring is empty, or its table row too short); it keeps its length, and
+ * its tokens have slot -1.
+ * NO_ROOM: more new tokens than max_tokens; those past it have no position and slot.
+ */
+#define IRIS_STATUS_BAD_INDEX 2
+#define IRIS_STATUS_NO_PAGES 4
+#define IRIS_STATUS_NO_ROOM 8
+
+/*
+ * Block tables of a paged key-value cache.  Request i has cached[i] tokens in the pages block_table[i][0 ..
+ * ceil(cached[i] / page_size)) and brings new_tokens[i] (0: none; below 0: it has ended and gives its pages back).
+ * Free pages are pool[x % pool_size] for x in [pool_state[0], pool_state[1]): the requests take from the front, in
+ * order; pages given back go to the end and may be taken from the next call on.  A request whose pages do not all
+ * fit gets none, and so do all later ones that need any.
+ * Writes the fresh table entries (in place), pool (in place, the pages given back), pool_state_out, lengths (tokens
+ * after the step), query_starts[requests + 1] (sums of new_tokens), and for token t of max_tokens its position in the
+ * request and its slot, page * page_size + position % page_size; position 0 and slot -1 past the last token.
+ * lengths and pool_state_out are not cached and pool_state.  At most 8192 requests.
+ */
+typedef struct iris_block_tables_args {
+  const int32_t* cached;
+  const int32_t* new_tokens;
+  int32_t* block_table;
+  int32_t* pool;
+  const int64_t* pool_state;
+  int64_t* pool_state_out;
+  int32_t* lengths;
+  int32_t* query_starts;
+  int32_t* positions;
+  int64_t* slots;
+  uint32_t* status;
+  int64_t stride_table;
+  int32_t requests, table_width, page_size, pool_size, max_tokens;
+} iris_block_tables_args;
+
+int iris_block_tables_launch(const iris_block_tables_args* args, void* stream);
+
+/*
+ * Norms and rotation of query and key heads.  A head x of head_dim elements becomes x / sqrt(mean(x^2) + eps) * weight
+ * (no weight: x itself), of which the first rotary_dim elements turn by the angles cos / sin[position][rotary_dim / 2]:
+ * pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved.  Strides are in elements, t: token, h: head; a head's
+ * elements are contiguous.  k_out may be NULL where there is a cache.  With slots, keys and values also go to
+ * k_cache / v_cache[slot / page_size][slot % page_size][head]; a negative slot is skipped.  Outputs may be the inputs.
+ */
+typedef struct iris_qk_norm_rope_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* positions;
+  const float* cos;
+  const float* sin;
+  const void* q_weight;
+  const void* k_weight;
+  void* q_out;
+  void* k_out;
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slots;
+  uint32_t* status;
+  int64_t stride_qt, stride_qh, stride_kt, stride_kh, stride_vt, stride_vh;
+  int64_t stride_qot, stride_qoh, stride_kot, stride_koh;
+  int64_t stride_kc_page, stride_kc_row, stride_kc_head, stride_vc_page, stride_vc_row, stride_vc_head;
+  int64_t stride_cos, stride_sin;
+  int64_t num_slots;
+  int32_t tokens, q_heads, k_heads, head_dim, rotary_dim, max_positions, page_size;
+  int32_t dtype, weight_fp32, positions_64, interleaved;
+  float eps;
+} iris_qk_norm_rope_args;
+
+int iris_qk_norm_rope_launch(const iris_qk_norm_rope_args* args, void* stream);
+
+/*
+ * Its gradient: dq, dk from dq_out, dk_out and the unnormed q, k; dq_weight / dk_weight (fp32, may be NULL) summed over
+ * tokens and heads in a fixed order.  workspace holds rows of 2 * head_dim floats, one a workgroup; more rows let
+ * more workgroups run.  Not needed without weight gradients.
+ */
+typedef struct iris_qk_norm_rope_backward_args {
+  const void* dq_out;
+  const void* dk_out;
+  const void* q;
+  const void* k;
+  const void* positions;
+  const float* cos;
+  const float* sin;
+  const void* q_weight;
+  const void* k_weight;
+  void* dq;
+  void* dk;
+  float* dq_weight;
+  float* dk_weight;
+  float* workspace;
+  uint32_t* status;
+  int64_t workspace_elems;
+  int64_t stride_dqot, stride_dqoh, stride_dkot, stride_dkoh, stride_qt, stride_qh, stride_kt, stride_kh;
+  int64_t stride_dqt, stride_dqh, stride_dkt, stride_dkh;
+  int64_t stride_cos, stride_sin;
+  int32_t tokens, q_heads, k_heads, head_dim, rotary_dim, max_positions;
+  int32_t dtype, weight_fp32, positions_64, interleaved;
+  float eps;
+} iris_qk_norm_rope_backward_args;
+
+int iris_qk_norm_rope_backward_launch(const iris_qk_norm_rope_backward_args* args, void* stream);
+
+/*
+ * Causal attention over a paged key-value cache.  Request i's keys are its lengths[i] tokens in the pages of block_table[i];
+ * its queries are tokens [query_starts[i], query_starts[i + 1]) and stand at the last positions of the context, or
+ * (query_starts NULL) there is one a request.  The query at position p sees key j <= p where j > p - window, or j < sinks, or
+ * window is 0; query head h goes to key head h / (q_heads / k_heads).  out = softmax(scale q k^T) v; lse (may be NULL,
+ * fp32 [tokens][q_heads]) the logarithm of the softmax's sum.  A row that sees no key is 0 with lse -inf.
+ * Tables, lengths and starts are read on the device; keys past a request's length are never read as numbers.
+ * workspace (fp32, 16-byte aligned, zeroed once before its first use, for one stream at a time) takes the parts that a long
+ * axis is split into; without it nothing is split.
+ */
+typedef struct iris_attention_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* block_table;
+  const int32_t* lengths;
+  const int32_t* query_starts;
+  void* out;
+  float* lse;
+  float* workspace;
+  uint32_t* status;
+  int64_t workspace_elems;
+  int64_t stride_qt, stride_qh, stride_ot, stride_oh, stride_lse;
+  int64_t stride_kc_page, stride_kc_row, stride_kc_head, stride_vc_page, stride_vc_row, stride_vc_head;
+  int64_t stride_table;
+  int32_t requests, tokens, q_heads, k_heads, head_dim, page_size, table_width, num_pages;
+  int32_t window, sinks, dtype;
+  float scale;
+} iris_attention_args;
+
+int iris_attention_launch(const iris_attention_args* args, void* stream);
+/* Elements of a workspace with which a launch for heads of head_dim splits as it likes. */
+int64_t iris_attention_workspace_elems(int32_t head_dim);
+
 /* Library version, bumped when a signature in this header changes. */
 int iris_amd_abi_version(void);
 

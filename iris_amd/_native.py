@@ -34,6 +34,8 @@ FLAG_SEM_WRITE_THROUGH, FLAG_SEM_RELEASE_ACQUIRE = 0, 1
 TOUCH_AUTO, TOUCH_ON, TOUCH_OFF = 0, 1, 2
 # status word (IRIS_STATUS_*)
 STATUS_OK, STATUS_SPIN_TIMEOUT = 0, 1
+# bits of the attention block's status word
+STATUS_BAD_INDEX, STATUS_NO_PAGES, STATUS_NO_ROOM = 2, 4, 8
 
 HIP_ERROR_INVALID_VALUE = 1
 
@@ -121,6 +123,59 @@ class ReduceArgs(ctypes.Structure):
     ]
 
 
+def _fields(*groups):
+    """Structure fields: (ctype, "names in order") pairs."""
+    return [(name, ctype) for ctype, names in groups for name in names.split()]
+
+
+class BlockTablesArgs(ctypes.Structure):
+    """``iris_block_tables_args``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "cached new_tokens block_table pool pool_state pool_state_out lengths query_starts positions slots status"),
+        (ctypes.c_int64, "stride_table"),
+        (ctypes.c_int32, "requests table_width page_size pool_size max_tokens"),
+    )
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    """``iris_qk_norm_rope_args``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "q k v positions cos sin q_weight k_weight q_out k_out k_cache v_cache slots status"),
+        (ctypes.c_int64, "stride_qt stride_qh stride_kt stride_kh stride_vt stride_vh stride_qot stride_qoh stride_kot stride_koh"),
+        (ctypes.c_int64, "stride_kc_page stride_kc_row stride_kc_head stride_vc_page stride_vc_row stride_vc_head"),
+        (ctypes.c_int64, "stride_cos stride_sin num_slots"),
+        (ctypes.c_int32, "tokens q_heads k_heads head_dim rotary_dim max_positions page_size"),
+        (ctypes.c_int32, "dtype weight_fp32 positions_64 interleaved"),
+        (ctypes.c_float, "eps"),
+    )
+
+
+class QkNormRopeBackwardArgs(ctypes.Structure):
+    """``iris_qk_norm_rope_backward_args``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "dq_out dk_out q k positions cos sin q_weight k_weight dq dk dq_weight dk_weight workspace status"),
+        (ctypes.c_int64, "workspace_elems stride_dqot stride_dqoh stride_dkot stride_dkoh stride_qt stride_qh stride_kt stride_kh"),
+        (ctypes.c_int64, "stride_dqt stride_dqh stride_dkt stride_dkh stride_cos stride_sin"),
+        (ctypes.c_int32, "tokens q_heads k_heads head_dim rotary_dim max_positions dtype weight_fp32 positions_64 interleaved"),
+        (ctypes.c_float, "eps"),
+    )
+
+
+class AttentionArgs(ctypes.Structure):
+    """``iris_attention_args``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "q k_cache v_cache block_table lengths query_starts out lse workspace status"),
+        (ctypes.c_int64, "workspace_elems stride_qt stride_qh stride_ot stride_oh stride_lse"),
+        (ctypes.c_int64, "stride_kc_page stride_kc_row stride_kc_head stride_vc_page stride_vc_row stride_vc_head stride_table"),
+        (ctypes.c_int32, "requests tokens q_heads k_heads head_dim page_size table_width num_pages window sinks dtype"),
+        (ctypes.c_float, "scale"),
+    )
+
+
 # every symbol include/iris_amd.h declares for libiris_amd.so:
 # name -> (restype, argtypes)
 _P = ctypes.c_void_p
@@ -156,6 +211,11 @@ SIGNATURES = {
                                          ctypes.POINTER(ctypes.c_int32)]),
     "iris_p2p_bench_launch": (_I, [ctypes.c_int32] * 2 + [_P, _P, ctypes.c_int64] + [ctypes.c_int32] * 3
                               + [_P, ctypes.c_int32, _P]),
+    "iris_block_tables_launch": (_I, [ctypes.POINTER(BlockTablesArgs), _P]),
+    "iris_qk_norm_rope_launch": (_I, [ctypes.POINTER(QkNormRopeArgs), _P]),
+    "iris_qk_norm_rope_backward_launch": (_I, [ctypes.POINTER(QkNormRopeBackwardArgs), _P]),
+    "iris_attention_launch": (_I, [ctypes.POINTER(AttentionArgs), _P]),
+    "iris_attention_workspace_elems": (ctypes.c_int64, [ctypes.c_int32]),
     "iris_amd_abi_version": (_I, []),
 }
 ALLOCATOR_SYMBOLS = ("finegrained_hipMalloc", "finegrained_hipFree")

@@ -1,0 +1,121 @@
+// iris_attention_launch: checks a call, and takes the kernel for it.
+#include <type_traits>
+
+#include "attention_rows.hpp"
+
+namespace iris_amd {
+namespace {
+
+constexpr int64_t COUNTERS = 4096;      // arrival counters, one a split unit, at the workspace's start
+constexpr int64_t ROW_SLOTS = 4096;     // partial results of 16 rows that a full workspace holds
+constexpr int MAX_HEAD_DIM = 256;
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+hipError_t check(const iris_attention_args& a) {
+  if (a.dtype != IRIS_DTYPE_F32 && a.dtype != IRIS_DTYPE_F16 && a.dtype != IRIS_DTYPE_BF16) return hipErrorInvalidValue;
+  if (a.requests < 0 || a.tokens < 0 || a.q_heads < 0 || a.k_heads < 0 || a.page_size <= 0 || a.table_width < 0 || a.num_pages < 0 ||
+      a.window < 0 || a.sinks < 0 || !(a.scale > 0.f) || !(a.scale < INFINITY))
+    return hipErrorInvalidValue;
+  const int es = dtype_size(a.dtype), vec = 16 / es;
+  if (a.head_dim <= 0 || a.head_dim > MAX_HEAD_DIM || a.head_dim % vec) return hipErrorInvalidValue;
+  if (a.tokens == 0 || a.q_heads == 0) return hipSuccess;
+  if (a.k_heads == 0 || a.q_heads % a.k_heads || a.requests == 0 || a.table_width == 0 || a.num_pages == 0) return hipErrorInvalidValue;
+  if (!a.query_starts && a.requests != a.tokens) return hipErrorInvalidValue;
+  if (!a.q || !a.k_cache || !a.v_cache || !a.block_table || !a.lengths || !a.out || a.stride_table < a.table_width) return hipErrorInvalidValue;
+  if ((int64_t)a.table_width * a.page_size > INT32_MAX) return hipErrorInvalidValue;
+  for (const void* p : {a.q, a.k_cache, a.v_cache, (const void*)a.out, (const void*)a.workspace})
+    if (!aligned16(p)) return hipErrorInvalidValue;
+  for (const int64_t s : {a.stride_qt, a.stride_qh, a.stride_ot, a.stride_oh, a.stride_kc_page, a.stride_kc_row, a.stride_kc_head, a.stride_vc_page,
+                          a.stride_vc_row, a.stride_vc_head})
+    if (s % vec) return hipErrorInvalidValue;
+  return hipSuccess;
+}
+
+template <class F>
+hipError_t with_types(const iris_attention_args& a, F f) {
+  using std::integral_constant;
+  auto paged = [&](auto dt, auto dp) {
+    return a.page_size % 16 == 0 ? f(dt, dp, std::true_type{}) : f(dt, dp, std::false_type{});
+  };
+  auto dims = [&](auto dt) {
+    switch (padded_dim(a.head_dim)) {
+      case 64: return paged(dt, integral_constant<int, 64>{});
+      case 128: return paged(dt, integral_constant<int, 128>{});
+      default: return paged(dt, integral_constant<int, 256>{});
+    }
+  };
+  if (a.dtype == IRIS_DTYPE_F32) return dims(integral_constant<int, IRIS_DTYPE_F32>{});
+  if (a.dtype == IRIS_DTYPE_F16) return dims(integral_constant<int, IRIS_DTYPE_F16>{});
+  return dims(integral_constant<int, IRIS_DTYPE_BF16>{});
+}
+
+}  // namespace
+}  // namespace iris_amd
+
+extern "C" int64_t iris_attention_workspace_elems(int32_t head_dim) {
+  using namespace iris_amd;
+  if (head_dim <= 0 || head_dim > MAX_HEAD_DIM) return 0;
+  return COUNTERS + ROW_SLOTS * rows::ROWS * (padded_dim(head_dim) + 2);
+}
+
+extern "C" int iris_attention_launch(const iris_attention_args* args, void* stream) {
+  using namespace iris_amd;
+  if (!args) return hipErrorInvalidValue;
+  const iris_attention_args& a = *args;
+  const hipError_t bad = check(a);
+  if (bad != hipSuccess) return bad;
+  if (a.tokens == 0 || a.q_heads == 0) return hipSuccess;
+
+  AttentionKArgs g{};
+  g.a = a;
+  g.page = make_page_div((uint32_t)a.page_size);
+  g.scale_log2 = a.scale * 1.4426950408889634f;
+  g.group = a.q_heads / a.k_heads;
+  g.splits = 1;
+  const int cus = current_cu_count();
+  int64_t slots = 0;
+  if (a.workspace && a.workspace_elems > COUNTERS) {
+    slots = (a.workspace_elems - COUNTERS) / (rows::ROWS * (padded_dim(a.head_dim) + 2));
+    g.counters = (int32_t*)a.workspace;
+    g.slots = a.workspace + COUNTERS;
+  }
+  // the most keys that a row may see
+  const int64_t room = (int64_t)a.table_width * a.page_size;
+  const int64_t most_keys = a.window > 0 && (int64_t)a.window + a.sinks < room ? (int64_t)a.window + a.sinks : room;
+  const hipStream_t s = (hipStream_t)stream;
+
+  return with_types(a, [&](auto dt, auto dp, auto pg) {
+    using C = rows::Cfg<dt.value, dp.value>;
+    constexpr int threads = rows::WAVES * 64;
+    if (!a.query_starts) {
+      const int64_t units = (int64_t)a.requests * a.k_heads * ((g.group + rows::ROWS - 1) / rows::ROWS);
+      int64_t grid = units * ((most_keys + C::BT - 1) / C::BT + 2);
+      if (grid > 2 * cus) grid = 2 * cus;
+      if (slots && grid > slots / 2) grid = slots / 2;
+      if (grid > COUNTERS) grid = COUNTERS;
+      if (grid < 1) {
+        grid = 1;
+        g.slots = nullptr;
+      }
+      g.grid_units = (int)grid;
+      rows::decode_kernel<dt.value, dp.value, pg.value><<<(int)grid, threads, 0, s>>>(g);
+      return hipGetLastError();
+    }
+    const int64_t row_tiles = (int64_t)a.tokens * g.group / rows::ROWS + a.requests;
+    const int64_t units = row_tiles * a.k_heads;
+    int64_t splits = 1;
+    if (units < 2 * cus && units <= COUNTERS) {
+      splits = 2 * cus / units;
+      if (splits > most_keys / (2 * C::BT)) splits = most_keys / (2 * C::BT);
+      if (splits > slots / units) splits = slots / units;
+      if (splits < 1) splits = 1;
+    }
+    g.splits = (int)splits;
+    if (row_tiles * splits > INT32_MAX || a.k_heads > 65535) return hipErrorInvalidValue;
+    rows::prompt_rows_kernel<dt.value, dp.value, pg.value><<<dim3((unsigned)(row_tiles * splits), a.k_heads), threads, 0, s>>>(g);
+    return hipGetLastError();
+  });
+}
