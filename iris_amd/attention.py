@@ -120,6 +120,14 @@ def _no_gradient(*tensors):
                            "and attention over a cache has none")
 
 
+def _launched(err):
+    """Whether the native code took the call.  What it declines, and what the launcher rejects, goes through the full checks, which
+    say what is wrong."""
+    if err > 0 and err != _native.HIP_ERROR_INVALID_VALUE:
+        _native.hip_try(err)
+    return err == 0
+
+
 def _launch(name, args, device):
     stream = torch.cuda.current_stream(device).cuda_stream
     with torch.cuda.device(device):
@@ -150,6 +158,9 @@ def build_block_tables(cached, new_tokens, block_table, pool, pool_state, page_s
     every token, up to their common length (0 and -1 past the last token).
     ``lengths`` and ``pool_state_out`` may not be ``cached`` and ``pool_state``.
     """
+    if _launched(_native.host().block_tables(cached, new_tokens, block_table, pool, pool_state, lengths, pool_state_out, query_starts,
+                                             positions, slots, status, page_size)):
+        return
     device = cached.device
     requests = cached.numel()
     _ints("cached", cached, device, torch.int32, requests)
@@ -296,8 +307,9 @@ def _rope_operands(a, device, dtype, tokens, dim, positions, cos, sin, q_weight,
 
 
 def _strides(a, prefix, t):
-    setattr(a, f"stride_{prefix}t", t.stride(0))
-    setattr(a, f"stride_{prefix}h", t.stride(1))
+    token, head = _steps(t, 2)
+    setattr(a, f"stride_{prefix}t", token)
+    setattr(a, f"stride_{prefix}h", head)
 
 
 def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, v=None,
@@ -316,6 +328,9 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
     slots of ``k_cache`` / ``v_cache`` [pages, page size, key heads, head size]; a negative
     slot is skipped, and with a cache ``k_out`` may be None.
     """
+    if _launched(_native.host().qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, q_weight, k_weight, v, k_cache, v_cache, slots,
+                                             status, eps, interleaved)):
+        return
     device, dtype = q.device, q.dtype
     if dtype not in _DTYPES:
         raise TypeError(f"q: unsupported dtype {dtype}")
@@ -354,8 +369,8 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
             raise ValueError("more slots than 31 bits count")
         a.v, a.slots, a.k_cache, a.v_cache = _ptr(v), _ptr(slots), _ptr(k_cache), _ptr(v_cache)
         _strides(a, "v", v)
-        a.stride_kc_page, a.stride_kc_row, a.stride_kc_head = k_cache.stride()[:3]
-        a.stride_vc_page, a.stride_vc_row, a.stride_vc_head = v_cache.stride()[:3]
+        a.stride_kc_page, a.stride_kc_row, a.stride_kc_head = _steps(k_cache, 3)
+        a.stride_vc_page, a.stride_vc_row, a.stride_vc_head = _steps(v_cache, 3)
         a.page_size = k_cache.shape[1]
     elif v is not None or k_cache is not None or v_cache is not None:
         raise ValueError("v, k_cache and v_cache need slots")
@@ -379,6 +394,9 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, 
     heads in a fixed order, in ``workspace`` (``make_gradient_workspace``; fp32, as
     few as 2 * head size elements).  ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out``.
     """
+    if _launched(_native.host().qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, q_weight, k_weight, dq_weight,
+                                                      dk_weight, workspace, status, eps, interleaved)):
+        return
     device, dtype = q.device, q.dtype
     if dtype not in _DTYPES:
         raise TypeError(f"q: unsupported dtype {dtype}")
@@ -459,6 +477,9 @@ def make_workspace(head_dim, *, device="cuda"):
 
 
 def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status):
+    if _launched(_native.host().attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale,
+                                          window, sinks)):
+        return
     device, dtype = q.device, q.dtype
     if dtype not in _DTYPES:
         raise TypeError(f"q: unsupported dtype {dtype}")
@@ -525,7 +546,6 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
         return
     a.q, a.k_cache, a.v_cache, a.out = _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out)
     a.block_table, a.lengths, a.query_starts, a.status = _ptr(block_table), _ptr(lengths), _ptr(query_starts), _ptr(status)
-    # (the stride of an axis of one element is never taken, and need not be a multiple of anything)
     a.stride_qt, a.stride_qh = _steps(q, 2)
     a.stride_ot, a.stride_oh = _steps(out, 2)
     a.stride_kc_page, a.stride_kc_row, a.stride_kc_head = _steps(k_cache, 3)
@@ -538,6 +558,7 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
 
 
 def _steps(t, n):
+    # (the stride of an axis of one element is never taken, and need not be a multiple of anything)
     return [s if size > 1 else 0 for s, size in zip(t.stride()[:n], t.shape[:n])]
 
 

@@ -19,6 +19,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "../../../include/iris_amd.h"
 
 namespace {
@@ -387,11 +390,353 @@ PyObject* memset_i32(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return PyLong_FromLong(unlocked([&] { return iris_memset_i32_launch(p, value, count, stream); }));
 }
 
+// ---- the attention block (iris_amd/attention.py documents what is checked) ----
+
+constexpr int MAX_REQUESTS = 8192, MAX_HEAD_DIM = 512, MAX_ATTENTION_HEAD_DIM = 256;
+
+bool real(PyObject* o, double* out) {
+  if (!PyFloat_Check(o) && !PyLong_Check(o)) return false;
+  *out = PyFloat_AsDouble(o);
+  return !PyErr_Occurred();
+}
+bool truth(PyObject* o, int32_t* out) { return (*out = PyObject_IsTrue(o)) >= 0; }
+
+bool differentiates(const Operand& t) { return t && at::GradMode::is_enabled() && t.t->requires_grad(); }
+
+// A tensor [tokens, heads, head size] of `type` whose head elements are contiguous; sizes below 0 are free.
+bool heads_of(const Operand& t, at::ScalarType type, int64_t tokens, int64_t heads, int64_t dim) {
+  return t && t.t->dim() == 3 && t.t->scalar_type() == type && (tokens < 0 || t.t->size(0) == tokens) && (heads < 0 || t.t->size(1) == heads) &&
+         (dim < 0 || t.t->size(2) == dim) && (t.t->size(2) <= 1 || t.t->stride(2) == 1) && t.t->size(0) <= INT32_MAX && t.t->size(1) <= INT32_MAX;
+}
+
+// Something that a kernel writes: elements of its own, and no gradient.
+bool output(const Operand& t) {
+  if (!t || differentiates(t)) return false;
+  const int64_t n = t.t->dim();
+  int64_t reach = 0, floor = -1;  // axes in the order of their strides
+  for (int64_t taken = 0; taken < n; ++taken) {
+    int64_t best = -1;
+    for (int64_t i = 0; i < n; ++i) {
+      const int64_t key = t.t->stride(i) * 8 + i;
+      if (key > floor && (best < 0 || key < t.t->stride(best) * 8 + best)) best = i;
+    }
+    if (best < 0) return false;
+    floor = t.t->stride(best) * 8 + best;
+    if (t.t->size(best) <= 1) continue;
+    if (t.t->stride(best) <= reach) return false;
+    reach += t.t->stride(best) * (t.t->size(best) - 1);
+  }
+  return true;
+}
+
+bool vector_of(const Operand& t, at::ScalarType type, int64_t numel) {
+  return t && t.t->dim() == 1 && t.t->scalar_type() == type && t.t->numel() == numel && t.t->is_contiguous();
+}
+bool status_ok(const Operand& t) {
+  return !t || ((t.t->scalar_type() == at::kInt || t.t->scalar_type() == at::kUInt32) && t.t->numel() >= 1);
+}
+bool rows_contiguous(const Operand& t) { return t && t.t->dim() == 2 && (t.t->size(1) <= 1 || t.t->stride(1) == 1); }
+
+// build_block_tables(cached, new_tokens, block_table, pool, pool_state, lengths, pool_state_out, query_starts, positions, slots,
+//                    status, page_size)
+PyObject* block_tables(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 12) {
+    PyErr_SetString(PyExc_TypeError, "block_tables takes 12 arguments");
+    return nullptr;
+  }
+  const int device = launch_device(v[0]);
+  Operand t[11];
+  iris_block_tables_args a{};
+  bool ok = device >= 0 && int32(v[11], &a.page_size) && a.page_size > 0;
+  for (int i = 0; ok && i < 11; ++i) ok = operand(v[i], device, &t[i]);
+  PyErr_Clear();
+  enum { CACHED, NEW, TABLE, POOL, STATE, LENGTHS, STATE_OUT, STARTS, POSITIONS, SLOTS, STATUS };
+  if (!ok || !t[CACHED] || !t[POOL] || !t[POSITIONS]) return PyLong_FromLong(DECLINED);
+  const int64_t requests = t[CACHED].t->numel(), pool = t[POOL].t->numel(), tokens = t[POSITIONS].t->numel();
+  if (requests > MAX_REQUESTS || pool < 1 || pool > INT32_MAX || tokens > INT32_MAX || !vector_of(t[CACHED], at::kInt, requests) ||
+      !vector_of(t[NEW], at::kInt, requests) || !vector_of(t[LENGTHS], at::kInt, requests) || !vector_of(t[STARTS], at::kInt, requests + 1) ||
+      !vector_of(t[POOL], at::kInt, pool) || !vector_of(t[STATE], at::kLong, 2) || !vector_of(t[STATE_OUT], at::kLong, 2) ||
+      !vector_of(t[POSITIONS], at::kInt, tokens) || !vector_of(t[SLOTS], at::kLong, tokens) || !status_ok(t[STATUS]) || !rows_contiguous(t[TABLE]) ||
+      t[TABLE].t->scalar_type() != at::kInt || t[TABLE].t->size(0) != requests || t[TABLE].t->size(1) > INT32_MAX ||
+      (requests > 1 && !output(t[TABLE])))
+    return PyLong_FromLong(DECLINED);
+  // no operand lies in another
+  for (int i = 0; i < STATUS; ++i) {
+    const auto span = [&](int k, const char** lo, const char** hi) {
+      int64_t reach = 1;
+      for (int64_t d = 0; d < t[k].t->dim(); ++d) reach += t[k].t->stride(d) * (t[k].t->size(d) - 1);
+      *lo = (const char*)t[k].ptr();
+      *hi = *lo + (t[k].t->numel() ? reach * (int64_t)t[k].t->element_size() : 0);
+    };
+    const char *lo, *hi, *lo2, *hi2;
+    span(i, &lo, &hi);
+    for (int k = 0; k < i; ++k) {
+      span(k, &lo2, &hi2);
+      if (lo < hi2 && lo2 < hi) return PyLong_FromLong(DECLINED);
+    }
+  }
+  a.cached = (const int32_t*)t[CACHED].ptr();
+  a.new_tokens = (const int32_t*)t[NEW].ptr();
+  a.block_table = (int32_t*)t[TABLE].ptr();
+  a.pool = (int32_t*)t[POOL].ptr();
+  a.pool_state = (const int64_t*)t[STATE].ptr();
+  a.pool_state_out = (int64_t*)t[STATE_OUT].ptr();
+  a.lengths = (int32_t*)t[LENGTHS].ptr();
+  a.query_starts = (int32_t*)t[STARTS].ptr();
+  a.positions = (int32_t*)t[POSITIONS].ptr();
+  a.slots = (int64_t*)t[SLOTS].ptr();
+  a.status = (uint32_t*)t[STATUS].ptr();
+  a.requests = (int32_t)requests;
+  a.table_width = (int32_t)t[TABLE].t->size(1);
+  a.stride_table = std::max<int64_t>(t[TABLE].t->stride(0), a.table_width);
+  a.pool_size = (int32_t)pool;
+  a.max_tokens = (int32_t)tokens;
+  void* stream = current_stream(device);
+  return PyLong_FromLong(unlocked([&] { return iris_block_tables_launch(&a, stream); }));
+}
+
+// What the norms and the rotation take beside the heads.
+template <class Args>
+bool rope_operands(const Operand& positions, const Operand& cos, const Operand& sin, const Operand& qw, const Operand& kw, at::ScalarType type,
+                   int64_t tokens, int64_t dim, Args* a) {
+  if (dim % 2 || dim <= 0 || dim > MAX_HEAD_DIM || (bool)cos != (bool)sin) return false;
+  if (cos) {
+    if (!positions || cos.t->scalar_type() != at::kFloat || sin.t->scalar_type() != at::kFloat || !rows_contiguous(cos) || !rows_contiguous(sin) ||
+        cos.t->sizes() != sin.t->sizes() || cos.t->size(0) < 1 || cos.t->size(0) > INT32_MAX || 2 * cos.t->size(1) > dim)
+      return false;
+    const bool wide = positions.t->scalar_type() == at::kLong;
+    if (!vector_of(positions, wide ? at::kLong : at::kInt, tokens)) return false;
+    a->cos = (const float*)cos.ptr();
+    a->sin = (const float*)sin.ptr();
+    a->positions = positions.ptr();
+    a->stride_cos = cos.t->stride(0);
+    a->stride_sin = sin.t->stride(0);
+    a->rotary_dim = (int32_t)(2 * cos.t->size(1));
+    a->max_positions = (int32_t)cos.t->size(0);
+    a->positions_64 = wide;
+  }
+  for (const Operand* w : {&qw, &kw})
+    if (*w && (!vector_of(*w, w->t->scalar_type(), dim) || (w->t->scalar_type() != type && w->t->scalar_type() != at::kFloat))) return false;
+  if (qw && kw && qw.t->scalar_type() != kw.t->scalar_type()) return false;
+  a->q_weight = qw.ptr();
+  a->k_weight = kw.ptr();
+  a->weight_fp32 = (qw && qw.t->scalar_type() == at::kFloat) || (kw && kw.t->scalar_type() == at::kFloat);
+  a->tokens = (int32_t)tokens;
+  a->head_dim = (int32_t)dim;
+  return true;
+}
+
+struct CacheStrides {
+  int64_t page, row, head;
+};
+bool cache_of(const Operand& t, at::ScalarType type, int64_t heads, int64_t dim, CacheStrides* s) {
+  if (!t || t.t->dim() != 4 || t.t->scalar_type() != type || t.t->size(1) < 1 || t.t->size(2) != heads || t.t->size(3) != dim ||
+      (dim > 1 && t.t->stride(3) != 1) || t.t->size(0) > INT32_MAX || t.t->size(1) > INT32_MAX)
+    return false;
+  int64_t* const out[3] = {&s->page, &s->row, &s->head};
+  for (int i = 0; i < 3; ++i) *out[i] = t.t->size(i) > 1 ? t.t->stride(i) : 0;  // (the stride of an axis of one is never taken)
+  return true;
+}
+
+void strides_of(const Operand& t, int64_t* token, int64_t* head) {
+  *token = t.t->size(0) > 1 ? t.t->stride(0) : 0;
+  *head = t.t->size(1) > 1 ? t.t->stride(1) : 0;
+}
+
+// qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, q_weight, k_weight, v, k_cache, v_cache, slots, status, eps, interleaved)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 16) {
+    PyErr_SetString(PyExc_TypeError, "qk_norm_rope takes 16 arguments");
+    return nullptr;
+  }
+  const int device = launch_device(x[0]);
+  Operand t[14];
+  iris_qk_norm_rope_args a{};
+  double eps = 0;
+  bool ok = device >= 0 && real(x[14], &eps) && truth(x[15], &a.interleaved);
+  for (int i = 0; ok && i < 14; ++i) ok = operand(x[i], device, &t[i]);
+  PyErr_Clear();
+  enum { Q, K, POSITIONS, COS, SIN, Q_OUT, K_OUT, QW, KW, V, K_CACHE, V_CACHE, SLOTS, STATUS };
+  if (!ok || !t[Q] || t[Q].t->dim() != 3 || dtype_code(*t[Q].t) < 0) return PyLong_FromLong(DECLINED);
+  const auto type = t[Q].t->scalar_type();
+  const int64_t tokens = t[Q].t->size(0), hq = t[Q].t->size(1), dim = t[Q].t->size(2);
+  if (!heads_of(t[Q], type, -1, -1, -1) || !heads_of(t[K], type, tokens, -1, dim) || !heads_of(t[Q_OUT], type, tokens, hq, dim) || !output(t[Q_OUT]))
+    return PyLong_FromLong(DECLINED);
+  const int64_t hk = t[K].t->size(1);
+  for (const int i : {Q, K, V, QW, KW})
+    if (differentiates(t[i])) return PyLong_FromLong(DECLINED);
+  if (!rope_operands(t[POSITIONS], t[COS], t[SIN], t[QW], t[KW], type, tokens, dim, &a) || !status_ok(t[STATUS])) return PyLong_FromLong(DECLINED);
+  if (t[K_OUT] ? !heads_of(t[K_OUT], type, tokens, hk, dim) || !output(t[K_OUT]) : !t[SLOTS] && hk) return PyLong_FromLong(DECLINED);
+  if (t[SLOTS]) {
+    CacheStrides k, w;
+    if (!heads_of(t[V], type, tokens, hk, dim) || !vector_of(t[SLOTS], at::kLong, tokens) || !cache_of(t[K_CACHE], type, hk, dim, &k) ||
+        !cache_of(t[V_CACHE], type, hk, dim, &w) || t[K_CACHE].t->sizes() != t[V_CACHE].t->sizes() || !output(t[K_CACHE]) || !output(t[V_CACHE]))
+      return PyLong_FromLong(DECLINED);
+    a.page_size = (int32_t)t[K_CACHE].t->size(1);
+    a.num_slots = t[K_CACHE].t->size(0) * t[K_CACHE].t->size(1);
+    if (a.num_slots > INT32_MAX) return PyLong_FromLong(DECLINED);
+    a.stride_kc_page = k.page, a.stride_kc_row = k.row, a.stride_kc_head = k.head;
+    a.stride_vc_page = w.page, a.stride_vc_row = w.row, a.stride_vc_head = w.head;
+    strides_of(t[V], &a.stride_vt, &a.stride_vh);
+  } else if (t[V] || t[K_CACHE] || t[V_CACHE]) {
+    return PyLong_FromLong(DECLINED);
+  }
+  a.q = t[Q].ptr();
+  a.k = t[K].ptr();
+  a.v = t[V].ptr();
+  a.q_out = t[Q_OUT].ptr();
+  a.k_out = t[K_OUT].ptr();
+  a.k_cache = t[K_CACHE].ptr();
+  a.v_cache = t[V_CACHE].ptr();
+  a.slots = (const int64_t*)t[SLOTS].ptr();
+  a.status = (uint32_t*)t[STATUS].ptr();
+  strides_of(t[Q], &a.stride_qt, &a.stride_qh);
+  strides_of(t[K], &a.stride_kt, &a.stride_kh);
+  strides_of(t[Q_OUT], &a.stride_qot, &a.stride_qoh);
+  if (t[K_OUT]) strides_of(t[K_OUT], &a.stride_kot, &a.stride_koh);
+  a.q_heads = (int32_t)hq;
+  a.k_heads = (int32_t)hk;
+  a.dtype = dtype_code(*t[Q].t);
+  a.eps = (float)eps;
+  void* stream = current_stream(device);
+  return PyLong_FromLong(unlocked([&] { return iris_qk_norm_rope_launch(&a, stream); }));
+}
+
+// qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, q_weight, k_weight, dq_weight, dk_weight, workspace,
+//                       status, eps, interleaved)
+PyObject* qk_norm_rope_backward(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 17) {
+    PyErr_SetString(PyExc_TypeError, "qk_norm_rope_backward takes 17 arguments");
+    return nullptr;
+  }
+  const int device = launch_device(x[2]);
+  Operand t[15];
+  iris_qk_norm_rope_backward_args a{};
+  double eps = 0;
+  bool ok = device >= 0 && real(x[15], &eps) && truth(x[16], &a.interleaved);
+  for (int i = 0; ok && i < 15; ++i) ok = operand(x[i], device, &t[i]);
+  PyErr_Clear();
+  enum { DQ_OUT, DK_OUT, Q, K, POSITIONS, COS, SIN, DQ, DK, QW, KW, DQW, DKW, WORKSPACE, STATUS };
+  if (!ok || !t[Q] || t[Q].t->dim() != 3 || dtype_code(*t[Q].t) < 0) return PyLong_FromLong(DECLINED);
+  const auto type = t[Q].t->scalar_type();
+  const int64_t tokens = t[Q].t->size(0), hq = t[Q].t->size(1), dim = t[Q].t->size(2);
+  if (!heads_of(t[Q], type, -1, -1, -1) || !heads_of(t[K], type, tokens, -1, dim)) return PyLong_FromLong(DECLINED);
+  const int64_t hk = t[K].t->size(1);
+  if (!heads_of(t[DQ_OUT], type, tokens, hq, dim) || !heads_of(t[DQ], type, tokens, hq, dim) || !heads_of(t[DK_OUT], type, tokens, hk, dim) ||
+      !heads_of(t[DK], type, tokens, hk, dim) || !output(t[DQ]) || !output(t[DK]) || !status_ok(t[STATUS]) ||
+      !rope_operands(t[POSITIONS], t[COS], t[SIN], t[QW], t[KW], type, tokens, dim, &a))
+    return PyLong_FromLong(DECLINED);
+  if (t[DQW] || t[DKW]) {
+    if ((t[DQW] && (!t[QW] || !vector_of(t[DQW], at::kFloat, dim) || !output(t[DQW]))) ||
+        (t[DKW] && (!t[KW] || !vector_of(t[DKW], at::kFloat, dim) || !output(t[DKW]))) || !t[WORKSPACE] ||
+        !contiguous(t[WORKSPACE], at::kFloat, 2 * dim))
+      return PyLong_FromLong(DECLINED);
+    a.workspace = (float*)t[WORKSPACE].ptr();
+    a.workspace_elems = t[WORKSPACE].t->numel();
+  }
+  a.dq_out = t[DQ_OUT].ptr();
+  a.dk_out = t[DK_OUT].ptr();
+  a.q = t[Q].ptr();
+  a.k = t[K].ptr();
+  a.dq = t[DQ].ptr();
+  a.dk = t[DK].ptr();
+  a.dq_weight = (float*)t[DQW].ptr();
+  a.dk_weight = (float*)t[DKW].ptr();
+  a.status = (uint32_t*)t[STATUS].ptr();
+  strides_of(t[DQ_OUT], &a.stride_dqot, &a.stride_dqoh);
+  strides_of(t[DK_OUT], &a.stride_dkot, &a.stride_dkoh);
+  strides_of(t[Q], &a.stride_qt, &a.stride_qh);
+  strides_of(t[K], &a.stride_kt, &a.stride_kh);
+  strides_of(t[DQ], &a.stride_dqt, &a.stride_dqh);
+  strides_of(t[DK], &a.stride_dkt, &a.stride_dkh);
+  a.q_heads = (int32_t)hq;
+  a.k_heads = (int32_t)hk;
+  a.dtype = dtype_code(*t[Q].t);
+  a.eps = (float)eps;
+  void* stream = current_stream(device);
+  return PyLong_FromLong(unlocked([&] { return iris_qk_norm_rope_backward_launch(&a, stream); }));
+}
+
+// attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale, window, sinks)
+PyObject* attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 13) {
+    PyErr_SetString(PyExc_TypeError, "attention takes 13 arguments");
+    return nullptr;
+  }
+  const int device = launch_device(x[0]);
+  Operand t[10];
+  iris_attention_args a{};
+  double scale = 0;
+  bool ok = device >= 0 && (x[10] == Py_None || real(x[10], &scale)) && int32(x[11], &a.window) && int32(x[12], &a.sinks);
+  for (int i = 0; ok && i < 10; ++i) ok = operand(x[i], device, &t[i]);
+  PyErr_Clear();
+  enum { Q, K_CACHE, V_CACHE, TABLE, LENGTHS, STARTS, OUT, LSE, WORKSPACE, STATUS };
+  if (!ok || !t[Q] || t[Q].t->dim() != 3 || dtype_code(*t[Q].t) < 0 || !t[K_CACHE] || t[K_CACHE].t->dim() != 4 || !rows_contiguous(t[TABLE]))
+    return PyLong_FromLong(DECLINED);
+  const auto type = t[Q].t->scalar_type();
+  const int64_t tokens = t[Q].t->size(0), hq = t[Q].t->size(1), dim = t[Q].t->size(2), hk = t[K_CACHE].t->size(2);
+  const int64_t requests = t[TABLE].t->size(0), width = t[TABLE].t->size(1), pages = t[K_CACHE].t->size(0), page_size = t[K_CACHE].t->size(1);
+  const int64_t vec = 16 / (int64_t)t[Q].t->element_size();
+  CacheStrides k, v;
+  // (calls with nothing to do, and those whose sizes are refused, are the Python code's)
+  if (!tokens || !hq || !hk || !requests || !width || !pages || hq % hk || dim % vec || dim <= 0 || dim > MAX_ATTENTION_HEAD_DIM ||
+      width > INT32_MAX || requests > INT32_MAX || width * page_size > INT32_MAX)
+    return PyLong_FromLong(DECLINED);
+  if (!heads_of(t[Q], type, -1, -1, -1) || !heads_of(t[OUT], type, tokens, hq, dim) || !cache_of(t[K_CACHE], type, hk, dim, &k) ||
+      !cache_of(t[V_CACHE], type, hk, dim, &v) || t[K_CACHE].t->sizes() != t[V_CACHE].t->sizes() || t[TABLE].t->scalar_type() != at::kInt ||
+      !vector_of(t[LENGTHS], at::kInt, requests) || (t[STARTS] ? !vector_of(t[STARTS], at::kInt, requests + 1) : requests != tokens) ||
+      !output(t[OUT]) || !status_ok(t[STATUS]))
+    return PyLong_FromLong(DECLINED);
+  for (const int i : {Q, K_CACHE, V_CACHE})
+    if (differentiates(t[i])) return PyLong_FromLong(DECLINED);
+  if (t[LSE]) {
+    if (t[LSE].t->scalar_type() != at::kFloat || !rows_contiguous(t[LSE]) || t[LSE].t->size(0) != tokens || t[LSE].t->size(1) != hq || !output(t[LSE]))
+      return PyLong_FromLong(DECLINED);
+    a.lse = (float*)t[LSE].ptr();
+    a.stride_lse = t[LSE].t->stride(0);
+  }
+  if (t[WORKSPACE]) {
+    if (!contiguous(t[WORKSPACE], at::kFloat, 0)) return PyLong_FromLong(DECLINED);
+    a.workspace = (float*)t[WORKSPACE].ptr();
+    a.workspace_elems = t[WORKSPACE].t->numel();
+  }
+  a.q = t[Q].ptr();
+  a.k_cache = t[K_CACHE].ptr();
+  a.v_cache = t[V_CACHE].ptr();
+  a.block_table = (const int32_t*)t[TABLE].ptr();
+  a.lengths = (const int32_t*)t[LENGTHS].ptr();
+  a.query_starts = (const int32_t*)t[STARTS].ptr();
+  a.out = t[OUT].ptr();
+  a.status = (uint32_t*)t[STATUS].ptr();
+  strides_of(t[Q], &a.stride_qt, &a.stride_qh);
+  strides_of(t[OUT], &a.stride_ot, &a.stride_oh);
+  a.stride_kc_page = k.page, a.stride_kc_row = k.row, a.stride_kc_head = k.head;
+  a.stride_vc_page = v.page, a.stride_vc_row = v.row, a.stride_vc_head = v.head;
+  a.stride_table = requests > 1 ? std::max(t[TABLE].t->stride(0), width) : width;
+  if (requests > 1 && t[TABLE].t->stride(0) < width) return PyLong_FromLong(DECLINED);
+  a.requests = (int32_t)requests;
+  a.tokens = (int32_t)tokens;
+  a.q_heads = (int32_t)hq;
+  a.k_heads = (int32_t)hk;
+  a.head_dim = (int32_t)dim;
+  a.page_size = (int32_t)page_size;
+  a.table_width = (int32_t)width;
+  a.num_pages = (int32_t)pages;
+  a.dtype = dtype_code(*t[Q].t);
+  a.scale = (float)(x[10] == Py_None ? 1.0 / std::sqrt((double)dim) : scale);
+  void* stream = current_stream(device);
+  return PyLong_FromLong(unlocked([&] { return iris_attention_launch(&a, stream); }));
+}
+
 PyMethodDef methods[] = {
     {"gemm", (PyCFunction)(void (*)(void))gemm, METH_FASTCALL, "launch a shard GEMM; -1: declined"},
     {"matmul_apply", (PyCFunction)(void (*)(void))matmul_apply, METH_FASTCALL, "matmul.apply; NotImplemented: declined, int: failed"},
     {"one_shot_reduce", (PyCFunction)(void (*)(void))one_shot_reduce, METH_FASTCALL, "launch the reduce; -1: declined"},
     {"memset_i32", (PyCFunction)(void (*)(void))memset_i32, METH_FASTCALL, "int32 fill; -1: declined"},
+    {"block_tables", (PyCFunction)(void (*)(void))block_tables, METH_FASTCALL, "launch the block tables; -1: declined"},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope, METH_FASTCALL, "launch norms and rotation; -1: declined"},
+    {"qk_norm_rope_backward", (PyCFunction)(void (*)(void))qk_norm_rope_backward, METH_FASTCALL, "launch their gradient; -1: declined"},
+    {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "launch attention over a paged cache; -1: declined"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "launches through the C-ABI on torch's current stream", -1, methods,
