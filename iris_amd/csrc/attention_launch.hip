@@ -2,6 +2,7 @@
 #include <type_traits>
 
 #include "attention_rows.hpp"
+#include "attention_tiles.hpp"
 
 namespace iris_amd {
 namespace {
@@ -103,6 +104,26 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
       g.grid_units = (int)grid;
       rows::decode_kernel<dt.value, dp.value, pg.value><<<(int)grid, threads, 0, s>>>(g);
       return hipGetLastError();
+    }
+    if constexpr (dt.value != IRIS_DTYPE_F32 && dp.value <= 128 && pg.value) {
+      const int64_t row_tiles = (int64_t)a.tokens * g.group / tiles::ROWS + a.requests;
+      // (a page's rows are addressed with 32 bits)
+      const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
+      if ((int64_t)a.tokens * g.group > 32 * (int64_t)a.requests && row_tiles <= INT32_MAX / 64 && a.k_heads <= 65535 && reach <= INT32_MAX &&
+          a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
+        const int64_t units = row_tiles * a.k_heads;
+        int64_t splits = 1;
+        if (units <= cus && units <= COUNTERS) {
+          splits = 2 * cus / units;
+          const int64_t room_for = slots * rows::ROWS * (dp.value + 2) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
+          if (splits > most_keys / (4 * tiles::BT)) splits = most_keys / (4 * tiles::BT);
+          if (splits > room_for) splits = room_for;
+          if (splits < 1) splits = 1;
+        }
+        g.splits = (int)splits;
+        tiles::prompt_tiles_kernel<dt.value, dp.value><<<dim3((unsigned)(row_tiles * splits), a.k_heads), tiles::WAVES * 64, 0, s>>>(g);
+        return hipGetLastError();
+      }
     }
     const int64_t row_tiles = (int64_t)a.tokens * g.group / rows::ROWS + a.requests;
     const int64_t units = row_tiles * a.k_heads;

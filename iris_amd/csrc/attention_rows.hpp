@@ -224,14 +224,14 @@ struct Unit {
       top = max_of_row(top * g.scale_log2 - C::LIFT);
       const float m_new = fmaxf(m, top);
       const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float shrink = exp2f(m - ref);
+      const float shrink = __builtin_amdgcn_exp2f(m - ref);
       m = m_new;
       l *= shrink;
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[u][r] = exp2f(s[u][r] * g.scale_log2 - ref);
+          s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - ref);
           l += s[u][r];
         }
 #pragma unroll
@@ -322,7 +322,7 @@ struct Unit {
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds.m[w][row]);
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      weight[w] = exp2f(lds.m[w][row] - (top == -INFINITY ? 0.f : top));
+      weight[w] = __builtin_amdgcn_exp2f(lds.m[w][row] - (top == -INFINITY ? 0.f : top));
       sum += weight[w] * lds.l[w][row];
     }
     if (p.parts > 1) {
@@ -351,7 +351,7 @@ struct Unit {
     if (row >= p.rows) return;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const Target t = target(p, row);
-    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 #pragma unroll
     for (int d = part * 8; d < DP; d += 128)
       if (d < a.head_dim) {
@@ -393,7 +393,7 @@ struct Unit {
       const u32x2 bits = ml;
       const float mi = __builtin_bit_cast(f32x2, bits)[0], li = __builtin_bit_cast(f32x2, bits)[1];
       const float t = fmaxf(top, mi), ref = t == -INFINITY ? 0.f : t;
-      const float old = exp2f(top - ref), now = exp2f(mi - ref);
+      const float old = __builtin_amdgcn_exp2f(top - ref), now = __builtin_amdgcn_exp2f(mi - ref);
       top = t;
       sum = sum * old + li * now;
 #pragma unroll
@@ -401,7 +401,7 @@ struct Unit {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const Target t = target(p, row);
-    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 #pragma unroll
     for (int d = 0; d < NV; ++d) {
       const int at = d * 64 + part * 4;

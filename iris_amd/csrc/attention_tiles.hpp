@@ -1,0 +1,355 @@
+// Attention of prompts in 16 bits: 128 query rows of one key head a workgroup, keys and values through LDS.
+//
+// Rows are (token, query head of the key head) pairs, token-major, so that heads that share keys share their tiles.  Four waves
+// take 32 rows each and walk the keys in tiles of 64:
+//   scores   S^T[key, row] = K Q^T on 32 x 32 x 16 matrix instructions; the queries stay in registers.
+//   weights  one pass with a running reference and sum a row (online softmax).  A lane holds half of a row's keys of the tile
+//            and only one row, so the maximum is one exchange and the rescaling factor the lane's own.  The
+//            reference follows the maximum only when that has grown by more than SLACK: weights stay below 2^(SLACK + LIFT), and
+//            almost no tile rescales the sums.
+//   output   O^T[d, row] += V^T P^T: the lane's weights are P^T's operand as they are, four consecutive keys at a time, and
+//            V^T's comes out of LDS transposed (ds_read_b64_tr_b16: four keys of sixteen columns).
+// Tiles go from the pages to LDS by LDS-DMA, 16 bytes a lane, two stages, with the 16-byte chunks of a row exchanged
+// (XOR) so that neither read meets its own banks; keys past the end and columns past the head are read out of
+// the buffer's range and arrive as zeros.
+#pragma once
+
+#include "attention_rows.hpp"
+
+namespace iris_amd {
+namespace tiles {
+
+constexpr int WAVES = 4, ROWS = 128, WAVE_ROWS = 32, BT = 64;
+
+template <int DT, int DP>
+struct Cfg {
+  static constexpr int ROW_BYTES = DP * 2;
+  static constexpr int TILE_BYTES = BT * ROW_BYTES;
+  static constexpr int CHUNKS = ROW_BYTES / 16;        // 16-byte chunks of a key
+  static constexpr int DMA_ROWS = 1024 / ROW_BYTES;    // keys that one LDS-DMA instruction of a wave moves
+  static constexpr int DMAS = 16 / DMA_ROWS;           // ... and how many move a wave's 16 keys of a tile
+  static constexpr int KC = DP / 16;                   // matrix instructions over a head
+  static constexpr int DTILES = DP / 32;               // 32-column tiles of the output
+  static constexpr int SLOT = ROWS * DP + WAVES * 64 * 4;  // floats of a partial result
+  static constexpr float SLACK = 4.f;
+  static constexpr float LIFT = DT == IRIS_DTYPE_F16 ? 11.f : 0.f;  // (fp16 weights below 2^-14 lose places, above 65504 they end)
+};
+
+// The chunk of its row that lies at chunk position p (and the other way round: both are XORs).
+template <int DP>
+__device__ inline int swizzle_k(int row, int p) {
+  return p ^ (DP == 64 ? (row >> 1) & 7 : row & 15);
+}
+template <int DP>
+__device__ inline int swizzle_v(int row, int p) {
+  return p ^ (DP == 64 ? 2 * ((row >> 1) & 3) : 2 * (row & 7));
+}
+
+template <int DT>
+__device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (DT == IRIS_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Larger of a lane's value and that of the lane 32 away.
+__device__ inline float max_of_halves(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
+
+template <int DT, int DP>
+__global__ __launch_bounds__(WAVES * 64, 2) void prompt_tiles_kernel(AttentionKArgs g) {
+  using C = Cfg<DT, DP>;
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][C::TILE_BYTES];  // [stage][keys, values]
+  const iris_attention_args& a = g.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, half = lane >> 5;
+
+  // The workgroup's rows: row tile x is the (x - bound)-th of the last request whose bound is not past x; late rows, which see
+  // the most keys, start first.
+  const int back = gridDim.x - 1 - blockIdx.x, x = back / g.splits, split = back - x * g.splits;
+  auto bound = [&](int r) { return (int)((int64_t)scalar_at(a.query_starts, r) * g.group / ROWS) + r; };
+  int request = 0;
+  for (int hi = a.requests; hi - request > 1;) {
+    const int mid = (request + hi) / 2;
+    if (bound(mid) <= x)
+      request = mid;
+    else
+      hi = mid;
+  }
+  const int token0 = scalar_at(a.query_starts, request);
+  const int tokens = min(scalar_at(a.query_starts, request + 1), a.tokens) - token0;
+  const int row0 = (x - bound(request)) * ROWS;
+  if (row0 < 0 || token0 < 0 || tokens <= 0 || row0 >= (int64_t)tokens * g.group) return;
+  const int num_rows = (int)min((int64_t)ROWS, (int64_t)tokens * g.group - row0);
+  const int head = blockIdx.y;
+  int length = max(scalar_at(a.lengths, request), 0);
+  if ((int64_t)length > (int64_t)a.table_width * g.page.d) {
+    if (tid == 0) report(a.status, IRIS_STATUS_BAD_INDEX);
+    length = (int)(a.table_width * g.page.d);
+  }
+  const int first = length - tokens;  // position of the request's first query
+  const KeyTiles list = key_tiles<BT>(a, first + row0 / g.group, first + (row0 + num_rows - 1) / g.group);
+  // the workgroup's share of the tiles
+  const int j0 = (int)((int64_t)list.count * split / g.splits), j1 = (int)((int64_t)list.count * (split + 1) / g.splits);
+
+  // the lane's row
+  const int wrow = wave * WAVE_ROWS;
+  const bool have_row = wrow + n < num_rows;
+  const int row = row0 + (have_row ? wrow + n : 0);
+  const int token = (int)((uint32_t)row / (uint32_t)g.group), qhead = head * g.group + row - token * g.group;
+  const int at = have_row ? first + token : -1;
+  // positions of the wave's rows, from .. to (no row: an empty range)
+  const int wave_first = first + (row0 + min(wrow, num_rows)) / g.group;
+  const int wave_last = wrow < num_rows ? first + (row0 + min(wrow + WAVE_ROWS, num_rows) - 1) / g.group : -1;
+
+  u32x4 q[C::KC];
+  {
+    const IRIS_GLOBAL char* qp = (const IRIS_GLOBAL char*)a.q + ((int64_t)(token0 + token) * a.stride_qt + (int64_t)qhead * a.stride_qh) * 2 + half * 16;
+#pragma unroll
+    for (int c = 0; c < C::KC; ++c) {
+      q[c] = u32x4{0, 0, 0, 0};
+      if (have_row && c * 16 + half * 8 < a.head_dim) q[c] = *(const IRIS_GLOBAL u32x4*)(qp + c * 32);
+    }
+  }
+
+  // What a wave fetches: 16 keys of each tile, DMA_ROWS an instruction.  Offsets of the lane's chunk from the first of the 16.
+  uint32_t k_off[C::DMAS], v_off[C::DMAS];
+#pragma unroll
+  for (int i = 0; i < C::DMAS; ++i) {
+    const int r = i * C::DMA_ROWS + lane / C::CHUNKS, p = lane % C::CHUNKS;
+    const int kc = swizzle_k<DP>(r, p), vc = swizzle_v<DP>(r, p);
+    k_off[i] = kc * 8 < a.head_dim ? (uint32_t)(r * a.stride_kc_row * 2) + kc * 16 : DEAD_OFFSET;
+    v_off[i] = vc * 8 < a.head_dim ? (uint32_t)(r * a.stride_vc_row * 2) + vc * 16 : DEAD_OFFSET;
+  }
+  bool bad_page = false;
+  auto fetch_page = [&](int j) {  // the page of the wave's keys of list tile j
+    const int key = list.tile(j) * BT + wave * 16;
+    return key < length ? scalar_at(a.block_table, (int64_t)request * a.stride_table + page_div((uint32_t)key, g.page)) : 0;
+  };
+  auto fetch = [&](int j, int page, int stage) {
+    const int key = list.tile(j) * BT + wave * 16;
+    if ((uint32_t)page >= (uint32_t)a.num_pages) {
+      bad_page = true;
+      page = 0;
+    }
+    const int in_page = key - (int)(page_div((uint32_t)key, g.page) * g.page.d);
+    const int valid = length - key;  // of the 16 keys
+    const __amdgpu_buffer_rsrc_t kr = tile_rsrc((const IRIS_GLOBAL char*)a.k_cache + ((int64_t)page * a.stride_kc_page + (int64_t)head * a.stride_kc_head) * 2, 0x7FFFFFFF);
+    const __amdgpu_buffer_rsrc_t vr = tile_rsrc((const IRIS_GLOBAL char*)a.v_cache + ((int64_t)page * a.stride_vc_page + (int64_t)head * a.stride_vc_head) * 2, 0x7FFFFFFF);
+    const int k_at = in_page * (int)(a.stride_kc_row * 2), v_at = in_page * (int)(a.stride_vc_row * 2);
+#pragma unroll
+    for (int i = 0; i < C::DMAS; ++i) {
+      uint32_t ko = k_off[i], vo = v_off[i];
+      if (valid < 16 && i * C::DMA_ROWS + lane / C::CHUNKS >= valid) ko = vo = DEAD_OFFSET;
+      lds_dma16(kr, (IRIS_LDS void*)&lds[stage][0][wave * 16 * C::ROW_BYTES + i * 1024], ko, k_at);
+      lds_dma16(vr, (IRIS_LDS void*)&lds[stage][1][wave * 16 * C::ROW_BYTES + i * 1024], vo, v_at);
+    }
+  };
+  // where the lane reads: keys by row, values by groups of four keys
+  int k_read[C::KC];
+#pragma unroll
+  for (int c = 0; c < C::KC; ++c) k_read[c] = n * C::ROW_BYTES + swizzle_k<DP>(n, 2 * c + half) * 16;
+  const int v_row = half * 4 + ((lane & 15) >> 2);  // (and eight further on for the second four)
+  int v_read[C::DTILES];
+#pragma unroll
+  for (int t = 0; t < C::DTILES; ++t) {
+    const int column = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    v_read[t] = v_row * C::ROW_BYTES + swizzle_v<DP>(v_row, column / 8) * 16 + (column & 7) * 2;
+  }
+  // (both swizzles repeat after 16 rows)
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  auto read_v = [&](const char* base, int t, int group) {  // V^T's operand: 16 keys of 32 columns
+    const IRIS_LDS char* p = (const IRIS_LDS char*)base + group * 16 * C::ROW_BYTES;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((IRIS_LDS s16x4*)(p + v_read[t]));
+    // rows eight further on: for 128 columns the swizzle is the same, for 64 it is too ((row >> 1) & 3 repeats after 8)
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((IRIS_LDS s16x4*)(p + v_read[t] + 8 * C::ROW_BYTES));
+    return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x16 o[C::DTILES];
+#pragma unroll
+  for (int t = 0; t < C::DTILES; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+  float ref = -INFINITY, l = 0.f;
+  bool poisoned = false;
+
+  int page = 0;
+  if (j0 < j1) {
+    fetch(j0, fetch_page(j0), j0 & 1);
+    if (j0 + 1 < j1) page = fetch_page(j0 + 1);
+  }
+  for (int j = j0; j < j1; ++j) {
+    const int stage = j & 1, base = list.tile(j) * BT;
+    IRIS_WAIT_VMCNT(0);  // this wave's share of the tile has arrived; behind the barrier everyone's has
+    block_barrier_raw();
+    if (j + 1 < j1) {
+      fetch(j + 1, page, stage ^ 1);
+      if (j + 2 < j1) page = fetch_page(j + 2);
+    }
+    if (base > wave_last) continue;
+    const char* kt = lds[stage][0];
+    const char* vt = lds[stage][1];
+    f32x16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C::KC; ++c) {
+        const u32x4 k = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)kt + u * 32 * C::ROW_BYTES + k_read[c]);
+        s[u] = mfma<DT>(k, q[c], s[u]);
+      }
+    }
+    // May some of the tile's keys be hidden from some of the wave's rows?
+    const bool edge = base + BT - 1 > wave_first || (a.window > 0 && wave_last - base >= a.window && base + BT > a.sinks);
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!sees(a, at, base + u * 32 + 8 * (r / 4) + 4 * half + r % 4)) s[u][r] = -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = max_of_halves(top) * g.scale_log2 - C::LIFT;
+    if (__any(top > ref + C::SLACK || ref == -INFINITY)) {
+      const float next = fmaxf(ref, top), from = next == -INFINITY ? 0.f : next;
+      const float shrink = __builtin_amdgcn_exp2f(ref - from);
+      ref = next;
+      l *= shrink;
+#pragma unroll
+      for (int t = 0; t < C::DTILES; ++t) o[t] *= shrink;
+    }
+    const float from = ref == -INFINITY ? 0.f : ref;
+    u32x4 p[4];  // P^T's operands: 16 keys each
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - from);
+        l += s[u][r];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        p[2 * u + i] = u32x4{pack2<DT>(s[u][8 * i], s[u][8 * i + 1]), pack2<DT>(s[u][8 * i + 2], s[u][8 * i + 3]),
+                             pack2<DT>(s[u][8 * i + 4], s[u][8 * i + 5]), pack2<DT>(s[u][8 * i + 6], s[u][8 * i + 7])};
+    }
+    if (edge) {  // is a value among the tile's, some of which some rows must not see, not a finite number?
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 most = {0, 0};
+#pragma unroll 1
+      for (int i = 0; i < C::TILE_BYTES; i += 1024) {
+        const u32x4 v = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)vt + i + lane * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[w] & 0x7FFF7FFFu));
+      }
+      constexpr unsigned short INF = DT == IRIS_DTYPE_BF16 ? 0x7F80 : 0x7C00;
+      poisoned |= most[0] >= INF || most[1] >= INF;
+    }
+#pragma unroll
+    for (int t = 0; t < C::DTILES; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[t] = mfma<DT>(read_v(vt, t, i), p[i], o[t]);
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  // what one wave found is every row's
+  bool redo = __syncthreads_or(poisoned);
+  float flags = __syncthreads_or(bad_page) ? __builtin_nanf("") : 0.f;
+  if (g.splits > 1) {
+    // The parts meet in the workspace, each in the order of its registers: the last to arrive has the rows of all in the same lanes.
+    const int unit = blockIdx.y * (gridDim.x / g.splits) + x;
+    auto slot = [&](int part) { return (IRIS_GLOBAL char*)(g.slots + ((int64_t)unit * g.splits + part) * C::SLOT); };
+    const uint32_t mine = (wave * 64 + lane) * 16;
+#pragma unroll
+    for (int t = 0; t < C::DTILES; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4 v = {o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
+        store16_any<AUX_SC1>(slot(split) + (t * 4 + r / 4) * (WAVES * 1024) + mine, __builtin_bit_cast(u32x4, v));
+      }
+    const f32x4 tail = {ref, l, flags, redo ? 1.f : 0.f};
+    store16_any<AUX_SC1>(slot(split) + C::DTILES * 4 * (WAVES * 1024) + mine, __builtin_bit_cast(u32x4, tail));
+    IRIS_WAIT_VMCNT(0);
+    __syncthreads();
+    int last = 0;
+    if (tid == 0) {
+      IRIS_GLOBAL int32_t* count = (IRIS_GLOBAL int32_t*)(g.counters + unit);
+      last = arrive(count, false, false) == g.splits - 1;
+      if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!__syncthreads_or(last)) return;
+#pragma unroll
+    for (int t = 0; t < C::DTILES; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+    ref = -INFINITY;
+    l = 0.f;
+    float again = 0.f;
+    for (int part = 0; part < g.splits; ++part) {
+      const __amdgpu_buffer_rsrc_t rs = tile_rsrc(slot(part), C::SLOT * 4);
+      const f32x4 m = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)mine, C::DTILES * 4 * (WAVES * 1024), AUX_SC1));
+      const float next = fmaxf(ref, m[0]), from = next == -INFINITY ? 0.f : next;
+      const float old = __builtin_amdgcn_exp2f(ref - from), now = __builtin_amdgcn_exp2f(m[0] - from);
+      ref = next;
+      l = l * old + m[1] * now;
+      flags += m[2];
+      again += m[3];
+#pragma unroll
+      for (int t = 0; t < C::DTILES; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const f32x4 v =
+              __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)mine, (t * 4 + r / 4) * (WAVES * 1024), AUX_SC1));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][r + i] = o[t][r + i] * old + v[i] * now;
+        }
+    }
+    redo = __builtin_amdgcn_readfirstlane(again > 0.f);
+  }
+  if (flags != 0.f && lane == 0) report(a.status, IRIS_STATUS_BAD_INDEX);
+
+  // A weight of 0 times a value that is no number is NaN: then the rows are computed again by the kernel that takes hidden values out.
+  if (redo) {
+    static_assert(sizeof(rows::Lds<DT, DP>) <= sizeof(lds), "the tiles' room is given over");
+    rows::Unit<DT, DP, true, false> unit(g, *(rows::Lds<DT, DP>*)lds);
+#pragma unroll 1
+    for (int r = 0; r < num_rows; r += rows::ROWS) {
+      rows::Piece p{};
+      p.request = request;
+      p.head = head;
+      p.row0 = row0 + r;
+      p.rows = min(rows::ROWS, num_rows - r);
+      p.token0 = token0;
+      p.length = length;
+      p.first = first;
+      p.tiles = key_tiles<rows::Cfg<DT, DP>::BT>(a, first + p.row0 / g.group, first + (p.row0 + p.rows - 1) / g.group);
+      p.j1 = p.tiles.count;
+      p.parts = 1;
+      unit.run(p);
+    }
+    return;
+  }
+  if (!have_row) return;
+  // (a page outside the cache: every number of the rows is NaN)
+  const float inv = flags != 0.f ? flags : l == 0.f ? 0.f : 1.f / l;
+  const int64_t out_token = token0 + token;
+  if (a.lse && half == 0)
+    a.lse[out_token * a.stride_lse + qhead] = flags != 0.f ? flags : l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  IRIS_GLOBAL char* out = (IRIS_GLOBAL char*)a.out + (out_token * a.stride_ot + (int64_t)qhead * a.stride_oh) * 2;
+#pragma unroll
+  for (int t = 0; t < C::DTILES; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = t * 32 + 2 * r + 4 * half;
+      if (d < a.head_dim)
+        *(IRIS_GLOBAL u32x2*)(out + d * 2) = u32x2{pack2<DT>(o[t][r] * inv, o[t][r + 1] * inv), pack2<DT>(o[t][r + 2] * inv, o[t][r + 3] * inv)};
+    }
+}
+
+}  // namespace tiles
+}  // namespace iris_amd
