@@ -4,9 +4,8 @@
 // take 32 rows each and walk the keys in tiles of 64:
 //   scores   S^T[key, row] = K Q^T on 32 x 32 x 16 matrix instructions; the queries stay in registers.
 //   weights  one pass with a running reference and sum a row (online softmax).  A lane holds half of a row's keys of the tile
-//            and only one row, so the maximum is one exchange and the rescaling factor the lane's own.  The
-//            reference follows the maximum only when that has grown by more than SLACK: weights stay below 2^(SLACK + LIFT), and
-//            almost no tile rescales the sums.
+//            and only one row, so a maximum is one exchange and a rescaling factor the lane's own; and the reference need not be the
+//            maximum, only near enough that weights and sums stay in range, so almost no tile looks for the one or needs the other.
 //   output   O^T[d, row] += V^T P^T: the lane's weights are P^T's operand as they are, four consecutive keys at a time, and
 //            V^T's comes out of LDS transposed (ds_read_b64_tr_b16: four keys of sixteen columns).
 // Tiles go from the pages to LDS by LDS-DMA, 16 bytes a lane, two stages, with the 16-byte chunks of a row exchanged
@@ -20,6 +19,8 @@ namespace iris_amd {
 namespace tiles {
 
 constexpr int WAVES = 4, ROWS = 128, WAVE_ROWS = 32, BT = 64;
+constexpr int AHEAD = 4;
+constexpr int SCHED_MFMA = 0x8, SCHED_DS_READ = 0x100;  // kinds of instructions of __builtin_amdgcn_sched_group_barrier
 
 template <int DT, int DP>
 struct Cfg {
@@ -31,8 +32,11 @@ struct Cfg {
   static constexpr int KC = DP / 16;                   // matrix instructions over a head
   static constexpr int DTILES = DP / 32;               // 32-column tiles of the output
   static constexpr int SLOT = ROWS * DP + WAVES * 64 * 4;  // floats of a partial result
-  static constexpr float SLACK = 4.f;
-  static constexpr float LIFT = DT == IRIS_DTYPE_F16 ? 11.f : 0.f;  // (fp16 weights below 2^-14 lose places, above 65504 they end)
+  // Weights are 2^(score - reference), and the reference is the maximum, less LIFT, of the first keys that the row sees; it stays
+  // until a lane's 32 weights of a tile sum up to more than MOST.  fp16 ends at 65504 and loses places below 2^-14, so that LIFT
+  // stands between; bf16 and the fp32 sums have room for any of it.
+  static constexpr float LIFT = DT == IRIS_DTYPE_F16 ? 6.f : 0.f;
+  static constexpr float MOST = DT == IRIS_DTYPE_F16 ? 32768.f : 1.1529215e18f;
 };
 
 // The chunk of its row that lies at chunk position p (and the other way round: both are XORs).
@@ -57,7 +61,7 @@ __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
 __device__ inline float max_of_halves(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 
 template <int DT, int DP>
-__global__ __launch_bounds__(WAVES * 64, 2) void prompt_tiles_kernel(AttentionKArgs g) {
+__global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_tiles_kernel(AttentionKArgs g) {
   using C = Cfg<DT, DP>;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][C::TILE_BYTES];  // [stage][keys, values]
   const iris_attention_args& a = g.a;
@@ -171,90 +175,133 @@ __global__ __launch_bounds__(WAVES * 64, 2) void prompt_tiles_kernel(AttentionKA
   for (int t = 0; t < C::DTILES; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
-  float ref = -INFINITY, l = 0.f;
+  float ref = have_row ? -INFINITY : 0.f, l = 0.f;
   bool poisoned = false;
 
+  // Tiles are fetched a stage ahead by all waves; the last ones of a workgroup may lie past a wave's own last key.
   int page = 0;
   if (j0 < j1) {
     fetch(j0, fetch_page(j0), j0 & 1);
     if (j0 + 1 < j1) page = fetch_page(j0 + 1);
   }
-  for (int j = j0; j < j1; ++j) {
-    const int stage = j & 1, base = list.tile(j) * BT;
+  auto next_stage = [&](int j) {
     IRIS_WAIT_VMCNT(0);  // this wave's share of the tile has arrived; behind the barrier everyone's has
     block_barrier_raw();
     if (j + 1 < j1) {
-      fetch(j + 1, page, stage ^ 1);
+      fetch(j + 1, page, (j + 1) & 1);
       if (j + 2 < j1) page = fetch_page(j + 2);
     }
-    if (base > wave_last) continue;
-    const char* kt = lds[stage][0];
-    const char* vt = lds[stage][1];
-    f32x16 s[2];
+  };
+  f32x16 s[2];
+  u32x4 p[4];  // P^T's operands: 16 keys each
+  float sum;
+  // The scores of list tile j.  Operands are read AHEAD matrix instructions before they are used; two sums in turn, so that
+  // neither waits for its own last step.
+  auto score = [&](int j) {
+    const char* kt = lds[j & 1][0];
+    u32x4 f[AHEAD];
+    auto read_k = [&](int i) { return *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)kt + (i & 1) * 32 * C::ROW_BYTES + k_read[i / 2]); };
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < C::KC; ++c) {
-        const u32x4 k = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)kt + u * 32 * C::ROW_BYTES + k_read[c]);
-        s[u] = mfma<DT>(k, q[c], s[u]);
+    for (int i = 0; i < AHEAD; ++i) f[i] = read_k(i);
+    __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * C::KC; ++i) {
+      s[i & 1] = mfma<DT>(f[i % AHEAD], q[i / 2], s[i & 1]);
+      __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 1, 0);
+      if (i + AHEAD < 2 * C::KC) {
+        f[i % AHEAD] = read_k(i + AHEAD);
+        __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, 1, 0);
       }
     }
     // May some of the tile's keys be hidden from some of the wave's rows?
-    const bool edge = base + BT - 1 > wave_first || (a.window > 0 && wave_last - base >= a.window && base + BT > a.sinks);
-    if (edge) {
+    const int base = list.tile(j) * BT;
+    if (base + BT - 1 > wave_first || (a.window > 0 && wave_last - base >= a.window && base + BT > a.sinks)) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (!sees(a, at, base + u * 32 + 8 * (r / 4) + 4 * half + r % 4)) s[u][r] = -INFINITY;
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    top = max_of_halves(top) * g.scale_log2 - C::LIFT;
-    if (__any(top > ref + C::SLACK || ref == -INFINITY)) {
-      const float next = fmaxf(ref, top), from = next == -INFINITY ? 0.f : next;
-      const float shrink = __builtin_amdgcn_exp2f(ref - from);
-      ref = next;
-      l *= shrink;
-#pragma unroll
-      for (int t = 0; t < C::DTILES; ++t) o[t] *= shrink;
-    }
-    const float from = ref == -INFINITY ? 0.f : ref;
-    u32x4 p[4];  // P^T's operands: 16 keys each
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - from);
-        l += s[u][r];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        p[2 * u + i] = u32x4{pack2<DT>(s[u][8 * i], s[u][8 * i + 1]), pack2<DT>(s[u][8 * i + 2], s[u][8 * i + 3]),
-                             pack2<DT>(s[u][8 * i + 4], s[u][8 * i + 5]), pack2<DT>(s[u][8 * i + 6], s[u][8 * i + 7])};
-    }
-    if (edge) {  // is a value among the tile's, some of which some rows must not see, not a finite number?
+      // is a value among the tile's, some of which some rows must not see, not a finite number?
       typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
       u16x2 most = {0, 0};
 #pragma unroll 1
       for (int i = 0; i < C::TILE_BYTES; i += 1024) {
-        const u32x4 v = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)vt + i + lane * 16);
+        const u32x4 v = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)lds[j & 1][1] + i + lane * 16);
 #pragma unroll
         for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[w] & 0x7FFF7FFFu));
       }
       constexpr unsigned short INF = DT == IRIS_DTYPE_BF16 ? 0x7F80 : 0x7C00;
       poisoned |= most[0] >= INF || most[1] >= INF;
     }
+  };
+  // The weights, against the reference as it stands.
+  auto weigh = [&] {
+    const float from = ref == -INFINITY ? 0.f : ref;
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < C::DTILES; ++t)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[t] = mfma<DT>(read_v(vt, t, i), p[i], o[t]);
+      for (int i = 0; i < 2; ++i) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * i + e], g.scale_log2, -from));
+          sums[e & 3] += w[e];
+        }
+        p[2 * u + i] = u32x4{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
+      }
+    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  };
+  auto add_values = [&](int j) {
+    l += sum;
+    const char* vt = lds[j & 1][1];
+    u32x4 f[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) f[i] = read_v(vt, i % C::DTILES, i / C::DTILES);
+    __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, 2 * AHEAD, 1);
+#pragma unroll
+    for (int i = 0; i < 4 * C::DTILES; ++i) {
+      o[i % C::DTILES] = mfma<DT>(f[i % AHEAD], p[i / C::DTILES], o[i % C::DTILES]);
+      __builtin_amdgcn_sched_group_barrier(SCHED_MFMA, 1, 1);
+      if (i + AHEAD < 4 * C::DTILES) {
+        f[i % AHEAD] = read_v(vt, (i + AHEAD) % C::DTILES, (i + AHEAD) / C::DTILES);
+        __builtin_amdgcn_sched_group_barrier(SCHED_DS_READ, 2, 1);
+      }
+    }
+  };
+  int j = j0, own_end = j0;  // the tiles that hold keys of the wave's
+  while (own_end < j1 && list.tile(own_end) * BT <= wave_last) ++own_end;
+  for (;; ++j) {
+    // The maximum is looked for only where there is no reference yet, or where the sum says that the reference is far too low: a
+    // tile in hundreds, outside the loop that the others stay in (sums that are rescaled in it would be kept twice).
+    for (; j < own_end; ++j) {
+      next_stage(j);
+      score(j);
+      if (__any(ref == -INFINITY)) break;
+      weigh();
+      if (__any(sum > C::MOST)) break;
+      add_values(j);
+    }
+    if (j >= own_end) break;
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    const float next = fmaxf(ref, max_of_halves(top) * g.scale_log2 - C::LIFT);
+    const float shrink = __builtin_amdgcn_exp2f(ref - (next == -INFINITY ? 0.f : next));
+    ref = next;
+    l *= shrink;
+#pragma unroll
+    for (int t = 0; t < C::DTILES; ++t) o[t] *= shrink;
+    weigh();
+    add_values(j);
   }
+  for (; j < j1; ++j) next_stage(j);
 
   l += __shfl_xor(l, 32, 64);
   // what one wave found is every row's
