@@ -25,6 +25,7 @@ struct AttentionKArgs {
   float scale_log2;   // scale * log2(e): scores are exponents of two
   int group;          // query heads to a key head
   int splits;         // parts of a unit's keys (prompts)
+  int by_length;      // rows that see the most keys start first (prompts in tiles)
   int grid_units;     // workgroups that share the work (decode)
   float* slots;       // partial results, `slot_elems` floats each
   int32_t* counters;  // arrivals at split units; zero between launches
@@ -54,6 +55,18 @@ __device__ inline KeyTiles key_tiles(const iris_attention_args& a, int first, in
 // Does the query at position `at` see key `key`?  (window 0: all up to its own)
 __device__ inline bool sees(const iris_attention_args& a, int at, int key) {
   return key <= at && (a.window <= 0 || at - key < a.window || key < a.sinks);
+}
+
+// sum + the two 16-bit weights of `w`: sums of the weights as they are multiplied, so that a row whose weight is one key's has that
+// key's value and nothing of the weight's rounding.  (Subnormal fp16 weights count.)
+template <int DT>
+__device__ inline float add_weights(uint32_t w, float sum) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == IRIS_DTYPE_BF16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
 }
 
 // Word i of an array that no kernel writes while this one runs, by a scalar load (i is the wave's).

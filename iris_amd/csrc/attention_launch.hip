@@ -13,6 +13,9 @@ constexpr int MAX_HEAD_DIM = 256;
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
+// Floats of a partial result of 16 rows.
+int64_t row_slot(int dim) { return rows::ROWS * (padded_dim(dim) + 4); }
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 hipError_t check(const iris_attention_args& a) {
@@ -59,7 +62,7 @@ hipError_t with_types(const iris_attention_args& a, F f) {
 extern "C" int64_t iris_attention_workspace_elems(int32_t head_dim) {
   using namespace iris_amd;
   if (head_dim <= 0 || head_dim > MAX_HEAD_DIM) return 0;
-  return COUNTERS + ROW_SLOTS * rows::ROWS * (padded_dim(head_dim) + 2);
+  return COUNTERS + ROW_SLOTS * row_slot(head_dim);
 }
 
 extern "C" int iris_attention_launch(const iris_attention_args* args, void* stream) {
@@ -79,7 +82,7 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
   const int cus = current_cu_count();
   int64_t slots = 0;
   if (a.workspace && a.workspace_elems > COUNTERS) {
-    slots = (a.workspace_elems - COUNTERS) / (rows::ROWS * (padded_dim(a.head_dim) + 2));
+    slots = (a.workspace_elems - COUNTERS) / row_slot(a.head_dim);
     g.counters = (int32_t*)a.workspace;
     g.slots = a.workspace + COUNTERS;
   }
@@ -109,19 +112,21 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
       const int64_t row_tiles = (int64_t)a.tokens * g.group / tiles::ROWS + a.requests;
       // (a page's rows are addressed with 32 bits)
       const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
-      if ((int64_t)a.tokens * g.group > 32 * (int64_t)a.requests && row_tiles <= INT32_MAX / 64 && a.k_heads <= 65535 && reach <= INT32_MAX &&
+      if ((int64_t)a.tokens * g.group > 32 * (int64_t)a.requests && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX &&
           a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
         const int64_t units = row_tiles * a.k_heads;
         int64_t splits = 1;
         if (units <= cus && units <= COUNTERS) {
           splits = 2 * cus / units;
-          const int64_t room_for = slots * rows::ROWS * (dp.value + 2) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
+          const int64_t room_for = slots * row_slot(a.head_dim) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
           if (splits > most_keys / (4 * tiles::BT)) splits = most_keys / (4 * tiles::BT);
           if (splits > room_for) splits = room_for;
           if (splits < 1) splits = 1;
         }
         g.splits = (int)splits;
-        tiles::prompt_tiles_kernel<dt.value, dp.value><<<dim3((unsigned)(row_tiles * splits), a.k_heads), tiles::WAVES * 64, 0, s>>>(g);
+        // (which starts first matters where not all run at once; a window leaves little between them)
+        g.by_length = units * splits > 2 * cus && a.window == 0 && a.requests <= 64;
+        tiles::prompt_tiles_kernel<dt.value, dp.value><<<(int)(units * splits), tiles::WAVES * 64, 0, s>>>(g);
         return hipGetLastError();
       }
     }

@@ -31,7 +31,7 @@ struct Cfg {
   static constexpr int VE = DP / 16;                 // elements of a value that a lane loads
   static constexpr int VB = VE * ES;                 // their bytes: 8, 16, 32 or 64
   static constexpr int VW = VB / 4;                  // their words
-  static constexpr int SLOT = ROWS * (DP + 2);       // floats of a partial result
+  static constexpr int SLOT = ROWS * (DP + 4);       // floats of a partial result
   // Weights are 2^(score - maximum + LIFT): fp16 ones of keys far below the maximum stay normal numbers (to 2^-28 of the largest
   // weight), and the sum, lifted alike, takes it out again.
   static constexpr float LIFT = DT == IRIS_DTYPE_F16 ? 14.f : 0.f;
@@ -67,7 +67,7 @@ __device__ inline int slot_of(const Piece& p, int part) { return part ? p.later_
 template <int DT, int DP>
 struct alignas(16) Lds {
   float o[WAVES][ROWS][DP + 4];
-  float m[WAVES][ROWS], l[WAVES][ROWS];
+  float m[WAVES][ROWS], l[WAVES][ROWS], lse_l[WAVES][ROWS];
   int last;
 };
 
@@ -147,7 +147,8 @@ struct Unit {
     f32x4 o[C::VE];
 #pragma unroll
     for (int e = 0; e < C::VE; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    // l: the sum of the weights as they are multiplied; lse_l: as they are, for the logarithm
+    float m = -INFINITY, l = 0.f, lse_l = 0.f;
 
     for (int j = p.j0; j < p.j1; ++j) {
       const int base = p.tiles.tile(j) * C::BT + wave * C::KS;
@@ -227,17 +228,28 @@ struct Unit {
       const float shrink = __builtin_amdgcn_exp2f(m - ref);
       m = m_new;
       l *= shrink;
+      lse_l *= shrink;
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - ref);
-          l += s[u][r];
+        for (int r = 0; r < 4; ++r) s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - ref);
+      u32x4 weights;  // in the operand's type: for fp32 themselves
+      if constexpr (C::F32) {
+        weights = __builtin_bit_cast(u32x4, s[0]);
+        l += (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
+        lse_l = l;
+      } else {
+        weights = u32x4{pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]), pack2<DT>(s[1][2], s[1][3])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          l = add_weights<DT>(weights[e], l);
+          lse_l += s[0][e] + s[1][e];
         }
+      }
 #pragma unroll
       for (int e = 0; e < C::VE; ++e) o[e] *= shrink;
       if (!poisoned) {
-        add_values(s, v, o);
+        add_values(weights, v, o);
       } else {
         // (0 times it would still be NaN: each row's keys apart, with what it does not see taken out)
         for (int x = 0; x < ROWS; ++x) {
@@ -254,7 +266,7 @@ struct Unit {
           f32x4 one[C::VE];
 #pragma unroll
           for (int e = 0; e < C::VE; ++e) one[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-          add_values(s, vx, one);
+          add_values(weights, vx, one);
 #pragma unroll
           for (int e = 0; e < C::VE; ++e)
             if (n == x) o[e] += one[e];
@@ -263,7 +275,9 @@ struct Unit {
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    finish(p, m, l, o);
+    lse_l += __shfl_xor(lse_l, 16, 64);
+    lse_l += __shfl_xor(lse_l, 32, 64);
+    finish(p, m, l, lse_l, o);
   }
 
   static __device__ inline bool not_finite(uint32_t w) {
@@ -273,16 +287,15 @@ struct Unit {
   }
 
   // O^T += V^T P^T
-  __device__ inline void add_values(const f32x4 (&s)[C::SUBS], const uint32_t (&v)[C::SUBS][4][C::VW], f32x4 (&o)[C::VE]) {
+  __device__ inline void add_values(u32x4 w, const uint32_t (&v)[C::SUBS][4][C::VW], f32x4 (&o)[C::VE]) {
     if constexpr (C::F32) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int e = 0; e < C::VE; ++e)
-          o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[0][r][e]), s[0][r], o[e], 0, 0, 0);
+          o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[0][r][e]), __builtin_bit_cast(f32x4, w)[r], o[e], 0, 0, 0);
     } else {
-      // (the weights in 16 bits, as the matrix instruction takes them: at most half a last place of the values' own type)
-      const u32x4 w = {pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]), pack2<DT>(s[1][2], s[1][3])};
+      // (the weights are in 16 bits, as the matrix instruction takes them: off by half a last place of the values' own type)
 #pragma unroll
       for (int e = 0; e < C::VE; ++e) {
         u32x4 t;
@@ -297,15 +310,16 @@ struct Unit {
   }
 
   // The waves' shares meet; the unit's result is written, or its part handed over.
-  __device__ inline void finish(const Piece& p, float m, float l, const f32x4 (&o)[C::VE]) {
+  __device__ inline void finish(const Piece& p, float m, float l, float lse_l, const f32x4 (&o)[C::VE]) {
     if (__any(bad_page)) {
       if (lane == 0) report(a.status, IRIS_STATUS_BAD_INDEX);
-      l = __builtin_nanf("");
+      l = lse_l = __builtin_nanf("");
     }
     __syncthreads();  // (the last unit's shares have been read)
     if (quad == 0) {
       lds.m[wave][n] = m;
       lds.l[wave][n] = l;
+      lds.lse_l[wave][n] = lse_l;
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -317,13 +331,14 @@ struct Unit {
     __syncthreads();
     // sixteen lanes a row
     const int row = threadIdx.x / 16, part = threadIdx.x % 16;
-    float top = -INFINITY, sum = 0.f, weight[WAVES];
+    float top = -INFINITY, sum = 0.f, lse_sum = 0.f, weight[WAVES];
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds.m[w][row]);
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       weight[w] = __builtin_amdgcn_exp2f(lds.m[w][row] - (top == -INFINITY ? 0.f : top));
       sum += weight[w] * lds.l[w][row];
+      lse_sum += weight[w] * lds.lse_l[w][row];
     }
     if (p.parts > 1) {
       float* slot = g.slots + (int64_t)slot_of(p, p.part) * C::SLOT;
@@ -335,7 +350,7 @@ struct Unit {
         store16_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + row * DP + d), __builtin_bit_cast(u32x4, x));
       }
       if (part == 0)
-        store8_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + ROWS * DP + 2 * row), u32x2{__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, sum)});
+        store16_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + ROWS * DP + 4 * row), __builtin_bit_cast(u32x4, f32x4{top, sum, lse_sum, 0.f}));
       // the stores have reached the agent's coherence point before the arrival is counted
       IRIS_WAIT_VMCNT(0);
       __syncthreads();
@@ -351,7 +366,7 @@ struct Unit {
     if (row >= p.rows) return;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const Target t = target(p, row);
-    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = lse_sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(lse_sum)) * 0.6931471805599453f;
 #pragma unroll
     for (int d = part * 8; d < DP; d += 128)
       if (d < a.head_dim) {
@@ -379,29 +394,29 @@ struct Unit {
   __device__ inline void join(const Piece& p, int row, int part) {
     if (row >= p.rows) return;
     auto buffer = [&](int i) { return tile_rsrc((const IRIS_GLOBAL char*)(g.slots + (int64_t)slot_of(p, i) * C::SLOT), C::SLOT * 4); };
-    float top = -INFINITY, sum = 0.f;
+    float top = -INFINITY, sum = 0.f, lse_sum = 0.f;
     constexpr int NV = (DP + 63) / 64;
     f32x4 x[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < p.parts; ++i) {
       const __amdgpu_buffer_rsrc_t rs = buffer(__builtin_amdgcn_readfirstlane(i));
-      const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(rs, (ROWS * DP + 2 * row) * 4, 0, AUX_SC1);
+      const f32x4 ml = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (ROWS * DP + 4 * row) * 4, 0, AUX_SC1));
       u32x4 y[NV];
 #pragma unroll
       for (int d = 0; d < NV; ++d) y[d] = __builtin_amdgcn_raw_buffer_load_b128(rs, (row * DP + d * 64 + part * 4) * 4, 0, AUX_SC1);
-      const u32x2 bits = ml;
-      const float mi = __builtin_bit_cast(f32x2, bits)[0], li = __builtin_bit_cast(f32x2, bits)[1];
+      const float mi = ml[0];
       const float t = fmaxf(top, mi), ref = t == -INFINITY ? 0.f : t;
       const float old = __builtin_amdgcn_exp2f(top - ref), now = __builtin_amdgcn_exp2f(mi - ref);
       top = t;
-      sum = sum * old + li * now;
+      sum = sum * old + ml[1] * now;
+      lse_sum = lse_sum * old + ml[2] * now;
 #pragma unroll
       for (int d = 0; d < NV; ++d) x[d] = x[d] * old + __builtin_bit_cast(f32x4, y[d]) * now;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const Target t = target(p, row);
-    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = lse_sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(lse_sum)) * 0.6931471805599453f;
 #pragma unroll
     for (int d = 0; d < NV; ++d) {
       const int at = d * 64 + part * 4;

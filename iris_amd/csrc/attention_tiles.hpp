@@ -60,6 +60,57 @@ __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
 // Larger of a lane's value and that of the lane 32 away.
 __device__ inline float max_of_halves(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 
+// The row tile that sees the k-th most keys (no window), later rows before earlier ones: workgroups that start last are then the
+// short ones.  (A prompt of 8192 tokens among others, 1153 row tiles of 1 to 128 key tiles on 512 places: 345 us in the requests'
+// order, BALANCED_US by length.)  Request r has tiles_r row tiles, and of those that see at least c key tiles the number is known in closed form;
+// the largest c with more than k of them in all is found by bisection, the lanes adding up the requests.
+__device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request, int* row_tile) {
+  const iris_attention_args& a = g.a;
+  const int lane = threadIdx.x & 63;
+  struct Rows {
+    int64_t rows;
+    int first, tiles;
+  };
+  // the lane's request (at most 64 of them)
+  Rows own{0, 0, 0};
+  if (lane < a.requests) {
+    const int begin = a.query_starts[lane], tokens = max(min(a.query_starts[lane + 1], a.tokens) - begin, 0);
+    own.rows = (int64_t)tokens * g.group;
+    own.first = (int)min((int64_t)max(a.lengths[lane], 0), (int64_t)a.table_width * g.page.d) - tokens;
+    own.tiles = (int)((own.rows + ROWS - 1) / ROWS);
+  }
+  auto at_least = [&](int c) {  // its row tiles that see at least c key tiles
+    const int64_t q = ((int64_t)(c - 1) * BT - own.first) * g.group;
+    return c <= 0 || q <= 0 ? own.tiles : own.rows <= q ? 0 : own.tiles - (int)(q / ROWS);
+  };
+  auto sum_of = [&](int x) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) x += __shfl_xor(x, d, 64);
+    return __builtin_amdgcn_readfirstlane(x);
+  };
+  if (k >= sum_of(own.tiles)) return false;
+  int lo = 0;
+  for (int hi = (int)(((int64_t)a.table_width * g.page.d + BT - 1) / BT) + 1; hi - lo > 1;) {
+    const int mid = (lo + hi) / 2;
+    if (sum_of(at_least(mid)) > k)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const int more = at_least(lo + 1), exactly = at_least(lo) - more;
+  k -= sum_of(more);  // the k-th of those with exactly lo, request by request
+  int sum = exactly;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(sum, d, 64);
+    if (lane >= d) sum += y;
+  }
+  const int at = __builtin_ctzll(__ballot(k < sum) | 1ull << 63);
+  *request = at;
+  *row_tile = __builtin_amdgcn_readlane(own.tiles - more - 1 - (k - (sum - exactly)), at);
+  return true;
+}
+
 template <int DT, int DP>
 __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_tiles_kernel(AttentionKArgs g) {
   using C = Cfg<DT, DP>;
@@ -68,24 +119,29 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, half = lane >> 5;
 
-  // The workgroup's rows: row tile x is the (x - bound)-th of the last request whose bound is not past x; late rows, which see
-  // the most keys, start first.
-  const int back = gridDim.x - 1 - blockIdx.x, x = back / g.splits, split = back - x * g.splits;
-  auto bound = [&](int r) { return (int)((int64_t)scalar_at(a.query_starts, r) * g.group / ROWS) + r; };
-  int request = 0;
-  for (int hi = a.requests; hi - request > 1;) {
-    const int mid = (request + hi) / 2;
-    if (bound(mid) <= x)
-      request = mid;
-    else
-      hi = mid;
+  // The workgroup's rows, and its share of their keys.  Key heads change fastest: with eight of them each XCD has one.
+  const int item = blockIdx.x / a.k_heads, head = blockIdx.x - item * a.k_heads, x = item / g.splits, split = item - x * g.splits;
+  int request, row_tile;
+  if (g.by_length) {
+    if (!nth_longest(g, x, &request, &row_tile)) return;
+  } else {
+    // x counts row tiles with room for each request's, without a sum over the requests: request r's begin at bound(r).
+    auto bound = [&](int r) { return (int)((int64_t)scalar_at(a.query_starts, r) * g.group / ROWS) + r; };
+    request = 0;
+    for (int hi = a.requests; hi - request > 1;) {
+      const int mid = (request + hi) / 2;
+      if (bound(mid) <= x)
+        request = mid;
+      else
+        hi = mid;
+    }
+    row_tile = x - bound(request);
   }
   const int token0 = scalar_at(a.query_starts, request);
   const int tokens = min(scalar_at(a.query_starts, request + 1), a.tokens) - token0;
-  const int row0 = (x - bound(request)) * ROWS;
+  const int row0 = row_tile * ROWS;
   if (row0 < 0 || token0 < 0 || tokens <= 0 || row0 >= (int64_t)tokens * g.group) return;
   const int num_rows = (int)min((int64_t)ROWS, (int64_t)tokens * g.group - row0);
-  const int head = blockIdx.y;
   int length = max(scalar_at(a.lengths, request), 0);
   if ((int64_t)length > (int64_t)a.table_width * g.page.d) {
     if (tid == 0) report(a.status, IRIS_STATUS_BAD_INDEX);
@@ -175,7 +231,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   for (int t = 0; t < C::DTILES; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
-  float ref = have_row ? -INFINITY : 0.f, l = 0.f;
+  // l: the sum of the weights as they are multiplied; lse_l: as they are, for the logarithm
+  float ref = have_row ? -INFINITY : 0.f, l = 0.f, lse_l = 0.f;
   bool poisoned = false;
 
   // Tiles are fetched a stage ahead by all waves; the last ones of a workgroup may lie past a wave's own last key.
@@ -194,7 +251,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   };
   f32x16 s[2];
   u32x4 p[4];  // P^T's operands: 16 keys each
-  float sum;
+  float sum, exact;
   // The scores of list tile j.  Operands are read AHEAD matrix instructions before they are used; two sums in turn, so that
   // neither waits for its own last step.
   auto score = [&](int j) {
@@ -242,6 +299,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   auto weigh = [&] {
     const float from = ref == -INFINITY ? 0.f : ref;
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    exact = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -250,14 +308,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * i + e], g.scale_log2, -from));
-          sums[e & 3] += w[e];
         }
         p[2 * u + i] = u32x4{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[e] = add_weights<DT>(p[2 * u + i][e], sums[e]);
+        if (a.lse) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) exact += w[e];
+        }
       }
     sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   };
   auto add_values = [&](int j) {
     l += sum;
+    lse_l += exact;
     const char* vt = lds[j & 1][1];
     u32x4 f[AHEAD];
 #pragma unroll
@@ -296,6 +360,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
     const float shrink = __builtin_amdgcn_exp2f(ref - (next == -INFINITY ? 0.f : next));
     ref = next;
     l *= shrink;
+    lse_l *= shrink;
 #pragma unroll
     for (int t = 0; t < C::DTILES; ++t) o[t] *= shrink;
     weigh();
@@ -304,12 +369,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   for (; j < j1; ++j) next_stage(j);
 
   l += __shfl_xor(l, 32, 64);
+  lse_l += __shfl_xor(lse_l, 32, 64);
   // what one wave found is every row's
   bool redo = __syncthreads_or(poisoned);
   float flags = __syncthreads_or(bad_page) ? __builtin_nanf("") : 0.f;
   if (g.splits > 1) {
     // The parts meet in the workspace, each in the order of its registers: the last to arrive has the rows of all in the same lanes.
-    const int unit = blockIdx.y * (gridDim.x / g.splits) + x;
+    const int unit = x * a.k_heads + head;
     auto slot = [&](int part) { return (IRIS_GLOBAL char*)(g.slots + ((int64_t)unit * g.splits + part) * C::SLOT); };
     const uint32_t mine = (wave * 64 + lane) * 16;
 #pragma unroll
@@ -319,7 +385,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
         const f32x4 v = {o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]};
         store16_any<AUX_SC1>(slot(split) + (t * 4 + r / 4) * (WAVES * 1024) + mine, __builtin_bit_cast(u32x4, v));
       }
-    const f32x4 tail = {ref, l, flags, redo ? 1.f : 0.f};
+    const f32x4 tail = {ref, l, lse_l, redo ? 1.f : flags};
     store16_any<AUX_SC1>(slot(split) + C::DTILES * 4 * (WAVES * 1024) + mine, __builtin_bit_cast(u32x4, tail));
     IRIS_WAIT_VMCNT(0);
     __syncthreads();
@@ -335,8 +401,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
     ref = -INFINITY;
-    l = 0.f;
-    float again = 0.f;
+    l = lse_l = 0.f;
+    bool bad = false, again = false;
     for (int part = 0; part < g.splits; ++part) {
       const __amdgpu_buffer_rsrc_t rs = tile_rsrc(slot(part), C::SLOT * 4);
       const f32x4 m = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)mine, C::DTILES * 4 * (WAVES * 1024), AUX_SC1));
@@ -344,8 +410,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
       const float old = __builtin_amdgcn_exp2f(ref - from), now = __builtin_amdgcn_exp2f(m[0] - from);
       ref = next;
       l = l * old + m[1] * now;
-      flags += m[2];
-      again += m[3];
+      lse_l = lse_l * old + m[2] * now;
+      again |= m[3] == 1.f;
+      bad |= __builtin_isnan(m[3]);
 #pragma unroll
       for (int t = 0; t < C::DTILES; ++t)
 #pragma unroll
@@ -356,7 +423,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
           for (int i = 0; i < 4; ++i) o[t][r + i] = o[t][r + i] * old + v[i] * now;
         }
     }
-    redo = __builtin_amdgcn_readfirstlane(again > 0.f);
+    redo = __any(again);
+    flags = __any(bad) ? __builtin_nanf("") : 0.f;
   }
   if (flags != 0.f && lane == 0) report(a.status, IRIS_STATUS_BAD_INDEX);
 
@@ -386,7 +454,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   const float inv = flags != 0.f ? flags : l == 0.f ? 0.f : 1.f / l;
   const int64_t out_token = token0 + token;
   if (a.lse && half == 0)
-    a.lse[out_token * a.stride_lse + qhead] = flags != 0.f ? flags : l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    a.lse[out_token * a.stride_lse + qhead] = flags != 0.f ? flags : lse_l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(lse_l)) * 0.6931471805599453f;
   IRIS_GLOBAL char* out = (IRIS_GLOBAL char*)a.out + (out_token * a.stride_ot + (int64_t)qhead * a.stride_oh) * 2;
 #pragma unroll
   for (int t = 0; t < C::DTILES; ++t)

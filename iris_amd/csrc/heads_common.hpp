@@ -6,48 +6,81 @@
 
 namespace iris_amd {
 
-// N consecutive elements of type DT at `p`, which is aligned to all of them (N 1 to 4), as fp32.
+// N elements of type DT as they lie in memory (N 1 or 4), and as fp32.
 template <int DT, int N>
-__device__ inline void load_elems(const IRIS_GLOBAL char* p, float (&v)[N]) {
-  static_assert(N == 1 || N == 4, "one element, or four");
-  if constexpr (DT == IRIS_DTYPE_F32) {
-    if constexpr (N == 4) {
-      const f32x4 x = *(const IRIS_GLOBAL f32x4*)p;
+struct Raw {
+  static constexpr bool F32 = DT == IRIS_DTYPE_F32;
+  static constexpr int WORDS = F32 ? N : (N + 1) / 2;
+  uint32_t w[WORDS];
+  __device__ inline void load(const IRIS_GLOBAL char* p) {
+    if constexpr (WORDS == 4) {
+      const u32x4 x = *(const IRIS_GLOBAL u32x4*)p;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = x[e];
+      for (int i = 0; i < 4; ++i) w[i] = x[i];
+    } else if constexpr (WORDS == 2) {
+      const u32x2 x = *(const IRIS_GLOBAL u32x2*)p;
+      w[0] = x[0], w[1] = x[1];
+    } else if constexpr (F32) {
+      w[0] = *(const IRIS_GLOBAL uint32_t*)p;
     } else {
-      v[0] = *(const IRIS_GLOBAL float*)p;
+      w[0] = *(const IRIS_GLOBAL unsigned short*)p;
     }
-  } else if constexpr (N == 4) {
-    const u32x2 x = *(const IRIS_GLOBAL u32x2*)p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = from16<DT>((unsigned short)(x[e / 2] >> (16 * (e & 1))));
-  } else {
-    v[0] = from16<DT>(*(const IRIS_GLOBAL unsigned short*)p);
   }
-}
-
-template <int DT, int N>
-__device__ inline void store_elems(IRIS_GLOBAL char* p, const float (&v)[N]) {
-  static_assert(N == 1 || N == 4, "one element, or four");
-  if constexpr (DT == IRIS_DTYPE_F32) {
-    if constexpr (N == 4)
-      *(IRIS_GLOBAL f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
+  __device__ inline void store(IRIS_GLOBAL char* p) const {
+    if constexpr (WORDS == 4)
+      *(IRIS_GLOBAL u32x4*)p = u32x4{w[0], w[1], w[2], w[3]};
+    else if constexpr (WORDS == 2)
+      *(IRIS_GLOBAL u32x2*)p = u32x2{w[0], w[1]};
+    else if constexpr (F32)
+      *(IRIS_GLOBAL uint32_t*)p = w[0];
     else
-      *(IRIS_GLOBAL float*)p = v[0];
-  } else if constexpr (N == 4) {
-    *(IRIS_GLOBAL u32x2*)p = u32x2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-  } else {
-    *(IRIS_GLOBAL unsigned short*)p = to16<DT>(v[0]);
+      *(IRIS_GLOBAL unsigned short*)p = (unsigned short)w[0];
   }
+  __device__ inline void get(float (&v)[N]) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if constexpr (F32)
+        v[e] = __builtin_bit_cast(float, w[e]);
+      else
+        v[e] = from16<DT>((unsigned short)(w[e / 2] >> (16 * (e & 1))));
+    }
+  }
+  __device__ inline void set(const float (&v)[N]) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] = __builtin_bit_cast(uint32_t, v[e]);
+    } else if constexpr (N == 4) {
+      w[0] = pack2<DT>(v[0], v[1]), w[1] = pack2<DT>(v[2], v[3]);
+    } else {
+      w[0] = to16<DT>(v[0]);
+    }
+  }
+};
+
+// A lane's value from the lane that CTRL (a DPP permutation within 16 lanes) names: a VALU operand, where a shuffle would go through LDS.
+template <int CTRL>
+__device__ inline float permuted(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ inline double permuted(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Sum over groups of `lanes` neighbouring lanes (a power of two up to 64), in every one of them; the same order for
-// every lane, so that all hold the same bits.
+// Sum over groups of LANES neighbouring lanes (8, 16, 32 or 64), the same bits in all of them: neighbours, pairs, and from
+// four lanes of equal sums on mirror images.
 template <int LANES, class T>
 __device__ inline T sum_lanes(T x) {
-#pragma unroll
-  for (int m = 1; m < LANES; m *= 2) x += __shfl_xor(x, m, 64);
+  constexpr int NEIGHBOURS = 0xB1, PAIRS = 0x4E, MIRROR_8 = 0x141, MIRROR_16 = 0x140;  // quad_perm [1,0,3,2], [2,3,0,1]; row_half_mirror, row_mirror
+  x += permuted<NEIGHBOURS>(x);
+  x += permuted<PAIRS>(x);
+  x += permuted<MIRROR_8>(x);
+  if constexpr (LANES >= 16) x += permuted<MIRROR_16>(x);
+  if constexpr (LANES >= 32) x += __shfl_xor(x, 16, 64);
+  if constexpr (LANES >= 64) x += __shfl_xor(x, 32, 64);
   return x;
 }
 

@@ -9,7 +9,10 @@
 //
 // The work is one read and one write of each head, so it is bound by memory: a head is held by the fewest lanes that
 // load it eight elements each, as two runs of four of which one holds a pair's first and one its second elements, so
-// that no rotation crosses lanes; the norm is the only exchange.  A lane keeps its angles for the heads of its token.
+// that no rotation crosses lanes; the norm is the only exchange, within 16 lanes by DPP.  A lane keeps its angles for the heads of
+// its token that it has.  bf16, heads of 128: 8191 tokens of 8 + 2 + 2 heads (54.6 MB) in 13.1 us, 4.2 TB/s, a copy of
+// 4 GB runs at 4.9; the gradient of 8192 tokens of 32 + 8 heads (256 MB) in 55.8 us, 4.6 TB/s.  (Loads unpacked as they
+// arrive and both weights in one workgroup took 208 registers and 105 us for the latter.)
 #include <type_traits>
 
 #include "heads_common.hpp"
@@ -20,7 +23,7 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int BATCH = 4;  // heads whose loads a lane has in flight together
 
-// Where a lane's V first and V second elements of a row lie.  ROT: the pairs that turn.
+// Where a lane's V first and V second elements of a row lie.
 template <int V>
 struct Place {
   int first, second;
@@ -81,8 +84,11 @@ __device__ inline void load_angles(const Args& a, int64_t t, const Place<V> (&at
 #pragma unroll
     for (int e = 0; e < V; ++e) g.c[i][e] = 1.f, g.s[i][e] = 0.f;
     if (at[i].turns) {
-      load_elems<IRIS_DTYPE_F32, V>((const IRIS_GLOBAL char*)(a.cos + row * a.stride_cos + at[i].pair), g.c[i]);
-      load_elems<IRIS_DTYPE_F32, V>((const IRIS_GLOBAL char*)(a.sin + row * a.stride_sin + at[i].pair), g.s[i]);
+      Raw<IRIS_DTYPE_F32, V> c, s;
+      c.load((const IRIS_GLOBAL char*)(a.cos + row * a.stride_cos + at[i].pair));
+      s.load((const IRIS_GLOBAL char*)(a.sin + row * a.stride_sin + at[i].pair));
+      c.get(g.c[i]);
+      s.get(g.s[i]);
       if (!inside) {
 #pragma unroll
         for (int e = 0; e < V; ++e) g.c[i][e] = g.s[i][e] = __builtin_nanf("");
@@ -91,262 +97,302 @@ __device__ inline void load_angles(const Args& a, int64_t t, const Place<V> (&at
   }
 }
 
+// A lane's elements of a head: in their own type, and as fp32.
 template <int DT, int V, int ITEMS>
-struct Row {
-  float a[ITEMS][V], b[ITEMS][V];
+struct Packed {
+  static constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2;
+  Raw<DT, V> a[ITEMS], b[ITEMS];
   __device__ inline void load(const IRIS_GLOBAL char* p, const Place<V> (&at)[ITEMS]) {
-    constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) a[i][e] = b[i][e] = 0.f;
+      a[i] = b[i] = Raw<DT, V>{};
       if (at[i].live) {
-        load_elems<DT, V>(p + at[i].first * ES, a[i]);
-        load_elems<DT, V>(p + at[i].second * ES, b[i]);
+        a[i].load(p + at[i].first * ES);
+        b[i].load(p + at[i].second * ES);
       }
     }
   }
   __device__ inline void store(IRIS_GLOBAL char* p, const Place<V> (&at)[ITEMS]) const {
-    constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
       if (at[i].live) {
-        store_elems<DT, V>(p + at[i].first * ES, a[i]);
-        store_elems<DT, V>(p + at[i].second * ES, b[i]);
+        a[i].store(p + at[i].first * ES);
+        b[i].store(p + at[i].second * ES);
       }
   }
 };
-
-// A weight vector at a lane's elements; ones where there is none.
-template <int DT, int V, int ITEMS>
-__device__ inline void load_weight(const void* w, bool fp32, const Place<V> (&at)[ITEMS], Row<DT, V, ITEMS>& out) {
+template <int V, int ITEMS>
+struct Wide {
+  float a[ITEMS][V], b[ITEMS][V];
+  template <int DT>
+  __device__ inline void get(const Packed<DT, V, ITEMS>& x) {
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) out.a[i][e] = out.b[i][e] = 1.f;
-  if (!w) return;
-  if (!fp32) {
-    out.load((const IRIS_GLOBAL char*)w, at);
-    return;
+    for (int i = 0; i < ITEMS; ++i) x.a[i].get(a[i]), x.b[i].get(b[i]);
   }
-  Row<IRIS_DTYPE_F32, V, ITEMS> wide;
-  wide.load((const IRIS_GLOBAL char*)w, at);
+  template <int DT>
+  __device__ inline void put(Packed<DT, V, ITEMS>& x) const {
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) out.a[i][e] = wide.a[i][e], out.b[i][e] = wide.b[i][e];
+    for (int i = 0; i < ITEMS; ++i) x.a[i].set(a[i]), x.b[i].set(b[i]);
+  }
+  // A weight vector at the lane's elements, in the heads' type DT or fp32.
+  template <int DT>
+  __device__ inline void load_weight(const void* w, bool fp32, const Place<V> (&at)[ITEMS]) {
+    if (fp32) {
+      Packed<IRIS_DTYPE_F32, V, ITEMS> x;
+      x.load((const IRIS_GLOBAL char*)w, at);
+      get(x);
+    } else {
+      Packed<DT, V, ITEMS> x;
+      x.load((const IRIS_GLOBAL char*)w, at);
+      get(x);
+    }
+  }
+};
+
+// The tokens and heads of one kind (queries, keys or values), as groups of lanes take them: `heads_each` heads of a token.
+struct Kind {
+  int heads, heads_each, parts, blocks;
+  FastDiv div;  // by parts
+};
+Kind make_kind(int64_t tokens, int heads, int heads_each, int64_t per_block) {
+  Kind k{};
+  if (!heads) return k;
+  k.heads = heads;
+  k.heads_each = heads_each < heads ? heads_each : heads;
+  k.parts = (heads + k.heads_each - 1) / k.heads_each;
+  k.blocks = (int)((tokens * k.parts + per_block - 1) / per_block);
+  k.div = make_fast_div((uint32_t)k.parts, (uint64_t)(k.blocks * per_block));
+  return k;
+}
+__device__ inline int64_t token_of(const Kind& k, int64_t group) {
+  return k.div.m || k.parts == 1 ? (int64_t)fast_div((uint32_t)group, k.div) : group / k.parts;
 }
 
-template <int V, int ITEMS, class A, class B>
-__device__ inline float dot_items(const A& x, const B& y) {
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) sum += x.a[i][e] * y.a[i][e] + x.b[i][e] * y.b[i][e];
-  return sum;
-}
-
-// LANES lanes hold a row, V elements twice and ITEMS times each.  A group of lanes takes `heads_each` of a token's rows:
-// query heads, key heads, and (with a cache) value heads, in this order.
+// LANES lanes hold a head, V elements twice and ITEMS times each.  The first kinds[0].blocks workgroups take queries, the next
+// kinds[1].blocks keys, and (with a cache) the last values: a workgroup has one weight and one way.
+struct ForwardArgs {
+  iris_qk_norm_rope_args a;
+  Kind kinds[3];
+};
 template <int DT, int V, int LANES, int ITEMS>
-__global__ __launch_bounds__(THREADS) void qk_norm_rope_kernel(iris_qk_norm_rope_args a, FastDiv parts, int heads_each) {
+__global__ __launch_bounds__(THREADS) void qk_norm_rope_kernel(ForwardArgs args) {
   constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2;
-  const int64_t group = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LANES;
+  const iris_qk_norm_rope_args& a = args.a;
+  int block = blockIdx.x, which = 0;
+  if (block >= args.kinds[0].blocks) block -= args.kinds[0].blocks, which = 1;
+  if (which == 1 && block >= args.kinds[1].blocks) block -= args.kinds[1].blocks, which = 2;
+  Kind kind = args.kinds[0];
+  if (which == 1) kind = args.kinds[1];
+  if (which == 2) kind = args.kinds[2];
+  const int64_t group = ((int64_t)block * THREADS + threadIdx.x) / LANES;
   const int lane = threadIdx.x % LANES;
-  const int64_t t = parts.m || parts.d == 1 ? (int64_t)fast_div((uint32_t)group, parts) : group / parts.d;
+  const int64_t t = token_of(kind, group);
   if (t >= a.tokens) return;  // (all lanes of a group together)
-  const int rows = a.q_heads + a.k_heads + (a.v ? a.k_heads : 0);
-  const int begin = (int)(group - t * parts.d) * heads_each, end = min(begin + heads_each, rows);
+  const int begin = (int)(group - t * kind.parts) * kind.heads_each, end = min(begin + kind.heads_each, kind.heads);
 
   Place<V> at[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) at[i] = place<V>(lane + i * LANES, a.head_dim, a.rotary_dim, a.interleaved);
-  // the slot of the token's keys and values; none where it is negative
-  int64_t slot = -1;
-  if (a.slots) {
-    slot = a.slots[t];
-    if (slot >= a.num_slots) {
-      report(a.status, IRIS_STATUS_BAD_INDEX);
-      slot = -1;
-    }
-  }
-  const int page = slot < 0 ? 0 : (int)((uint32_t)slot / (uint32_t)a.page_size);
-  const int in_page = slot < 0 ? 0 : (int)slot - page * a.page_size;
-
-  auto source = [&](int r) -> const IRIS_GLOBAL char* {
-    const char* base = (const char*)(r < a.q_heads ? a.q : r < a.q_heads + a.k_heads ? a.k : a.v);
-    const int64_t off = r < a.q_heads                ? t * a.stride_qt + r * a.stride_qh
-                        : r < a.q_heads + a.k_heads ? t * a.stride_kt + (r - a.q_heads) * a.stride_kh
-                                                    : t * a.stride_vt + (r - a.q_heads - a.k_heads) * a.stride_vh;
-    return (const IRIS_GLOBAL char*)(base + off * ES);
-  };
-  Row<DT, V, ITEMS> x[BATCH];
-  auto fetch = [&](int r0) {
+  const IRIS_GLOBAL char* source = (const IRIS_GLOBAL char*)(which == 0 ? a.q : which == 1 ? a.k : a.v) +
+                                   t * (which == 0 ? a.stride_qt : which == 1 ? a.stride_kt : a.stride_vt) * ES;
+  const int64_t source_step = (which == 0 ? a.stride_qh : which == 1 ? a.stride_kh : a.stride_vh) * ES;
+  Packed<DT, V, ITEMS> x[BATCH];
+  auto fetch = [&](int h0) {
 #pragma unroll
     for (int u = 0; u < BATCH; ++u)
-      if (r0 + u < end) x[u].load(source(r0 + u), at);
+      if (h0 + u < end) x[u].load(source + (h0 + u) * source_step, at);
   };
   fetch(begin);
   Angles<V, ITEMS> angle;
-  load_angles(a, t, at, angle);
-  Row<DT, V, ITEMS> wq, wk;
-  load_weight(a.q_weight, a.weight_fp32, at, wq);
-  load_weight(a.k_weight, a.weight_fp32, at, wk);
+  if (which < 2) load_angles(a, t, at, angle);
+  const void* weight = which == 0 ? a.q_weight : which == 1 ? a.k_weight : nullptr;
+  Wide<V, ITEMS> w;
+  if (weight) w.template load_weight<DT>(weight, a.weight_fp32, at);
+  // where the heads go: a tensor, and for keys and values the token's slot of the cache (none where it is negative)
+  IRIS_GLOBAL char* out = which == 0 ? (IRIS_GLOBAL char*)a.q_out + t * a.stride_qot * ES
+                          : which == 1 && a.k_out ? (IRIS_GLOBAL char*)a.k_out + t * a.stride_kot * ES
+                                                  : nullptr;
+  const int64_t out_step = (which == 0 ? a.stride_qoh : a.stride_koh) * ES;
+  IRIS_GLOBAL char* cached = nullptr;
+  int64_t cached_step = 0;
+  if (which > 0 && a.slots) {
+    const int64_t slot = a.slots[t];
+    if (slot >= a.num_slots) report(a.status, IRIS_STATUS_BAD_INDEX);
+    if (slot >= 0 && slot < a.num_slots) {
+      const int64_t page = (uint32_t)slot / (uint32_t)a.page_size, row = (int)slot - (int)page * a.page_size;
+      cached = which == 1 ? (IRIS_GLOBAL char*)a.k_cache + (page * a.stride_kc_page + row * a.stride_kc_row) * ES
+                          : (IRIS_GLOBAL char*)a.v_cache + (page * a.stride_vc_page + row * a.stride_vc_row) * ES;
+    }
+    cached_step = (which == 1 ? a.stride_kc_head : a.stride_vc_head) * ES;
+  }
 
-  for (int r0 = begin; r0 < end; r0 += BATCH) {
-    if (r0 > begin) fetch(r0);
+  for (int h0 = begin; h0 < end; h0 += BATCH) {
+    if (h0 > begin) fetch(h0);
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const int r = r0 + u;
-      if (r >= end) break;
-      const bool is_q = r < a.q_heads, is_v = r >= a.q_heads + a.k_heads;
-      if (!is_v) {
-        const bool normed = (is_q ? a.q_weight : a.k_weight) != nullptr;
-        if (normed) {
-          const float rs = rsqrtf(sum_lanes<LANES>(dot_items<V, ITEMS>(x[u], x[u])) / (float)a.head_dim + a.eps);
+      const int h = h0 + u;
+      if (h >= end) break;
+      if (which < 2) {
+        Wide<V, ITEMS> y;
+        y.get(x[u]);
+        if (weight) {
+          float square = 0.f;
 #pragma unroll
           for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              x[u].a[i][e] *= rs * (is_q ? wq.a[i][e] : wk.a[i][e]);
-              x[u].b[i][e] *= rs * (is_q ? wq.b[i][e] : wk.b[i][e]);
-            }
+            for (int e = 0; e < V; ++e) square += y.a[i][e] * y.a[i][e] + y.b[i][e] * y.b[i][e];
+          const float rs = rsqrtf(sum_lanes<LANES>(square) / (float)a.head_dim + a.eps);
+#pragma unroll
+          for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) y.a[i][e] *= rs * w.a[i][e], y.b[i][e] *= rs * w.b[i][e];
         }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-          if (at[i].turns) turn<V, false>(x[u].a[i], x[u].b[i], angle.c[i], angle.s[i], a.interleaved);
+          if (at[i].turns) turn<V, false>(y.a[i], y.b[i], angle.c[i], angle.s[i], a.interleaved);
+        y.put(x[u]);
       }
-      if (is_q) {
-        x[u].store((IRIS_GLOBAL char*)a.q_out + (t * a.stride_qot + r * a.stride_qoh) * ES, at);
-      } else if (!is_v) {
-        const int h = r - a.q_heads;
-        if (a.k_out) x[u].store((IRIS_GLOBAL char*)a.k_out + (t * a.stride_kot + h * a.stride_koh) * ES, at);
-        if (slot >= 0)
-          x[u].store((IRIS_GLOBAL char*)a.k_cache + (page * a.stride_kc_page + in_page * a.stride_kc_row + h * a.stride_kc_head) * ES, at);
-      } else if (slot >= 0) {
-        const int h = r - a.q_heads - a.k_heads;
-        x[u].store((IRIS_GLOBAL char*)a.v_cache + (page * a.stride_vc_page + in_page * a.stride_vc_row + h * a.stride_vc_head) * ES, at);
-      }
+      if (out) x[u].store(out + h * out_step, at);
+      if (cached) x[u].store(cached + h * cached_step, at);
     }
   }
 }
 
-// The gradient.  A group takes whole tokens, `step` groups apart, and keeps its share of the weights' gradients in
-// registers; a workgroup adds its groups' shares in LDS in a fixed order and leaves one row of partial sums, which
-// weight_gradient_kernel adds in a fixed order: the same inputs give the same bits.
+// The gradient.  The first kinds[0].blocks workgroups take queries, the others keys.  A group of lanes takes `heads_each` heads of a
+// token, then those `blocks` workgroups further on, and keeps its share of the weight's gradient in registers; a workgroup
+// adds its groups' shares in LDS in a fixed order and leaves one row of partial sums, which weight_gradient_kernel
+// adds in a fixed order: the same inputs give the same bits.
+struct BackwardArgs {
+  iris_qk_norm_rope_backward_args a;
+  Kind kinds[2];
+};
 template <int DT, int V, int LANES, int ITEMS>
-__global__ __launch_bounds__(THREADS) void qk_norm_rope_backward_kernel(iris_qk_norm_rope_backward_args a) {
-  constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, GROUPS = THREADS / LANES;
+__global__ __launch_bounds__(THREADS) void qk_norm_rope_backward_kernel(BackwardArgs args) {
+  constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, GROUPS = THREADS / LANES, PAIR = BATCH / 2;
+  const iris_qk_norm_rope_backward_args& a = args.a;
+  const bool keys = (int)blockIdx.x >= args.kinds[0].blocks;
+  Kind kind = args.kinds[0];
+  if (keys) kind = args.kinds[1];
+  const int block = blockIdx.x - (keys ? args.kinds[0].blocks : 0);
   const int lane = threadIdx.x % LANES, in_block = threadIdx.x / LANES;
   Place<V> at[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) at[i] = place<V>(lane + i * LANES, a.head_dim, a.rotary_dim, a.interleaved);
-  Row<DT, V, ITEMS> w[2], dw[2];
-  load_weight(a.q_weight, a.weight_fp32, at, w[0]);
-  load_weight(a.k_weight, a.weight_fp32, at, w[1]);
+  const void* weight = keys ? a.k_weight : a.q_weight;
+  Wide<V, ITEMS> w, dw;
+  if (weight) w.template load_weight<DT>(weight, a.weight_fp32, at);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) dw[k].a[i][e] = dw[k].b[i][e] = 0.f;
+    for (int e = 0; e < V; ++e) dw.a[i][e] = dw.b[i][e] = 0.f;
 
   const float inv_dim = 1.f / (float)a.head_dim;
-  for (int64_t t = (int64_t)blockIdx.x * GROUPS + in_block; t < a.tokens; t += (int64_t)gridDim.x * GROUPS) {
+  const int64_t xh = (keys ? a.stride_kh : a.stride_qh) * ES, zh = (keys ? a.stride_dkoh : a.stride_dqoh) * ES,
+                dh = (keys ? a.stride_dkh : a.stride_dqh) * ES;
+  const int64_t groups = (int64_t)a.tokens * kind.parts, step = (int64_t)kind.blocks * GROUPS;
+  for (int64_t group = (int64_t)block * GROUPS + in_block; group < groups; group += step) {
+    const int64_t t = token_of(kind, group);
+    const int begin = (int)(group - t * kind.parts) * kind.heads_each, end = min(begin + kind.heads_each, kind.heads);
+    const IRIS_GLOBAL char* xs = (const IRIS_GLOBAL char*)(keys ? a.k : a.q) + t * (keys ? a.stride_kt : a.stride_qt) * ES;
+    const IRIS_GLOBAL char* zs = (const IRIS_GLOBAL char*)(keys ? a.dk_out : a.dq_out) + t * (keys ? a.stride_dkot : a.stride_dqot) * ES;
+    IRIS_GLOBAL char* ds = (IRIS_GLOBAL char*)(keys ? a.dk : a.dq) + t * (keys ? a.stride_dkt : a.stride_dqt) * ES;
+    Packed<DT, V, ITEMS> x[PAIR], z[PAIR];
+    auto fetch = [&](int h0) {
+#pragma unroll
+      for (int u = 0; u < PAIR; ++u)
+        if (h0 + u < end) {
+          z[u].load(zs + (h0 + u) * zh, at);
+          if (weight) x[u].load(xs + (h0 + u) * xh, at);
+        }
+    };
+    fetch(begin);
     Angles<V, ITEMS> angle;
     load_angles(a, t, at, angle);
+    for (int h0 = begin; h0 < end; h0 += PAIR) {
+      if (h0 > begin) fetch(h0);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int heads = k ? a.k_heads : a.q_heads;
-      const bool normed = (k ? a.k_weight : a.q_weight) != nullptr;
-      const IRIS_GLOBAL char* xs = (const IRIS_GLOBAL char*)(k ? a.k : a.q) + t * (k ? a.stride_kt : a.stride_qt) * ES;
-      const IRIS_GLOBAL char* zs = (const IRIS_GLOBAL char*)(k ? a.dk_out : a.dq_out) + t * (k ? a.stride_dkot : a.stride_dqot) * ES;
-      IRIS_GLOBAL char* ds = (IRIS_GLOBAL char*)(k ? a.dk : a.dq) + t * (k ? a.stride_dkt : a.stride_dqt) * ES;
-      const int64_t xh = (k ? a.stride_kh : a.stride_qh) * ES, zh = (k ? a.stride_dkoh : a.stride_dqoh) * ES,
-                    dh = (k ? a.stride_dkh : a.stride_dqh) * ES;
-      for (int h0 = 0; h0 < heads; h0 += BATCH) {
-        Row<DT, V, ITEMS> x[BATCH], g[BATCH];
+      for (int u = 0; u < PAIR; ++u) {
+        if (h0 + u >= end) break;
+        Wide<V, ITEMS> g;
+        g.get(z[u]);
 #pragma unroll
-        for (int u = 0; u < BATCH; ++u)
-          if (h0 + u < heads) {
-            g[u].load(zs + (h0 + u) * zh, at);
-            if (normed) x[u].load(xs + (h0 + u) * xh, at);
-          }
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-          if (h0 + u >= heads) break;
+        for (int i = 0; i < ITEMS; ++i)
+          if (at[i].turns) turn<V, true>(g.a[i], g.b[i], angle.c[i], angle.s[i], a.interleaved);
+        if (weight) {
+          Wide<V, ITEMS> y;
+          y.get(x[u]);
+          // dx is what is left of g w when its part along x is taken out: in short heads very little, so those (which single
+          // pairs serve) take it out in 64 bits
+          using Acc = std::conditional_t<V == 1, double, float>;
+          Acc square = 0, along = 0;
 #pragma unroll
           for (int i = 0; i < ITEMS; ++i)
-            if (at[i].turns) turn<V, true>(g[u].a[i], g[u].b[i], angle.c[i], angle.s[i], a.interleaved);
-          if (normed) {
-            // dx is what is left of g w when its part along x is taken out: in short heads very little, so those (which single
-            // pairs serve) take it out in 64 bits
-            using Acc = std::conditional_t<V == 1, double, float>;
-            Acc square = 0, along = 0;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
+            for (int e = 0; e < V; ++e) {
+              square += (Acc)y.a[i][e] * y.a[i][e] + (Acc)y.b[i][e] * y.b[i][e];
+              along += (Acc)g.a[i][e] * w.a[i][e] * y.a[i][e] + (Acc)g.b[i][e] * w.b[i][e] * y.b[i][e];
+            }
+          square = sum_lanes<LANES>(square);
+          along = sum_lanes<LANES>(along);
+          const float rs = rsqrtf((float)(square * inv_dim) + a.eps);
+          const Acc back = along / (square + (Acc)a.head_dim * a.eps);
 #pragma unroll
-              for (int e = 0; e < V; ++e) {
-                square += (Acc)x[u].a[i][e] * x[u].a[i][e] + (Acc)x[u].b[i][e] * x[u].b[i][e];
-                along += (Acc)g[u].a[i][e] * w[k].a[i][e] * x[u].a[i][e] + (Acc)g[u].b[i][e] * w[k].b[i][e] * x[u].b[i][e];
-              }
-            square = sum_lanes<LANES>(square);
-            along = sum_lanes<LANES>(along);
-            const float rs = rsqrtf((float)(square * inv_dim) + a.eps);
-            const Acc back = along / (square + (Acc)a.head_dim * a.eps);
+          for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-              for (int e = 0; e < V; ++e) {
-                dw[k].a[i][e] += g[u].a[i][e] * x[u].a[i][e] * rs;
-                dw[k].b[i][e] += g[u].b[i][e] * x[u].b[i][e] * rs;
-                g[u].a[i][e] = rs * (float)((Acc)g[u].a[i][e] * w[k].a[i][e] - x[u].a[i][e] * back);
-                g[u].b[i][e] = rs * (float)((Acc)g[u].b[i][e] * w[k].b[i][e] - x[u].b[i][e] * back);
-              }
-          }
-          g[u].store(ds + (h0 + u) * dh, at);
+            for (int e = 0; e < V; ++e) {
+              dw.a[i][e] += g.a[i][e] * y.a[i][e] * rs;
+              dw.b[i][e] += g.b[i][e] * y.b[i][e] * rs;
+              g.a[i][e] = rs * (float)((Acc)g.a[i][e] * w.a[i][e] - y.a[i][e] * back);
+              g.b[i][e] = rs * (float)((Acc)g.b[i][e] * w.b[i][e] - y.b[i][e] * back);
+            }
         }
+        g.put(z[u]);
+        z[u].store(ds + (h0 + u) * dh, at);
       }
     }
   }
-  if (!a.dq_weight && !a.dk_weight) return;
-  // the groups' shares: rows of `width` floats in LDS, added by column
+  if (!(keys ? a.dk_weight : a.dq_weight)) return;
+  // the groups' shares: rows of head_dim floats in LDS, added by column
   extern __shared__ float shares[];
-  const int width = 2 * a.head_dim;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int i = 0; i < ITEMS; ++i)
+    if (at[i].live)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if (at[i].live)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          shares[in_block * width + k * a.head_dim + at[i].first + e] = dw[k].a[i][e];
-          shares[in_block * width + k * a.head_dim + at[i].second + e] = dw[k].b[i][e];
-        }
+      for (int e = 0; e < V; ++e) {
+        shares[in_block * a.head_dim + at[i].first + e] = dw.a[i][e];
+        shares[in_block * a.head_dim + at[i].second + e] = dw.b[i][e];
+      }
   __syncthreads();
-  for (int c = threadIdx.x; c < width; c += THREADS) {
+  for (int c = threadIdx.x; c < a.head_dim; c += THREADS) {
     float sum = 0.f;
-    for (int g = 0; g < GROUPS; ++g) sum += shares[g * width + c];
-    a.workspace[(int64_t)blockIdx.x * width + c] = sum;
+    for (int g = 0; g < GROUPS; ++g) sum += shares[g * a.head_dim + c];
+    a.workspace[(int64_t)blockIdx.x * a.head_dim + c] = sum;
   }
 }
 
-// Adds the workgroups' partial sums: 16 columns a workgroup, 16 lanes a column.
-__global__ __launch_bounds__(THREADS) void weight_gradient_kernel(const float* partials, int rows, int dim, float* dq_weight, float* dk_weight) {
-  __shared__ float sums[16][17];
-  const int c = threadIdx.x % 16, part = threadIdx.x / 16, column = blockIdx.x * 16 + c, width = 2 * dim;
+// Adds the workgroups' partial sums, those of the queries' weight in the first `q_rows` rows and of the keys' in the next `k_rows`:
+// 16 columns a workgroup, 64 lanes a column.
+constexpr int SUM_THREADS = 1024;
+__global__ __launch_bounds__(SUM_THREADS) void weight_gradient_kernel(const float* partials, int q_rows, int k_rows, int dim, float* dq_weight,
+                                                                      float* dk_weight) {
+  __shared__ float sums[SUM_THREADS / 16][17];
+  const int c = threadIdx.x % 16, part = threadIdx.x / 16, column = blockIdx.x * 16 + c;
+  const bool keys = blockIdx.y;
+  float* out = keys ? dk_weight : dq_weight;
+  if (!out) return;
+  const int begin = keys ? q_rows : 0, end = keys ? q_rows + k_rows : q_rows;
   float sum = 0.f;
-  if (column < width)
-    for (int r = part; r < rows; r += 16) sum += partials[(int64_t)r * width + column];
+  if (column < dim) {
+#pragma unroll 4
+    for (int r = begin + part; r < end; r += SUM_THREADS / 16) sum += partials[(int64_t)r * dim + column];
+  }
   sums[part][c] = sum;
   __syncthreads();
-  if (part == 0 && column < width) {
-    float all = 0.f;
-    for (int p = 0; p < 16; ++p) all += sums[p][c];
-    float* out = column < dim ? dq_weight : dk_weight;
-    if (out) out[column < dim ? column : column - dim] = all;
+  for (int n = SUM_THREADS / 32; n > 0; n /= 2) {
+    if (part < n) sums[part][c] += sums[part + n][c];
+    __syncthreads();
   }
+  if (part == 0 && column < dim) out[column] = sums[0][c];
 }
 
 bool known_dtype(int dt) { return dt == IRIS_DTYPE_F32 || dt == IRIS_DTYPE_F16 || dt == IRIS_DTYPE_BF16; }
@@ -375,6 +421,17 @@ hipError_t with_dtype(int dt, F f) {
 }
 
 constexpr int MAX_HEAD_DIM = 512;
+constexpr int MOST_GROUPS = 4;  // workgroups a CU of the gradient; each costs a row of partial sums (8 a CU: 59 us where 4 take 56)
+
+// Heads of a token that a group of lanes takes: they share the token's angles, up to four (eight gain nothing), as long as two
+// workgroups a CU are left.  Forward, bf16 heads of 128, us at 1 / 2 / 4 / 8 heads: 500 tokens of 8 + 2 + 2 heads 3.6 / 3.9 / 4.3 / 6.0,
+// 2000 of them 6.3 / 5.8 / 5.8 / 7.7, 8191 15.3 / 13.8 / 13.1 / 13.6, 2000 of 32 + 8 + 8 15.6 / 12.6 / 11.7 / 12.7.
+int heads_each(int64_t tokens, int heads, int64_t per_block) {
+  const int64_t enough = 2 * (int64_t)current_cu_count() * per_block;
+  int each = 1;
+  while (each < 4 && tokens * ((heads + 2 * each - 1) / (2 * each)) >= enough) each *= 2;
+  return each;
+}
 
 }  // namespace
 }  // namespace iris_amd
@@ -402,19 +459,15 @@ extern "C" int iris_qk_norm_rope_launch(const iris_qk_norm_rope_args* args, void
   wide = wide && aligned(a.cos, 16) && aligned(a.sin, 16) && a.stride_cos % 4 == 0 && a.stride_sin % 4 == 0 && aligned(a.q_weight, 4 * wes) &&
          aligned(a.k_weight, 4 * wes);
 
-  const int rows = a.q_heads + a.k_heads + (a.v ? a.k_heads : 0);
   return with_dtype(a.dtype, [&](auto dt) {
     return with_layout(wide, a.head_dim, [&](auto v, auto lanes, auto items) {
-      // All of a token's heads in one group share its angles; few tokens are spread over more groups.
-      const int64_t per_block = THREADS / lanes.value, enough = (int64_t)4 * current_cu_count() * per_block;
-      int heads_each = rows;
-      while (heads_each > BATCH && (int64_t)a.tokens * ((rows + heads_each - 1) / heads_each) < enough) heads_each = (heads_each + 1) / 2;
-      if ((int64_t)a.tokens * rows <= enough) heads_each = 1;
-      const int parts = (rows + heads_each - 1) / heads_each;
-      const int64_t groups = (int64_t)a.tokens * parts, grid = (groups + per_block - 1) / per_block;
+      const int64_t per_block = THREADS / lanes.value;
+      const int each = heads_each(a.tokens, a.q_heads + (a.v ? 2 : 1) * a.k_heads, per_block);
+      ForwardArgs f{a, {make_kind(a.tokens, a.q_heads, each, per_block), make_kind(a.tokens, a.k_heads, each, per_block),
+                        make_kind(a.tokens, a.v ? a.k_heads : 0, each, per_block)}};
+      const int64_t grid = (int64_t)f.kinds[0].blocks + f.kinds[1].blocks + f.kinds[2].blocks;
       if (grid > INT32_MAX) return hipErrorInvalidValue;
-      qk_norm_rope_kernel<dt.value, v.value, lanes.value, items.value>
-          <<<(int)grid, THREADS, 0, (hipStream_t)stream>>>(a, make_fast_div((uint32_t)parts, (uint64_t)(grid * per_block)), heads_each);
+      qk_norm_rope_kernel<dt.value, v.value, lanes.value, items.value><<<(int)grid, THREADS, 0, (hipStream_t)stream>>>(f);
       return hipGetLastError();
     });
   });
@@ -447,15 +500,25 @@ extern "C" int iris_qk_norm_rope_backward_launch(const iris_qk_norm_rope_backwar
   return with_dtype(a.dtype, [&](auto dt) {
     return with_layout(wide, a.head_dim, [&](auto v, auto lanes, auto items) {
       const int64_t per_block = THREADS / lanes.value;
-      int64_t grid = (a.tokens + per_block - 1) / per_block, most = 4 * (int64_t)current_cu_count();
-      if (weights && a.workspace_elems / (2 * a.head_dim) < most) most = a.workspace_elems / (2 * a.head_dim);
-      grid = grid < 1 ? 1 : grid > most ? most : grid;
-      const size_t lds = weights ? per_block * 2 * a.head_dim * sizeof(float) : 0;
-      qk_norm_rope_backward_kernel<dt.value, v.value, lanes.value, items.value><<<(int)grid, THREADS, lds, (hipStream_t)stream>>>(a);
+      const int each = heads_each(a.tokens, a.q_heads + a.k_heads, per_block);
+      BackwardArgs f{a, {make_kind(a.tokens, a.q_heads, each, per_block), make_kind(a.tokens, a.k_heads, each, per_block)}};
+      // persistent workgroups, each with a row of the workspace; the kinds have their shares of them, one at least
+      const int64_t room = weights ? a.workspace_elems / a.head_dim : INT32_MAX, most = room < MOST_GROUPS * current_cu_count() ? room : MOST_GROUPS * current_cu_count();
+      const int64_t all = (int64_t)f.kinds[0].blocks + f.kinds[1].blocks;
+      if (all > most) {
+        int64_t q = most * f.kinds[0].blocks / all;
+        if (f.kinds[0].blocks && q < 1) q = 1;
+        if (f.kinds[1].blocks && q > most - 1) q = most - 1;
+        if (q < f.kinds[0].blocks) f.kinds[0].blocks = (int)q;
+        if (most - q < f.kinds[1].blocks) f.kinds[1].blocks = (int)(most - q);
+      }
+      const int q_blocks = f.kinds[0].blocks, k_blocks = f.kinds[1].blocks;
+      const size_t lds = weights ? per_block * a.head_dim * sizeof(float) : 0;
+      if (q_blocks + k_blocks) qk_norm_rope_backward_kernel<dt.value, v.value, lanes.value, items.value><<<q_blocks + k_blocks, THREADS, lds, (hipStream_t)stream>>>(f);
       hipError_t err = hipGetLastError();
       if (err != hipSuccess || !weights) return err;
-      weight_gradient_kernel<<<(2 * a.head_dim + 15) / 16, THREADS, 0, (hipStream_t)stream>>>(a.workspace, (int)grid, a.head_dim, a.dq_weight,
-                                                                                              a.dk_weight);
+      weight_gradient_kernel<<<dim3((a.head_dim + 15) / 16, 2), SUM_THREADS, 0, (hipStream_t)stream>>>(a.workspace, q_blocks, k_blocks, a.head_dim,
+                                                                                                      a.dq_weight, a.dk_weight);
       return hipGetLastError();
     });
   });
