@@ -96,10 +96,16 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
     constexpr int threads = rows::WAVES * 64;
     if (!a.query_starts) {
       const int64_t units = (int64_t)a.requests * a.k_heads * ((g.group + rows::ROWS - 1) / rows::ROWS);
-      int64_t grid = units * ((most_keys + C::BT - 1) / C::BT + 2);
-      if (grid > 2 * cus) grid = 2 * cus;
+      const int64_t line = units * ((most_keys + C::BT - 1) / C::BT + 2 + rows::REST);  // at most
+      if (line > INT32_MAX) return hipErrorInvalidValue;
+      int64_t grid = line;
+      // As many workgroups as have 64 KiB of keys and values in flight a CU; more only leave more parts to join (us at 1 / 2 / 3 a CU:
+      // heads of 128, 64 requests of up to 8192 keys 20.6 / 22.1 / 23.1, 16 of up to 131072 119 / 120 / 123; heads of 64, 128
+      // requests that see 1028 keys 24.3 / 19.6 / 20.1).
+      constexpr int per_cu = 2 * C::BT * dp.value * C::ES <= 32 * 1024 ? 2 : 1;
+      if (grid > per_cu * cus) grid = per_cu * cus;
       if (slots && grid > slots / 2) grid = slots / 2;
-      if (grid > COUNTERS) grid = COUNTERS;
+      if (grid > rows::LATER) grid = rows::LATER;
       if (grid < 1) {
         grid = 1;
         g.slots = nullptr;
@@ -116,7 +122,7 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
           a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
         const int64_t units = row_tiles * a.k_heads;
         int64_t splits = 1;
-        if (units <= cus && units <= COUNTERS) {
+        if (units <= cus && units <= rows::LATER) {
           splits = 2 * cus / units;
           const int64_t room_for = slots * row_slot(a.head_dim) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
           if (splits > most_keys / (4 * tiles::BT)) splits = most_keys / (4 * tiles::BT);
@@ -133,10 +139,11 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
     const int64_t row_tiles = (int64_t)a.tokens * g.group / rows::ROWS + a.requests;
     const int64_t units = row_tiles * a.k_heads;
     int64_t splits = 1;
-    if (units < 2 * cus && units <= COUNTERS) {
+    if (units < 2 * cus && units <= rows::LATER) {
       splits = 2 * cus / units;
       if (splits > most_keys / (2 * C::BT)) splits = most_keys / (2 * C::BT);
       if (splits > slots / units) splits = slots / units;
+      if (splits > rows::FLAT) splits = rows::FLAT;
       if (splits < 1) splits = 1;
     }
     g.splits = (int)splits;

@@ -19,6 +19,9 @@ namespace iris_amd {
 namespace rows {
 
 constexpr int WAVES = 4, ROWS = 16;
+constexpr int FLAT = 24, FAN = 16, MEET = 64;     // parts that meet at once, how many do where there are more, and fans at most
+constexpr int REST = 2;                           // tiles that cost as much as beginning and ending a unit does
+constexpr int LATER = 1024, TOP = 2048;           // counters of fans but the first (by their first workgroup), and of a unit's fans
 
 template <int DT, int DP>
 struct Cfg {
@@ -67,15 +70,9 @@ __device__ inline int slot_of(const Piece& p, int part) { return part ? p.later_
 template <int DT, int DP>
 struct alignas(16) Lds {
   float o[WAVES][ROWS][DP + 4];
-  float m[WAVES][ROWS], l[WAVES][ROWS], lse_l[WAVES][ROWS];
+  f32x4 ml[WAVES][ROWS];  // maximum, sums
   int last;
 };
-
-// One row's maximum (sum) over the four lanes that hold its keys.
-__device__ inline float max_of_row(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
-}
 
 // Writes eight (fewer at the head's end) elements of an output row.
 template <int DT>
@@ -105,179 +102,225 @@ struct Unit {
 
   __device__ inline Unit(const AttentionKArgs& g, Lds<DT, DP>& lds) : g(g), a(g.a), lds(lds) {}
 
-  __device__ inline int64_t page_at(const Piece& p, int key, bool uniform) {
-    const int64_t at = (int64_t)p.request * a.stride_table + page_div((uint32_t)key, g.page);
-    int page = uniform ? scalar_at(a.block_table, at) : a.block_table[at];
-    if ((uint32_t)page >= (uint32_t)a.num_pages) {
-      bad_page = true;
-      page = 0;
-    }
-    return page;
-  }
-  // byte offset of key `key` (below the request's length) in a cache
-  struct Where {
-    int64_t k, v;
+  // The table's entries for a step's keys (for the wave, or for each of the lane's keys), and the keys and values themselves.
+  struct Pages {
+    int k[C::SUBS], v[C::SUBS][4];
   };
-  __device__ inline Where where(const Piece& p, int64_t page, int key) {
-    const int in_page = key - (int)(page_div((uint32_t)key, g.page) * g.page.d);
-    return {(page * a.stride_kc_page + (int64_t)in_page * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::ES,
-            (page * a.stride_vc_page + (int64_t)in_page * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::ES};
-  }
+  struct Step {
+    u32x4 k[C::SUBS][C::KC];
+    uint32_t v[C::SUBS][4][C::VW];
+  };
+  __device__ inline int step_base(const Piece& p, int j) { return p.tiles.tile(j) * C::BT + wave * C::KS; }
 
-  __device__ inline void run(const Piece& p) {
-    bad_page = false;
-    // the lane's row: its query, and its position
-    const int row = p.row0 + n;
-    const bool have_row = n < p.rows;
-    const int token = ONE ? 0 : (int)((uint32_t)(have_row ? row : p.row0) / (uint32_t)g.group);
-    const int head = p.head * g.group + (have_row ? row : p.row0) - token * g.group;
-    const int at = have_row ? p.first + token : -1;
-    const int first_at = ONE ? p.first : p.first + p.row0 / g.group;
-    const int last_at = ONE ? p.first : p.first + (p.row0 + p.rows - 1) / g.group;
+  // The state of the lane's row.  l: the sum of the weights as they are multiplied; lse_l: as they are, for the logarithm.
+  struct Row {
     u32x4 q[C::KC];
-    {
-      const IRIS_GLOBAL char* qp =
-          (const IRIS_GLOBAL char*)a.q + ((int64_t)(p.token0 + token) * a.stride_qt + (int64_t)head * a.stride_qh) * C::ES + quad * 16;
+    f32x4 o[C::VE];
+    float m, l, lse_l;
+    int at;                // the row's position
+    int first_at, last_at; // of the unit's rows
+  };
+
+  // Steps of a tile that no row sees a key of (the wave's share of the last keys, of the window's edge, behind the first
+  // tokens) are left out: their loads all go to the request's first key.
+  __device__ inline bool seen(const Piece& p, const Row& row, int j) {
+    const int base = step_base(p, j);
+    return base <= row.last_at && (a.window <= 0 || row.first_at - (base + C::KS - 1) < a.window || base < a.sinks);
+  }
+  __device__ inline void look_up(const Piece& p, int j, int last, Pages& pages) {
+    const int base = step_base(p, j);
+    const int64_t row = (int64_t)p.request * a.stride_table;
+#pragma unroll
+    for (int s = 0; s < C::SUBS; ++s) {
+      const int first_key = base + 16 * s;
+      if constexpr (PG) {
+        pages.k[s] = scalar_at(a.block_table, row + page_div((uint32_t)min(first_key, last), g.page));
+      } else {
+        pages.k[s] = a.block_table[row + page_div((uint32_t)min(first_key + n, last), g.page)];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pages.v[s][r] = a.block_table[row + page_div((uint32_t)min(first_key + quad * 4 + r, last), g.page)];
+      }
+    }
+  }
+  __device__ inline int64_t checked(int page) {
+    if ((uint32_t)page < (uint32_t)a.num_pages) return page;
+    bad_page = true;
+    return 0;
+  }
+  __device__ inline int in_page(int key) { return key - (int)(page_div((uint32_t)key, g.page) * g.page.d); }
+
+  // Keys past `last` are read as that one, and hidden later.
+  __device__ inline void load(const Piece& p, int j, int last, const Pages& pages, Step& x) {
+    const int base = step_base(p, j);
+#pragma unroll
+    for (int s = 0; s < C::SUBS; ++s) {
+      const int first_key = base + 16 * s, own = min(first_key + n, last);
+      const int64_t page = checked(pages.k[s]);
+      const IRIS_GLOBAL char* kp = (const IRIS_GLOBAL char*)a.k_cache +
+                                   (page * a.stride_kc_page + (int64_t)in_page(own) * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::ES + quad * 16;
 #pragma unroll
       for (int c = 0; c < C::KC; ++c) {
-        q[c] = u32x4{0, 0, 0, 0};
-        if (have_row && (c * 64 + quad * 16) / C::ES < a.head_dim) q[c] = *(const IRIS_GLOBAL u32x4*)(qp + c * 64);
+        x.k[s][c] = u32x4{0, 0, 0, 0};
+        if ((c * 64 + quad * 16) / C::ES < a.head_dim) x.k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + c * 64);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = min(first_key + quad * 4 + r, last);
+        const int64_t vpage = PG ? page : checked(pages.v[s][r]);
+        const IRIS_GLOBAL char* vp = (const IRIS_GLOBAL char*)a.v_cache +
+                                     (vpage * a.stride_vc_page + (int64_t)in_page(key) * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::ES + n * C::VB;
+#pragma unroll
+        for (int w = 0; w < C::VW; ++w) x.v[s][r][w] = 0;
+        if constexpr (C::VB == 8) {
+          if (n * C::VE < a.head_dim) {
+            const u32x2 y = *(const IRIS_GLOBAL u32x2*)vp;
+            x.v[s][r][0] = y[0], x.v[s][r][1] = y[1];
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < C::VW; w += 4)
+            if (n * C::VE + w * 4 / C::ES < a.head_dim) {
+              const u32x4 y = *(const IRIS_GLOBAL u32x4*)(vp + w * 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x.v[s][r][w + i] = y[i];
+            }
+        }
       }
     }
-    f32x4 o[C::VE];
-#pragma unroll
-    for (int e = 0; e < C::VE; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // l: the sum of the weights as they are multiplied; lse_l: as they are, for the logarithm
-    float m = -INFINITY, l = 0.f, lse_l = 0.f;
+  }
 
-    for (int j = p.j0; j < p.j1; ++j) {
-      const int base = p.tiles.tile(j) * C::BT + wave * C::KS;
-      if (base > last_at) continue;
-      const int last_key = p.length - 1;
-      u32x4 k[C::SUBS][C::KC];
-      uint32_t v[C::SUBS][4][C::VW];
+  __device__ inline void compute(const Piece& p, int j, Step& x, Row& row) {
+    const int base = step_base(p, j);
+    auto& v = x.v;
+    f32x4 s[C::SUBS];
 #pragma unroll
-      for (int s = 0; s < C::SUBS; ++s) {
-        const int first_key = base + 16 * s, own = min(first_key + n, last_key);
-        const int64_t page = page_at(p, PG ? min(first_key, last_key) : own, PG);
-        const IRIS_GLOBAL char* kp = (const IRIS_GLOBAL char*)a.k_cache + where(p, page, own).k + quad * 16;
+    for (int u = 0; u < C::SUBS; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < C::KC; ++c) {
-          k[s][c] = u32x4{0, 0, 0, 0};
-          if ((c * 64 + quad * 16) / C::ES < a.head_dim) k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + c * 64);
-        }
+      for (int c = 0; c < C::KC; ++c) s[u] = mfma<DT>(x.k[u][c], row.q[c], s[u]);
+    }
+    // Some of the step's keys may be hidden from some of the rows?  (the last keys; the window's edge)
+    const bool edge = base + C::KS - 1 > row.first_at || (a.window > 0 && row.last_at - base >= a.window && base + C::KS > a.sinks);
+    bool poisoned = false;  // a value that some row must not see is not a finite number
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int key = min(first_key + quad * 4 + r, last_key);
-          const int64_t vpage = PG ? page : page_at(p, key, false);
-          const IRIS_GLOBAL char* vp = (const IRIS_GLOBAL char*)a.v_cache + where(p, vpage, key).v + n * C::VB;
+          const int key = base + 16 * u + quad * 4 + r;
+          if (!sees(a, row.at, key)) s[u][r] = -INFINITY;
+          // hidden from every row: no product may see it either, whatever it is
+          const bool any = ONE ? sees(a, p.first, key) : key <= row.last_at && (a.window <= 0 || row.first_at - key < a.window || key < a.sinks);
 #pragma unroll
-          for (int w = 0; w < C::VW; ++w) v[s][r][w] = 0;
-          if constexpr (C::VB == 8) {
-            if (n * C::VE < a.head_dim) {
-              const u32x2 x = *(const IRIS_GLOBAL u32x2*)vp;
-              v[s][r][0] = x[0], v[s][r][1] = x[1];
-            }
-          } else {
-#pragma unroll
-            for (int w = 0; w < C::VW; w += 4)
-              if (n * C::VE + w * 4 / C::ES < a.head_dim) {
-                const u32x4 x = *(const IRIS_GLOBAL u32x4*)(vp + w * 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[s][r][w + i] = x[i];
-              }
+          for (int w = 0; w < C::VW; ++w) {
+            if (!any) v[u][r][w] = 0;
+            if (!ONE) poisoned |= not_finite(v[u][r][w]);
           }
         }
-      }
-      f32x4 s[C::SUBS];
+      if (!ONE) poisoned = __any(poisoned);
+    }
+    // the running maximum (less LIFT) and sum
+    float top = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < C::SUBS; ++u) {
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
-        for (int c = 0; c < C::KC; ++c) s[u] = mfma<DT>(k[u][c], q[c], s[u]);
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
+    top = over_32(over_16(top * g.scale_log2 - C::LIFT, Larger{}), Larger{});
+    const float m_new = fmaxf(row.m, top);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    const float shrink = __builtin_amdgcn_exp2f(row.m - ref);
+    row.m = m_new;
+    row.l *= shrink;
+    row.lse_l *= shrink;
+#pragma unroll
+    for (int u = 0; u < C::SUBS; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - ref);
+    u32x4 weights;  // in the operand's type: for fp32 themselves
+    if constexpr (C::F32) {
+      weights = __builtin_bit_cast(u32x4, s[0]);
+      row.l += (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
+      row.lse_l = row.l;
+    } else {
+      weights = u32x4{pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]), pack2<DT>(s[1][2], s[1][3])};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        row.l = add_weights<DT>(weights[e], row.l);
+        row.lse_l += s[0][e] + s[1][e];
       }
-      // Some of the step's keys may be hidden from some of the rows?  (the last keys; the window's edge)
-      const bool edge = base + C::KS - 1 > first_at || (a.window > 0 && last_at - base >= a.window && base + C::KS > a.sinks);
-      bool poisoned = false;  // a value that some row must not see is not a finite number
-      if (edge) {
+    }
+#pragma unroll
+    for (int e = 0; e < C::VE; ++e) row.o[e] *= shrink;
+    if (!poisoned) {
+      add_values(weights, v, row.o);
+    } else {
+      // (0 times it would still be NaN: each row's keys apart, with what it does not see taken out)
+      for (int y = 0; y < ROWS; ++y) {
+        const int at_y = __shfl(row.at, y, 64);
+        uint32_t vy[C::SUBS][4][C::VW];
 #pragma unroll
         for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int key = base + 16 * u + quad * 4 + r;
-            if (!sees(a, at, key)) s[u][r] = -INFINITY;
-            // hidden from every row: no product may see it either, whatever it is
-            const bool any = ONE ? sees(a, p.first, key) : key <= last_at && (a.window <= 0 || first_at - key < a.window || key < a.sinks);
+            const bool seen = sees(a, at_y, base + 16 * u + quad * 4 + r);
 #pragma unroll
-            for (int w = 0; w < C::VW; ++w) {
-              if (!any) v[u][r][w] = 0;
-              if (!ONE) poisoned |= not_finite(v[u][r][w]);
-            }
+            for (int w = 0; w < C::VW; ++w) vy[u][r][w] = seen ? v[u][r][w] : 0;
           }
-        if (!ONE) poisoned = __any(poisoned);
-      }
-      // the running maximum (less LIFT) and sum
-      float top = -INFINITY;
+        f32x4 one[C::VE];
 #pragma unroll
-      for (int u = 0; u < C::SUBS; ++u)
+        for (int e = 0; e < C::VE; ++e) one[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        add_values(weights, vy, one);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
-      top = max_of_row(top * g.scale_log2 - C::LIFT);
-      const float m_new = fmaxf(m, top);
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float shrink = __builtin_amdgcn_exp2f(m - ref);
-      m = m_new;
-      l *= shrink;
-      lse_l *= shrink;
-#pragma unroll
-      for (int u = 0; u < C::SUBS; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - ref);
-      u32x4 weights;  // in the operand's type: for fp32 themselves
-      if constexpr (C::F32) {
-        weights = __builtin_bit_cast(u32x4, s[0]);
-        l += (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
-        lse_l = l;
-      } else {
-        weights = u32x4{pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]), pack2<DT>(s[1][2], s[1][3])};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          l = add_weights<DT>(weights[e], l);
-          lse_l += s[0][e] + s[1][e];
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < C::VE; ++e) o[e] *= shrink;
-      if (!poisoned) {
-        add_values(weights, v, o);
-      } else {
-        // (0 times it would still be NaN: each row's keys apart, with what it does not see taken out)
-        for (int x = 0; x < ROWS; ++x) {
-          const int at_x = __shfl(at, x, 64);
-          uint32_t vx[C::SUBS][4][C::VW];
-#pragma unroll
-          for (int u = 0; u < C::SUBS; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool seen = sees(a, at_x, base + 16 * u + quad * 4 + r);
-#pragma unroll
-              for (int w = 0; w < C::VW; ++w) vx[u][r][w] = seen ? v[u][r][w] : 0;
-            }
-          f32x4 one[C::VE];
-#pragma unroll
-          for (int e = 0; e < C::VE; ++e) one[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-          add_values(weights, vx, one);
-#pragma unroll
-          for (int e = 0; e < C::VE; ++e)
-            if (n == x) o[e] += one[e];
-        }
+        for (int e = 0; e < C::VE; ++e)
+          if (n == y) row.o[e] += one[e];
       }
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    lse_l += __shfl_xor(lse_l, 16, 64);
-    lse_l += __shfl_xor(lse_l, 32, 64);
-    finish(p, m, l, lse_l, o);
+  }
+
+  __device__ inline void run(const Piece& p) {
+    bad_page = false;
+    Row row;
+    // the lane's row: its query, and its position
+    const bool have_row = n < p.rows;
+    const int index = p.row0 + (have_row ? n : 0);
+    const int token = ONE ? 0 : (int)((uint32_t)index / (uint32_t)g.group);
+    const int head = p.head * g.group + index - token * g.group;
+    row.at = have_row ? p.first + token : -1;
+    row.first_at = ONE ? p.first : p.first + p.row0 / g.group;
+    row.last_at = ONE ? p.first : p.first + (p.row0 + p.rows - 1) / g.group;
+    Pages pages;
+    Step x;
+        {
+      const IRIS_GLOBAL char* qp =
+          (const IRIS_GLOBAL char*)a.q + ((int64_t)(p.token0 + token) * a.stride_qt + (int64_t)head * a.stride_qh) * C::ES + quad * 16;
+#pragma unroll
+      for (int c = 0; c < C::KC; ++c) {
+        row.q[c] = u32x4{0, 0, 0, 0};
+        if (have_row && (c * 64 + quad * 16) / C::ES < a.head_dim) row.q[c] = *(const IRIS_GLOBAL u32x4*)(qp + c * 64);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < C::VE; ++e) row.o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    row.m = -INFINITY;
+    row.l = row.lse_l = 0.f;
+
+    // A step's pages are looked up while the step before it is worked on.  (Its keys and values as well, in registers of their own,
+    // took 116 us where this takes 119 for 606 MB, and the same for everything shorter, with half as much code again.)
+    int last = 0;
+    auto prepare = [&](int j) {
+      last = seen(p, row, j) ? p.length - 1 : 0;
+      look_up(p, j, last, pages);
+    };
+    if (p.j0 < p.j1) prepare(p.j0);
+    int j = p.j0;
+    for (; j < p.j1; ++j) {
+      load(p, j, last, pages, x);
+      if (j + 1 < p.j1) prepare(j + 1);
+      if (seen(p, row, j)) compute(p, j, x, row);
+    }
+    row.l = over_32(over_16(row.l, Sum{}), Sum{});
+    row.lse_l = over_32(over_16(row.lse_l, Sum{}), Sum{});
+    finish(p, row.m, row.l, row.lse_l, row.o);
   }
 
   static __device__ inline bool not_finite(uint32_t w) {
@@ -316,11 +359,7 @@ struct Unit {
       l = lse_l = __builtin_nanf("");
     }
     __syncthreads();  // (the last unit's shares have been read)
-    if (quad == 0) {
-      lds.m[wave][n] = m;
-      lds.l[wave][n] = l;
-      lds.lse_l[wave][n] = lse_l;
-    }
+    if (quad == 0) lds.ml[wave][n] = f32x4{m, l, lse_l, 0.f};
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -332,35 +371,40 @@ struct Unit {
     // sixteen lanes a row
     const int row = threadIdx.x / 16, part = threadIdx.x % 16;
     float top = -INFINITY, sum = 0.f, lse_sum = 0.f, weight[WAVES];
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds.m[w][row]);
+    f32x4 ml[WAVES];
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      weight[w] = __builtin_amdgcn_exp2f(lds.m[w][row] - (top == -INFINITY ? 0.f : top));
-      sum += weight[w] * lds.l[w][row];
-      lse_sum += weight[w] * lds.lse_l[w][row];
+      ml[w] = lds.ml[w][row];
+      top = fmaxf(top, ml[w][0]);
+    }
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      weight[w] = __builtin_amdgcn_exp2f(ml[w][0] - (top == -INFINITY ? 0.f : top));
+      sum += weight[w] * ml[w][1];
+      lse_sum += weight[w] * ml[w][2];
     }
     if (p.parts > 1) {
-      float* slot = g.slots + (int64_t)slot_of(p, p.part) * C::SLOT;
+      if (row < p.rows) {
+        float* slot = g.slots + (int64_t)slot_of(p, p.part) * C::SLOT;
 #pragma unroll
-      for (int d = part * 4; d < DP; d += 64) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int d = part * 4; d < DP; d += 64) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) x += weight[w] * *(const f32x4*)&lds.o[w][row][d];
-        store16_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + row * DP + d), __builtin_bit_cast(u32x4, x));
+          for (int w = 0; w < WAVES; ++w) x += weight[w] * *(const f32x4*)&lds.o[w][row][d];
+          store16_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + row * DP + d), __builtin_bit_cast(u32x4, x));
+        }
+        if (part == 0)
+          store16_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + ROWS * DP + 4 * row), __builtin_bit_cast(u32x4, f32x4{top, sum, lse_sum, 0.f}));
       }
-      if (part == 0)
-        store16_any<AUX_SC1>((IRIS_GLOBAL char*)(slot + ROWS * DP + 4 * row), __builtin_bit_cast(u32x4, f32x4{top, sum, lse_sum, 0.f}));
-      // the stores have reached the agent's coherence point before the arrival is counted
-      IRIS_WAIT_VMCNT(0);
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        IRIS_GLOBAL int32_t* count = (IRIS_GLOBAL int32_t*)(g.counters + p.counter);
-        lds.last = arrive(count, false, false) == p.parts - 1;
-        if (lds.last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      // Up to FLAT parts meet at once; more meet FAN by FAN, and then what they left in their first ones' slots.
+      const int fan = p.parts <= FLAT ? p.parts : FAN, mine = p.part / fan * fan, members = min(fan, p.parts - mine);
+      if (members > 1) {
+        if (!last_to_arrive(mine ? LATER + p.counter + mine : p.counter, members)) return;
+        join(p, mine, 1, members, fan == p.parts);
       }
-      __syncthreads();
-      if (lds.last) join(p, row, part);
+      if (fan == p.parts) return;
+      const int fans = (p.parts + fan - 1) / fan;
+      if (last_to_arrive(TOP + p.counter, fans)) join(p, 0, fan, fans, true);
       return;
     }
     if (row >= p.rows) return;
@@ -390,44 +434,103 @@ struct Unit {
     return {p.token0 + token, p.head * g.group + r - token * g.group};
   }
 
-  // The last part to arrive adds all parts, in their order.
-  __device__ inline void join(const Piece& p, int row, int part) {
-    if (row >= p.rows) return;
-    auto buffer = [&](int i) { return tile_rsrc((const IRIS_GLOBAL char*)(g.slots + (int64_t)slot_of(p, i) * C::SLOT), C::SLOT * 4); };
-    float top = -INFINITY, sum = 0.f, lse_sum = 0.f;
-    constexpr int NV = (DP + 63) / 64;
-    f32x4 x[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < p.parts; ++i) {
-      const __amdgpu_buffer_rsrc_t rs = buffer(__builtin_amdgcn_readfirstlane(i));
-      const f32x4 ml = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (ROWS * DP + 4 * row) * 4, 0, AUX_SC1));
-      u32x4 y[NV];
-#pragma unroll
-      for (int d = 0; d < NV; ++d) y[d] = __builtin_amdgcn_raw_buffer_load_b128(rs, (row * DP + d * 64 + part * 4) * 4, 0, AUX_SC1);
-      const float mi = ml[0];
-      const float t = fmaxf(top, mi), ref = t == -INFINITY ? 0.f : t;
-      const float old = __builtin_amdgcn_exp2f(top - ref), now = __builtin_amdgcn_exp2f(mi - ref);
-      top = t;
-      sum = sum * old + ml[1] * now;
-      lse_sum = lse_sum * old + ml[2] * now;
-#pragma unroll
-      for (int d = 0; d < NV; ++d) x[d] = x[d] * old + __builtin_bit_cast(f32x4, y[d]) * now;
+  // Counts this workgroup at counter `index`, once its stores have reached the agent's coherence point; true for the last of `all`,
+  // which takes the counter back to zero.
+  __device__ inline bool last_to_arrive(int index, int all) {
+    IRIS_WAIT_VMCNT(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      IRIS_GLOBAL int32_t* count = (IRIS_GLOBAL int32_t*)(g.counters + index);
+      lds.last = arrive(count, false, false) == all - 1;
+      if (lds.last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const Target t = target(p, row);
-    if (part == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = lse_sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(lse_sum)) * 0.6931471805599453f;
+    __syncthreads();
+    return lds.last;
+  }
+
+  // Adds the parts first, first + step, ... (`count` of them, no more than MEET): into the output, or back into the first one's slot.
+  // LANES lanes hold a row, and the first `count` of them (of LANES twice or four times in turn) its parts' maxima and sums, from
+  // which every part's weight follows at once; where there are few rows, sets of lanes take every so many-th part's output
+  // and add up in LDS.  Fixed orders all the way.
+  __device__ inline void join(const Piece& p, int first, int step, int count, bool whole) {
+    constexpr int LANES = DP / 4, GROUPS = WAVES * 64 / LANES, AT_ONCE = 8, HOLD = (MEET + LANES - 1) / LANES;
+    int abreast = 1;  // rows that are worked on at once
+    while (abreast < p.rows && abreast < GROUPS) abreast *= 2;
+    const int sets = GROUPS / abreast, group = threadIdx.x / LANES, set = group / abreast, in_row = threadIdx.x % LANES, d = in_row * 4;
+    float* const flat = &lds.o[0][0][0];         // sets' sums
+    float* const weights = flat + GROUPS * DP;   // the groups' weights of the parts
+    for (int row0 = 0; row0 < p.rows; row0 += abreast) {
+      const int row = row0 + group % abreast, used = min(row, p.rows - 1);  // (groups without a row repeat the last)
+      auto slot = [&](int i) { return (const char*)(g.slots + (int64_t)slot_of(p, first + i * step) * C::SLOT); };
+      f32x4 ml[HOLD];
 #pragma unroll
-    for (int d = 0; d < NV; ++d) {
-      const int at = d * 64 + part * 4;
-      if (at >= a.head_dim) continue;
-      IRIS_GLOBAL char* out = (IRIS_GLOBAL char*)a.out + (t.token * a.stride_ot + t.head * a.stride_oh + at) * C::ES;
-      x[d] *= inv;
+      for (int i = 0; i < HOLD; ++i) {
+        ml[i] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+        if (i * LANES + in_row < count) ml[i] = load_slot(slot(i * LANES + in_row) + (ROWS * DP + 4 * used) * 4);
+      }
+      f32x4 y[AT_ONCE];
+      auto fetch = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+          if (i0 + i * sets < count) y[i] = load_slot(slot(i0 + i * sets) + (used * DP + d) * 4);
+      };
+      fetch(set);
+      float top = -INFINITY, sum = 0.f, lse_sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) top = fmaxf(top, ml[i][0]);
+      top = over_lanes<LANES>(top, Larger{});
+      __syncthreads();  // (what LDS held has been read)
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) {
+        const float w = __builtin_amdgcn_exp2f(ml[i][0] - (top == -INFINITY ? 0.f : top));
+        sum += w * ml[i][1];
+        lse_sum += w * ml[i][2];
+        if (i * LANES + in_row < MEET) weights[group * MEET + i * LANES + in_row] = w;
+      }
+      sum = over_lanes<LANES>(sum, Sum{});
+      lse_sum = over_lanes<LANES>(lse_sum, Sum{});
+      __syncthreads();
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      for (int i0 = set; i0 < count; i0 += sets * AT_ONCE) {
+        if (i0 > set) fetch(i0);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+          if (i0 + i * sets < count) x += y[i] * weights[group * MEET + i0 + i * sets];
+      }
+      if (sets > 1) {
+        *(f32x4*)(flat + group * DP + d) = x;
+        __syncthreads();
+        if (set == 0) {
+          x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < GROUPS; ++i)
+            if (i < sets) x += *(const f32x4*)(flat + (group + i * abreast) * DP + d);
+        }
+      }
+      if (set > 0 || row >= p.rows) continue;
+      if (!whole) {
+        char* slot = (char*)(g.slots + (int64_t)slot_of(p, first) * C::SLOT);
+        store16_any<AUX_SC1>((IRIS_GLOBAL char*)slot + (row * DP + d) * 4, __builtin_bit_cast(u32x4, x));
+        if (d == 0) store16_any<AUX_SC1>((IRIS_GLOBAL char*)slot + (ROWS * DP + 4 * row) * 4, __builtin_bit_cast(u32x4, f32x4{top, sum, lse_sum, 0.f}));
+        continue;
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const Target t = target(p, row);
+      if (d == 0 && a.lse) a.lse[t.token * a.stride_lse + t.head] = lse_sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(lse_sum)) * 0.6931471805599453f;
+      if (d >= a.head_dim) continue;
+      IRIS_GLOBAL char* out = (IRIS_GLOBAL char*)a.out + (t.token * a.stride_ot + t.head * a.stride_oh + d) * C::ES;
+      x *= inv;
       if constexpr (C::F32)
-        *(IRIS_GLOBAL f32x4*)out = x[d];
+        *(IRIS_GLOBAL f32x4*)out = x;
       else
-        *(IRIS_GLOBAL u32x2*)out = u32x2{pack2<DT>(x[d][0], x[d][1]), pack2<DT>(x[d][2], x[d][3])};
+        *(IRIS_GLOBAL u32x2*)out = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
     }
+  }
+  // 16 bytes that another workgroup has written through.
+  __device__ inline f32x4 load_slot(const char* p) {
+    const u32x2 lo = __builtin_bit_cast(u32x2, __hip_atomic_load((const IRIS_GLOBAL uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __hip_atomic_load((const IRIS_GLOBAL uint64_t*)(p + 8), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    return __builtin_bit_cast(f32x4, u32x4{lo[0], lo[1], hi[0], hi[1]});
   }
 };
 
@@ -451,111 +554,113 @@ __device__ inline int keys_of(const AttentionKArgs& g, int request) {
   return length;
 }
 
-// Single tokens.  All units' key tiles lie in one line (request, key head, rows of 16, tile), which the workgroups cut into
-// equal runs: requests of any lengths load every workgroup alike.  A run's first and last unit may be shared with
-// the workgroups beside it.
+// Single tokens.  All units (request, key head, rows of 16) lie in one line, each as long as its key tiles and REST more for what a
+// unit costs beside them, and the workgroups cut the line into equal runs: requests of any lengths load every workgroup
+// alike.  A run's first and last unit may be shared with the workgroups beside it.
 template <int DT, int DP, bool PG>
 __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void decode_kernel(AttentionKArgs g) {
   using C = Cfg<DT, DP>;
   __shared__ Lds<DT, DP> lds;
   __shared__ int wave_sum[WAVES];
-  __shared__ int found_request, found_before;
+  __shared__ int found_request, found_before, found_length;
+  touch_args<sizeof(AttentionKArgs)>();
   const iris_attention_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row_tiles = (g.group + ROWS - 1) / ROWS, units = a.k_heads * row_tiles;
   constexpr int STEP = WAVES * 64;
 
-  auto tiles_of = [&](int request) {
-    const int length = keys_of(g, request);
-    return key_tiles<C::BT>(a, length - 1, length - 1).count;
-  };
-  // idle requests
-  for (int64_t r = blockIdx.x * WAVES + wave; r < a.requests; r += (int64_t)gridDim.x * WAVES)
-    if (keys_of(g, (int)r) == 0)
-      for (int h = 0; h < a.q_heads; ++h) clear_row<DT>(a, r, h);
-
-  // all tiles, then the request in which this workgroup's run begins
-  int64_t total = 0;
-  int mine = 0;
-  for (int r = tid; r < a.requests; r += STEP) mine += tiles_of(r);
-  for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d, 64);
-  if (lane == 0) wave_sum[wave] = mine;
-  __syncthreads();
-  for (int w = 0; w < WAVES; ++w) total += wave_sum[w];
-  const int64_t all = total * units;
-  if (all == 0) return;
-  const int64_t groups = all < g.grid_units ? all : g.grid_units;
-  if (blockIdx.x >= groups) return;
-  const int64_t begin = all * blockIdx.x / groups, end = all * (blockIdx.x + 1) / groups;
-  int before = 0;
-  for (int base = 0; base < a.requests; base += STEP) {
-    __syncthreads();
-    const int r = base + tid, own = r < a.requests ? tiles_of(r) : 0;
-    int sum = own;
+  // what a unit of `length` keys takes of the line
+  auto span_of = [&](int length) { return length > 0 ? key_tiles<C::BT>(a, length - 1, length - 1).count + REST : 0; };
+  // The line's length, and the request in which this workgroup's run begins: sums over the requests, STEP of them at a time, once
+  // where they are no more than that.  (The launcher has seen to it that the line is no longer than 31 bits count.)
+  int length = 0, own = 0, sum = 0;  // keys and span of the lane's request, and spans up to it in the wave
+  auto add_up = [&](int base) {
+    const int r = base + tid;
+    length = r < a.requests ? keys_of(g, r) : 0;
+    own = span_of(length);
+    sum = own;
+#pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int x = __shfl_up(sum, d, 64);
       if (lane >= d) sum += x;
     }
+    __syncthreads();
     if (lane == 63) wave_sum[wave] = sum;
     __syncthreads();
-    int ahead = before, chunk = 0;
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) ahead += wave_sum[w];
-      chunk += wave_sum[w];
+    int chunk = 0;
+    for (int w = 0; w < WAVES; ++w) chunk += wave_sum[w];
+    return chunk;
+  };
+  int total = 0;
+  for (int base = 0; base < a.requests; base += STEP) total += add_up(base);
+  const uint32_t all = (uint32_t)total * units, groups = min(all, (uint32_t)g.grid_units);
+  if (blockIdx.x < groups) {
+    // runs of `each`, the first `longer` of them one longer
+    const uint32_t each = all / groups, longer = all - each * groups;
+    const uint32_t begin = blockIdx.x * each + min(blockIdx.x, longer), end = begin + each + (blockIdx.x < longer);
+    auto group_at = [&](uint32_t x) { return x < longer * (each + 1) ? x / (each + 1) : longer + (x - longer * (each + 1)) / each; };
+    int before = 0;  // spans of earlier chunks
+    for (int base = 0; base < a.requests; base += STEP) {
+      const int chunk = a.requests > STEP ? add_up(base) : total;
+      int ahead = before;
+      for (int w = 0; w < wave; ++w) ahead += wave_sum[w];
+      const uint32_t lo = (uint32_t)(ahead + sum - own) * units, hi = (uint32_t)(ahead + sum) * units;
+      if (lo <= begin && begin < hi) {
+        found_request = base + tid;
+        found_before = ahead + sum - own;
+        found_length = length;
+      }
+      before += chunk;
+      if ((uint32_t)before * units > begin) break;
     }
-    const int64_t lo = (int64_t)(ahead + sum - own) * units, hi = (int64_t)(ahead + sum) * units;
-    if (lo <= begin && begin < hi) {
-      found_request = r;
-      found_before = ahead + sum - own;
-    }
-    before += chunk;
-    if ((int64_t)before * units > begin) break;
-  }
-  __syncthreads();
-  int request = __builtin_amdgcn_readfirstlane(found_request);
-  int64_t base = (int64_t)__builtin_amdgcn_readfirstlane(found_before) * units;  // the request's first tile in the line
+    __syncthreads();
+    int request = __builtin_amdgcn_readfirstlane(found_request), next_length = __builtin_amdgcn_readfirstlane(found_length);
+    uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane(found_before) * units;  // the request's place in the line
 
-  Unit<DT, DP, PG, true> unit(g, lds);
-  for (int64_t at = begin; at < end;) {
-    Piece p;
-    p.request = request;
-    p.length = __builtin_amdgcn_readfirstlane(keys_of(g, request));
-    p.first = p.length - 1;
-    p.tiles = key_tiles<C::BT>(a, p.first, p.first);
-    const int64_t request_end = base + (int64_t)p.tiles.count * units;
-    if (at >= request_end) {  // (idle requests have no tiles)
+    Unit<DT, DP, PG, true> unit(g, lds);
+    for (uint32_t at = begin; at < end; ++request) {
+      Piece p;
+      p.request = request;
+      p.length = next_length;
+      p.first = p.length - 1;
+      p.tiles = key_tiles<C::BT>(a, p.first, p.first);
+      const uint32_t span = p.length > 0 ? p.tiles.count + REST : 0, request_end = base + span * units;
+      while (at < end && at < request_end) {
+        const uint32_t u = (at - base) / span, unit_begin = base + u * span, tiles_begin = unit_begin + REST, unit_end = unit_begin + span;
+        const uint32_t from = max(at, tiles_begin), to = min(end, unit_end);
+        at = unit_end;
+        if (from >= to) continue;  // (the run ends in what stands before the tiles)
+        p.head = row_tiles == 1 ? u : u / row_tiles;
+        p.row0 = (u - p.head * row_tiles) * ROWS;
+        p.rows = min(ROWS, g.group - p.row0);
+        p.token0 = request;
+        p.parts = 1;
+        p.j0 = from - tiles_begin;
+        p.j1 = to - tiles_begin;
+        if (g.slots) {
+          // the workgroups of the first and the last tile
+          const int first = tiles_begin >= begin ? (int)blockIdx.x : group_at(tiles_begin);
+          const int last = unit_end <= end ? (int)blockIdx.x : group_at(unit_end - 1);
+          p.parts = last - first + 1;
+          p.part = (int)blockIdx.x - first;
+          p.first_slot = 2 * first + 1;
+          p.later_slot = 2 * first;
+          p.slot_step = 2;
+          p.counter = first;
+        } else {  // nothing is split: a unit is its first tile's workgroup's
+          if (p.j0) continue;
+          p.j1 = p.tiles.count;
+        }
+        unit.run(p);
+      }
       base = request_end;
-      ++request;
-      continue;
+      if (at < end) next_length = min(max(scalar_at(a.lengths, request + 1), 0), (int)(a.table_width * g.page.d));
     }
-    const int u = (int)((at - base) / p.tiles.count);
-    const int64_t unit_begin = base + (int64_t)u * p.tiles.count, unit_end = unit_begin + p.tiles.count;
-    p.head = u / row_tiles;
-    p.row0 = (u - p.head * row_tiles) * ROWS;
-    p.rows = min(ROWS, g.group - p.row0);
-    p.token0 = request;
-    if (!g.slots) {  // nothing is split: a unit is its first tile's workgroup's
-      at = unit_end;
-      if (at - p.tiles.count < begin) continue;
-      p.j0 = 0;
-      p.j1 = p.tiles.count;
-      p.parts = 1;
-      unit.run(p);
-      continue;
-    }
-    p.j0 = (int)(at - unit_begin);
-    p.j1 = (int)((end < unit_end ? end : unit_end) - unit_begin);
-    // the workgroups that hold the unit's first and last tile
-    const int first = (int)(((unit_begin + 1) * groups - 1) / all), last = (int)((unit_end * groups - 1) / all);
-    p.parts = last - first + 1;
-    p.part = (int)blockIdx.x - first;
-    p.first_slot = 2 * first + 1;
-    p.later_slot = 2 * first;
-    p.slot_step = 2;
-    p.counter = first;
-    unit.run(p);
-    at = unit_begin + p.j1;
   }
+  // idle requests
+  for (int64_t r = blockIdx.x * WAVES + wave; r < a.requests; r += (int64_t)gridDim.x * WAVES)
+    if (a.lengths[r] <= 0)
+      for (int h = 0; h < a.q_heads; ++h) clear_row<DT>(a, r, h);
 }
 
 // Prompts: a workgroup for 16 rows of a request and key head, and a share of the keys they see.  Row tile x of the grid is the

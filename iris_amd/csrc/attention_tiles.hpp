@@ -57,9 +57,6 @@ __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Larger of a lane's value and that of the lane 32 away.
-__device__ inline float max_of_halves(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
-
 // The row tile that sees the k-th most keys (no window), later rows before earlier ones: workgroups that start last are then the
 // short ones.  (A prompt of 8192 tokens among others, 1153 row tiles of 1 to 128 key tiles on 512 places: 345 us in the requests'
 // order, BALANCED_US by length.)  Request r has tiles_r row tiles, and of those that see at least c key tiles the number is known in closed form;
@@ -356,7 +353,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    const float next = fmaxf(ref, max_of_halves(top) * g.scale_log2 - C::LIFT);
+    const float next = fmaxf(ref, over_32(top, Larger{}) * g.scale_log2 - C::LIFT);
     const float shrink = __builtin_amdgcn_exp2f(ref - (next == -INFINITY ? 0.f : next));
     ref = next;
     l *= shrink;
@@ -368,8 +365,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   }
   for (; j < j1; ++j) next_stage(j);
 
-  l += __shfl_xor(l, 32, 64);
-  lse_l += __shfl_xor(lse_l, 32, 64);
+  l = over_32(l, Sum{});
+  lse_l = over_32(lse_l, Sum{});
   // what one wave found is every row's
   bool redo = __syncthreads_or(poisoned);
   float flags = __syncthreads_or(bad_page) ? __builtin_nanf("") : 0.f;

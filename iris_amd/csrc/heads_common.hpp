@@ -62,25 +62,49 @@ template <int CTRL>
 __device__ inline float permuted(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
 }
-template <int CTRL>
-__device__ inline double permuted(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, true);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+// op over the lanes 16 (32) apart, in each of them.
+template <class Op>
+__device__ inline float over_16(float x, Op op) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return op(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+template <class Op>
+__device__ inline float over_32(float x, Op op) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return op(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-// Sum over groups of LANES neighbouring lanes (8, 16, 32 or 64), the same bits in all of them: neighbours, pairs, and from
-// four lanes of equal sums on mirror images.
-template <int LANES, class T>
-__device__ inline T sum_lanes(T x) {
+// op over groups of LANES neighbouring lanes (8, 16, 32 or 64), the same bits in all of them: neighbours, pairs, from four equal
+// lanes on mirror images, and rows and halves of the wave that change places between two copies.
+template <int LANES, class Op>
+__device__ inline float over_lanes(float x, Op op) {
   constexpr int NEIGHBOURS = 0xB1, PAIRS = 0x4E, MIRROR_8 = 0x141, MIRROR_16 = 0x140;  // quad_perm [1,0,3,2], [2,3,0,1]; row_half_mirror, row_mirror
-  x += permuted<NEIGHBOURS>(x);
-  x += permuted<PAIRS>(x);
-  x += permuted<MIRROR_8>(x);
-  if constexpr (LANES >= 16) x += permuted<MIRROR_16>(x);
-  if constexpr (LANES >= 32) x += __shfl_xor(x, 16, 64);
-  if constexpr (LANES >= 64) x += __shfl_xor(x, 32, 64);
+  x = op(x, permuted<NEIGHBOURS>(x));
+  x = op(x, permuted<PAIRS>(x));
+  x = op(x, permuted<MIRROR_8>(x));
+  if constexpr (LANES >= 16) x = op(x, permuted<MIRROR_16>(x));
+  if constexpr (LANES >= 32) x = over_16(x, op);
+  if constexpr (LANES >= 64) x = over_32(x, op);
+  return x;
+}
+struct Larger {
+  __device__ inline float operator()(float x, float y) const { return fmaxf(x, y); }
+};
+struct Sum {
+  template <class T>
+  __device__ inline T operator()(T x, T y) const {
+    return x + y;
+  }
+};
+template <int LANES>
+__device__ inline float sum_lanes(float x) {
+  return over_lanes<LANES>(x, Sum{});
+}
+template <int LANES>
+__device__ inline double sum_lanes(double x) {
+  static_assert(LANES == 64, "as single pairs are laid out");
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
   return x;
 }
 
