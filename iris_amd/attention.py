@@ -184,6 +184,8 @@ def build_block_tables(cached, new_tokens, block_table, pool, pool_state, page_s
         raise ValueError(f"at most {MAX_REQUESTS} requests, got {requests}")
     if page_size < 1:
         raise ValueError("page_size must be positive")
+    if block_table.shape[1] * page_size > INT32_MAX:
+        raise ValueError("block_table has room for more tokens than 31 bits count")
     written = (block_table, pool, lengths, pool_state_out, query_starts, positions, slots)
     spans = [(t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape))))
              for t in written + (cached, new_tokens, pool_state) if t.numel()]

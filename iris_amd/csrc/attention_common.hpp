@@ -5,20 +5,6 @@
 
 namespace iris_amd {
 
-// Division by the launch's page size for dividends below 2^31: with s = ceil(log2 d), m = ceil(2^(31 + s) / d) < 2^32 + 1 and
-// m d - 2^(31 + s) < 2^s, so that floor(n m / 2^(31 + s)) = floor(n / d) for n < 2^31.
-struct PageDiv {
-  uint32_t d, shift;
-  uint64_t m;
-};
-__host__ __device__ inline PageDiv make_page_div(uint32_t d) {
-  PageDiv p{d, 31, 0};
-  while ((1ull << (p.shift - 31)) < d) ++p.shift;
-  p.m = ((1ull << p.shift) + d - 1) / d;
-  return p;
-}
-__host__ __device__ inline uint32_t page_div(uint32_t n, const PageDiv& p) { return (uint32_t)(((uint64_t)n * p.m) >> p.shift); }
-
 struct AttentionKArgs {
   iris_attention_args a;
   PageDiv page;

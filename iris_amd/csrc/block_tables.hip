@@ -11,29 +11,50 @@
 namespace iris_amd {
 namespace {
 
-constexpr int MAX_REQUESTS = 8192;  // three sums of them fit in LDS
+constexpr int MAX_REQUESTS = 8192;  // three sums and the lengths of them fit in LDS
+constexpr int THREADS = 1024;
 
 struct Sums {
   int need, back, tokens;
 };
+__device__ inline Sums operator+(Sums a, Sums b) { return {a.need + b.need, a.back + b.back, a.tokens + b.tokens}; }
 
-// What request i asks for, before the ring's end is looked at.
+struct Args {
+  iris_block_tables_args a;
+  PageDiv page;
+  int room;  // tokens that a table row has pages for
+};
+
+__device__ inline int pages(int tokens, const PageDiv& p) { return tokens > 0 ? (int)page_div((uint32_t)tokens - 1, p) + 1 : 0; }
+
+// What a request asks for, before the ring's end is looked at.
 struct Request {
-  int cached, add, held, want;
+  int cached, add;
   bool ended, fits;
 };
-__device__ inline Request request(const iris_block_tables_args& a, int i) {
+__device__ inline Request request(const Args& g, int i) {
   Request r;
-  const int n = a.new_tokens[i];
-  r.cached = max(a.cached[i], 0);
+  const int n = g.a.new_tokens[i];
+  r.cached = max(g.a.cached[i], 0);
   r.ended = n < 0;
   r.add = max(n, 0);
-  const int64_t want = ((int64_t)r.cached + r.add + a.page_size - 1) / a.page_size;
-  r.held = (int)(((int64_t)r.cached + a.page_size - 1) / a.page_size);
-  r.fits = !r.ended && want <= a.table_width;
-  r.want = r.fits ? (int)want : r.held;
-  if (r.ended) r.held = min(r.held, a.table_width);
+  r.fits = !r.ended && (int64_t)r.cached + r.add <= g.room;
   return r;
+}
+
+// Inclusive sum over the wave.  DPP: shifts within rows of 16, then the rows' and halves' last lanes to the next ones.
+template <int CTRL, int ROWS>
+__device__ inline int shifted(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ inline int wave_prefix(int x) {
+  x += shifted<0x111, 0xF>(x);
+  x += shifted<0x112, 0xF>(x);
+  x += shifted<0x114, 0xF>(x);
+  x += shifted<0x118, 0xF>(x);
+  x += shifted<0x142, 0xA>(x);
+  x += shifted<0x143, 0xC>(x);
+  return x;
 }
 
 // The largest i < n with before[i] <= x, where before[0] == 0.
@@ -49,97 +70,91 @@ __device__ inline int owner(const int* before, int n, int x) {
   return lo;
 }
 
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void block_tables_kernel(iris_block_tables_args a) {
+// ITEMS requests a thread, neighbours.
+template <int ITEMS>
+__global__ __launch_bounds__(THREADS) void block_tables_kernel(Args g) {
   extern __shared__ int lds[];
   __shared__ Sums wave_sums[THREADS / 64];
   __shared__ int granted;  // pages taken by the requests that were served
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.requests;
+  const iris_block_tables_args& a = g.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x / 64, n = a.requests;
   int* const need_before = lds;
   int* const back_before = lds + n;
   int* const tokens_before = lds + 2 * n;
+  int* const lengths = lds + 3 * n;  // tokens in the cache; of requests that are not served, the complement
   const int64_t taken = a.pool_state[0], returned = a.pool_state[1];
   const int64_t free64 = returned - taken;
   const int free_pages = (int)(free64 < 0 ? 0 : free64 > a.pool_size ? a.pool_size : free64);
   if (tid == 0) granted = 0;
 
-  // exclusive prefix sums of the requests, THREADS of them at a time
-  Sums carry{0, 0, 0};
-  for (int base = 0; base < n; base += THREADS) {
-    const int i = base + tid;
-    Sums own{0, 0, 0};
-    if (i < n) {
-      const Request r = request(a, i);
-      own.need = r.fits ? r.want - r.held : 0;
-      own.back = r.ended ? r.held : 0;
-      own.tokens = r.add;
-    }
-    Sums s = own;
+  // exclusive prefix sums of the requests
+  Request r[ITEMS];
+  Sums own[ITEMS], mine{0, 0, 0};
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(s.need, d, 64), y = __shfl_up(s.back, d, 64), z = __shfl_up(s.tokens, d, 64);
-      if (lane >= d) {
-        s.need += x;
-        s.back += y;
-        s.tokens += z;
-      }
-    }
-    __syncthreads();  // (the last chunk's sums have been read)
-    if (lane == 63) wave_sums[wave] = s;
-    __syncthreads();
-    Sums before = carry;
-    for (int w = 0; w < THREADS / 64; ++w) {
-      const Sums t = wave_sums[w];
-      if (w < wave) {
-        before.need += t.need;
-        before.back += t.back;
-        before.tokens += t.tokens;
-      }
-      carry.need += t.need;
-      carry.back += t.back;
-      carry.tokens += t.tokens;
-    }
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = tid * ITEMS + k;
+    own[k] = Sums{0, 0, 0};
     if (i < n) {
-      need_before[i] = before.need + s.need - own.need;
-      back_before[i] = before.back + s.back - own.back;
-      tokens_before[i] = before.tokens + s.tokens - own.tokens;
-      // The requests that need pages are served while the ring lasts: a prefix of them, whose last sum is the number taken.
-      if (own.need && before.need + s.need <= free_pages) atomicMax(&granted, before.need + s.need);
+      r[k] = request(g, i);
+      const int held = pages(r[k].cached, g.page);
+      if (r[k].fits) own[k].need = pages(r[k].cached + r[k].add, g.page) - held;
+      if (r[k].ended) own[k].back = min(held, a.table_width);
+      own[k].tokens = r[k].add;
     }
+    mine = mine + own[k];
+  }
+  const Sums upto{wave_prefix(mine.need), wave_prefix(mine.back), wave_prefix(mine.tokens)};
+  if (lane == 63) wave_sums[wave] = upto;
+  __syncthreads();
+  Sums before{upto.need - mine.need, upto.back - mine.back, upto.tokens - mine.tokens}, all{0, 0, 0};
+  for (int w = 0; w < waves; ++w) {
+    const Sums t = wave_sums[w];
+    if (w < wave) before = before + t;
+    all = all + t;
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = tid * ITEMS + k;
+    if (i < n) {
+      // The requests that need pages are served while the ring lasts: a prefix of them, whose last sum is the number taken.
+      const int after = before.need + own[k].need;
+      const bool served = r[k].fits && (!own[k].need || after <= free_pages);
+      if (own[k].need && served) atomicMax(&granted, after);
+      need_before[i] = before.need;
+      back_before[i] = before.back;
+      tokens_before[i] = before.tokens;
+      lengths[i] = served || r[k].ended ? r[k].cached : ~r[k].cached;
+      if (blockIdx.x == 0) {
+        a.lengths[i] = r[k].ended ? 0 : served ? r[k].cached + r[k].add : r[k].cached;
+        a.query_starts[i] = before.tokens;
+        if (!r[k].ended && !served) report(a.status, IRIS_STATUS_NO_PAGES);
+      }
+    }
+    before = before + own[k];
   }
   __syncthreads();
-  const int total = carry.tokens;
   const uint32_t ring = (uint32_t)a.pool_size;
   const uint32_t taken_at = (uint32_t)(taken % ring), returned_at = (uint32_t)(returned % ring);
-  // served: does request i get what it needs
-  auto served = [&](const Request& r, int i) { return r.fits && (r.want == r.held || need_before[i] + r.want - r.held <= free_pages); };
   auto page_of = [&](int nth) { return a.pool[(taken_at + (uint32_t)nth) % ring]; };
 
-  const int gid = blockIdx.x * THREADS + tid, step = gridDim.x * THREADS;
-  for (int i = gid; i < n; i += step) {
-    const Request r = request(a, i);
-    const bool ok = served(r, i);
-    a.lengths[i] = r.ended ? 0 : ok ? r.cached + r.add : r.cached;
-    a.query_starts[i] = tokens_before[i];
-    if (!r.ended && !ok) report(a.status, IRIS_STATUS_NO_PAGES);
-  }
+  const int gid = blockIdx.x * blockDim.x + tid, step = gridDim.x * blockDim.x;
   if (gid == 0) {
-    a.query_starts[n] = total;
+    a.query_starts[n] = all.tokens;
     a.pool_state_out[0] = taken + granted;
-    a.pool_state_out[1] = returned + carry.back;
-    if (total > a.max_tokens) report(a.status, IRIS_STATUS_NO_ROOM);
+    a.pool_state_out[1] = returned + all.back;
+    if (all.tokens > a.max_tokens) report(a.status, IRIS_STATUS_NO_ROOM);
   }
   for (int t = gid; t < a.max_tokens; t += step) {
     int position = 0;
     int64_t slot = -1;
-    if (t < total) {
-      const int i = owner(tokens_before, n, t);
-      const Request r = request(a, i);
-      position = r.cached + t - tokens_before[i];
-      const int j = position / a.page_size;
-      if (served(r, i) && position >= 0 && j < a.table_width) {
-        const int page = j < r.held ? a.block_table[(int64_t)i * a.stride_table + j] : page_of(need_before[i] + j - r.held);
-        slot = (int64_t)page * a.page_size + position % a.page_size;
+    if (t < all.tokens) {
+      const int i = owner(tokens_before, n, t), length = lengths[i];
+      position = (length < 0 ? ~length : length) + t - tokens_before[i];
+      // (a sum past 31 bits, of lengths that are none, may leave a position that is none)
+      if (length >= 0 && position >= 0 && position < g.room) {
+        const int j = (int)page_div((uint32_t)position, g.page), held = pages(length, g.page);
+        const int page = j < held ? a.block_table[(int64_t)i * a.stride_table + j] : page_of(need_before[i] + j - held);
+        slot = (int64_t)page * a.page_size + (position - j * a.page_size);
       }
     }
     a.positions[t] = position;
@@ -147,13 +162,12 @@ __global__ __launch_bounds__(THREADS) void block_tables_kernel(iris_block_tables
   }
   // (a request that was not served has sums past `granted`, and needs nothing where it has not)
   for (int x = gid; x < granted; x += step) {
-    const int i = owner(need_before, n, x);
-    const Request r = request(a, i);
-    a.block_table[(int64_t)i * a.stride_table + r.held + x - need_before[i]] = page_of(x);
+    const int i = owner(need_before, n, x), j = pages(lengths[i], g.page) + x - need_before[i];
+    if ((uint32_t)j < (uint32_t)a.table_width) a.block_table[(int64_t)i * a.stride_table + j] = page_of(x);
   }
-  for (int x = gid; x < carry.back; x += step) {
-    const int i = owner(back_before, n, x);
-    a.pool[(returned_at + (uint32_t)x) % ring] = a.block_table[(int64_t)i * a.stride_table + x - back_before[i]];
+  for (int x = gid; x < all.back; x += step) {
+    const int i = owner(back_before, n, x), j = x - back_before[i];
+    if ((uint32_t)j < (uint32_t)a.table_width) a.pool[(returned_at + (uint32_t)x) % ring] = a.block_table[(int64_t)i * a.stride_table + j];
   }
 }
 
@@ -169,21 +183,24 @@ extern "C" int iris_block_tables_launch(const iris_block_tables_args* args, void
       (a.max_tokens && (!a.positions || !a.slots)) || (a.requests && (!a.cached || !a.new_tokens || !a.lengths)) ||
       (a.requests && a.table_width && !a.block_table) || (int64_t)a.requests * a.table_width > INT32_MAX)
     return hipErrorInvalidValue;
-  const size_t lds = (size_t)a.requests * 3 * sizeof(int);
-  const int threads = a.requests > 1024 ? 1024 : 256;
-  // a workgroup repeats the sums, so it is given a few items a thread to write
-  const int64_t items = (int64_t)a.max_tokens + a.requests;
-  const int64_t groups = (items + 2 * threads - 1) / (2 * threads);
+  if ((int64_t)a.table_width * a.page_size > INT32_MAX) return hipErrorInvalidValue;
+  const Args g{a, make_page_div((uint32_t)a.page_size), a.table_width * a.page_size};
+  const size_t lds = (size_t)a.requests * 4 * sizeof(int);
+  // Four waves where they hold the requests, so that a small step's sums meet sooner; sixteen beyond.  An item (token) a thread: a
+  // workgroup repeats the sums, but what it writes it looks for in several dependent reads.
+  const int threads = a.requests > 256 ? THREADS : 256;
+  const int64_t groups = ((int64_t)a.max_tokens + threads - 1) / threads;
   const int cus = current_cu_count();
   const int grid = (int)(groups < 1 ? 1 : groups > cus ? cus : groups);
-  if (threads == 1024) {
+  if (a.requests > THREADS) {
+    constexpr int ITEMS = MAX_REQUESTS / THREADS;
     if (lds > 64 * 1024) {
-      const hipError_t err = hipFuncSetAttribute((const void*)block_tables_kernel<1024>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      const hipError_t err = hipFuncSetAttribute((const void*)block_tables_kernel<ITEMS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
       if (err != hipSuccess) return err;
     }
-    block_tables_kernel<1024><<<grid, 1024, lds, (hipStream_t)stream>>>(a);
+    block_tables_kernel<ITEMS><<<grid, threads, lds, (hipStream_t)stream>>>(g);
   } else {
-    block_tables_kernel<256><<<grid, 256, lds, (hipStream_t)stream>>>(a);
+    block_tables_kernel<1><<<grid, threads, lds, (hipStream_t)stream>>>(g);
   }
   return hipGetLastError();
 }
