@@ -120,10 +120,10 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
       const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
       if ((int64_t)a.tokens * g.group > 32 * (int64_t)a.requests && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX &&
           a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
-        const int64_t units = row_tiles * a.k_heads;
+        const int64_t units = row_tiles * a.k_heads, places = tiles::waves_a_simd(dp.value) * cus;
         int64_t splits = 1;
-        if (units <= cus && units <= rows::LATER) {
-          splits = 2 * cus / units;
+        if (2 * units <= places && units <= rows::LATER) {
+          splits = places / units;
           const int64_t room_for = slots * row_slot(a.head_dim) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
           if (splits > most_keys / (4 * tiles::BT)) splits = most_keys / (4 * tiles::BT);
           if (splits > room_for) splits = room_for;
@@ -131,8 +131,11 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
         }
         g.splits = (int)splits;
         // (which starts first matters where not all run at once; a window leaves little between them)
-        g.by_length = units * splits > 2 * cus && a.window == 0 && a.requests <= 64;
-        tiles::prompt_tiles_kernel<dt.value, dp.value><<<(int)(units * splits), tiles::WAVES * 64, 0, s>>>(g);
+        g.by_length = units * splits > places && a.window == 0 && a.requests <= 64;
+        if (a.lse)
+          tiles::prompt_tiles_kernel<dt.value, dp.value, true><<<(int)(units * splits), tiles::WAVES * 64, 0, s>>>(g);
+        else
+          tiles::prompt_tiles_kernel<dt.value, dp.value, false><<<(int)(units * splits), tiles::WAVES * 64, 0, s>>>(g);
         return hipGetLastError();
       }
     }

@@ -18,9 +18,13 @@
 namespace iris_amd {
 namespace tiles {
 
+
 constexpr int WAVES = 4, ROWS = 128, WAVE_ROWS = 32, BT = 64;
 constexpr int AHEAD = 4;
 constexpr int SCHED_MFMA = 0x8, SCHED_DS_READ = 0x100;  // kinds of instructions of __builtin_amdgcn_sched_group_barrier
+
+// As many as their registers let in.  (Heads of 64, a window of 1024: two 58 us, three 55, four 77, for they spill.)
+constexpr int waves_a_simd(int dp) { return dp == 64 ? 3 : 2; }
 
 template <int DT, int DP>
 struct Cfg {
@@ -55,6 +59,13 @@ __device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Which of the keys base .. base + 31 the query at position `at` sees, as bits.
+__device__ inline uint32_t visible(const iris_attention_args& a, int at, int base) {
+  auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+  const uint32_t past = below(at + 1 - base);
+  return a.window > 0 ? past & (~below(at - a.window + 1 - base) | below(a.sinks - base)) : past;
 }
 
 // The row tile that sees the k-th most keys (no window), later rows before earlier ones: workgroups that start last are then the
@@ -108,8 +119,9 @@ __device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request,
   return true;
 }
 
-template <int DT, int DP>
-__global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_tiles_kernel(AttentionKArgs g) {
+// LSE: the logarithms of the rows' sums are wanted.
+template <int DT, int DP, bool LSE>
+__global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu_waves_per_eu(waves_a_simd(DP), waves_a_simd(DP)))) void prompt_tiles_kernel(AttentionKArgs g) {
   using C = Cfg<DT, DP>;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][C::TILE_BYTES];  // [stage][keys, values]
   const iris_attention_args& a = g.a;
@@ -145,7 +157,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
     length = (int)(a.table_width * g.page.d);
   }
   const int first = length - tokens;  // position of the request's first query
-  const KeyTiles list = key_tiles<BT>(a, first + row0 / g.group, first + (row0 + num_rows - 1) / g.group);
+  const int rows_first = first + row0 / g.group, rows_last = first + (row0 + num_rows - 1) / g.group;
+  const KeyTiles list = key_tiles<BT>(a, rows_first, rows_last);
   // the workgroup's share of the tiles
   const int j0 = (int)((int64_t)list.count * split / g.splits), j1 = (int)((int64_t)list.count * (split + 1) / g.splits);
 
@@ -194,12 +207,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
     const __amdgpu_buffer_rsrc_t kr = tile_rsrc((const IRIS_GLOBAL char*)a.k_cache + ((int64_t)page * a.stride_kc_page + (int64_t)head * a.stride_kc_head) * 2, 0x7FFFFFFF);
     const __amdgpu_buffer_rsrc_t vr = tile_rsrc((const IRIS_GLOBAL char*)a.v_cache + ((int64_t)page * a.stride_vc_page + (int64_t)head * a.stride_vc_head) * 2, 0x7FFFFFFF);
     const int k_at = in_page * (int)(a.stride_kc_row * 2), v_at = in_page * (int)(a.stride_vc_row * 2);
+    char* const to = &lds[stage][0][wave * 16 * C::ROW_BYTES];
+    auto dma = [&](int i, uint32_t ko, uint32_t vo) {
+      lds_dma16(kr, (IRIS_LDS void*)(to + i * 1024), ko, k_at);
+      lds_dma16(vr, (IRIS_LDS void*)(to + C::TILE_BYTES + i * 1024), vo, v_at);
+    };
+    if (valid >= 16) {
 #pragma unroll
-    for (int i = 0; i < C::DMAS; ++i) {
-      uint32_t ko = k_off[i], vo = v_off[i];
-      if (valid < 16 && i * C::DMA_ROWS + lane / C::CHUNKS >= valid) ko = vo = DEAD_OFFSET;
-      lds_dma16(kr, (IRIS_LDS void*)&lds[stage][0][wave * 16 * C::ROW_BYTES + i * 1024], ko, k_at);
-      lds_dma16(vr, (IRIS_LDS void*)&lds[stage][1][wave * 16 * C::ROW_BYTES + i * 1024], vo, v_at);
+      for (int i = 0; i < C::DMAS; ++i) dma(i, k_off[i], v_off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::DMAS; ++i) {
+        const bool there = i * C::DMA_ROWS + lane / C::CHUNKS < valid;
+        dma(i, there ? k_off[i] : DEAD_OFFSET, there ? v_off[i] : DEAD_OFFSET);
+      }
     }
   };
   // where the lane reads: keys by row, values by groups of four keys
@@ -240,6 +261,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   }
   auto next_stage = [&](int j) {
     IRIS_WAIT_VMCNT(0);  // this wave's share of the tile has arrived; behind the barrier everyone's has
+    const int base = list.tile(j) * BT;
+    if (base + BT - 1 > rows_first || (a.window > 0 && rows_last - base >= a.window && base + BT > a.sinks)) {
+      // some rows must not see some of the tile's values: is any among the wave's share of them not a finite number?
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 most = {0, 0};
+#pragma unroll
+      for (int i = 0; i < C::DMAS; ++i) {
+        const u32x4 v = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)lds[j & 1][1] + wave * 16 * C::ROW_BYTES + i * 1024 + lane * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[w] & 0x7FFF7FFFu));
+      }
+      constexpr unsigned short INF = DT == IRIS_DTYPE_BF16 ? 0x7F80 : 0x7C00;
+      poisoned |= most[0] >= INF || most[1] >= INF;
+    }
     block_barrier_raw();
     if (j + 1 < j1) {
       fetch(j + 1, page, (j + 1) & 1);
@@ -275,21 +310,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
     const int base = list.tile(j) * BT;
     if (base + BT - 1 > wave_first || (a.window > 0 && wave_last - base >= a.window && base + BT > a.sinks)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        // the keys that the row sees as bits, those of the lane from bit 0 on: two instructions a score
+        const uint32_t mask = visible(a, at, base + 32 * u) >> (4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!sees(a, at, base + u * 32 + 8 * (r / 4) + 4 * half + r % 4)) s[u][r] = -INFINITY;
-      // is a value among the tile's, some of which some rows must not see, not a finite number?
-      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-      u16x2 most = {0, 0};
-#pragma unroll 1
-      for (int i = 0; i < C::TILE_BYTES; i += 1024) {
-        const u32x4 v = *(const IRIS_LDS u32x4*)((const IRIS_LDS char*)lds[j & 1][1] + i + lane * 16);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[w] & 0x7FFF7FFFu));
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t keep = (uint32_t)((int)(mask << (31 - (8 * (r / 4) + r % 4))) >> 31);
+          const float score = s[u][r];  // (a bit_cast of a vector's element would read its first)
+          s[u][r] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, score) & keep) | (~keep & 0xFF800000u));
+        }
       }
-      constexpr unsigned short INF = DT == IRIS_DTYPE_BF16 ? 0x7F80 : 0x7C00;
-      poisoned |= most[0] >= INF || most[1] >= INF;
     }
   };
   // The weights, against the reference as it stands.
@@ -309,7 +339,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
         p[2 * u + i] = u32x4{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[e] = add_weights<DT>(p[2 * u + i][e], sums[e]);
-        if (a.lse) {
+        if (LSE) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) exact += w[e];
         }
@@ -450,7 +480,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) __attribute__((amdgpu_waves_per_eu(2
   // (a page outside the cache: every number of the rows is NaN)
   const float inv = flags != 0.f ? flags : l == 0.f ? 0.f : 1.f / l;
   const int64_t out_token = token0 + token;
-  if (a.lse && half == 0)
+  if (LSE && half == 0)
     a.lse[out_token * a.stride_lse + qhead] = flags != 0.f ? flags : lse_l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(lse_l)) * 0.6931471805599453f;
   IRIS_GLOBAL char* out = (IRIS_GLOBAL char*)a.out + (out_token * a.stride_ot + (int64_t)qhead * a.stride_oh) * 2;
 #pragma unroll
