@@ -114,7 +114,7 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
       rows::decode_kernel<dt.value, dp.value, pg.value><<<(int)grid, threads, 0, s>>>(g);
       return hipGetLastError();
     }
-    if constexpr (dt.value != IRIS_DTYPE_F32 && dp.value <= 128 && pg.value) {
+    if constexpr (dt.value != IRIS_DTYPE_F32 && pg.value) {
       const int64_t row_tiles = (int64_t)a.tokens * g.group / tiles::ROWS + a.requests;
       // (a page's rows are addressed with 32 bits)
       const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;

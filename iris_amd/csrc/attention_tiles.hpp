@@ -24,7 +24,7 @@ constexpr int AHEAD = 4;
 constexpr int SCHED_MFMA = 0x8, SCHED_DS_READ = 0x100;  // kinds of instructions of __builtin_amdgcn_sched_group_barrier
 
 // As many as their registers let in.  (Heads of 64, a window of 1024: two 58 us, three 55, four 77, for they spill.)
-constexpr int waves_a_simd(int dp) { return dp == 64 ? 3 : 2; }
+constexpr int waves_a_simd(int dp) { return dp == 64 ? 3 : dp == 128 ? 2 : 1; }
 
 template <int DT, int DP>
 struct Cfg {
