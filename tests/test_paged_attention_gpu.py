@@ -393,3 +393,83 @@ def test_nothing_to_do():
     attention.decode_attention(q, cache[:0], cache[:0], torch.zeros((2, 1), dtype=torch.int32, device="cuda"),
                                torch.zeros(2, dtype=torch.int32, device="cuda"), out)
     assert bool((out == 0).all())
+
+
+# ---- many prompts, against the definition on the GPU ---------------------------
+
+
+def dense_on_gpu(p):
+    """The definition in 64 bits with whole score matrices, one head at a time: for problems too large for the CPU's."""
+    hq, hk, d = p.shape
+    out, at = [], 0
+    for i, n in enumerate(p.lengths):
+        new = p.news[i]
+        q, k, v = p.q[at:at + new].double(), p.k[i].double().cuda(), p.v[i].double().cuda()
+        rows, keys = torch.arange(n - new, n, device="cuda")[:, None], torch.arange(n, device="cuda")
+        heads = []
+        for h in range(hq):
+            s = (q[:, h] @ k[:, h // (hq // hk)].T) * d ** -0.5
+            weights = torch.softmax(s.masked_fill(~R.sees(rows, keys, p.window, p.sinks), -math.inf), -1)
+            heads.append((weights @ v[:, h // (hq // hk)], weights @ v[:, h // (hq // hk)].abs()))
+        out.append(tuple(torch.stack([h[j] for h in heads], 1) for j in (0, 1)))
+        at += new
+    return tuple(torch.cat([o[j] for o in out]).cpu() for j in (0, 1))
+
+
+@pytest.mark.parametrize("lengths,news,hq,hk,dim,dtype,window", [
+    # more row tiles than run at once: those that see the most keys start first
+    ([900, 700, 1300, 64, 2000], [900, 500, 300, 64, 1999], 40, 8, 128, BF16, 0),
+    ([800, 1500, 700], [800, 1500, 1], 48, 8, 64, F16, 0),
+    ([2100], [2100], 36, 4, 64, BF16, 200),
+    ([700, 650], [600, 650], 32, 4, 256, BF16, 0),
+])
+def test_more_prompts_than_run_at_once(lengths, news, hq, hk, dim, dtype, window):
+    p = Problem(lengths, news, hq, hk, dim, dtype, 16, window=window, sinks=3 if window else 0)
+    p.launch()
+    assert p.word.item() == 0
+    want, spread = dense_on_gpu(p)
+    off, bound = (p.out.double().cpu() - want).abs(), R.attention_error(dtype, want, spread, dim)
+    assert bool((off <= bound).all()), f"off by up to {(off / bound).max().item()} times the bound"
+    first = p.out.clone()
+    p.launch()
+    assert torch.equal(p.out, first)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 256), (F32, 64)])
+def test_a_page_outside_the_cache_is_reported_for_prompts(dtype, dim):
+    for lengths, news in (([300, 300], [300, 300]), ([3000, 3000], [40, 40])):  # (the second: keys split over workgroups)
+        p = Problem(lengths, news, 4, 1, dim, dtype, 16)
+        p.table[1, 5] = 1 << 30
+        p.launch()
+        assert p.word.item() == attention.STATUS_BAD_INDEX
+        at = news[0]
+        reached = 5 * 16 - (lengths[1] - news[1])  # the first query that sees the page
+        assert bool(p.out[at + max(reached, 0):].isnan().all())
+        assert not bool(p.out[:at].isnan().any())
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+def test_values_that_are_no_numbers_where_keys_are_split(dtype, dim):
+    n, new = 2500, 40
+    p = Problem([n], [new], 4, 1, dim, dtype, 16)
+    p.v_cache[p.table[0, (n - 20) // 16], (n - 20) % 16, 0, 1] = math.nan
+    p.v[0][n - 20, 0, 1] = math.nan
+    p.launch()
+    p.check(skip=lambda request, at: at >= n - 20)
+    assert bool(p.out[new - 20:, :, 1].isnan().all()) and bool(p.out[new - 20:, :, 2:].isfinite().all())
+
+
+def test_scores_that_grow_along_the_context():
+    """Each stretch of keys outweighs those before it: the reference of the weights moves again and again."""
+    for dtype, new in ((F16, 70), (BF16, 70), (F16, 1)):
+        n, d = 700, 64
+        p = Problem([n], [new], 1, 1, d, dtype, 16)
+        p.q_host[:] = 0
+        p.q_host[..., 0] = 16
+        p.q.copy_(p.q_host)
+        p.k[0][..., 0] = (torch.arange(n) // 50).to(dtype)[:, None]  # two more a stretch, 28 in all
+        for j in range(R.cdiv(n, 16)):
+            part = p.k[0][16 * j:16 * j + 16].cuda()
+            p.k_cache[p.table[0, j], :len(part)] = part
+        p.launch()
+        p.check()
