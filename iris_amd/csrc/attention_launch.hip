@@ -114,18 +114,29 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
       rows::decode_kernel<dt.value, dp.value, pg.value><<<(int)grid, threads, 0, s>>>(g);
       return hipGetLastError();
     }
+    const int64_t few_tiles = (int64_t)a.tokens * g.group / rows::ROWS + a.requests, few_units = few_tiles * a.k_heads;  // of 16 rows
     if constexpr (dt.value != IRIS_DTYPE_F32 && pg.value) {
+      // Tiles of 128 rows read keys once for all of them, tiles of 16 fill the chip with fewer rows and end sooner.  us in tiles of 128 /
+      // of 16, bf16, 8 + 1 heads of 128 unless stated.  By rows a request: 64 requests behind up to 4096 tokens, 19 rows each
+      // 41 / 37, 27 each 41 / 46, 42 each 42 / 49.  By 16-row units and the most keys a row may see: 102 x 200 11.3 / 7.7,
+      // 93 x 2004 20.5 / 17.2, 201 x 400 16.4 / 10.9, 460 x 500 17.1 / 13.4, 57 x 8001 31 / 26; 501 x 1000 20.2 / 20.5,
+      // 188 x 4113 29 / 39, 268 x 2001 (4 + 4 heads) 27 / 37, 55 x 46398 79 / 86; 537 x 180 12.6 / 14.1.
+      const bool few_rows = (int64_t)a.tokens * g.group <= 24 * (int64_t)a.requests ||
+                            (few_units <= 2 * cus && few_units * most_keys <= (int64_t)1536 * cus);
       const int64_t row_tiles = (int64_t)a.tokens * g.group / tiles::ROWS + a.requests;
       // (a page's rows are addressed with 32 bits)
       const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
-      if ((int64_t)a.tokens * g.group > 32 * (int64_t)a.requests && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX &&
+      if (!few_rows && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX &&
           a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
         const int64_t units = row_tiles * a.k_heads, places = tiles::waves_a_simd(dp.value) * cus;
+        // Where places are left, several take a row tile, of four tiles of keys each or more.  (One prompt of 1000 tokens, us in one part / of
+        // four / of two key tiles: 28 / 20 / 26; of 2000: 49 / 34 / 34.)
         int64_t splits = 1;
         if (2 * units <= places && units <= rows::LATER) {
           splits = places / units;
           const int64_t room_for = slots * row_slot(a.head_dim) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
           if (splits > most_keys / (4 * tiles::BT)) splits = most_keys / (4 * tiles::BT);
+          if (splits > tiles::MOST_PARTS) splits = tiles::MOST_PARTS;
           if (splits > room_for) splits = room_for;
           if (splits < 1) splits = 1;
         }
@@ -139,19 +150,19 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
         return hipGetLastError();
       }
     }
-    const int64_t row_tiles = (int64_t)a.tokens * g.group / rows::ROWS + a.requests;
-    const int64_t units = row_tiles * a.k_heads;
+    // (8 prompts of up to 4 tokens behind up to 4096, us in one part / as many as make one / two workgroups a CU: 65 / 15 / 16; fp32, a
+    // prompt of 500: 25 / 19 / 19; more a CU the same)
     int64_t splits = 1;
-    if (units < 2 * cus && units <= rows::LATER) {
-      splits = 2 * cus / units;
+    if (few_units < 2 * cus && few_units <= rows::LATER) {
+      splits = 2 * cus / few_units;
       if (splits > most_keys / (2 * C::BT)) splits = most_keys / (2 * C::BT);
-      if (splits > slots / units) splits = slots / units;
+      if (splits > slots / few_units) splits = slots / few_units;
       if (splits > rows::FLAT) splits = rows::FLAT;
       if (splits < 1) splits = 1;
     }
     g.splits = (int)splits;
-    if (row_tiles * splits > INT32_MAX || a.k_heads > 65535) return hipErrorInvalidValue;
-    rows::prompt_rows_kernel<dt.value, dp.value, pg.value><<<dim3((unsigned)(row_tiles * splits), a.k_heads), threads, 0, s>>>(g);
+    if (few_tiles * splits > INT32_MAX || a.k_heads > 65535) return hipErrorInvalidValue;
+    rows::prompt_rows_kernel<dt.value, dp.value, pg.value><<<dim3((unsigned)(few_tiles * splits), a.k_heads), threads, 0, s>>>(g);
     return hipGetLastError();
   });
 }

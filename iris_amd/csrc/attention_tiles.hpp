@@ -18,9 +18,12 @@
 namespace iris_amd {
 namespace tiles {
 
-
 constexpr int WAVES = 4, ROWS = 128, WAVE_ROWS = 32, BT = 64;
-constexpr int AHEAD = 4;
+constexpr int AHEAD = 4;  // operands in flight ahead of the matrix instructions (three, four or six: the same time)
+// Parts of a row tile's keys: of no fewer than LEAST tiles (rows that see few keys are not cut as the longest are: 8 prompts of up to
+// 32 tokens behind up to 4096, 40.5 us for 41.9), and no more than MOST_PARTS, for the last adds them up one by one (8 of up to
+// 30 behind up to 8000, us at 4 / 8 / 16 / 31 parts: 51 / 35 / 31 / 53).
+constexpr int LEAST = 2, MOST_PARTS = 16;
 constexpr int SCHED_MFMA = 0x8, SCHED_DS_READ = 0x100;  // kinds of instructions of __builtin_amdgcn_sched_group_barrier
 
 // As many as their registers let in.  (Heads of 64, a window of 1024: two 58 us, three 55, four 77, for they spill.)
@@ -69,9 +72,10 @@ __device__ inline uint32_t visible(const iris_attention_args& a, int at, int bas
 }
 
 // The row tile that sees the k-th most keys (no window), later rows before earlier ones: workgroups that start last are then the
-// short ones.  (A prompt of 8192 tokens among others, 1153 row tiles of 1 to 128 key tiles on 512 places: 345 us in the requests'
-// order, BALANCED_US by length.)  Request r has tiles_r row tiles, and of those that see at least c key tiles the number is known in closed form;
-// the largest c with more than k of them in all is found by bisection, the lanes adding up the requests.
+// short ones.  (A prompt of 8192 tokens among others, 1153 row tiles of 1 to 128 key tiles on 512 places: 396 us in the requests'
+// order, 334 by length; one such prompt alone 209 and 191.)  Request r has tiles_r row tiles, and of those that see at least c
+// key tiles the number is known in closed form; the largest c with more than k of them in all is found by bisection, the
+// lanes adding up the requests.
 __device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request, int* row_tile) {
   const iris_attention_args& a = g.a;
   const int lane = threadIdx.x & 63;
@@ -160,7 +164,9 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
   const int rows_first = first + row0 / g.group, rows_last = first + (row0 + num_rows - 1) / g.group;
   const KeyTiles list = key_tiles<BT>(a, rows_first, rows_last);
   // the workgroup's share of the tiles
-  const int j0 = (int)((int64_t)list.count * split / g.splits), j1 = (int)((int64_t)list.count * (split + 1) / g.splits);
+  const int parts = max(min(g.splits, list.count / LEAST), 1);
+  if (split >= parts) return;
+  const int j0 = (int)((int64_t)list.count * split / parts), j1 = (int)((int64_t)list.count * (split + 1) / parts);
 
   // the lane's row
   const int wrow = wave * WAVE_ROWS;
@@ -400,7 +406,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
   // what one wave found is every row's
   bool redo = __syncthreads_or(poisoned);
   float flags = __syncthreads_or(bad_page) ? __builtin_nanf("") : 0.f;
-  if (g.splits > 1) {
+  if (parts > 1) {
     // The parts meet in the workspace, each in the order of its registers: the last to arrive has the rows of all in the same lanes.
     const int unit = x * a.k_heads + head;
     auto slot = [&](int part) { return (IRIS_GLOBAL char*)(g.slots + ((int64_t)unit * g.splits + part) * C::SLOT); };
@@ -419,7 +425,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
     int last = 0;
     if (tid == 0) {
       IRIS_GLOBAL int32_t* count = (IRIS_GLOBAL int32_t*)(g.counters + unit);
-      last = arrive(count, false, false) == g.splits - 1;
+      last = arrive(count, false, false) == parts - 1;
       if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (!__syncthreads_or(last)) return;
@@ -430,7 +436,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
     ref = -INFINITY;
     l = lse_l = 0.f;
     bool bad = false, again = false;
-    for (int part = 0; part < g.splits; ++part) {
+    for (int part = 0; part < parts; ++part) {
       const __amdgpu_buffer_rsrc_t rs = tile_rsrc(slot(part), C::SLOT * 4);
       const f32x4 m = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)mine, C::DTILES * 4 * (WAVES * 1024), AUX_SC1));
       const float next = fmaxf(ref, m[0]), from = next == -INFINITY ? 0.f : next;

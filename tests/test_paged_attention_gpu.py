@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 class Problem:
     """Requests with ``lengths`` keys and ``news`` queries each (None: one each), in a cache whose other places hold NaN."""
 
-    def __init__(self, lengths, news, hq, hk, d, dtype, page, *, window=0, sinks=0, seed=0, heads_first=False, fused=False, spare=3):
+    def __init__(self, lengths, news, hq, hk, d, dtype, page, *, window=0, sinks=0, seed=0, heads_first=False, fused=False, spare=3, room=2):
         self.lengths, self.news, self.dtype, self.window, self.sinks = lengths, news, dtype, window, sinks
         self.shape = (hq, hk, d)
         g = torch.Generator().manual_seed(seed)
@@ -30,7 +30,7 @@ class Problem:
         random.Random(seed).shuffle(order)
         shape = (pages, hk, page, d) if heads_first else (pages, page, hk, d)
         caches = [torch.full(shape, math.nan, dtype=dtype) for _ in range(2)]
-        width = max(counts + [1]) + 2
+        width = max(counts + [1]) + room
         table = torch.full((len(lengths), width), 1 << 30, dtype=torch.int32)  # (entries past a request's pages are not read)
         at = 0
         for i, n in enumerate(counts):
@@ -252,58 +252,67 @@ def test_decode_addresses_past_32_bits():
 
 
 # ---- prompts -----------------------------------------------------------------
+# (Few rows of few keys at most go in tiles of 16 rows; block tables with room for more keys take the same problems to tiles of 128.)
+
+@pytest.fixture(params=[2, 30000], ids=["tight", "roomy"])
+def room(request):
+    return request.param
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("dim", [64, 128, 256, 80, 96, 192])
-def test_prompt_types_and_head_sizes(dtype, dim):
-    run([70, 33, 1, 0, 150], [70, 5, 1, 0, 1], 4, 2, dim, dtype, 16)
+def test_prompt_types_and_head_sizes(dtype, dim, room):
+    run([70, 33, 1, 0, 150], [70, 5, 1, 0, 1], 4, 2, dim, dtype, 16, room=room)
 
 
 @pytest.mark.parametrize("hq,hk", [(1, 1), (4, 4), (3, 1), (8, 1), (7, 1), (16, 1), (20, 1), (6, 2)])
-def test_prompt_heads(hq, hk):
-    run([90, 20], [40, 20], hq, hk, 64, BF16, 32)
+def test_prompt_heads(hq, hk, room):
+    run([90, 20], [40, 20], hq, hk, 64, BF16, 32, room=room)
 
 
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 20, 64])
 @pytest.mark.parametrize("heads_first", [False, True])
-def test_prompt_pages(page, heads_first):
-    run([150, 31, 64], [130, 31, 2], 2, 1, 128, BF16, page, heads_first=heads_first)
+def test_prompt_pages(page, heads_first, room):
+    run([150, 31, 64], [130, 31, 2], 2, 1, 128, BF16, page, heads_first=heads_first, room=room)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (50, 70), (64, 64), (200, 5)])
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_prompt_window_and_first_tokens(window, sinks, dtype):
-    run([260, 100, 7], [260, 30, 7], 4, 2, 64, dtype, 16, window=window, sinks=sinks)
+@pytest.mark.parametrize("hq,hk", [(4, 2), (32, 16)])  # (tiles of 16 rows, and of 128)
+def test_prompt_window_and_first_tokens(window, sinks, dtype, hq, hk):
+    run([260, 100, 7], [260, 30, 7], hq, hk, 64, dtype, 16, window=window, sinks=sinks)
 
 
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 64), (F16, 128), (BF16, 96)])
-def test_prompts_of_many_tiles(dtype, dim):
-    run([700, 513], [700, 257], 2, 1, dim, dtype, 16)
+def test_prompts_of_many_tiles(dtype, dim, room):
+    run([700, 513], [700, 257], 2, 1, dim, dtype, 16, room=room)
     run([700, 513], [700, 257], 2, 1, dim, dtype, 16, window=100, sinks=3)
+    run([700, 513], [700, 257], 10, 5, dim, dtype, 16, window=100, sinks=3)
 
 
-def test_prompt_pieces_behind_a_long_context():
-    run([5000, 3000], [9, 64], 4, 1, 128, BF16, 16)
-    run([5000, 3000], [9, 64], 4, 1, 128, BF16, 16, workspace=None)
+def test_prompt_pieces_behind_a_long_context(room):
+    run([5000, 3000], [9, 64], 4, 1, 128, BF16, 16, room=room)
+    run([5000, 3000], [9, 64], 4, 1, 128, BF16, 16, workspace=None, room=room)
+    run([5000, 3500], [300, 310], 4, 1, 64, F16, 16, window=3000, sinks=4, room=room)
     run([5000, 3000], [9, 64], 4, 1, 64, F16, 16, window=900, sinks=4)
 
 
-def test_prompt_of_more_queries_than_keys_leaves_rows_empty():
-    p = run([3, 40], [10, 12], 2, 1, 64, BF16, 16)
+def test_prompt_of_more_queries_than_keys_leaves_rows_empty(room):
+    p = run([3, 40], [10, 12], 2, 1, 64, BF16, 16, room=room)
     assert bool((p.out[:7] == 0).all())
-    run([0, 40], [4, 12], 2, 1, 128, BF16, 16)
+    run([0, 40], [4, 12], 2, 1, 128, BF16, 16, room=room)
 
 
 @pytest.mark.parametrize("window", [0, 40])
 @pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 128), (F32, 64), (BF16, 192)])
-def test_a_value_that_is_no_number_reaches_only_the_queries_that_see_it(dtype, dim, window):
+@pytest.mark.parametrize("hq,hk", [(2, 1), (64, 32)])
+def test_a_value_that_is_no_number_reaches_only_the_queries_that_see_it(dtype, dim, window, hq, hk, room):
     n = 150
-    p = Problem([n], [n], 2, 1, dim, dtype, 16, window=window)
+    p = Problem([n], [n], hq, hk, dim, dtype, 16, window=window, room=room)
     bad = {60: math.nan, 100: math.inf, 101: -math.inf, n - 1: math.nan}
     for key, value in bad.items():
-        p.v_cache[p.table[0, key // 16], key % 16, 0, ::2] = value
-        p.v[0][key, 0, ::2] = value
+        p.v_cache[p.table[0, key // 16], key % 16, :, ::2] = value
+        p.v[0][key, :, ::2] = value
     p.launch()
 
     def reached(request, at):
@@ -315,17 +324,17 @@ def test_a_value_that_is_no_number_reaches_only_the_queries_that_see_it(dtype, d
     assert bool((~out[touched][..., ::2].isfinite()).all()) and bool(out[..., 1::2].isfinite().all())
 
 
-def test_a_key_that_is_no_number_reaches_only_the_queries_that_see_it():
+def test_a_key_that_is_no_number_reaches_only_the_queries_that_see_it(room):
     n = 140
-    p = Problem([n], [n], 2, 1, 64, BF16, 16)
+    p = Problem([n], [n], 2, 1, 64, BF16, 16, room=room)
     p.k_cache[p.table[0, 90 // 16], 90 % 16] = math.nan
     p.launch()
     p.check(skip=lambda request, at: at >= 90)
     assert bool(p.out[90:].isnan().all())
 
 
-def test_prompt_views_padding_and_repeats():
-    p = Problem([200, 90], [150, 90], 6, 2, 128, BF16, 16, fused=True)
+def test_prompt_views_padding_and_repeats(room):
+    p = Problem([200, 90], [150, 90], 6, 2, 128, BF16, 16, fused=True, room=room)
     pad = 20  # tokens of no request behind the last one's
     q, out = torch.zeros((260, 6, 128), dtype=BF16, device="cuda"), torch.full((260, 6, 128), -7.0, dtype=BF16, device="cuda")
     lse = torch.full((260, 6), -7.0, device="cuda")
@@ -419,7 +428,7 @@ def dense_on_gpu(p):
 @pytest.mark.parametrize("lengths,news,hq,hk,dim,dtype,window", [
     # more row tiles than run at once: those that see the most keys start first
     ([900, 700, 1300, 64, 2000], [900, 500, 300, 64, 1999], 40, 8, 128, BF16, 0),
-    ([800, 1500, 700], [800, 1500, 1], 48, 8, 64, F16, 0),
+    ([800, 1500, 700], [800, 1500, 1], 40, 8, 64, F16, 0),
     ([2100], [2100], 36, 4, 64, BF16, 200),
     ([700, 650], [600, 650], 32, 4, 256, BF16, 0),
 ])
@@ -436,9 +445,9 @@ def test_more_prompts_than_run_at_once(lengths, news, hq, hk, dim, dtype, window
 
 
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (BF16, 256), (F32, 64)])
-def test_a_page_outside_the_cache_is_reported_for_prompts(dtype, dim):
+def test_a_page_outside_the_cache_is_reported_for_prompts(dtype, dim, room):
     for lengths, news in (([300, 300], [300, 300]), ([3000, 3000], [40, 40])):  # (the second: keys split over workgroups)
-        p = Problem(lengths, news, 4, 1, dim, dtype, 16)
+        p = Problem(lengths, news, 4, 1, dim, dtype, 16, room=room)
         p.table[1, 5] = 1 << 30
         p.launch()
         assert p.word.item() == attention.STATUS_BAD_INDEX
@@ -449,9 +458,9 @@ def test_a_page_outside_the_cache_is_reported_for_prompts(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
-def test_values_that_are_no_numbers_where_keys_are_split(dtype, dim):
+def test_values_that_are_no_numbers_where_keys_are_split(dtype, dim, room):
     n, new = 2500, 40
-    p = Problem([n], [new], 4, 1, dim, dtype, 16)
+    p = Problem([n], [new], 4, 1, dim, dtype, 16, room=room)
     p.v_cache[p.table[0, (n - 20) // 16], (n - 20) % 16, 0, 1] = math.nan
     p.v[0][n - 20, 0, 1] = math.nan
     p.launch()
@@ -459,11 +468,11 @@ def test_values_that_are_no_numbers_where_keys_are_split(dtype, dim):
     assert bool(p.out[new - 20:, :, 1].isnan().all()) and bool(p.out[new - 20:, :, 2:].isfinite().all())
 
 
-def test_scores_that_grow_along_the_context():
+def test_scores_that_grow_along_the_context(room):
     """Each stretch of keys outweighs those before it: the reference of the weights moves again and again."""
     for dtype, new in ((F16, 70), (BF16, 70), (F16, 1)):
         n, d = 700, 64
-        p = Problem([n], [new], 1, 1, d, dtype, 16)
+        p = Problem([n], [new], 1, 1, d, dtype, 16, room=room)
         p.q_host[:] = 0
         p.q_host[..., 0] = 16
         p.q.copy_(p.q_host)
