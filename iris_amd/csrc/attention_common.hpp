@@ -11,7 +11,7 @@ struct AttentionKArgs {
   float scale_log2;   // scale * log2(e): scores are exponents of two
   int group;          // query heads to a key head
   int splits;         // parts of a unit's keys (prompts)
-  int by_length;      // rows that see the most keys start first (prompts in tiles)
+  int by_length;      // rows that see the most keys start first (prompts in tiles): row tiles that take one place a CU; 0: no order
   int grid_units;     // workgroups that share the work (decode)
   float* slots;       // partial results, `slot_elems` floats each
   int32_t* counters;  // arrivals at split units; zero between launches

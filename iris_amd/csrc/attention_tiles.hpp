@@ -11,6 +11,12 @@
 // Tiles go from the pages to LDS by LDS-DMA, 16 bytes a lane, two stages, with the 16-byte chunks of a row exchanged
 // (XOR) so that neither read meets its own banks; keys past the end and columns past the head are read out of
 // the buffer's range and arrive as zeros.
+//
+// bf16, heads of 128, four prompts of up to 8192 tokens (310 GFLOP): 332 us, 0.93 PFLOP/s, where a large matrix product runs at
+// 1.19; fp16, heads of 64, a window of 1024 (25 GFLOP): 52 us, 0.47.  The matrix cores are busy for 0.40 of the time and
+// vector instructions issue for 0.32, the one wave's beside the other's; the rest is LDS reads, barriers and
+// power (zeros take an eighth less).  Tiles of 64 rows a wave, or a tile's scores taken ahead of the last one's values, took
+// more registers than there are and 394 us and more.
 #pragma once
 
 #include "attention_rows.hpp"
@@ -71,9 +77,10 @@ __device__ inline uint32_t visible(const iris_attention_args& a, int at, int bas
   return a.window > 0 ? past & (~below(at - a.window + 1 - base) | below(a.sinks - base)) : past;
 }
 
-// The row tile that sees the k-th most keys (no window), later rows before earlier ones: workgroups that start last are then the
-// short ones.  (A prompt of 8192 tokens among others, 1153 row tiles of 1 to 128 key tiles on 512 places: 396 us in the requests'
-// order, 334 by length; one such prompt alone 209 and 191.)  Request r has tiles_r row tiles, and of those that see at least c
+// The row tile that sees the k-th most keys, later rows before earlier ones: workgroups that start last are then the
+// short ones.  (A prompt of 8192 tokens among others, 1153 row tiles of 1 to 128 key tiles on 512 places: 382 us in the requests'
+// order, 336 by length; with a window, 796 row tiles of heads of 64 on 768, 54.8 and 52.3; heads of 256, a prompt of
+// 6000, 320 and 279.)  Request r has tiles_r row tiles, and of those that see at least c
 // key tiles the number is known in closed form; the largest c with more than k of them in all is found by bisection, the
 // lanes adding up the requests.
 __device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request, int* row_tile) {
@@ -91,7 +98,9 @@ __device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request,
     own.first = (int)min((int64_t)max(a.lengths[lane], 0), (int64_t)a.table_width * g.page.d) - tokens;
     own.tiles = (int)((own.rows + ROWS - 1) / ROWS);
   }
-  auto at_least = [&](int c) {  // its row tiles that see at least c key tiles
+  const int all = (int)(((int64_t)a.table_width * g.page.d + BT - 1) / BT), most = a.window > 0 ? min(all, a.window / BT + 1) : all;
+  auto at_least = [&](int c) {  // its row tiles that see at least c key tiles (a window: `most` and more are one)
+    if (c > most) return 0;
     const int64_t q = ((int64_t)(c - 1) * BT - own.first) * g.group;
     return c <= 0 || q <= 0 ? own.tiles : own.rows <= q ? 0 : own.tiles - (int)(q / ROWS);
   };
@@ -102,7 +111,7 @@ __device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request,
   };
   if (k >= sum_of(own.tiles)) return false;
   int lo = 0;
-  for (int hi = (int)(((int64_t)a.table_width * g.page.d + BT - 1) / BT) + 1; hi - lo > 1;) {
+  for (int hi = most + 1; hi - lo > 1;) {
     const int mid = (lo + hi) / 2;
     if (sum_of(at_least(mid)) > k)
       lo = mid;
@@ -136,7 +145,11 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
   const int item = blockIdx.x / a.k_heads, head = blockIdx.x - item * a.k_heads, x = item / g.splits, split = item - x * g.splits;
   int request, row_tile;
   if (g.by_length) {
-    if (!nth_longest(g, x, &request, &row_tile)) return;
+    // Of those that take one place a CU every other batch is turned round: beside the longest runs the shortest of the next.  (One prompt
+    // of 8192 tokens, 512 row tiles: 199 us without, 189 with.)
+    const int batch = x / g.by_length, first_of = batch * g.by_length;
+    const int k = batch % 2 ? first_of + min(g.by_length, (int)gridDim.x / a.k_heads - first_of) - 1 - (x - first_of) : x;
+    if (!nth_longest(g, k, &request, &row_tile)) return;
   } else {
     // x counts row tiles with room for each request's, without a sum over the requests: request r's begin at bound(r).
     auto bound = [&](int r) { return (int)((int64_t)scalar_at(a.query_starts, r) * g.group / ROWS) + r; };

@@ -10,8 +10,8 @@
 // The work is one read and one write of each head, so it is bound by memory: a head is held by the fewest lanes that
 // load it eight elements each, as two runs of four of which one holds a pair's first and one its second elements, so
 // that no rotation crosses lanes; the norm is the only exchange, within 16 lanes by DPP.  A lane keeps its angles for the heads of
-// its token that it has.  bf16, heads of 128: 8191 tokens of 8 + 2 + 2 heads (54.6 MB) in 13.1 us, 4.2 TB/s, a copy of
-// 4 GB runs at 4.9; the gradient of 8192 tokens of 32 + 8 heads (256 MB) in 55.8 us, 4.6 TB/s.  (Loads unpacked as they
+// its token that it has.  bf16, heads of 128: 8191 tokens of 8 + 2 + 2 heads (54.6 MB) in 11.9 us, 4.6 TB/s, a copy of
+// 4 GB runs at 4.9; the gradient of 8192 tokens of 32 + 8 heads (256 MB) in 55.6 us, 4.6 TB/s.  (Loads unpacked as they
 // arrive and both weights in one workgroup took 208 registers and 105 us for the latter.)
 #include <type_traits>
 
