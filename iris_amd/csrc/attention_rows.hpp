@@ -456,30 +456,52 @@ struct Unit {
   // Adds the parts first, first + step, ... (`count` of them, no more than MEET): into the output, or back into the first one's slot.
   // LANES lanes hold a row, and the first `count` of them (of LANES twice or four times in turn) its parts' maxima and sums, from
   // which every part's weight follows at once; where there are few rows, sets of lanes take every so many-th part's output
-  // and add up in LDS.  Fixed orders all the way.
+  // and add up in LDS.  Fixed orders all the way.  Heads of 256 load 16 bytes and 16 parts at once (two requests of up to 16602 keys,
+  // 16 rows: 32.7 us, 37.6 with 8); for shorter ones that costs the rest of the kernel as much as it gives (606 MB in heads of 128
+  // 121 us for 118.5, one request of 1999 keys 11.0 for 10.3).
   __device__ inline void join(const Piece& p, int first, int step, int count, bool whole) {
-    constexpr int LANES = DP / 4, GROUPS = WAVES * 64 / LANES, AT_ONCE = 8, HOLD = (MEET + LANES - 1) / LANES;
+    constexpr int LANES = DP / 4, GROUPS = WAVES * 64 / LANES, AT_ONCE = DP == 256 ? FAN : 8, HOLD = (MEET + LANES - 1) / LANES;
     int abreast = 1;  // rows that are worked on at once
     while (abreast < p.rows && abreast < GROUPS) abreast *= 2;
     const int sets = GROUPS / abreast, group = threadIdx.x / LANES, set = group / abreast, in_row = threadIdx.x % LANES, d = in_row * 4;
     float* const flat = &lds.o[0][0][0];         // sets' sums
     float* const weights = flat + GROUPS * DP;   // the groups' weights of the parts
-    for (int row0 = 0; row0 < p.rows; row0 += abreast) {
-      const int row = row0 + group % abreast, used = min(row, p.rows - 1);  // (groups without a row repeat the last)
-      auto slot = [&](int i) { return (const char*)(g.slots + (int64_t)slot_of(p, first + i * step) * C::SLOT); };
-      f32x4 ml[HOLD];
+    // What other workgroups have written through, 16 bytes at float `at` of part i.  (The parts of a launch lie within 31 bits: at most
+    // two a workgroup or 24 a unit of 512.)
+    auto load_slot = [&](int i, int at) {
+      const int64_t word = (int64_t)slot_of(p, first + i * step) * C::SLOT + at;
+      if constexpr (DP == 256) {
+        const __amdgpu_buffer_rsrc_t slots = tile_rsrc((const IRIS_GLOBAL char*)g.slots, 0x7FFFFFFF);
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(slots, (int)word * 4, 0, AUX_SC1));
+      } else {
+        const IRIS_GLOBAL uint64_t* at16 = (const IRIS_GLOBAL uint64_t*)(g.slots + word);
+        const u32x2 lo = __builtin_bit_cast(u32x2, __hip_atomic_load(at16, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __hip_atomic_load(at16 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        return __builtin_bit_cast(f32x4, u32x4{lo[0], lo[1], hi[0], hi[1]});
+      }
+    };
+    auto row_of = [&](int row0) { return min(row0 + group % abreast, p.rows - 1); };  // (groups without a row repeat the last)
+    f32x4 ml[HOLD], next_ml[HOLD];
+    auto fetch_ml = [&](int row0) {
 #pragma unroll
       for (int i = 0; i < HOLD; ++i) {
-        ml[i] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
-        if (i * LANES + in_row < count) ml[i] = load_slot(slot(i * LANES + in_row) + (ROWS * DP + 4 * used) * 4);
+        next_ml[i] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+        if (i * LANES + in_row < count) next_ml[i] = load_slot(i * LANES + in_row, ROWS * DP + 4 * row_of(row0));
       }
+    };
+    fetch_ml(0);
+    for (int row0 = 0; row0 < p.rows; row0 += abreast) {
+      const int row = row0 + group % abreast, used = row_of(row0);
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) ml[i] = next_ml[i];
       f32x4 y[AT_ONCE];
       auto fetch = [&](int i0) {
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i)
-          if (i0 + i * sets < count) y[i] = load_slot(slot(i0 + i * sets) + (used * DP + d) * 4);
+          if (i0 + i * sets < count) y[i] = load_slot(i0 + i * sets, used * DP + d);
       };
       fetch(set);
+      if (row0 + abreast < p.rows) fetch_ml(row0 + abreast);
       float top = -INFINITY, sum = 0.f, lse_sum = 0.f;
 #pragma unroll
       for (int i = 0; i < HOLD; ++i) top = fmaxf(top, ml[i][0]);
@@ -530,12 +552,6 @@ struct Unit {
       else
         *(IRIS_GLOBAL u32x2*)out = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
     }
-  }
-  // 16 bytes that another workgroup has written through.
-  __device__ inline f32x4 load_slot(const char* p) {
-    const u32x2 lo = __builtin_bit_cast(u32x2, __hip_atomic_load((const IRIS_GLOBAL uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    const u32x2 hi = __builtin_bit_cast(u32x2, __hip_atomic_load((const IRIS_GLOBAL uint64_t*)(p + 8), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    return __builtin_bit_cast(f32x4, u32x4{lo[0], lo[1], hi[0], hi[1]});
   }
 };
 
