@@ -12,8 +12,8 @@
 //            of keys meet in a register by one byte permute each (16-bit types; none for fp32).
 // At the end the four waves' maxima, sums and outputs meet in LDS; the parts of a split unit meet in the workspace.
 //
-// Single tokens, heads of 128: 606 MB of keys and values in 118 us, 5.1 TB/s, where a copy of 4 GB runs at 4.9; 56 MB in 20.7 us,
-// of which 10 are a chain of latencies, as is all of one request's 10.5 (1999 keys, 4 MB): launch 2.4, lengths and the cut of
+// Single tokens, heads of 128: 606 MB of keys and values in 119 us, 5.1 TB/s, where a copy of 4 GB runs at 4.9; 56 MB in 20.6 us,
+// of which 10 are a chain of latencies, as is all of one request's 10.3 (1999 keys, 4 MB): launch 2.4, lengths and the cut of
 // the line 1.5, table, keys and values 2.3 a step, the waves' meeting 1, hand-over 0.8, join 2.2.
 #pragma once
 

@@ -12,8 +12,8 @@
 // (XOR) so that neither read meets its own banks; keys past the end and columns past the head are read out of
 // the buffer's range and arrive as zeros.
 //
-// bf16, heads of 128, four prompts of up to 8192 tokens (310 GFLOP): 332 us, 0.93 PFLOP/s, where a large matrix product runs at
-// 1.19; fp16, heads of 64, a window of 1024 (25 GFLOP): 52 us, 0.47.  The matrix cores are busy for 0.40 of the time and
+// bf16, heads of 128, four prompts of up to 8192 tokens (310 GFLOP): 325 to 332 us, 0.93 to 0.96 PFLOP/s, where a large matrix product runs at
+// 1.19; fp16, heads of 64, a window of 1024 (25 GFLOP): 51 to 52 us, 0.48.  The matrix cores are busy for 0.40 of the time and
 // vector instructions issue for 0.32, the one wave's beside the other's; the rest is LDS reads, barriers and
 // power (zeros take an eighth less).  Tiles of 64 rows a wave, or a tile's scores taken ahead of the last one's values, took
 // more registers than there are and 394 us and more.
