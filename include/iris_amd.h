@@ -536,6 +536,19 @@ int iris_attention_launch(const iris_attention_args* args, void* stream);
 /* Elements of a workspace with which a launch for heads of head_dim splits as it likes. */
 int64_t iris_attention_workspace_elems(int32_t head_dim);
 
+/* What iris_attention_launch does with args on num_cus compute units (0: the current device's); refuses what it refuses. */
+#define IRIS_ATTENTION_NOTHING 0      /* no query */
+#define IRIS_ATTENTION_DECODE 1       /* one token a request */
+#define IRIS_ATTENTION_PROMPT_TILES 2 /* 128 rows a workgroup */
+#define IRIS_ATTENTION_PROMPT_ROWS 3  /* 16 rows a workgroup */
+typedef struct iris_attention_plan_info {
+  int64_t workspace_elems; /* the workspace's elements that may be touched, from its start; 0: no unit is split */
+  int64_t workgroups;
+  int32_t kernel;
+  int32_t parts; /* of a prompt unit's keys, at most; single tokens are cut into one equal run a workgroup where workspace_elems is not 0 */
+} iris_attention_plan_info;
+int iris_attention_plan(const iris_attention_args* args, int32_t num_cus, iris_attention_plan_info* plan);
+
 /* Library version, bumped when a signature in this header changes. */
 int iris_amd_abi_version(void);
 

@@ -176,6 +176,15 @@ class AttentionArgs(ctypes.Structure):
     )
 
 
+class AttentionPlanInfo(ctypes.Structure):
+    """``iris_attention_plan_info``."""
+
+    _fields_ = _fields((ctypes.c_int64, "workspace_elems workgroups"), (ctypes.c_int32, "kernel parts"))
+
+
+ATTENTION_NOTHING, ATTENTION_DECODE, ATTENTION_PROMPT_TILES, ATTENTION_PROMPT_ROWS = 0, 1, 2, 3
+
+
 # every symbol include/iris_amd.h declares for libiris_amd.so:
 # name -> (restype, argtypes)
 _P = ctypes.c_void_p
@@ -216,6 +225,7 @@ SIGNATURES = {
     "iris_qk_norm_rope_backward_launch": (_I, [ctypes.POINTER(QkNormRopeBackwardArgs), _P]),
     "iris_attention_launch": (_I, [ctypes.POINTER(AttentionArgs), _P]),
     "iris_attention_workspace_elems": (ctypes.c_int64, [ctypes.c_int32]),
+    "iris_attention_plan": (_I, [ctypes.POINTER(AttentionArgs), ctypes.c_int32, ctypes.POINTER(AttentionPlanInfo)]),
     "iris_amd_abi_version": (_I, []),
 }
 ALLOCATOR_SYMBOLS = ("finegrained_hipMalloc", "finegrained_hipFree")

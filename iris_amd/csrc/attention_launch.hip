@@ -1,4 +1,4 @@
-// iris_attention_launch: checks a call, and takes the kernel for it.
+// iris_attention_launch: checks a call, plans it from the sizes that the host has, and launches the kernel that the plan names.
 #include <type_traits>
 
 #include "attention_rows.hpp"
@@ -56,6 +56,92 @@ hipError_t with_types(const iris_attention_args& a, F f) {
   return dims(integral_constant<int, IRIS_DTYPE_BF16>{});
 }
 
+// What a launch does.
+struct Plan {
+  int kernel = IRIS_ATTENTION_NOTHING;
+  int64_t workgroups = 0;
+  int64_t splits = 1;   // parts of a unit's keys (prompts)
+  int by_length = 0;    // (AttentionKArgs)
+  int64_t parted = 0;   // floats behind the workspace's counters that parts are left in; 0: no unit is split
+};
+
+template <int DT, int DP, bool PG>
+hipError_t make_plan(const iris_attention_args& a, int cus, Plan* p) {
+  using C = rows::Cfg<DT, DP>;
+  const int group = a.q_heads / a.k_heads;
+  const int64_t slots = a.workspace && a.workspace_elems > COUNTERS ? (a.workspace_elems - COUNTERS) / C::SLOT : 0;
+  // the most keys that a row may see
+  const int64_t room = (int64_t)a.table_width * a.page_size;
+  const int64_t most_keys = a.window > 0 && (int64_t)a.window + a.sinks < room ? (int64_t)a.window + a.sinks : room;
+  if (!a.query_starts) {
+    p->kernel = IRIS_ATTENTION_DECODE;
+    const int64_t units = (int64_t)a.requests * a.k_heads * ((group + rows::ROWS - 1) / rows::ROWS);
+    const int64_t line = units * ((most_keys + C::BT - 1) / C::BT + 2 + rows::REST);  // at most
+    if (line > INT32_MAX) return hipErrorInvalidValue;
+    int64_t grid = line;
+    // As many workgroups as have 64 KiB of keys and values in flight a CU; more only leave more parts to join (us at 1 / 2 / 3 a CU:
+    // heads of 128, 64 requests of up to 8192 keys 20.6 / 22.1 / 23.1, 16 of up to 131072 119 / 120 / 123; heads of 64, 128
+    // requests that see 1028 keys 24.3 / 19.6 / 20.1).
+    constexpr int per_cu = 2 * C::BT * DP * C::ES <= 32 * 1024 ? 2 : 1;
+    if (grid > per_cu * cus) grid = per_cu * cus;
+    // A workgroup may leave a part of its run's first unit and one of its last: two slots for each, or nothing is split.
+    const bool split = slots >= 2;
+    if (split && grid > slots / 2) grid = slots / 2;
+    if (grid > rows::LATER) grid = rows::LATER;
+    p->workgroups = grid;
+    if (split) p->parted = 2 * grid * C::SLOT;
+    return hipSuccess;
+  }
+  const int64_t few_tiles = (int64_t)a.tokens * group / rows::ROWS + a.requests, few_units = few_tiles * a.k_heads;  // of 16 rows
+  if constexpr (DT != IRIS_DTYPE_F32 && PG) {
+    // Tiles of 128 rows read keys once for all of them, tiles of 16 fill the chip with fewer rows and end sooner.  us in tiles of 128 /
+    // of 16, bf16, 8 + 1 heads of 128 unless stated.  By rows a request: 64 requests behind up to 4096 tokens, 19 rows each
+    // 41 / 37, 27 each 41 / 46, 42 each 42 / 49.  By 16-row units and the most keys a row may see: 102 x 200 11.3 / 7.7,
+    // 93 x 2004 20.5 / 17.2, 201 x 400 16.4 / 10.9, 460 x 500 17.1 / 13.4, 57 x 8001 31 / 26; 501 x 1000 20.2 / 20.5,
+    // 188 x 4113 29 / 39, 268 x 2001 (4 + 4 heads) 27 / 37, 55 x 46398 79 / 86; 537 x 180 12.6 / 14.1.
+    const bool few_rows = (int64_t)a.tokens * group <= 24 * (int64_t)a.requests ||
+                          (few_units <= 2 * cus && few_units * most_keys <= (int64_t)1536 * cus);
+    const int64_t row_tiles = (int64_t)a.tokens * group / tiles::ROWS + a.requests;
+    // (a page's rows are addressed with 32 bits)
+    const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
+    if (!few_rows && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX && a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
+      constexpr int64_t SLOT = tiles::Cfg<DT, DP>::SLOT;
+      p->kernel = IRIS_ATTENTION_PROMPT_TILES;
+      const int64_t units = row_tiles * a.k_heads, places = tiles::waves_a_simd(DP) * cus;
+      // Where places are left, several take a row tile, of four tiles of keys each or more.  (One prompt of 1000 tokens, us in one part / of
+      // four / of two key tiles: 28 / 20 / 26; of 2000: 49 / 34 / 34.)
+      if (2 * units <= places && units <= rows::LATER) {
+        p->splits = places / units;
+        const int64_t room_for = slots * C::SLOT / (SLOT * units);
+        if (p->splits > most_keys / (4 * tiles::BT)) p->splits = most_keys / (4 * tiles::BT);
+        if (p->splits > tiles::MOST_PARTS) p->splits = tiles::MOST_PARTS;
+        if (p->splits > room_for) p->splits = room_for;
+        if (p->splits < 1) p->splits = 1;
+      }
+      // Which starts first matters where places are taken twice: a CU's, or with a window (whose rows are nearly alike) all of them.  (us in the
+      // requests' order / by length: window of 1024, 642 row tiles on 768 places 44.4 / 46.3; no window, 381 on 512 99.7 / 97.)
+      if (p->splits == 1 && a.requests <= 64 && units > (a.window > 0 ? places : cus)) p->by_length = cus > a.k_heads ? cus / a.k_heads : 1;
+      p->workgroups = units * p->splits;
+      if (p->splits > 1) p->parted = units * p->splits * SLOT;
+      return hipSuccess;
+    }
+  }
+  // (8 prompts of up to 4 tokens behind up to 4096, us in one part / as many as make one / two workgroups a CU: 65 / 15 / 16; fp32, a
+  // prompt of 500: 25 / 19 / 19; more a CU the same)
+  p->kernel = IRIS_ATTENTION_PROMPT_ROWS;
+  if (few_units < 2 * cus && few_units <= rows::LATER) {
+    p->splits = 2 * cus / few_units;
+    if (p->splits > most_keys / (2 * C::BT)) p->splits = most_keys / (2 * C::BT);
+    if (p->splits > slots / few_units) p->splits = slots / few_units;
+    if (p->splits > rows::FLAT) p->splits = rows::FLAT;
+    if (p->splits < 1) p->splits = 1;
+  }
+  if (few_tiles * p->splits > INT32_MAX || a.k_heads > 65535) return hipErrorInvalidValue;
+  p->workgroups = few_units * p->splits;
+  if (p->splits > 1) p->parted = few_units * p->splits * C::SLOT;
+  return hipSuccess;
+}
+
 }  // namespace
 }  // namespace iris_amd
 
@@ -78,92 +164,51 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
   g.page = make_page_div((uint32_t)a.page_size);
   g.scale_log2 = a.scale * 1.4426950408889634f;
   g.group = a.q_heads / a.k_heads;
-  g.splits = 1;
-  const int cus = current_cu_count();
-  int64_t slots = 0;
-  if (a.workspace && a.workspace_elems > COUNTERS) {
-    slots = (a.workspace_elems - COUNTERS) / row_slot(a.head_dim);
-    g.counters = (int32_t*)a.workspace;
-    g.slots = a.workspace + COUNTERS;
-  }
-  // the most keys that a row may see
-  const int64_t room = (int64_t)a.table_width * a.page_size;
-  const int64_t most_keys = a.window > 0 && (int64_t)a.window + a.sinks < room ? (int64_t)a.window + a.sinks : room;
   const hipStream_t s = (hipStream_t)stream;
-
   return with_types(a, [&](auto dt, auto dp, auto pg) {
-    using C = rows::Cfg<dt.value, dp.value>;
-    constexpr int threads = rows::WAVES * 64;
-    if (!a.query_starts) {
-      const int64_t units = (int64_t)a.requests * a.k_heads * ((g.group + rows::ROWS - 1) / rows::ROWS);
-      const int64_t line = units * ((most_keys + C::BT - 1) / C::BT + 2 + rows::REST);  // at most
-      if (line > INT32_MAX) return hipErrorInvalidValue;
-      int64_t grid = line;
-      // As many workgroups as have 64 KiB of keys and values in flight a CU; more only leave more parts to join (us at 1 / 2 / 3 a CU:
-      // heads of 128, 64 requests of up to 8192 keys 20.6 / 22.1 / 23.1, 16 of up to 131072 119 / 120 / 123; heads of 64, 128
-      // requests that see 1028 keys 24.3 / 19.6 / 20.1).
-      constexpr int per_cu = 2 * C::BT * dp.value * C::ES <= 32 * 1024 ? 2 : 1;
-      if (grid > per_cu * cus) grid = per_cu * cus;
-      if (slots && grid > slots / 2) grid = slots / 2;
-      if (grid > rows::LATER) grid = rows::LATER;
-      if (grid < 1) {
-        grid = 1;
-        g.slots = nullptr;
-      }
-      g.grid_units = (int)grid;
-      rows::decode_kernel<dt.value, dp.value, pg.value><<<(int)grid, threads, 0, s>>>(g);
+    constexpr int DT = dt.value, DP = dp.value;
+    constexpr bool PG = pg.value;
+    Plan p;
+    const hipError_t refused = make_plan<DT, DP, PG>(a, current_cu_count(), &p);
+    if (refused != hipSuccess) return refused;
+    g.splits = (int)p.splits;
+    g.by_length = p.by_length;
+    g.grid_units = (int)p.workgroups;
+    if (p.parted) {
+      g.counters = (int32_t*)a.workspace;
+      g.slots = a.workspace + COUNTERS;
+    }
+    const unsigned workgroups = (unsigned)p.workgroups;
+    if (p.kernel == IRIS_ATTENTION_DECODE) {
+      rows::decode_kernel<DT, DP, PG><<<workgroups, rows::WAVES * 64, 0, s>>>(g);
       return hipGetLastError();
     }
-    const int64_t few_tiles = (int64_t)a.tokens * g.group / rows::ROWS + a.requests, few_units = few_tiles * a.k_heads;  // of 16 rows
-    if constexpr (dt.value != IRIS_DTYPE_F32 && pg.value) {
-      // Tiles of 128 rows read keys once for all of them, tiles of 16 fill the chip with fewer rows and end sooner.  us in tiles of 128 /
-      // of 16, bf16, 8 + 1 heads of 128 unless stated.  By rows a request: 64 requests behind up to 4096 tokens, 19 rows each
-      // 41 / 37, 27 each 41 / 46, 42 each 42 / 49.  By 16-row units and the most keys a row may see: 102 x 200 11.3 / 7.7,
-      // 93 x 2004 20.5 / 17.2, 201 x 400 16.4 / 10.9, 460 x 500 17.1 / 13.4, 57 x 8001 31 / 26; 501 x 1000 20.2 / 20.5,
-      // 188 x 4113 29 / 39, 268 x 2001 (4 + 4 heads) 27 / 37, 55 x 46398 79 / 86; 537 x 180 12.6 / 14.1.
-      const bool few_rows = (int64_t)a.tokens * g.group <= 24 * (int64_t)a.requests ||
-                            (few_units <= 2 * cus && few_units * most_keys <= (int64_t)1536 * cus);
-      const int64_t row_tiles = (int64_t)a.tokens * g.group / tiles::ROWS + a.requests;
-      // (a page's rows are addressed with 32 bits)
-      const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
-      if (!few_rows && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX &&
-          a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
-        const int64_t units = row_tiles * a.k_heads, places = tiles::waves_a_simd(dp.value) * cus;
-        // Where places are left, several take a row tile, of four tiles of keys each or more.  (One prompt of 1000 tokens, us in one part / of
-        // four / of two key tiles: 28 / 20 / 26; of 2000: 49 / 34 / 34.)
-        int64_t splits = 1;
-        if (2 * units <= places && units <= rows::LATER) {
-          splits = places / units;
-          const int64_t room_for = slots * row_slot(a.head_dim) / (tiles::Cfg<dt.value, dp.value>::SLOT * units);
-          if (splits > most_keys / (4 * tiles::BT)) splits = most_keys / (4 * tiles::BT);
-          if (splits > tiles::MOST_PARTS) splits = tiles::MOST_PARTS;
-          if (splits > room_for) splits = room_for;
-          if (splits < 1) splits = 1;
-        }
-        // Which starts first matters where places are taken twice: a CU's, or with a window (whose rows are nearly alike) all of them.  (us in the
-        // requests' order / by length: window of 1024, 642 row tiles on 768 places 44.4 / 46.3; no window, 381 on 512 99.7 / 97.)
-        if (splits == 1 && a.requests <= 64 && units > (a.window > 0 ? places : cus)) g.by_length = cus > a.k_heads ? cus / a.k_heads : 1;
-        g.splits = (int)splits;
+    if constexpr (DT != IRIS_DTYPE_F32 && PG) {
+      if (p.kernel == IRIS_ATTENTION_PROMPT_TILES) {
         if (a.lse)
-          tiles::prompt_tiles_kernel<dt.value, dp.value, true><<<(int)(units * splits), tiles::WAVES * 64, 0, s>>>(g);
+          tiles::prompt_tiles_kernel<DT, DP, true><<<workgroups, tiles::WAVES * 64, 0, s>>>(g);
         else
-          tiles::prompt_tiles_kernel<dt.value, dp.value, false><<<(int)(units * splits), tiles::WAVES * 64, 0, s>>>(g);
+          tiles::prompt_tiles_kernel<DT, DP, false><<<workgroups, tiles::WAVES * 64, 0, s>>>(g);
         return hipGetLastError();
       }
     }
-    // (8 prompts of up to 4 tokens behind up to 4096, us in one part / as many as make one / two workgroups a CU: 65 / 15 / 16; fp32, a
-    // prompt of 500: 25 / 19 / 19; more a CU the same)
-    int64_t splits = 1;
-    if (few_units < 2 * cus && few_units <= rows::LATER) {
-      splits = 2 * cus / few_units;
-      if (splits > most_keys / (2 * C::BT)) splits = most_keys / (2 * C::BT);
-      if (splits > slots / few_units) splits = slots / few_units;
-      if (splits > rows::FLAT) splits = rows::FLAT;
-      if (splits < 1) splits = 1;
-    }
-    g.splits = (int)splits;
-    if (few_tiles * splits > INT32_MAX || a.k_heads > 65535) return hipErrorInvalidValue;
-    rows::prompt_rows_kernel<dt.value, dp.value, pg.value><<<dim3((unsigned)(few_tiles * splits), a.k_heads), threads, 0, s>>>(g);
+    rows::prompt_rows_kernel<DT, DP, PG><<<dim3(workgroups / a.k_heads, a.k_heads), rows::WAVES * 64, 0, s>>>(g);
     return hipGetLastError();
+  });
+}
+
+extern "C" int iris_attention_plan(const iris_attention_args* args, int32_t num_cus, iris_attention_plan_info* plan) {
+  using namespace iris_amd;
+  if (!args || !plan || num_cus < 0) return hipErrorInvalidValue;
+  const iris_attention_args& a = *args;
+  const hipError_t bad = check(a);
+  if (bad != hipSuccess) return bad;
+  *plan = iris_attention_plan_info{0, 0, IRIS_ATTENTION_NOTHING, 1};
+  if (a.tokens == 0 || a.q_heads == 0) return hipSuccess;
+  return with_types(a, [&](auto dt, auto dp, auto pg) {
+    Plan p;
+    const hipError_t refused = make_plan<dt.value, dp.value, pg.value>(a, num_cus ? num_cus : current_cu_count(), &p);
+    if (refused == hipSuccess) *plan = iris_attention_plan_info{p.parted ? COUNTERS + p.parted : 0, p.workgroups, p.kernel, (int32_t)p.splits};
+    return refused;
   });
 }
