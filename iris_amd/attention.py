@@ -508,6 +508,8 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise TypeError("block_table must be an int32 matrix with contiguous rows")
     requests, width = block_table.shape
+    if requests > 1 and block_table.stride(0) < width:
+        raise ValueError("the rows of block_table must not overlap")
     _ints("lengths", lengths, device, torch.int32, requests)
     if query_starts is None:
         if requests != tokens:
@@ -552,7 +554,7 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     a.stride_ot, a.stride_oh = _steps(out, 2)
     a.stride_kc_page, a.stride_kc_row, a.stride_kc_head = _steps(k_cache, 3)
     a.stride_vc_page, a.stride_vc_row, a.stride_vc_head = _steps(v_cache, 3)
-    a.stride_table = max(block_table.stride(0), width) if requests > 1 else width
+    a.stride_table = block_table.stride(0) if requests > 1 else width
     a.requests, a.tokens, a.q_heads, a.k_heads, a.head_dim = requests, tokens, hq, hk, dim
     a.page_size, a.table_width, a.num_pages = page_size, width, pages
     a.window, a.sinks, a.dtype, a.scale = window, sinks, _DTYPES[dtype], scale
