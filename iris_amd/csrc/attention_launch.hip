@@ -103,7 +103,7 @@ hipError_t make_plan(const iris_attention_args& a, int cus, Plan* p) {
                           (few_units <= 2 * cus && few_units * most_keys <= (int64_t)1536 * cus);
     const int64_t row_tiles = (int64_t)a.tokens * group / tiles::ROWS + a.requests;
     // (a page's rows are addressed with 32 bits)
-    const int64_t reach = a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
+    const int64_t reach = (int64_t)a.page_size * 2 * (a.stride_kc_row > a.stride_vc_row ? a.stride_kc_row : a.stride_vc_row) + 512;
     if (!few_rows && row_tiles * a.k_heads <= INT32_MAX / 64 && reach <= INT32_MAX && a.stride_kc_row >= 0 && a.stride_vc_row >= 0) {
       constexpr int64_t SLOT = tiles::Cfg<DT, DP>::SLOT;
       p->kernel = IRIS_ATTENTION_PROMPT_TILES;

@@ -82,3 +82,10 @@ def test_kernels():
         assert lib.iris_attention_plan(ctypes.byref(bad), CUS, ctypes.byref(info)) == _native.HIP_ERROR_INVALID_VALUE
     assert lib.iris_attention_plan(ctypes.byref(call()), -1, ctypes.byref(info)) == _native.HIP_ERROR_INVALID_VALUE
     assert lib.iris_attention_plan(None, CUS, ctypes.byref(info)) == _native.HIP_ERROR_INVALID_VALUE
+
+
+@pytest.mark.parametrize("page,row,kernel", [(1 << 20, 64, "TILES"), (1 << 20, 1 << 11, "ROWS"), (1 << 30, 1, "ROWS"), ((1 << 31) - 16, 8, "ROWS")])
+def test_pages_past_what_31_bits_address_are_not_for_the_tiles(page, row, kernel):
+    """The tiles address a page's rows with 31 bits: the others do with 64."""
+    p = plan(tokens=4000, requests=2, hq=8, dim=8, width=1, page=page, stride_kc_row=row * 8, stride_vc_row=8)
+    assert p.kernel == getattr(_native, f"ATTENTION_PROMPT_{kernel}")
