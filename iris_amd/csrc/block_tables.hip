@@ -189,6 +189,7 @@ extern "C" int iris_block_tables_launch(const iris_block_tables_args* args, void
   if ((int64_t)a.table_width * a.page_size > INT32_MAX) return hipErrorInvalidValue;
   const Args g{a, make_page_div((uint32_t)a.page_size), a.table_width * a.page_size};
   const size_t lds = (size_t)a.requests * 4 * sizeof(int);
+  constexpr size_t FIXED_LDS = THREADS / 64 * sizeof(Sums) + sizeof(int);  // the waves' sums, and what is granted
   // Four waves where they hold the requests, so that a small step's sums meet sooner; sixteen beyond.  An item (token) a thread: a
   // workgroup repeats the sums, but what it writes it looks for in several dependent reads.
   const int threads = a.requests > 256 ? THREADS : 256;
@@ -197,7 +198,7 @@ extern "C" int iris_block_tables_launch(const iris_block_tables_args* args, void
   const int grid = (int)(groups < 1 ? 1 : groups > cus ? cus : groups);
   if (a.requests > THREADS) {
     constexpr int ITEMS = MAX_REQUESTS / THREADS;
-    if (lds > 64 * 1024) {
+    if (lds + FIXED_LDS > 64 * 1024) {  // (4084 requests and more)
       const hipError_t err = hipFuncSetAttribute((const void*)block_tables_kernel<ITEMS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
       if (err != hipSuccess) return err;
     }
