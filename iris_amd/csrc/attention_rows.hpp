@@ -128,11 +128,15 @@ struct Unit {
     int first_at, last_at; // of the unit's rows
   };
 
+  // Does some row of the unit see one of the keys first .. last?  (Positions of a unit's rows are neighbours.)
+  __device__ inline bool some_see(const Row& row, int first, int last) {
+    return first <= row.last_at && (a.window <= 0 || row.first_at - last < a.window || first < a.sinks);
+  }
   // Steps of a tile that no row sees a key of (the wave's share of the last keys, of the window's edge, behind the first
   // tokens) are left out: their loads all go to the request's first key.
   __device__ inline bool seen(const Piece& p, const Row& row, int j) {
     const int base = step_base(p, j);
-    return base <= row.last_at && (a.window <= 0 || row.first_at - (base + C::KS - 1) < a.window || base < a.sinks);
+    return some_see(row, base, base + C::KS - 1);
   }
   __device__ inline void look_up(const Piece& p, int j, int last, Pages& pages) {
     const int base = step_base(p, j);
@@ -149,20 +153,22 @@ struct Unit {
       }
     }
   }
-  __device__ inline int64_t checked(int page) {
+  // A table's entry for the keys first .. last.  One that is no page of the cache is none of the rows' business where they see none of
+  // its keys (pages behind a window may be gone): then, as otherwise, what is read for it is the first page's.
+  __device__ inline int64_t checked(int page, const Row& row, int first, int last) {
     if ((uint32_t)page < (uint32_t)a.num_pages) return page;
-    bad_page = true;
+    bad_page |= some_see(row, first, last);
     return 0;
   }
   __device__ inline int in_page(int key) { return key - (int)(page_div((uint32_t)key, g.page) * g.page.d); }
 
   // Keys past `last` are read as that one, and hidden later.
-  __device__ inline void load(const Piece& p, int j, int last, const Pages& pages, Step& x) {
+  __device__ inline void load(const Piece& p, const Row& row, int j, int last, const Pages& pages, Step& x) {
     const int base = step_base(p, j);
 #pragma unroll
     for (int s = 0; s < C::SUBS; ++s) {
       const int first_key = base + 16 * s, own = min(first_key + n, last);
-      const int64_t page = checked(pages.k[s]);
+      const int64_t page = PG ? checked(pages.k[s], row, first_key, first_key + 15) : checked(pages.k[s], row, first_key + n, first_key + n);
       const IRIS_GLOBAL char* kp = (const IRIS_GLOBAL char*)a.k_cache +
                                    (page * a.stride_kc_page + (int64_t)in_page(own) * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::ES + quad * 16;
 #pragma unroll
@@ -172,8 +178,8 @@ struct Unit {
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int key = min(first_key + quad * 4 + r, last);
-        const int64_t vpage = PG ? page : checked(pages.v[s][r]);
+        const int own_key = first_key + quad * 4 + r, key = min(own_key, last);
+        const int64_t vpage = PG ? page : checked(pages.v[s][r], row, own_key, own_key);
         const IRIS_GLOBAL char* vp = (const IRIS_GLOBAL char*)a.v_cache +
                                      (vpage * a.stride_vc_page + (int64_t)in_page(key) * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::ES + n * C::VB;
 #pragma unroll
@@ -321,7 +327,7 @@ struct Unit {
     if (p.j0 < p.j1) prepare(p.j0);
     int j = p.j0;
     for (; j < p.j1; ++j) {
-      load(p, j, last, pages, x);
+      load(p, row, j, last, pages, x);
       if (j + 1 < p.j1) prepare(j + 1);
       if (seen(p, row, j)) compute(p, j, x, row);
     }

@@ -30,3 +30,48 @@ def test_nothing_is_written_behind_a_workspace(dtype, dim, news):
             p.check()
         assert bool((room[COUNTERS + behind:] == -7).all()), f"{behind} elements behind the counters"
         assert bool((room[:COUNTERS].view(torch.int32) == 0).all())
+
+
+def forget(p, first_row_at, page, entries=(-1, 1 << 30)):
+    """Table entries of pages that no query of a request sees (its first one stands at ``first_row_at[i]``) become none."""
+    for i, first in enumerate(first_row_at):
+        for j in range(p.table.shape[1]):
+            lo, hi = j * page, (j + 1) * page - 1  # its keys
+            if lo >= p.sinks and hi < first - p.window + 1:
+                p.table[i, j] = entries[j % 2]
+
+
+@pytest.mark.parametrize("page", [16, 20, 64, 8])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 128), (F32, 64), (BF16, 256)])
+@pytest.mark.parametrize("window,sinks", [(50, 0), (50, 3), (16, 0), (200, 70), (1, 0)])
+def test_pages_behind_the_window_may_be_gone_for_single_tokens(window, sinks, dtype, dim, page):
+    lengths = [500, 40, 51, 300, 0, 129]
+    p = Problem(lengths, None, 4, 2, dim, dtype, page, window=window, sinks=sinks)
+    forget(p, [n - 1 for n in lengths], page)
+    p.launch()
+    p.check()
+
+
+@pytest.mark.parametrize("dtype,dim,page,hq,hk", [
+    (BF16, 64, 16, 4, 2), (F16, 128, 16, 4, 2), (F32, 64, 16, 4, 2), (BF16, 256, 16, 4, 2), (BF16, 64, 20, 4, 2), (F16, 128, 20, 4, 2), (F32, 64, 20, 4, 2),
+    (F16, 128, 64, 4, 2), (BF16, 64, 16, 48, 24), (F16, 128, 16, 48, 24), (BF16, 256, 64, 48, 24)])  # (tiles of 16 rows, and of 128)
+@pytest.mark.parametrize("window,sinks", [(50, 0), (50, 3), (200, 70)])
+def test_pages_behind_the_window_may_be_gone_for_prompts(window, sinks, dtype, dim, page, hq, hk):
+    lengths, news = [500, 40, 700, 300], [40, 40, 130, 1]
+    p = Problem(lengths, news, hq, hk, dim, dtype, page, window=window, sinks=sinks)
+    forget(p, [n - new for n, new in zip(lengths, news)], page)
+    p.launch()
+    p.check()
+
+
+@pytest.mark.parametrize("dtype,dim,heads", [(BF16, 128, 1), (F16, 64, 1), (F32, 64, 1), (BF16, 128, 20), (F16, 64, 20)])
+def test_a_page_that_is_none_reaches_the_tiles_whose_rows_see_it(dtype, dim, heads):
+    n, window, page = 700, 100, 16
+    p = Problem([n], [n], heads, heads, dim, dtype, page, window=window)
+    lo, hi = 304, 304 + page - 1  # its keys: rows 304 .. 418 see some of them
+    p.table[0, lo // page] = -1
+    p.launch()
+    assert p.word.item() == attention.STATUS_BAD_INDEX
+    out = p.out[:, 0].isnan()
+    assert bool(out[lo:hi + window].all())
+    assert not bool(out[:lo // 128 * 128].any()) and not bool(out[-(-(hi + window) // 128) * 128:].any())
