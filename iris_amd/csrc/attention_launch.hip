@@ -84,10 +84,11 @@ hipError_t make_plan(const iris_attention_args& a, int cus, Plan* p) {
     // requests that see 1028 keys 24.3 / 19.6 / 20.1).
     constexpr int per_cu = 2 * C::BT * DP * C::ES <= 32 * 1024 ? 2 : 1;
     if (grid > per_cu * cus) grid = per_cu * cus;
-    // A workgroup may leave a part of its run's first unit and one of its last: two slots for each, or nothing is split.
-    const bool split = slots >= 2;
-    if (split && grid > slots / 2) grid = slots / 2;
     if (grid > rows::LATER) grid = rows::LATER;
+    // A workgroup may leave a part of its run's first unit and one of its last, in two slots of its own.  Where the slots are for no more
+    // workgroups than there are units, nothing is split and a unit is a workgroup's.
+    const bool split = slots / 2 >= (units < grid ? units + 1 : grid);
+    if (split && grid > slots / 2) grid = slots / 2;
     p->workgroups = grid;
     if (split) p->parted = 2 * grid * C::SLOT;
     return hipSuccess;

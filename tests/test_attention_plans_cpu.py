@@ -89,3 +89,16 @@ def test_pages_past_what_31_bits_address_are_not_for_the_tiles(page, row, kernel
     """The tiles address a page's rows with 31 bits: the others do with 64."""
     p = plan(tokens=4000, requests=2, hq=8, dim=8, width=1, page=page, stride_kc_row=row * 8, stride_vc_row=8)
     assert p.kernel == getattr(_native, f"ATTENTION_PROMPT_{kernel}")
+
+
+@pytest.mark.parametrize("requests,hk", [(1, 1), (4, 1), (64, 1), (64, 8), (300, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_small_workspace_leaves_no_less_workgroups_than_none(requests, hk, dim):
+    """Equal runs of the line for fewer workgroups than there are units would be slower than a unit a workgroup."""
+    problem = dict(requests=requests, hq=8 * hk, hk=hk, dim=dim, width=400)
+    none, units = plan(**problem), requests * hk
+    for slots in (0, 1, 2, 3, 5, 9, 40, 64, 65, 200, 600, 1000, 4096):
+        p = plan(workspace=COUNTERS + slots * slot(dim), **problem)
+        assert p.workgroups >= min(units, none.workgroups)
+        # split where that is more workgroups than units, or as many as there are without a workspace
+        assert (p.workspace_elems > 0) == (slots // 2 >= min(units + 1, none.workgroups))
