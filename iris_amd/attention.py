@@ -120,12 +120,26 @@ def _no_gradient(*tensors):
                            "and attention over a cache has none")
 
 
-def _launched(err):
-    """Whether the native code took the call.  What it declines, and what the launcher rejects, goes through the full checks, which
-    say what is wrong."""
+DECLINED = -1  # the native module: not a call of the ordinary kind, nothing was launched
+
+
+def _native_call(err):
+    """Whether a call is done.  What the native code declined, or its launcher may have refused, goes through the full checks, which say
+    what is wrong; then ``_rest``."""
     if err > 0 and err != _native.HIP_ERROR_INVALID_VALUE:
         _native.hip_try(err)
     return err == 0
+
+
+def _rest(err, name, args, device):
+    """Launches a call that the native code declined.  Any other status may have come from behind a launch, which is not made again."""
+    if err != DECLINED:
+        _rejected(name)
+    _launch(name, args, device)
+
+
+def _rejected(name):
+    raise ValueError(f"{name} rejected the arguments (sizes, strides or alignment it does not take)")
 
 
 def _launch(name, args, device):
@@ -133,7 +147,7 @@ def _launch(name, args, device):
     with torch.cuda.device(device):
         err = getattr(_native.lib(), name)(ctypes.byref(args), stream)
     if err == _native.HIP_ERROR_INVALID_VALUE:
-        raise ValueError(f"{name} rejected the arguments (sizes, strides or alignment it does not take)")
+        _rejected(name)
     _native.hip_try(err)
 
 
@@ -158,8 +172,9 @@ def build_block_tables(cached, new_tokens, block_table, pool, pool_state, page_s
     every token, up to their common length (0 and -1 past the last token).
     ``lengths`` and ``pool_state_out`` may not be ``cached`` and ``pool_state``.
     """
-    if _launched(_native.host().block_tables(cached, new_tokens, block_table, pool, pool_state, lengths, pool_state_out, query_starts,
-                                             positions, slots, status, page_size)):
+    err = _native.host().block_tables(cached, new_tokens, block_table, pool, pool_state, lengths, pool_state_out, query_starts,
+                                      positions, slots, status, page_size)
+    if _native_call(err):
         return
     device = cached.device
     requests = cached.numel()
@@ -199,7 +214,7 @@ def build_block_tables(cached, new_tokens, block_table, pool, pool_state, page_s
     a.requests, a.table_width, a.page_size = requests, block_table.shape[1], page_size
     a.stride_table = max(block_table.stride(0), block_table.shape[1])
     a.pool_size, a.max_tokens = pool.numel(), positions.numel()
-    _launch("iris_block_tables_launch", a, device)
+    _rest(err, "iris_block_tables_launch", a, device)
 
 
 # ---- norms and rotation ------------------------------------------------------
@@ -330,8 +345,9 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
     slots of ``k_cache`` / ``v_cache`` [pages, page size, key heads, head size]; a negative
     slot is skipped, and with a cache ``k_out`` may be None.
     """
-    if _launched(_native.host().qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, q_weight, k_weight, v, k_cache, v_cache, slots,
-                                             status, eps, interleaved)):
+    err = _native.host().qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, q_weight, k_weight, v, k_cache, v_cache, slots,
+                                      status, eps, interleaved)
+    if _native_call(err):
         return
     device, dtype = q.device, q.dtype
     if dtype not in _DTYPES:
@@ -380,7 +396,7 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
         raise ValueError("k_out is required without a cache")
     for name, t in outputs:
         _output(name, t)
-    _launch("iris_qk_norm_rope_launch", a, device)
+    _rest(err, "iris_qk_norm_rope_launch", a, device)
 
 
 def make_gradient_workspace(head_dim, *, device="cuda"):
@@ -396,8 +412,9 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, 
     heads in a fixed order, in ``workspace`` (``make_gradient_workspace``; fp32, as
     few as 2 * head size elements).  ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out``.
     """
-    if _launched(_native.host().qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, q_weight, k_weight, dq_weight,
-                                                      dk_weight, workspace, status, eps, interleaved)):
+    err = _native.host().qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, q_weight, k_weight, dq_weight,
+                                               dk_weight, workspace, status, eps, interleaved)
+    if _native_call(err):
         return
     device, dtype = q.device, q.dtype
     if dtype not in _DTYPES:
@@ -433,7 +450,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, 
     a.dq_weight, a.dk_weight, a.status = _ptr(dq_weight), _ptr(dk_weight), _ptr(status)
     for prefix, t in (("dqo", dq_out), ("dko", dk_out), ("q", q), ("k", k), ("dq", dq), ("dk", dk)):
         _strides(a, prefix, t)
-    _launch("iris_qk_norm_rope_backward_launch", a, device)
+    _rest(err, "iris_qk_norm_rope_backward_launch", a, device)
 
 
 class QkNormRope(torch.autograd.Function):
@@ -479,8 +496,9 @@ def make_workspace(head_dim, *, device="cuda"):
 
 
 def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status):
-    if _launched(_native.host().attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale,
-                                          window, sinks)):
+    err = _native.host().attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale,
+                                   window, sinks)
+    if _native_call(err):
         return
     device, dtype = q.device, q.dtype
     if dtype not in _DTYPES:
@@ -558,7 +576,7 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     a.requests, a.tokens, a.q_heads, a.k_heads, a.head_dim = requests, tokens, hq, hk, dim
     a.page_size, a.table_width, a.num_pages = page_size, width, pages
     a.window, a.sinks, a.dtype, a.scale = window, sinks, _DTYPES[dtype], scale
-    _launch("iris_attention_launch", a, device)
+    _rest(err, "iris_attention_launch", a, device)
 
 
 def _steps(t, n):

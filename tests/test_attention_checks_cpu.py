@@ -55,3 +55,56 @@ def test_rows_of_a_block_table_lie_apart(calls):
         with pytest.raises(ValueError, match="overlap"):
             decode(**dict(base, block_table=table))
     assert len(calls.launched) == done
+
+
+def tables_operands(requests=3, width=5, tokens=6):
+    i32, i64 = torch.int32, torch.int64
+    return [torch.zeros(requests, dtype=i32), torch.zeros(requests, dtype=i32), torch.zeros((requests, width), dtype=i32), torch.zeros(16, dtype=i32),
+            torch.zeros(2, dtype=i64), 16], dict(lengths=torch.zeros(requests, dtype=i32), pool_state_out=torch.zeros(2, dtype=i64),
+                                                 query_starts=torch.zeros(requests + 1, dtype=i32), positions=torch.zeros(tokens, dtype=i32),
+                                                 slots=torch.zeros(tokens, dtype=i64))
+
+
+def rope_operands(tokens=5, hq=4, hk=2, dim=64):
+    heads = [torch.zeros((tokens, h, dim), dtype=BF16) for h in (hq, hk, hq, hk)]
+    cos = torch.zeros((10, dim // 2))
+    return heads[:2] + [torch.zeros(tokens, dtype=torch.int32), cos, cos.clone()] + heads[2:]
+
+
+CALLS = {
+    "tables": lambda: (lambda args, kw: attention.build_block_tables(*args, **kw))(*tables_operands()),
+    "rope": lambda: attention.qk_norm_rope(*rope_operands()),
+    "in place": lambda: (lambda x: attention.qk_norm_rope(*x[:5], x[0], x[1]))(rope_operands()),
+    "gradient": lambda: (lambda x, y: attention.qk_norm_rope_backward(*x[:2], *y))(rope_operands(), rope_operands()),
+    "gradient in place": lambda: (lambda x, y: attention.qk_norm_rope_backward(*x[:2], *y[:5], *x[:2]))(rope_operands(), rope_operands()),
+    "decode": lambda: decode(**operands()),
+    "prompt": lambda: (lambda a: attention.prompt_attention(*[a[n] for n in ("q", "k_cache", "v_cache", "block_table", "lengths")],
+                                                            torch.zeros(4, dtype=torch.int32), a["out"]))(operands(tokens=7)),
+}
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_what_the_native_code_launched_is_not_launched_again(calls, name, monkeypatch):
+    """A status that is an error may come from behind a launch (one that was left by an earlier call, a second launch that failed): work
+    in place would be done twice."""
+    calls.answer = 0
+    CALLS[name]()
+    assert not calls.launched
+    calls.answer = _native.HIP_ERROR_INVALID_VALUE
+    with pytest.raises(ValueError, match="rejected"):
+        CALLS[name]()
+    assert not calls.launched
+    calls.answer = 719
+    monkeypatch.setattr(_native, "hip_try", lambda err: (_ for _ in ()).throw(RuntimeError(f"HIP error code {err}")))
+    with pytest.raises(RuntimeError, match="719"):
+        CALLS[name]()
+    assert not calls.launched
+    calls.answer = DECLINED
+    CALLS[name]()
+    assert len(calls.launched) == 1
+
+
+def test_what_the_launcher_refuses_is_explained_where_the_checks_know_it(calls):
+    calls.answer = _native.HIP_ERROR_INVALID_VALUE
+    with pytest.raises(ValueError, match="16 bytes"):
+        decode(**dict(operands(), q=torch.zeros(3 * 4 * 64 + 1, dtype=BF16)[1:].view(3, 4, 64)))
