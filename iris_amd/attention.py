@@ -199,7 +199,7 @@ def build_block_tables(cached, new_tokens, block_table, pool, pool_state, page_s
         raise ValueError(f"at most {MAX_REQUESTS} requests, got {requests}")
     if page_size < 1:
         raise ValueError("page_size must be positive")
-    if block_table.shape[1] * page_size > INT32_MAX:
+    if max(block_table.shape[1], 1) * page_size > INT32_MAX:
         raise ValueError("block_table has room for more tokens than 31 bits count")
     written = (block_table, pool, lengths, pool_state_out, query_starts, positions, slots)
     spans = [(t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape))))
@@ -575,7 +575,8 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     a.stride_table = block_table.stride(0) if requests > 1 else width
     a.requests, a.tokens, a.q_heads, a.k_heads, a.head_dim = requests, tokens, hq, hk, dim
     a.page_size, a.table_width, a.num_pages = page_size, width, pages
-    a.window, a.sinks, a.dtype, a.scale = window, sinks, _DTYPES[dtype], scale
+    # (no context is longer than 31 bits count, so that the most they hold is all keys)
+    a.window, a.sinks, a.dtype, a.scale = min(window, INT32_MAX), min(sinks, INT32_MAX), _DTYPES[dtype], scale
     _rest(err, "iris_attention_launch", a, device)
 
 

@@ -108,3 +108,22 @@ def test_what_the_launcher_refuses_is_explained_where_the_checks_know_it(calls):
     calls.answer = _native.HIP_ERROR_INVALID_VALUE
     with pytest.raises(ValueError, match="16 bytes"):
         decode(**dict(operands(), q=torch.zeros(3 * 4 * 64 + 1, dtype=BF16)[1:].view(3, 4, 64)))
+
+
+def test_numbers_past_31_bits_keep_their_meaning(calls):
+    """No context is longer than 31 bits count: a window or first tokens beyond it are all keys."""
+    most = 2 ** 31 - 1
+    for value, want in ((2 ** 32 + 16, most), (2 ** 32, most), (2 ** 31, most), (most, most), (2 ** 70, most), (17, 17), (0, 0)):
+        decode(**dict(operands(), window=value, sinks=5))
+        assert (calls.launched[-1][1].window, calls.launched[-1][1].sinks) == (want, 5)
+        decode(**dict(operands(), window=9, sinks=value))
+        assert (calls.launched[-1][1].window, calls.launched[-1][1].sinks) == (9, want)
+    done = len(calls.launched)
+    for wrong in (dict(window=-2 ** 32 + 16), dict(sinks=-1)):
+        with pytest.raises(ValueError):
+            decode(**dict(operands(), **wrong))
+    args, kw = tables_operands(width=0)
+    for page_size in (2 ** 32 + 16, 2 ** 31):
+        with pytest.raises(ValueError, match="31 bits"):
+            attention.build_block_tables(*args[:5], page_size, **kw)
+    assert len(calls.launched) == done

@@ -75,3 +75,12 @@ def test_a_page_that_is_none_reaches_the_tiles_whose_rows_see_it(dtype, dim, hea
     out = p.out[:, 0].isnan()
     assert bool(out[lo:hi + window].all())
     assert not bool(out[:lo // 128 * 128].any()) and not bool(out[-(-(hi + window) // 128) * 128:].any())
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 32 + 16, 0), (2 ** 31 - 1, 0), (16, 2 ** 32), (16, 2 ** 31 - 1), (2 ** 31, 2 ** 40)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_windows_and_first_tokens_past_31_bits_are_all_keys(window, sinks, dtype):
+    for news, heads in ((None, (4, 2)), ([200, 30], (4, 2)), ([200, 30], (80, 40))):
+        p = Problem([300, 40], news, *heads, 64, dtype, 16, window=window, sinks=sinks)
+        p.launch()
+        p.check()
