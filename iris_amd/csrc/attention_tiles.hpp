@@ -219,7 +219,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
     const int key = list.tile(j) * BT + wave * 16;
     if ((uint32_t)page >= (uint32_t)a.num_pages) {
       // (of the rows' business only where one of them sees one of the 16 keys; pages behind a window may be gone)
-      bad_page |= key <= rows_last && (a.window <= 0 || rows_first - (key + 15) < a.window || key < a.sinks);
+      bad_page |= key <= rows_last && (key + 15 >= list.lo || key < a.sinks);
       page = 0;
     }
     const int in_page = key - (int)(page_div((uint32_t)key, g.page) * g.page.d);
