@@ -47,9 +47,11 @@ struct Cfg {
   static constexpr int SLOT = ROWS * DP + WAVES * 64 * 4;  // floats of a partial result
   // Weights are 2^(score - reference), and the reference is the maximum, less LIFT, of the first keys that the row sees; it stays
   // until a lane's 32 weights of a tile sum up to more than MOST.  fp16 ends at 65504 and loses places below 2^-14, so that LIFT
-  // stands between; bf16 and the fp32 sums have room for any of it.
-  static constexpr float LIFT = DT == IRIS_DTYPE_F16 ? 6.f : 0.f;
-  static constexpr float MOST = DT == IRIS_DTYPE_F16 ? 32768.f : 1.1529215e18f;
+  // stands between.  bf16 has fp32's range, but so have its values: weights begin at 2^-16 at most and are not let past 1, so that
+  // their products with values sum up to no more than those against the running maximum would.  (The same time as with a
+  // reference at the maximum and sums of up to 2^60, where values of 3e20 and more could leave fp32's range.)
+  static constexpr float LIFT = DT == IRIS_DTYPE_F16 ? 6.f : -16.f;
+  static constexpr float MOST = DT == IRIS_DTYPE_F16 ? 32768.f : 1.f;
 };
 
 // The chunk of its row that lies at chunk position p (and the other way round: both are XORs).

@@ -84,3 +84,29 @@ def test_windows_and_first_tokens_past_31_bits_are_all_keys(window, sinks, dtype
         p = Problem([300, 40], news, *heads, 64, dtype, 16, window=window, sinks=sinks)
         p.launch()
         p.check()
+
+
+@pytest.mark.parametrize("size", [1e20, 1e25, 1e35])
+@pytest.mark.parametrize("news", [70, 650, 1])
+@pytest.mark.parametrize("room", [2, 30000], ids=["tight", "roomy"])
+@pytest.mark.parametrize("steps", [14, 7])
+def test_large_values_under_scores_that_grow(size, news, room, steps):
+    """Averages of finite values are finite, whatever the scores of the keys before: bf16 has fp32's range, and products of weights and
+    values must not leave it."""
+    n, d = 700, 64
+    p = Problem([n], [news] if news > 1 else None, 1, 1, d, BF16, 16, room=room)
+    p.q_host[:] = 0
+    p.q_host[..., 0] = 16
+    p.q.copy_(p.q_host)
+    p.k[0][..., 0] = (torch.arange(n) * steps // n).to(BF16)[:, None] * (19 / steps)  # 38 more at the end than at the beginning
+    p.k[0][..., 0] = p.k[0][..., 0].float().round().to(BF16)
+    p.v[0] = (p.v[0].float() * size).to(BF16)
+    for j in range(-(-n // 16)):
+        for cache, rows in ((p.k_cache, p.k[0]), (p.v_cache, p.v[0])):
+            part = rows[16 * j:16 * j + 16].cuda()
+            cache[p.table[0, j], :len(part)] = part
+    p.launch()
+    p.check()
+    p.out.fill_(-7)
+    p.launch(None)  # (in one part)
+    p.check()
