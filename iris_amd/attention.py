@@ -81,7 +81,7 @@ def _output(name, t):
         if stride <= reach:
             raise ValueError(f"{name}: elements of an output must not overlap")
         reach += stride * (n - 1)
-    if t.requires_grad and torch.is_grad_enabled():
+    if _differentiated(t):
         raise RuntimeError(f"{name} requires a gradient; outputs are written in place")
 
 
@@ -114,10 +114,19 @@ def _cache(name, t, device, dtype, heads, dim):
         raise ValueError(f"{name}: the elements of a head must be contiguous")
 
 
+def _tangent(t):
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
+def _differentiated(t):
+    """Whether autograd has business with a tensor: a gradient, or a tangent (forward mode)."""
+    return t is not None and ((torch.is_grad_enabled() and t.requires_grad) or _tangent(t))
+
+
 def _no_gradient(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("no gradient flows through this call; QkNormRope is the differentiable form of qk_norm_rope, "
-                           "and attention over a cache has none")
+    if any(_differentiated(t) for t in tensors):
+        raise RuntimeError("no gradient flows through this call; QkNormRope is the differentiable form of qk_norm_rope "
+                           "(in heads and weights), and attention over a cache has none")
 
 
 DECLINED = -1  # the native module: not a call of the ordinary kind, nothing was launched
@@ -357,7 +366,7 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
     _heads("k", k, device, dtype, tokens, None, dim)
     hk = k.shape[1]
     _heads("q_out", q_out, device, dtype, tokens, hq, dim)
-    _no_gradient(q, k, v, q_weight, k_weight)
+    _no_gradient(q, k, v, cos, sin, q_weight, k_weight)
     outputs = [("q_out", q_out)]
     a = _native.QkNormRopeArgs()
     _rope_operands(a, device, dtype, tokens, dim, positions, cos, sin, q_weight, k_weight, eps, interleaved)
@@ -425,6 +434,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, 
     hk = k.shape[1]
     for name, t, heads in (("dq_out", dq_out, hq), ("dq", dq, hq), ("dk_out", dk_out, hk), ("dk", dk, hk)):
         _heads(name, t, device, dtype, tokens, heads, dim)
+    if any(t is not None and _tangent(t) for t in (dq_out, dk_out, q, k, cos, sin, q_weight, k_weight)):
+        raise RuntimeError("no gradient flows through this call, and no tangent")
     a = _native.QkNormRopeBackwardArgs()
     _rope_operands(a, device, dtype, tokens, dim, positions, cos, sin, q_weight, k_weight, eps, interleaved)
     _status(status, device)
@@ -459,6 +470,8 @@ class QkNormRope(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, positions, cos, sin, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+        if any(ctx.needs_input_grad[3:5]):
+            raise RuntimeError("no gradient flows to the angles")
         q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
         qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved)
         ctx.save_for_backward(q, k, positions, cos, sin, q_weight, k_weight)

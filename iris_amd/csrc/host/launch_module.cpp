@@ -401,7 +401,9 @@ bool real(PyObject* o, double* out) {
 }
 bool truth(PyObject* o, int32_t* out) { return (*out = PyObject_IsTrue(o)) >= 0; }
 
-bool differentiates(const Operand& t) { return t && at::GradMode::is_enabled() && t.t->requires_grad(); }
+// Autograd's business with an operand: a tangent (forward mode), or a gradient.
+bool tangent(const Operand& t) { return t && t.t->_fw_grad(/*level=*/0).defined(); }
+bool differentiates(const Operand& t) { return t && ((at::GradMode::is_enabled() && t.t->requires_grad()) || tangent(t)); }
 
 // A tensor [tokens, heads, head size] of `type` whose head elements are contiguous; sizes below 0 are free.
 bool heads_of(const Operand& t, at::ScalarType type, int64_t tokens, int64_t heads, int64_t dim) {
@@ -563,7 +565,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* x, Py_ssize_t n) {
   if (!heads_of(t[Q], type, -1, -1, -1) || !heads_of(t[K], type, tokens, -1, dim) || !heads_of(t[Q_OUT], type, tokens, hq, dim) || !output(t[Q_OUT]))
     return PyLong_FromLong(DECLINED);
   const int64_t hk = t[K].t->size(1);
-  for (const int i : {Q, K, V, QW, KW})
+  for (const int i : {Q, K, V, COS, SIN, QW, KW})
     if (differentiates(t[i])) return PyLong_FromLong(DECLINED);
   if (!rope_operands(t[POSITIONS], t[COS], t[SIN], t[QW], t[KW], type, tokens, dim, &a) || !status_ok(t[STATUS])) return PyLong_FromLong(DECLINED);
   if (t[K_OUT] ? !heads_of(t[K_OUT], type, tokens, hk, dim) || !output(t[K_OUT]) : !t[SLOTS] && hk) return PyLong_FromLong(DECLINED);
@@ -626,6 +628,8 @@ PyObject* qk_norm_rope_backward(PyObject*, PyObject* const* x, Py_ssize_t n) {
       !heads_of(t[DK], type, tokens, hk, dim) || !output(t[DQ]) || !output(t[DK]) || !status_ok(t[STATUS]) ||
       !rope_operands(t[POSITIONS], t[COS], t[SIN], t[QW], t[KW], type, tokens, dim, &a))
     return PyLong_FromLong(DECLINED);
+  for (const int i : {DQ_OUT, DK_OUT, Q, K, COS, SIN, QW, KW})
+    if (tangent(t[i])) return PyLong_FromLong(DECLINED);
   if (t[DQW] || t[DKW]) {
     if ((t[DQW] && (!t[QW] || !vector_of(t[DQW], at::kFloat, dim) || !output(t[DQW]))) ||
         (t[DKW] && (!t[KW] || !vector_of(t[DKW], at::kFloat, dim) || !output(t[DKW]))) || !t[WORKSPACE] ||

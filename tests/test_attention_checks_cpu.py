@@ -127,3 +127,41 @@ def test_numbers_past_31_bits_keep_their_meaning(calls):
         with pytest.raises(ValueError, match="31 bits"):
             attention.build_block_tables(*args[:5], page_size, **kw)
     assert len(calls.launched) == done
+
+
+def test_gradients_and_tangents_that_would_be_lost_are_refused(calls):
+    """Of every operand that results depend on: heads, caches, weights, angles."""
+    forward_ad = torch.autograd.forward_ad
+    cache = torch.zeros((3, 16, 2, 64), dtype=BF16)
+    serving = dict(v=torch.zeros((5, 2, 64), dtype=BF16), k_cache=cache, v_cache=cache.clone(), slots=torch.zeros(5, dtype=torch.int64),
+                   q_weight=torch.ones(64), k_weight=torch.ones(64))
+    q, k, positions, cos, sin, q_out, k_out = rope_operands()
+    rope = dict(serving, q=q, k=k, cos=cos, sin=sin, q_out=q_out, k_out=k_out)
+    heads = [torch.zeros_like(t) for t in (q, k)]
+    gradient = dict(dq_out=heads[0], dk_out=heads[1], q=q, k=k, cos=cos, sin=sin, dq=q_out, dk=k_out, q_weight=torch.ones(64), k_weight=torch.ones(64))
+
+    def run_rope(**a):
+        first = [a.pop(n) for n in ("q", "k")] + [positions] + [a.pop(n) for n in ("cos", "sin", "q_out", "k_out")]
+        attention.qk_norm_rope(*first, **a)
+
+    def run_gradient(**a):
+        first = [a.pop(n) for n in ("dq_out", "dk_out", "q", "k")] + [positions] + [a.pop(n) for n in ("cos", "sin", "dq", "dk")]
+        attention.qk_norm_rope_backward(*first, **a)
+
+    attended = {n: t for n, t in operands().items() if t.is_floating_point()}
+    for run, names, args in ((run_rope, rope, rope), (decode, attended, operands()), (run_gradient, gradient, gradient)):
+        run(**args)
+        for name in names:
+            if not args[name].is_floating_point():
+                continue
+            done = len(calls.launched)
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(args[name].clone(), torch.ones_like(args[name]))
+                with pytest.raises(RuntimeError, match="gradient"):
+                    run(**dict(args, **{name: dual}))
+            if run is not run_gradient or name in ("dq", "dk"):  # (a gradient's inputs are what autograd holds)
+                with pytest.raises(RuntimeError, match="gradient"):
+                    run(**dict(args, **{name: args[name].clone().requires_grad_()}))
+            assert len(calls.launched) == done, name
+    with pytest.raises(RuntimeError, match="gradient"):
+        attention.QkNormRope.apply(q, k, positions, cos.clone().requires_grad_(), sin)

@@ -110,3 +110,27 @@ def test_large_values_under_scores_that_grow(size, news, room, steps):
     p.out.fill_(-7)
     p.launch(None)  # (in one part)
     p.check()
+
+
+def test_tangents_are_refused():
+    forward_ad = torch.autograd.forward_ad
+    p = Problem([20, 30], None, 4, 2, 64, BF16, 16)
+    k, cos = torch.zeros((2, 2, 64), dtype=BF16, device="cuda"), torch.ones((4, 32), device="cuda")
+    positions = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def attend(q):
+        attention.decode_attention(q, p.k_cache, p.v_cache, p.table, p.lens, p.out)
+
+    def turn(q):
+        attention.qk_norm_rope(q, k, positions, cos, cos, p.out, torch.empty_like(k))
+
+    def back(q):
+        attention.qk_norm_rope_backward(q, k, p.q, k, positions, cos, cos, p.out, torch.empty_like(k))
+
+    for call in (attend, turn, back):
+        call(p.q)
+        p.out.fill_(-7)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="gradient"):
+            call(forward_ad.make_dual(p.q, torch.ones_like(p.q)))
+        assert bool((p.out == -7).all())
+        call(p.q.detach())
