@@ -85,6 +85,22 @@ def _output(name, t):
         raise RuntimeError(f"{name} requires a gradient; outputs are written in place")
 
 
+def _same_view(a, b):
+    return (a.data_ptr() == b.data_ptr() and a.dtype == b.dtype and a.shape == b.shape
+            and all(n <= 1 or s == z for n, s, z in zip(a.shape, a.stride(), b.stride())))
+
+
+def _apart(outputs, inputs, in_place=()):
+    """(name, tensor) outputs share no memory with each other or with the inputs, but for an output that is one of its own inputs,
+    element by element: (output, input) names ``in_place``."""
+    outputs, inputs = ([(name, t) for name, t in operands if t is not None] for operands in (outputs, inputs))
+    for i, (name, t) in enumerate(outputs):
+        others = outputs[:i] + [(other, x) for other, x in inputs if not ((name, other) in in_place and _same_view(t, x))]
+        for other, x in others:
+            if _native.host().overlap(t, x):
+                raise ValueError(f"{name} shares memory with {other}: an output lies in memory of its own, or is its own input")
+
+
 def _ints(name, t, device, dtype, numel, exact=True):
     _require_cuda(name, t, device)
     if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous():
@@ -405,6 +421,8 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
         raise ValueError("k_out is required without a cache")
     for name, t in outputs:
         _output(name, t)
+    _apart(outputs, [("q", q), ("k", k), ("v", v), ("positions", positions), ("cos", cos), ("sin", sin), ("q_weight", q_weight),
+                     ("k_weight", k_weight), ("slots", slots)], [("q_out", "q"), ("k_out", "k")])
     _rest(err, "iris_qk_norm_rope_launch", a, device)
 
 
@@ -457,6 +475,11 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, 
         a.workspace, a.workspace_elems = _ptr(workspace), workspace.numel()
     for name, t in (("dq", dq), ("dk", dk)):
         _output(name, t)
+    written = [("dq", dq), ("dk", dk), ("workspace", workspace)]
+    _apart(written, [("dq_out", dq_out), ("dk_out", dk_out), ("q", q), ("k", k), ("positions", positions), ("cos", cos), ("sin", sin),
+                     ("q_weight", q_weight), ("k_weight", k_weight)], [("dq", "dq_out"), ("dq", "q"), ("dk", "dk_out"), ("dk", "k")])
+    # (the weights' gradients are written by a launch of their own, behind the last read of an input)
+    _apart(written + [("dq_weight", dq_weight), ("dk_weight", dk_weight)], [])
     a.dq_out, a.dk_out, a.q, a.k, a.dq, a.dk = _ptr(dq_out), _ptr(dk_out), _ptr(q), _ptr(k), _ptr(dq), _ptr(dk)
     a.dq_weight, a.dk_weight, a.status = _ptr(dq_weight), _ptr(dk_weight), _ptr(status)
     for prefix, t in (("dqo", dq_out), ("dko", dk_out), ("q", q), ("k", k), ("dq", dq), ("dk", dk)):
@@ -570,6 +593,9 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
         if workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.data_ptr() % 16:
             raise TypeError("workspace must be contiguous fp32 at a multiple of 16 bytes (make_workspace)")
         a.workspace, a.workspace_elems = _ptr(workspace), workspace.numel()
+    _apart([("out", out), ("lse", lse), ("workspace", workspace)],
+           [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("lengths", lengths), ("query_starts", query_starts)],
+           [("out", "q")])
     if tokens == 0 or hq == 0:
         return
     if requests == 0:

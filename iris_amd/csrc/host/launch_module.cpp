@@ -21,6 +21,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <utility>
 
 #include "../../../include/iris_amd.h"
 
@@ -431,6 +433,107 @@ bool output(const Operand& t) {
   return true;
 }
 
+// A tensor's elements lie in [lo, hi).
+struct Span {
+  const char *lo = nullptr, *hi = nullptr;
+  bool meets(const Span& other) const { return lo < other.hi && other.lo < hi; }
+};
+Span span_of(const at::Tensor& t) {
+  const auto sizes = t.sizes(), strides = t.strides();
+  Span s;
+  int64_t reach = 1;
+  for (size_t d = 0; d < sizes.size(); ++d) {
+    if (!sizes[d]) return s;
+    reach += (sizes[d] - 1) * strides[d];
+  }
+  s.lo = (const char*)t.data_ptr();
+  s.hi = s.lo + reach * (int64_t)t.element_size();
+  return s;
+}
+// ... as runs of `run` bytes at every combination of its axes' steps, the longest step first.
+struct Lattice {
+  static constexpr int MOST_AXES = 8;
+  int64_t step[MOST_AXES], count[MOST_AXES], run;
+  int axes = 0;
+};
+Lattice lattice_of(const at::Tensor& t) {
+  Lattice l;
+  l.run = (int64_t)t.element_size();
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    const int64_t n = t.size(d), step = t.stride(d) * (int64_t)t.element_size();
+    if (n <= 1 || step == 0) continue;
+    int i = l.axes++;
+    for (; i > 0 && l.step[i - 1] < step; --i) l.step[i] = l.step[i - 1], l.count[i] = l.count[i - 1];
+    l.step[i] = step, l.count[i] = n;
+  }
+  while (l.axes && l.step[l.axes - 1] == l.run) l.run *= l.count[--l.axes];
+  return l;
+}
+// Whether the axes from i and j on of two lattices, the second `by` bytes further on, have a byte in common.  A step of the longest axis
+// is looked at only where what is left of both can meet, which for tensors whose axes lie inside each other are two or three.
+// `budget` ends the rest: what cannot be told apart counts as common.
+bool meet(const Lattice& a, int i, const Lattice& b, int j, int64_t by, int* budget) {
+  if (--*budget < 0) return true;
+  int64_t reach_a = a.run, reach_b = b.run;
+  for (int k = i; k < a.axes; ++k) reach_a += (a.count[k] - 1) * a.step[k];
+  for (int k = j; k < b.axes; ++k) reach_b += (b.count[k] - 1) * b.step[k];
+  if (by >= reach_a || -by >= reach_b) return false;
+  if (i == a.axes && j == b.axes) return true;
+  const int64_t step = std::max(i < a.axes ? a.step[i] : 0, j < b.axes ? b.step[j] : 0);
+  const bool in_a = i < a.axes && a.step[i] == step, in_b = j < b.axes && b.step[j] == step;
+  const int64_t most = in_a ? a.count[i] - 1 : 0, least = in_b ? 1 - b.count[j] : 0;  // of a's index less b's
+  if (in_a) reach_a -= most * step;
+  if (in_b) reach_b += least * step;
+  // -reach_b < by - k step < reach_a
+  const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t first = std::max(least, floor_div(by - reach_a, step) + 1), last = std::min(most, floor_div(by + reach_b - 1, step));
+  for (int64_t k = first; k <= last; ++k)
+    if (meet(a, i + in_a, b, j + in_b, by - k * step, budget)) return true;
+  return false;
+}
+bool common(const at::Tensor& a, const at::Tensor& b) {
+  if (a.dim() > Lattice::MOST_AXES || b.dim() > Lattice::MOST_AXES) return true;
+  int budget = 4096;
+  return meet(lattice_of(a), 0, lattice_of(b), 0, (const char*)b.data_ptr() - (const char*)a.data_ptr(), &budget);
+}
+bool same_view(const at::Tensor& a, const at::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+// Operands t[outs] lie apart from each other and, but for those in `late` (which are written when all inputs have been read), from
+// t[ins].  An output may be one of its own inputs, element by element: (output, input) pairs in `in_place`.
+bool apart(const Operand* t, std::initializer_list<int> outs, std::initializer_list<int> ins, std::initializer_list<std::pair<int, int>> in_place,
+           std::initializer_list<int> late = {}) {
+  Span span[16];
+  for (const auto& list : {outs, ins})
+    for (const int i : list)
+      if (t[i]) span[i] = span_of(*t[i].t);
+  for (auto o = outs.begin(); o != outs.end(); ++o) {
+    for (auto p = outs.begin(); p != o; ++p)
+      if (span[*o].meets(span[*p]) && common(*t[*o].t, *t[*p].t)) return false;
+    if (std::find(late.begin(), late.end(), *o) != late.end()) continue;
+    for (const int i : ins) {
+      if (!span[*o].meets(span[i])) continue;
+      if (std::find(in_place.begin(), in_place.end(), std::make_pair(*o, i)) != in_place.end() && same_view(*t[*o].t, *t[i].t)) continue;
+      if (common(*t[*o].t, *t[i].t)) return false;
+    }
+  }
+  return true;
+}
+
+// overlap(a, b) -> whether two tensors (of any device) have memory in common, or may have.
+PyObject* overlap(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 2 || !THPVariable_Check(x[0]) || !THPVariable_Check(x[1])) {
+    PyErr_SetString(PyExc_TypeError, "overlap takes two tensors");
+    return nullptr;
+  }
+  const at::Tensor &a = THPVariable_Unpack(x[0]), &b = THPVariable_Unpack(x[1]);
+  if (!plain(a) || !plain(b)) Py_RETURN_TRUE;
+  return PyBool_FromLong(a.device() == b.device() && span_of(a).meets(span_of(b)) && common(a, b));
+}
+
 bool vector_of(const Operand& t, at::ScalarType type, int64_t numel) {
   return t && t.t->dim() == 1 && t.t->scalar_type() == type && t.t->numel() == numel && t.t->is_contiguous();
 }
@@ -583,6 +686,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* x, Py_ssize_t n) {
   } else if (t[V] || t[K_CACHE] || t[V_CACHE]) {
     return PyLong_FromLong(DECLINED);
   }
+  if (!apart(t, {Q_OUT, K_OUT, K_CACHE, V_CACHE}, {Q, K, V, POSITIONS, COS, SIN, QW, KW, SLOTS}, {{Q_OUT, Q}, {K_OUT, K}}))
+    return PyLong_FromLong(DECLINED);
   a.q = t[Q].ptr();
   a.k = t[K].ptr();
   a.v = t[V].ptr();
@@ -638,6 +743,10 @@ PyObject* qk_norm_rope_backward(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.workspace = (float*)t[WORKSPACE].ptr();
     a.workspace_elems = t[WORKSPACE].t->numel();
   }
+  // (the weights' gradients are written by a launch of their own)
+  if (!apart(t, {DQ, DK, WORKSPACE, DQW, DKW}, {DQ_OUT, DK_OUT, Q, K, POSITIONS, COS, SIN, QW, KW}, {{DQ, DQ_OUT}, {DQ, Q}, {DK, DK_OUT}, {DK, K}},
+             {DQW, DKW}))
+    return PyLong_FromLong(DECLINED);
   a.dq_out = t[DQ_OUT].ptr();
   a.dk_out = t[DK_OUT].ptr();
   a.q = t[Q].ptr();
@@ -704,6 +813,7 @@ PyObject* attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.workspace = (float*)t[WORKSPACE].ptr();
     a.workspace_elems = t[WORKSPACE].t->numel();
   }
+  if (!apart(t, {OUT, LSE, WORKSPACE}, {Q, K_CACHE, V_CACHE, TABLE, LENGTHS, STARTS}, {{OUT, Q}})) return PyLong_FromLong(DECLINED);
   a.q = t[Q].ptr();
   a.k_cache = t[K_CACHE].ptr();
   a.v_cache = t[V_CACHE].ptr();
@@ -740,6 +850,7 @@ PyMethodDef methods[] = {
     {"block_tables", (PyCFunction)(void (*)(void))block_tables, METH_FASTCALL, "launch the block tables; -1: declined"},
     {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope, METH_FASTCALL, "launch norms and rotation; -1: declined"},
     {"qk_norm_rope_backward", (PyCFunction)(void (*)(void))qk_norm_rope_backward, METH_FASTCALL, "launch their gradient; -1: declined"},
+    {"overlap", (PyCFunction)(void (*)(void))overlap, METH_FASTCALL, "whether two tensors have memory in common"},
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "launch attention over a paged cache; -1: declined"},
     {nullptr, nullptr, 0, nullptr}};
 

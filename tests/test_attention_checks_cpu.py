@@ -8,6 +8,7 @@ from iris_amd import _native, attention
 
 BF16 = torch.bfloat16
 DECLINED = -1
+HOST = _native.host()
 
 
 class Calls:
@@ -15,6 +16,7 @@ class Calls:
 
     def __init__(self):
         self.answer, self.launched = DECLINED, []
+        self.overlap = HOST.overlap  # (of tensors anywhere)
 
     def __getattr__(self, name):  # the native module's functions
         return lambda *args: self.answer
@@ -165,3 +167,105 @@ def test_gradients_and_tangents_that_would_be_lost_are_refused(calls):
             assert len(calls.launched) == done, name
     with pytest.raises(RuntimeError, match="gradient"):
         attention.QkNormRope.apply(q, k, positions, cos.clone().requires_grad_(), sin)
+
+
+def test_overlap_of_strided_tensors():
+    """Against the elements' addresses one by one: nested axes in any order, windows into each other, expanded axes."""
+    import random
+
+    overlap = HOST.overlap
+    rng = random.Random(1)
+    both = [0, 0]
+    for _ in range(3000):
+        base = torch.zeros(20000, dtype=rng.choice([torch.int16, torch.int32]))
+
+        def view(t):
+            if rng.random() < 0.5:  # axes inside each other, with gaps
+                sizes = [rng.randint(1, 4) for _ in range(rng.randint(1, 4))]
+                strides, reach = [], 1
+                for n in sizes:
+                    strides.append(reach * rng.choice([1, 1, 2]) + rng.choice([0, 0, 1, 5]))
+                    reach = strides[-1] * n
+                order = list(range(len(sizes)))
+                rng.shuffle(order)
+                sizes, strides = [sizes[i] for i in order], [strides[i] for i in order]
+            else:
+                sizes = [rng.randint(0 if rng.random() < 0.1 else 1, 5) for _ in range(3)]
+                strides = [rng.randint(0, 30) for _ in range(3)]
+            return t.as_strided(sizes, strides, rng.randint(0, 300))
+
+        a, b = view(base), view(base.view(torch.int16) if rng.random() < 0.3 else base)
+
+        def touched(t):
+            at = torch.zeros(t.shape, dtype=torch.int64)
+            for d, (n, s) in enumerate(zip(t.shape, t.stride())):
+                at = at + (torch.arange(n) * s).view([-1 if i == d else 1 for i in range(t.dim())])
+            start = (t.data_ptr() - base.data_ptr()) + at.flatten() * t.element_size()
+            return {x + i for x in start.tolist() for i in range(t.element_size())}
+
+        want = not touched(a).isdisjoint(touched(b))
+        assert overlap(a, b) == overlap(b, a) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        both[want] += 1
+    assert min(both) > 500
+    big = torch.zeros(1).expand(1 << 30)  # (nothing of that size is walked through)
+    assert overlap(big, big)
+    qkv = torch.zeros((1 << 16, 12, 64), dtype=BF16)
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+    assert not any(overlap(*pair) for pair in ((q, k), (q, v), (k, v))) and overlap(q, qkv[:, 7:9])
+    by_head = qkv.view(1 << 16, 4, 3, 64)
+    assert not overlap(by_head[:, :, 0], by_head[:, :, 1]) and overlap(by_head[:, :, 0], qkv[:, :1])
+    assert not overlap(q[::2], q[1::2]) and overlap(q[::2], q[::3])
+
+
+def test_outputs_lie_apart(calls):
+    """In place is element by element; anything else that shares memory would be read by one workgroup while another writes it."""
+
+    def check(good, bad):
+        for call in good:
+            done = len(calls.launched)
+            call()
+            assert len(calls.launched) == done + 1
+        for call in bad:
+            done = len(calls.launched)
+            with pytest.raises(ValueError, match="memory"):
+                call()
+            assert len(calls.launched) == done
+
+    tokens, hq, hk, d = 6, 4, 2, 64
+    wide = torch.zeros((tokens, hq + 2 * hk + 2, d), dtype=BF16)  # a fused projection, and room behind it
+    q, k, v = wide[:, :hq], wide[:, hq:hq + hk], wide[:, hq + hk:hq + 2 * hk]
+    cos, sin, positions = torch.zeros((10, d // 2)), torch.zeros((10, d // 2)), torch.zeros(tokens, dtype=torch.int32)
+    q_new, k_new = torch.zeros((tokens, hq, d), dtype=BF16), torch.zeros((tokens, hk, d), dtype=BF16)
+    caches = torch.zeros((2, 4, 16, hk, d), dtype=BF16)
+    cache = dict(v=v, k_cache=caches[0], v_cache=caches[1], slots=torch.zeros(tokens, dtype=torch.int64))
+    pages = caches.view(4, 2, 16, hk, d)  # keys and values of a page beside each other
+
+    def turn(q_out, k_out, **kw):
+        attention.qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, **kw)
+
+    check([lambda: turn(q, k), lambda: turn(q, k, **cache), lambda: turn(q_new, k_new, **cache), lambda: turn(q, None, **cache),
+           lambda: turn(q, wide[:, -hk:], **cache), lambda: turn(q_new, k, **dict(cache, k_cache=pages[:, 0], v_cache=pages[:, 1]))],
+          [lambda: turn(wide[:, 1:1 + hq], k_new), lambda: turn(q_new, wide[:, hq + 1:hq + 1 + hk]), lambda: turn(q, q[:, :hk]),
+           lambda: turn(wide[:, hk:hk + hq], k), lambda: turn(q, v, **cache), lambda: turn(q_new, q_new[:, 1:1 + hk]),
+           lambda: turn(q, k, **dict(cache, v_cache=caches[0])), lambda: turn(q, k, **dict(cache, v=caches[1, 0, :tokens])),
+           lambda: turn(q, caches[0, 0, :tokens], **cache)])
+
+    dq_out, dk_out, room = torch.zeros((tokens, hq, d), dtype=BF16), torch.zeros((tokens, hk, d), dtype=BF16), torch.zeros(20 * d)
+    weights = dict(q_weight=torch.ones(d), k_weight=torch.ones(d), dq_weight=torch.zeros(d), dk_weight=torch.zeros(d), workspace=room)
+
+    def back(dq, dk, **kw):
+        attention.qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, **kw)
+
+    check([lambda: back(dq_out, dk_out), lambda: back(q, k), lambda: back(q_new, k_new, **weights), lambda: back(wide[:, -hq:], k_new),
+           lambda: back(dq_out, dk_out, **dict(weights, dq_weight=weights["q_weight"]))],  # (written when all has been read)
+          [lambda: back(q_new, q_new[:, :hk]), lambda: back(wide[:, 1:1 + hq], k_new), lambda: back(q_new, q[:, :hk]), lambda: back(q_new, dq_out[:, :hk]),
+           lambda: back(q_new, k_new, **dict(weights, dk_weight=weights["dq_weight"])), lambda: back(q_new, k_new, **dict(weights, dq_weight=room[:d])),
+           lambda: back(q_new, k_new, **dict(weights, workspace=cos.flatten()[:2 * d]))])
+
+    a = operands(requests=3)
+    flat, scratch = torch.zeros(768 + 64, dtype=BF16), torch.zeros(5000)
+    check([lambda: decode(**dict(a, out=a["q"])), lambda: decode(**dict(a, lse=torch.zeros(3, 4), workspace=scratch)),
+           lambda: decode(**dict(a, v_cache=a["k_cache"]))],
+          [lambda: decode(**dict(a, q=flat[:768].view(3, 4, 64), out=flat[64:].view(3, 4, 64))), lambda: decode(**dict(a, out=a["k_cache"].view(-1, 4, 64)[:3])),
+           lambda: decode(**dict(a, out=a["q"].as_strided((3, 4, 64), (64, 192, 1)))), lambda: decode(**dict(a, lse=scratch[100:112].view(3, 4), workspace=scratch)),
+           lambda: decode(**dict(a, lse=a["block_table"].view(torch.float32).flatten()[:12].view(3, 4)))])

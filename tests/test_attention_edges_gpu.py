@@ -134,3 +134,28 @@ def test_tangents_are_refused():
             call(forward_ad.make_dual(p.q, torch.ones_like(p.q)))
         assert bool((p.out == -7).all())
         call(p.q.detach())
+
+
+def test_outputs_over_other_operands_are_refused():
+    """(What is refused and what is not: the checks' own tests, without a GPU.)"""
+    wide = torch.zeros((6, 10, 64), dtype=BF16, device="cuda")
+    q, k, fresh = wide[:, :4], wide[:, 4:6], torch.zeros((6, 4, 64), dtype=BF16, device="cuda")
+    positions, cos = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.ones((4, 32), device="cuda")
+    attention.qk_norm_rope(q, k, positions, cos, cos, q, k)
+    with pytest.raises(ValueError, match="shares memory"):
+        attention.qk_norm_rope(q, k, positions, cos, cos, wide[:, 1:5], k)
+    attention.qk_norm_rope_backward(fresh, fresh[:, :2], q, k, positions, cos, cos, q, k)
+    with pytest.raises(ValueError, match="shares memory"):
+        attention.qk_norm_rope_backward(fresh, fresh[:, :2], q, k, positions, cos, cos, fresh[:, :4], fresh[:, 1:3])
+    p = Problem([20, 30], None, 4, 2, 64, BF16, 16)
+    with pytest.raises(ValueError, match="shares memory"):
+        attention.decode_attention(p.q, p.k_cache, p.v_cache, p.table, p.lens, p.k_cache.view(-1, 4, 64)[:2])
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F32, 64)])
+def test_outputs_in_place_of_the_queries(dtype, dim):
+    for lengths, news in (([3000, 700, 0], None), ([900, 300], [900, 40]), ([4000], [20])):
+        p = Problem(lengths, news, 8, 1, dim, dtype, 16)
+        p.out = p.q
+        p.launch()
+        p.check()
