@@ -531,6 +531,25 @@ def make_workspace(head_dim, *, device="cuda"):
     return torch.zeros(elems, dtype=torch.float32, device=device)
 
 
+def _without_a_page(out, lse, status, lengths, query_starts, room):
+    """The rows of a call that has no page to read: NaN where one sees a key, else zeros, and reported as the kernels do."""
+    tokens = torch.arange(out.shape[0], device=out.device)
+    if query_starts is None:
+        row, begin, new, mine = tokens, tokens, 1, torch.ones_like(tokens, dtype=torch.bool)
+    else:
+        row = torch.searchsorted(query_starts[1:].contiguous(), tokens, right=True).clamp(max=len(lengths) - 1)
+        begin, new = query_starts[row], query_starts[row + 1] - query_starts[row]
+        mine = (tokens >= query_starts[0]) & (tokens < query_starts[-1])
+    sees = mine & (lengths.clamp(0, room)[row] - new + tokens - begin >= 0)
+    for t, none in ((out, 0.0), (lse, -math.inf)):
+        if t is not None:
+            shape = [-1] + [1] * (t.dim() - 1)
+            t.masked_fill_(mine.view(shape), none).masked_fill_(sees.view(shape), math.nan)
+    if status is not None:
+        bits = (sees.any() | (lengths > room).any()).int() * STATUS_BAD_INDEX
+        status.view(torch.int32).as_strided((1,), (1,)).bitwise_or_(bits)
+
+
 def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status):
     err = _native.host().attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale,
                                    window, sinks)
@@ -600,10 +619,8 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
         return
     if requests == 0:
         raise ValueError("queries of no request")
-    if width == 0 or pages == 0:  # no key anywhere
-        out.zero_()
-        if lse is not None:
-            lse.fill_(-math.inf)
+    if width == 0 or pages == 0:
+        _without_a_page(out, lse, status, lengths, query_starts, width * page_size)
         return
     a.q, a.k_cache, a.v_cache, a.out = _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out)
     a.block_table, a.lengths, a.query_starts, a.status = _ptr(block_table), _ptr(lengths), _ptr(query_starts), _ptr(status)

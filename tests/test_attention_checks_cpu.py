@@ -269,3 +269,39 @@ def test_outputs_lie_apart(calls):
           [lambda: decode(**dict(a, q=flat[:768].view(3, 4, 64), out=flat[64:].view(3, 4, 64))), lambda: decode(**dict(a, out=a["k_cache"].view(-1, 4, 64)[:3])),
            lambda: decode(**dict(a, out=a["q"].as_strided((3, 4, 64), (64, 192, 1)))), lambda: decode(**dict(a, lse=scratch[100:112].view(3, 4), workspace=scratch)),
            lambda: decode(**dict(a, lse=a["block_table"].view(torch.float32).flatten()[:12].view(3, 4)))])
+
+
+@pytest.mark.parametrize("width,pages", [(0, 4), (3, 0), (0, 0)])
+def test_without_a_page_the_rows_are_as_with_one(calls, width, pages):
+    """Rows that see a key have no page to read it from (NaN, reported) where the table has room for it; a length beyond the table's
+    room is none (reported); rows of no request stay as they are."""
+    q, nan, inf = torch.ones((9, 4, 64), dtype=BF16), float("nan"), float("inf")
+    cache = torch.zeros((pages, 16, 2, 64), dtype=BF16)
+
+    def run(lengths, starts):
+        n = len(lengths)
+        out, lse, word = torch.full((9, 4, 64), 7.0, dtype=BF16), torch.full((9, 4), 7.0), torch.tensor([64], dtype=torch.uint32)
+        table = torch.zeros((n, width), dtype=torch.int32)
+        args = [cache, cache, table, torch.tensor(lengths, dtype=torch.int32)]
+        if starts is None:
+            attention.decode_attention(q, *args, out, lse=lse, status=word)
+        else:
+            attention.prompt_attention(q, *args, torch.tensor(starts, dtype=torch.int32), out, lse=lse, status=word)
+        return out, lse, word.item()
+
+    def expect(got, rows, bits):
+        """rows: what each row's elements are, 0 (no key), nan (no page) or 7 (untouched)."""
+        want = torch.tensor(rows)
+        torch.testing.assert_close(got[0].float(), want[:, None, None].expand(9, 4, 64), equal_nan=True, rtol=0, atol=0)
+        torch.testing.assert_close(got[1], torch.where(want == 0, -inf, want)[:, None].expand(9, 4), equal_nan=True, rtol=0, atol=0)
+        assert got[2] == 64 | bits
+
+    bad = attention.STATUS_BAD_INDEX
+    see = nan if width else 0.0
+    expect(run([0] * 9, None), [0.0] * 9, 0)
+    expect(run([0, 5] + [0] * 7, None), [0.0, see] + [0.0] * 7, bad)
+    # the requests' tokens are 1 .. 2, 3 .. 6 (of which the last two have keys), none, and none is 0, 7 and 8
+    expect(run([0, 0, 0], [1, 3, 7, 7]), [7.0] + [0.0] * 6 + [7.0] * 2, 0)
+    expect(run([0, 2, 0], [1, 3, 7, 7]), [7.0] + [0.0] * 4 + [see] * 2 + [7.0] * 2, bad)
+    expect(run([0, 1000, 0], [1, 3, 7, 7]), [7.0] + [0.0] * 2 + [see] * 4 + [7.0] * 2, bad)
+    assert not calls.launched
