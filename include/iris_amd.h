@@ -441,7 +441,8 @@ int iris_block_tables_launch(const iris_block_tables_args* args, void* stream);
  * (no weight: x itself), of which the first rotary_dim elements turn by the angles cos / sin[position][rotary_dim / 2]:
  * pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved.  Strides are in elements, t: token, h: head; a head's
  * elements are contiguous.  k_out may be NULL where there is a cache.  With slots, keys and values also go to
- * k_cache / v_cache[slot / page_size][slot % page_size][head]; a negative slot is skipped.  Outputs may be the inputs.
+ * k_cache / v_cache[slot / page_size][slot % page_size][head]; a negative slot is skipped.  q_out may be q and
+ * k_out k; outputs share no other memory with each other or with inputs.
  */
 typedef struct iris_qk_norm_rope_args {
   const void* q;
@@ -472,8 +473,9 @@ int iris_qk_norm_rope_launch(const iris_qk_norm_rope_args* args, void* stream);
 
 /*
  * Its gradient: dq, dk from dq_out, dk_out and the unnormed q, k; dq_weight / dk_weight (fp32, may be NULL) summed over
- * tokens and heads in a fixed order.  workspace holds rows of 2 * head_dim floats, one a workgroup; more rows let
- * more workgroups run.  Not needed without weight gradients.
+ * tokens and heads in a fixed order.  workspace holds rows of head_dim floats, one a workgroup: two at least, and up to
+ * four a CU let as many workgroups run.  Not needed without weight gradients.  dq may be dq_out or q, dk dk_out or k; outputs
+ * share no other memory with each other or with inputs.
  */
 typedef struct iris_qk_norm_rope_backward_args {
   const void* dq_out;
@@ -508,9 +510,13 @@ int iris_qk_norm_rope_backward_launch(const iris_qk_norm_rope_backward_args* arg
  * (query_starts NULL) there is one a request.  The query at position p sees key j <= p where j > p - window, or j < sinks, or
  * window is 0; query head h goes to key head h / (q_heads / k_heads).  out = softmax(scale q k^T) v; lse (may be NULL,
  * fp32 [tokens][q_heads]) the logarithm of the softmax's sum.  A row that sees no key is 0 with lse -inf.
- * Tables, lengths and starts are read on the device; keys past a request's length are never read as numbers.
- * workspace (fp32, 16-byte aligned, zeroed once before its first use, for one stream at a time) takes the parts that a long
- * axis is split into; without it nothing is split.
+ * Tables, lengths and starts are read on the device; keys past a request's length are never read as numbers, and a table's entry
+ * need be no page where none of its keys is seen (behind a window).  Sums are fp32.  With heads of 16 bits the weights (exponentials
+ * of the scores, against the largest) are rounded to the heads' type for the product with the values and for the sum that divides
+ * it; lse is that of the unrounded ones.  Values times the number of keys have to stay in fp32's range.  out may be q; outputs and
+ * workspace share no other memory with each other or with inputs.
+ * workspace (fp32, 16-byte aligned, zeroed once before its first use, for one stream at a time, of any size) takes the parts that
+ * a long axis is split into; where it is none, or too small for it, nothing is split.
  */
 typedef struct iris_attention_args {
   const void* q;

@@ -12,6 +12,7 @@ and ``qk_norm_rope_backward`` (``QkNormRope`` under autograd) is the gradient
 of the norms and the rotation for training.
 
 Like ``iris_amd.ops`` these check operands against what the kernels assume
+(types, shapes, strides, and that outputs share no memory with other operands, but for work in place)
 *before* anything is launched, launch on torch's current stream, write into the
 tensors they are given, and neither synchronise nor allocate.  What only the
 device can see (an index outside of what it indexes, a ring of free pages
@@ -427,8 +428,9 @@ def qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, *, q_weight=None, k_we
 
 
 def make_gradient_workspace(head_dim, *, device="cuda"):
-    """A workspace for the weight gradients of ``qk_norm_rope_backward``: a row of partial sums for each of 1024 workgroups."""
-    return torch.empty(1024 * 2 * head_dim, dtype=torch.float32, device=device)
+    """A workspace for the weight gradients of ``qk_norm_rope_backward``: a row of ``head_dim`` partial sums for each of the (at most)
+    1024 workgroups of a launch."""
+    return torch.empty(1024 * head_dim, dtype=torch.float32, device=device)
 
 
 def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, q_weight=None, k_weight=None, dq_weight=None,
@@ -437,7 +439,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, *, 
 
     ``dq_weight`` / ``dk_weight`` fp32 [head size] (None: not wanted) are summed over tokens and
     heads in a fixed order, in ``workspace`` (``make_gradient_workspace``; fp32, as
-    few as 2 * head size elements).  ``dq`` and ``dk`` may be ``dq_out`` and ``dk_out``.
+    few as 2 * head size elements).  ``dq`` may be ``dq_out`` or ``q``, and ``dk`` ``dk_out`` or ``k``.
     """
     err = _native.host().qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, q_weight, k_weight, dq_weight,
                                                dk_weight, workspace, status, eps, interleaved)
@@ -650,7 +652,12 @@ def decode_attention(q, k_cache, v_cache, block_table, lengths, out, *, scale: O
     (written before, ``qk_norm_rope``) among them; 0 gives zeros.  Query head h reads key head ``h // (query heads // key heads)``.
     ``window`` > 0: only the last ``window`` keys are seen, and the first ``sinks``.
     ``scale`` is ``head size ** -0.5`` by default; ``lse`` fp32 [requests, query heads] takes the logarithms of the
-    softmax sums.  With a ``workspace`` (``make_workspace``) long contexts are split over the GPU and joined.
+    softmax sums.  With a ``workspace`` (``make_workspace``) long contexts are split over the GPU and joined; one too small for that is none.
+
+    With heads of 16 bits the softmax's weights are rounded to the heads' type for the product with the values, and divided by
+    the sum of the rounded ones; sums are fp32 (and values times the number of keys have to stay in its range).  A
+    table's entry need be no page where no query sees one of its keys: pages behind a window may be given back.
+    ``out`` may be ``q``, and shares no other memory with an operand.
     """
     _attention(q, k_cache, v_cache, block_table, lengths, None, out, scale, window, sinks, lse, workspace, status)
 
