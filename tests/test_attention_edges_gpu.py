@@ -1,11 +1,15 @@
 """Attention over a paged cache at the edges of what a caller may hand in."""
 
+import ctypes
+
 import pytest
 import torch
 
+import attention_reference as R
 from attention_reference import BF16, F16, F32
-from iris_amd import attention
-from test_paged_attention_gpu import Problem
+from iris_amd import _native, attention
+from test_block_tables_gpu import mixed, step
+from test_paged_attention_gpu import Problem, dense_on_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +163,118 @@ def test_outputs_in_place_of_the_queries(dtype, dim):
         p.out = p.q
         p.launch()
         p.check()
+
+
+# ---- which launch a call is --------------------------------------------------
+
+
+def planned(p, workspace, monkeypatch):
+    """What the launcher does with a problem's call (which is not made)."""
+    got = []
+    with monkeypatch.context() as m:
+        m.setattr(_native, "host", lambda: Declining())
+        m.setattr(attention, "_launch", lambda name, args, device: got.append(args))
+        p.launch(workspace)
+    info = _native.AttentionPlanInfo()
+    assert _native.lib().iris_attention_plan(ctypes.byref(got[0]), 0, ctypes.byref(info)) == 0
+    return info
+
+
+class Declining:
+    """A native module that takes no call."""
+
+    overlap = staticmethod(_native.host().overlap)
+
+    def __getattr__(self, name):
+        return lambda *args: attention.DECLINED
+
+
+@pytest.mark.parametrize("requests", [63, 64, 65, 150])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+def test_prompts_of_about_as_many_requests_as_are_put_in_order(dtype, dim, requests, monkeypatch):
+    """Up to 64 requests' row tiles start by the keys they see, those of more in the requests' order."""
+    news = [60 + (7 * i) % 41 for i in range(requests)]
+    lengths = [n + (13 * i) % 200 for i, n in enumerate(news)]
+    p = Problem(lengths, news, 40, 8, dim, dtype, 16)
+    assert planned(p, None, monkeypatch).kernel == _native.ATTENTION_PROMPT_TILES
+    p.launch()
+    assert p.word.item() == 0
+    want, spread = dense_on_gpu(p)
+    off, bound = (p.out.double().cpu() - want).abs(), R.attention_error(dtype, want, spread, dim)
+    assert bool((off <= bound).all()), f"off by up to {(off / bound).max().item()} times the bound"
+
+
+@pytest.mark.parametrize("news,hq,hk,kernel", [([300, 200], 8, 1, _native.ATTENTION_PROMPT_TILES), ([9, 4], 4, 2, _native.ATTENTION_PROMPT_ROWS)])
+def test_prompts_in_a_captured_graph_whose_parts_join(news, hq, hk, kernel, monkeypatch):
+    most = [3000, 2100]
+    p = Problem(most, news, hq, hk, 128, BF16, 16)
+    workspace = attention.make_workspace(128)
+    info = planned(p, workspace, monkeypatch)
+    assert info.kernel == kernel and info.parts > 1
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            p.launch(workspace)
+    torch.cuda.synchronize()
+    k, v, tokens = p.k, p.v, sum(news)
+    for lengths, first in ((most, news[0]), ([1000, 700], tokens - 1), ([3000, 40], 3), ([500, 0], tokens), (most, news[0])):
+        news = [first, tokens - first]
+        p.lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        p.starts.copy_(torch.tensor([0, first, tokens], dtype=torch.int32))
+        p.lengths, p.news = lengths, news
+        p.k, p.v = [x[:n] for x, n in zip(k, lengths)], [x[:n] for x, n in zip(v, lengths)]
+        p.out.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        p.check()
+        eager = p.out.clone()
+        p.launch(workspace)
+        assert torch.equal(p.out, eager)
+    assert bool((workspace[:COUNTERS].view(torch.int32) == 0).all())
+
+
+# ---- the Python code's own launches: what the native module declines ----------
+
+
+@pytest.mark.parametrize("news", [None, [300, 20]])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F32, 64)])
+def test_attention_launched_by_the_python_code_is_the_same(dtype, dim, news, monkeypatch):
+    p = Problem([1500, 200], news, 8, 2, dim, dtype, 16, window=400, sinks=3, fused=True)
+    workspace = p.launch()
+    out, lse = p.out.clone(), p.lse.clone()
+    p.out.fill_(-7)
+    p.lse.fill_(-7)
+    monkeypatch.setattr(_native, "host", lambda: Declining())
+    p.launch(workspace)
+    assert torch.equal(p.out, out) and torch.equal(p.lse, lse)
+    p.check()
+
+
+def test_heads_launched_by_the_python_code_are_the_same(monkeypatch):
+    t, hq, hk, d = 50, 6, 2, 128
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn((t, (hq + 2 * hk) * d), generator=g).to(BF16).cuda()
+    q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split((hq * d, hk * d, hk * d), 1))
+    wq, wk = (1 + torch.randn(d, generator=g).cuda() * 0.1 for _ in range(2))
+    cos, sin = attention.rope_tables(64, d)
+    positions, slots = torch.arange(t, device="cuda", dtype=torch.int32), torch.randperm(64, generator=g)[:t].cuda()
+
+    def run():
+        caches = torch.zeros((2, 4, 16, hk, d), dtype=BF16, device="cuda")
+        q_out, k_out, dq, dk = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, q, k))
+        attention.qk_norm_rope(q, k, positions, cos, sin, q_out, k_out, q_weight=wq, k_weight=wk, v=v, k_cache=caches[0], v_cache=caches[1], slots=slots)
+        dwq, dwk = torch.empty(d, device="cuda"), torch.empty(d, device="cuda")
+        attention.qk_norm_rope_backward(q, k, q, k, positions, cos, sin, dq, dk, q_weight=wq, k_weight=wk, dq_weight=dwq, dk_weight=dwk,
+                                        workspace=attention.make_gradient_workspace(d))
+        return caches, q_out, k_out, dq, dk, dwq, dwk
+
+    native = run()
+    monkeypatch.setattr(_native, "host", lambda: Declining())
+    assert all(torch.equal(a, b) for a, b in zip(native, run()))
+
+
+def test_block_tables_launched_by_the_python_code_are_right(monkeypatch):
+    monkeypatch.setattr(_native, "host", lambda: Declining())
+    step(mixed(70, 5), 16, seed=5, table_stride=3)
