@@ -554,6 +554,8 @@ typedef struct iris_attention_plan_info {
   int32_t parts; /* of a prompt unit's keys, at most; single tokens are cut into one equal run a workgroup where workspace_elems is not 0 */
 } iris_attention_plan_info;
 int iris_attention_plan(const iris_attention_args* args, int32_t num_cus, iris_attention_plan_info* plan);
+/* Registers of the kernel that iris_attention_launch would run for args, and its scratch bytes a lane. */
+int iris_attention_kernel_info(const iris_attention_args* args, int* n_regs, int* n_spills);
 
 /* Library version, bumped when a signature in this header changes. */
 int iris_amd_abi_version(void);

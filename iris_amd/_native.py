@@ -226,6 +226,7 @@ SIGNATURES = {
     "iris_attention_launch": (_I, [ctypes.POINTER(AttentionArgs), _P]),
     "iris_attention_workspace_elems": (ctypes.c_int64, [ctypes.c_int32]),
     "iris_attention_plan": (_I, [ctypes.POINTER(AttentionArgs), ctypes.c_int32, ctypes.POINTER(AttentionPlanInfo)]),
+    "iris_attention_kernel_info": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),
     "iris_amd_abi_version": (_I, []),
 }
 ALLOCATOR_SYMBOLS = ("finegrained_hipMalloc", "finegrained_hipFree")

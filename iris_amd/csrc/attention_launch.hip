@@ -143,6 +143,15 @@ hipError_t make_plan(const iris_attention_args& a, int cus, Plan* p) {
   return hipSuccess;
 }
 
+using Kernel = void (*)(AttentionKArgs);
+template <int DT, int DP, bool PG>
+Kernel kernel_of(int kernel, bool lse) {
+  if (kernel == IRIS_ATTENTION_DECODE) return rows::decode_kernel<DT, DP, PG>;
+  if constexpr (DT != IRIS_DTYPE_F32 && PG)
+    if (kernel == IRIS_ATTENTION_PROMPT_TILES) return lse ? tiles::prompt_tiles_kernel<DT, DP, true> : tiles::prompt_tiles_kernel<DT, DP, false>;
+  return rows::prompt_rows_kernel<DT, DP, PG>;
+}
+
 }  // namespace
 }  // namespace iris_amd
 
@@ -179,21 +188,9 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
       g.counters = (int32_t*)a.workspace;
       g.slots = a.workspace + COUNTERS;
     }
-    const unsigned workgroups = (unsigned)p.workgroups;
-    if (p.kernel == IRIS_ATTENTION_DECODE) {
-      rows::decode_kernel<DT, DP, PG><<<workgroups, rows::WAVES * 64, 0, s>>>(g);
-      return hipGetLastError();
-    }
-    if constexpr (DT != IRIS_DTYPE_F32 && PG) {
-      if (p.kernel == IRIS_ATTENTION_PROMPT_TILES) {
-        if (a.lse)
-          tiles::prompt_tiles_kernel<DT, DP, true><<<workgroups, tiles::WAVES * 64, 0, s>>>(g);
-        else
-          tiles::prompt_tiles_kernel<DT, DP, false><<<workgroups, tiles::WAVES * 64, 0, s>>>(g);
-        return hipGetLastError();
-      }
-    }
-    rows::prompt_rows_kernel<DT, DP, PG><<<dim3(workgroups / a.k_heads, a.k_heads), rows::WAVES * 64, 0, s>>>(g);
+    static_assert(tiles::WAVES == rows::WAVES, "one size of workgroups");
+    const unsigned heads = p.kernel == IRIS_ATTENTION_PROMPT_ROWS ? a.k_heads : 1;
+    kernel_of<DT, DP, PG>(p.kernel, a.lse)<<<dim3((unsigned)(p.workgroups / heads), heads), rows::WAVES * 64, 0, s>>>(g);
     return hipGetLastError();
   });
 }
@@ -211,5 +208,25 @@ extern "C" int iris_attention_plan(const iris_attention_args* args, int32_t num_
     const hipError_t refused = make_plan<dt.value, dp.value, pg.value>(a, num_cus ? num_cus : current_cu_count(), &p);
     if (refused == hipSuccess) *plan = iris_attention_plan_info{p.parted ? COUNTERS + p.parted : 0, p.workgroups, p.kernel, (int32_t)p.splits};
     return refused;
+  });
+}
+
+extern "C" int iris_attention_kernel_info(const iris_attention_args* args, int* n_regs, int* n_spills) {
+  using namespace iris_amd;
+  if (!args || !n_regs || !n_spills) return hipErrorInvalidValue;
+  const iris_attention_args& a = *args;
+  const hipError_t bad = check(a);
+  if (bad != hipSuccess) return bad;
+  if (a.tokens == 0 || a.q_heads == 0) return hipErrorInvalidValue;
+  return with_types(a, [&](auto dt, auto dp, auto pg) {
+    Plan p;
+    hipError_t err = make_plan<dt.value, dp.value, pg.value>(a, current_cu_count(), &p);
+    if (err != hipSuccess) return err;
+    hipFuncAttributes at;
+    err = hipFuncGetAttributes(&at, (const void*)kernel_of<dt.value, dp.value, pg.value>(p.kernel, a.lse));
+    if (err != hipSuccess) return err;
+    *n_regs = at.numRegs;
+    *n_spills = (int)at.localSizeBytes;
+    return hipSuccess;
   });
 }
