@@ -278,3 +278,24 @@ def test_heads_launched_by_the_python_code_are_the_same(monkeypatch):
 def test_block_tables_launched_by_the_python_code_are_right(monkeypatch):
     monkeypatch.setattr(_native, "host", lambda: Declining())
     step(mixed(70, 5), 16, seed=5, table_stride=3)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 8), (F16, 16), (BF16, 24), (F16, 72), (BF16, 120), (F16, 136), (BF16, 248), (F32, 4), (F32, 60), (F32, 132), (F32, 252)])
+def test_odd_head_sizes(dtype, dim):
+    for lengths, news, heads in (([300, 40, 0], None, (6, 2)), ([200, 33, 7], [150, 33, 1], (6, 2)), ([400, 200], [300, 130], (40, 20))):
+        p = Problem(lengths, news, *heads, dim, dtype, 16)
+        p.launch()
+        p.check()
+
+
+@pytest.mark.parametrize("slots", [6, 7, 33, 100, 513, 1000])
+def test_single_tokens_in_parts_of_a_small_workspace(slots, monkeypatch):
+    p = Problem([3000, 700], None, 8, 1, 64, BF16, 16)
+    workspace = torch.zeros(COUNTERS + slots * slot(64), device="cuda")
+    info = planned(p, workspace, monkeypatch)
+    assert COUNTERS < info.workspace_elems <= len(workspace) and info.workgroups > 2
+    p.launch(workspace)
+    p.check()
+    first = p.out.clone()
+    p.launch(workspace)
+    assert torch.equal(p.out, first) and bool((workspace[:COUNTERS].view(torch.int32) == 0).all())
