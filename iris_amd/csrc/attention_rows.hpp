@@ -12,8 +12,8 @@
 //            of keys meet in a register by one byte permute each (16-bit types; none for fp32).
 // At the end the four waves' maxima, sums and outputs meet in LDS; the parts of a split unit meet in the workspace.
 //
-// Single tokens, heads of 128: 606 MB of keys and values in 119 us, 5.1 TB/s, where a copy of 4 GB runs at 4.9; 56 MB in 20.6 us,
-// of which 10 are a chain of latencies, as is all of one request's 10.3 (1999 keys, 4 MB): launch 2.4, lengths and the cut of
+// Single tokens, heads of 128: 606 MB of keys and values in 116 us, 5.2 TB/s, where a copy of 4 GB runs at 4.9; 56 MB in 20.2 us,
+// of which 10 are a chain of latencies, as is all of one request's 9.9 (1999 keys, 4 MB): launch 2.4, lengths and the cut of
 // the line 1.5, table, keys and values 2.3 a step, the waves' meeting 1, hand-over 0.8, join 2.2.
 #pragma once
 
@@ -133,7 +133,7 @@ struct Unit {
     return first <= row.last_at && (a.window <= 0 || row.first_at - last < a.window || first < a.sinks);
   }
   // Steps of a tile that no row sees a key of (the wave's share of the last keys, of the window's edge, behind the first
-  // tokens) are left out: their loads all go to the request's first key.
+  // tokens) are left out: their loads all go to one key, the request's first or (where its page is none) the cache's.
   __device__ inline bool seen(const Piece& p, const Row& row, int j) {
     const int base = step_base(p, j);
     return some_see(row, base, base + C::KS - 1);
@@ -351,7 +351,9 @@ struct Unit {
         for (int e = 0; e < C::VE; ++e)
           o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[0][r][e]), __builtin_bit_cast(f32x4, w)[r], o[e], 0, 0, 0);
     } else {
-      // (the weights are in 16 bits, as the matrix instruction takes them: off by half a last place of the values' own type)
+      // The weights are in 16 bits, as the matrix instruction takes both its operands: off by half a last place of the values' own
+      // type, which the output is rounded to as well.  (Errors against 64 bits 0.0015 to 0.0016 of the output where fp32 weights
+      // have 0.0014 to 0.0015, fp16 4.9e-5 for 4.5e-5; a second product for the rest of each weight would double these instructions.)
 #pragma unroll
       for (int e = 0; e < C::VE; ++e) {
         u32x4 t;

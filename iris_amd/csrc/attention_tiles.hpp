@@ -12,11 +12,14 @@
 // (XOR) so that neither read meets its own banks; keys past the end and columns past the head are read out of
 // the buffer's range and arrive as zeros.
 //
-// bf16, heads of 128, four prompts of up to 8192 tokens (310 GFLOP): 325 to 332 us, 0.93 to 0.96 PFLOP/s, where a large matrix product runs at
-// 1.19; fp16, heads of 64, a window of 1024 (25 GFLOP): 51 to 52 us, 0.48.  The matrix cores are busy for 0.40 of the time and
-// vector instructions issue for 0.32, the one wave's beside the other's; the rest is LDS reads, barriers and
+// bf16, heads of 128, four prompts of up to 8192 tokens (310 GFLOP): 327 to 335 us, 0.93 to 0.95 PFLOP/s, where a large matrix product runs at
+// 1.19; fp16, heads of 64, a window of 1024 (25 GFLOP): 51 to 52 us, 0.48.  The matrix cores are busy for 0.41 of the time and
+// vector instructions issue for 0.33, the one wave's beside the other's; the rest is LDS reads, barriers and
 // power (zeros take an eighth less).  Tiles of 64 rows a wave, or a tile's scores taken ahead of the last one's values, took
 // more registers than there are and 394 us and more.
+// The waves take all the registers that so many a SIMD have, and spill: 15 to 21 words a lane for heads of 64, 21 to 26 for 128, of
+// which the loop reads none (with log-sums one); 90 for heads of 256, whose loop reads eight, behind a wait that the next tile's
+// loads are part of (0.59 PFLOP/s on prompts of 4096 and 2500 tokens, 8 + 2 heads, where heads of 128 have 0.48).
 #pragma once
 
 #include "attention_rows.hpp"
@@ -358,6 +361,8 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
         for (int e = 0; e < 8; ++e) {
           w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * i + e], g.scale_log2, -from));
         }
+        // (in 16 bits for the product with the values, and summed as rounded: bf16 outputs are off by 0.0022 of themselves, fp16 by
+        // 0.00026, where fp32 weights have 0.0017 and 0.00021; the rest of each weight would be half as many matrix instructions again)
         p[2 * u + i] = u32x4{pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[e] = add_weights<DT>(p[2 * u + i][e], sums[e]);

@@ -321,8 +321,8 @@ __global__ __launch_bounds__(THREADS) void qk_norm_rope_backward_kernel(Backward
         if (weight) {
           Wide<V, ITEMS> y;
           y.get(x[u]);
-          // dx is what is left of g w when its part along x is taken out: in short heads very little, so those (which single
-          // pairs serve) take it out in 64 bits
+          // dx is what is left of g w when its part along x is taken out: of heads of two elements very little.  Those are laid out as
+          // single pairs, and single pairs (heads of any size whose sizes or addresses allow no runs of four) take it out in 64 bits.
           using Acc = std::conditional_t<V == 1, double, float>;
           Acc square = 0, along = 0;
 #pragma unroll
