@@ -174,7 +174,6 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
   g.page = make_page_div((uint32_t)a.page_size);
   g.scale_log2 = a.scale * 1.4426950408889634f;
   g.group = a.q_heads / a.k_heads;
-  const hipStream_t s = (hipStream_t)stream;
   return with_types(a, [&](auto dt, auto dp, auto pg) {
     constexpr int DT = dt.value, DP = dp.value;
     constexpr bool PG = pg.value;
@@ -190,8 +189,7 @@ extern "C" int iris_attention_launch(const iris_attention_args* args, void* stre
     }
     static_assert(tiles::WAVES == rows::WAVES, "one size of workgroups");
     const unsigned heads = p.kernel == IRIS_ATTENTION_PROMPT_ROWS ? a.k_heads : 1;
-    kernel_of<DT, DP, PG>(p.kernel, a.lse)<<<dim3((unsigned)(p.workgroups / heads), heads), rows::WAVES * 64, 0, s>>>(g);
-    return hipGetLastError();
+    return launch(kernel_of<DT, DP, PG>(p.kernel, a.lse), dim3((unsigned)(p.workgroups / heads), heads), rows::WAVES * 64, 0, stream, g);
   });
 }
 

@@ -202,9 +202,7 @@ extern "C" int iris_block_tables_launch(const iris_block_tables_args* args, void
       const hipError_t err = hipFuncSetAttribute((const void*)block_tables_kernel<ITEMS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
       if (err != hipSuccess) return err;
     }
-    block_tables_kernel<ITEMS><<<grid, threads, lds, (hipStream_t)stream>>>(g);
-  } else {
-    block_tables_kernel<1><<<grid, threads, lds, (hipStream_t)stream>>>(g);
+    return launch(block_tables_kernel<ITEMS>, dim3(grid), threads, lds, stream, g);
   }
-  return hipGetLastError();
+  return launch(block_tables_kernel<1>, dim3(grid), threads, lds, stream, g);
 }

@@ -6,6 +6,13 @@
 
 namespace iris_amd {
 
+// Launches a kernel; its own status, whatever error an earlier call of the thread has left.
+template <class Args>
+inline hipError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t lds, void* stream, Args args) {
+  void* const list[] = {&args};
+  return hipLaunchKernel((const void*)kernel, grid, dim3(threads), const_cast<void**>(list), lds, (hipStream_t)stream);
+}
+
 // Division by the launch's page size for dividends below 2^31: with s = ceil(log2 d), m = ceil(2^(31 + s) / d) < 2^32 + 1 and
 // m d - 2^(31 + s) < 2^s, so that floor(n m / 2^(31 + s)) = floor(n / d) for n < 2^31.
 struct PageDiv {

@@ -373,18 +373,23 @@ __global__ __launch_bounds__(THREADS) void qk_norm_rope_backward_kernel(Backward
 // Adds the workgroups' partial sums, those of the queries' weight in the first `q_rows` rows and of the keys' in the next `k_rows`:
 // 16 columns a workgroup, 64 lanes a column.
 constexpr int SUM_THREADS = 1024;
-__global__ __launch_bounds__(SUM_THREADS) void weight_gradient_kernel(const float* partials, int q_rows, int k_rows, int dim, float* dq_weight,
-                                                                      float* dk_weight) {
+struct SumArgs {
+  const float* partials;
+  int q_rows, k_rows, dim;
+  float* dq_weight;
+  float* dk_weight;
+};
+__global__ __launch_bounds__(SUM_THREADS) void weight_gradient_kernel(SumArgs a) {
   __shared__ float sums[SUM_THREADS / 16][17];
   const int c = threadIdx.x % 16, part = threadIdx.x / 16, column = blockIdx.x * 16 + c;
   const bool keys = blockIdx.y;
-  float* out = keys ? dk_weight : dq_weight;
+  float* out = keys ? a.dk_weight : a.dq_weight;
   if (!out) return;
-  const int begin = keys ? q_rows : 0, end = keys ? q_rows + k_rows : q_rows;
+  const int begin = keys ? a.q_rows : 0, end = keys ? a.q_rows + a.k_rows : a.q_rows;
   float sum = 0.f;
-  if (column < dim) {
+  if (column < a.dim) {
 #pragma unroll 4
-    for (int r = begin + part; r < end; r += SUM_THREADS / 16) sum += partials[(int64_t)r * dim + column];
+    for (int r = begin + part; r < end; r += SUM_THREADS / 16) sum += a.partials[(int64_t)r * a.dim + column];
   }
   sums[part][c] = sum;
   __syncthreads();
@@ -392,7 +397,7 @@ __global__ __launch_bounds__(SUM_THREADS) void weight_gradient_kernel(const floa
     if (part < n) sums[part][c] += sums[part + n][c];
     __syncthreads();
   }
-  if (part == 0 && column < dim) out[column] = sums[0][c];
+  if (part == 0 && column < a.dim) out[column] = sums[0][c];
 }
 
 bool known_dtype(int dt) { return dt == IRIS_DTYPE_F32 || dt == IRIS_DTYPE_F16 || dt == IRIS_DTYPE_BF16; }
@@ -467,8 +472,7 @@ extern "C" int iris_qk_norm_rope_launch(const iris_qk_norm_rope_args* args, void
                         make_kind(a.tokens, a.v ? a.k_heads : 0, each, per_block)}};
       const int64_t grid = (int64_t)f.kinds[0].blocks + f.kinds[1].blocks + f.kinds[2].blocks;
       if (grid > INT32_MAX) return hipErrorInvalidValue;
-      qk_norm_rope_kernel<dt.value, v.value, lanes.value, items.value><<<(int)grid, THREADS, 0, (hipStream_t)stream>>>(f);
-      return hipGetLastError();
+      return launch(qk_norm_rope_kernel<dt.value, v.value, lanes.value, items.value>, dim3((unsigned)grid), THREADS, 0, stream, f);
     });
   });
 }
@@ -514,12 +518,14 @@ extern "C" int iris_qk_norm_rope_backward_launch(const iris_qk_norm_rope_backwar
       }
       const int q_blocks = f.kinds[0].blocks, k_blocks = f.kinds[1].blocks;
       const size_t lds = weights ? per_block * a.head_dim * sizeof(float) : 0;
-      if (q_blocks + k_blocks) qk_norm_rope_backward_kernel<dt.value, v.value, lanes.value, items.value><<<q_blocks + k_blocks, THREADS, lds, (hipStream_t)stream>>>(f);
-      hipError_t err = hipGetLastError();
-      if (err != hipSuccess || !weights) return err;
-      weight_gradient_kernel<<<dim3((a.head_dim + 15) / 16, 2), SUM_THREADS, 0, (hipStream_t)stream>>>(a.workspace, q_blocks, k_blocks, a.head_dim,
-                                                                                                      a.dq_weight, a.dk_weight);
-      return hipGetLastError();
+      if (q_blocks + k_blocks) {
+        const hipError_t err =
+            launch(qk_norm_rope_backward_kernel<dt.value, v.value, lanes.value, items.value>, dim3(q_blocks + k_blocks), THREADS, lds, stream, f);
+        if (err != hipSuccess) return err;
+      }
+      if (!weights) return hipSuccess;
+      return launch(weight_gradient_kernel, dim3((a.head_dim + 15) / 16, 2), SUM_THREADS, 0, stream,
+                    SumArgs{a.workspace, q_blocks, k_blocks, a.head_dim, a.dq_weight, a.dk_weight});
     });
   });
 }

@@ -299,3 +299,36 @@ def test_single_tokens_in_parts_of_a_small_workspace(slots, monkeypatch):
     first = p.out.clone()
     p.launch(workspace)
     assert torch.equal(p.out, first) and bool((workspace[:COUNTERS].view(torch.int32) == 0).all())
+
+
+def test_an_error_that_an_earlier_call_left_is_not_a_launchs(monkeypatch):
+    """What a call reports is its own launch's status, by the native module's way and by the Python code's."""
+    t, hq, hk, d = 5, 4, 2, 64
+    q, k, dq_out, dk_out = (torch.randn((t, h, d), device="cuda").to(BF16) for h in (hq, hk, hq, hk))
+    cos, sin = attention.rope_tables(16, d)
+    positions, weight = torch.arange(t, device="cuda", dtype=torch.int32), torch.ones(d, device="cuda")
+    q_out, k_out, dq, dk, dw = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q), torch.empty_like(k), torch.empty(d, device="cuda")
+    room = attention.make_gradient_workspace(d)
+    p, prompts = Problem([50, 20], None, 4, 2, 64, BF16, 16), Problem([50, 20], [30, 20], 4, 2, 64, BF16, 16)
+    workspace = attention.make_workspace(64)
+    i32, i64 = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    tables = [i32.clone() for _ in range(2)] + [torch.zeros((3, 4), dtype=torch.int32, device="cuda"), i32.clone(), i64[:2].clone(), 16]
+    written = dict(lengths=i32.clone(), pool_state_out=i64[:2].clone(), query_starts=torch.zeros(4, dtype=torch.int32, device="cuda"),
+                   positions=i32.clone(), slots=i64.clone())
+    calls = [lambda: p.launch(workspace), lambda: prompts.launch(workspace), lambda: attention.qk_norm_rope(q, k, positions, cos, sin, q_out, k_out),
+             lambda: attention.qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, dq, dk, q_weight=weight, dq_weight=dw, workspace=room),
+             lambda: attention.build_block_tables(*tables, **written)]
+    torch.cuda.synchronize()
+    loaded = {line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line}
+    assert len(loaded) == 1
+    hip = ctypes.CDLL(loaded.pop())
+    for host in (_native.host(), Declining()):
+        monkeypatch.setattr(_native, "host", lambda: host)
+        for call in calls:
+            call()
+            assert _native.lib().iris_hip_set_device(9999) != 0
+            call()
+            assert hip.hipGetLastError() == 101  # (still there for whom it concerns; cleared)
+    torch.cuda.synchronize()
+    p.check()
+    prompts.check()
