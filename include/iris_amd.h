@@ -78,6 +78,9 @@ int iris_hip_arch_name(int device, char* buf, size_t len);
 #define IRIS_DTYPE_I8 3
 #define IRIS_DTYPE_I16 4
 #define IRIS_DTYPE_I32 5
+/* 8-bit floats, the codes of a quantised cache: 4 bits of exponent and 3 of fraction (no infinity), 5 and 2 */
+#define IRIS_DTYPE_E4M3 6
+#define IRIS_DTYPE_E5M2 7
 #define IRIS_DTYPE_I64 6
 
 /* epilogues of the persistent shard GEMM */
@@ -556,6 +559,80 @@ typedef struct iris_attention_plan_info {
 int iris_attention_plan(const iris_attention_args* args, int32_t num_cus, iris_attention_plan_info* plan);
 /* Registers of the kernel that iris_attention_launch would run for args, and its scratch bytes a lane. */
 int iris_attention_kernel_info(const iris_attention_args* args, int* n_regs, int* n_spills);
+
+/*
+ * A paged cache in 8 bits: codes (8-bit floats, `code` IRIS_DTYPE_E4M3 or _E5M2) laid out as the 16-bit cache is, strides in elements,
+ * and for every `block` tokens of a page (a multiple of 16 that divides the page size) and key head a scale: a power of two 2^(x - 127) held
+ * as the byte x (255: not a number).  Element = code * scale.  Scales lie at k_scales / v_scales[page][row / block][head], strides
+ * in bytes.  head_dim is a multiple of 16 up to 256, and every head begins at a multiple of 16 bytes.
+ */
+typedef struct iris_cache_scales {
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  int64_t stride_ks_page, stride_ks_block, stride_ks_head, stride_vs_page, stride_vs_block, stride_vs_head;
+  int32_t block, code;
+} iris_cache_scales;
+
+/*
+ * Attention over such a cache: args as in iris_attention_launch (dtype that of q and out), k_cache and v_cache the codes.  The products are
+ * taken in dtype, in which a code times its scale is a number without rounding as long as it is in dtype's range.
+ */
+int iris_quantized_attention_launch(const iris_attention_args* args, const iris_cache_scales* scales, void* stream);
+int iris_quantized_attention_plan(const iris_attention_args* args, const iris_cache_scales* scales, int32_t num_cus, iris_attention_plan_info* plan);
+int iris_quantized_attention_kernel_info(const iris_attention_args* args, const iris_cache_scales* scales, int* n_regs, int* n_spills);
+
+/*
+ * Keys and values of new tokens into such a cache.  Token t goes to slots[t] (a negative slot is skipped; one past num_slots is
+ * reported and skipped).  The new tokens of a block are neighbours in k and v with slots in a row; one that follows a token of
+ * its own block at any other slot is reported and skipped, and no block may come up again further on.  Rows of a block before
+ * its first new one are earlier tokens and stay, rows behind the last new one are left as they are and count as empty.
+ * A block's scale becomes the smallest power of two, 2^-100 at least, by which the largest finite new element does not exceed the largest code
+ * (448 or 57344), or stays as it is where earlier tokens have a larger one; earlier tokens' codes are rounded to a scale
+ * that grew.  Roundings are to nearest, ties to even; what is not finite becomes the code that is not a number.
+ */
+typedef struct iris_write_cache_args {
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  uint8_t* k_scales;
+  uint8_t* v_scales;
+  const int64_t* slots;
+  uint32_t* status;
+  int64_t stride_kt, stride_kh, stride_vt, stride_vh;
+  int64_t stride_kc_page, stride_kc_row, stride_kc_head, stride_vc_page, stride_vc_row, stride_vc_head;
+  int64_t stride_ks_page, stride_ks_block, stride_ks_head, stride_vs_page, stride_vs_block, stride_vs_head;
+  int64_t num_slots;
+  int32_t tokens, heads, head_dim, page_size, block, dtype, code;
+} iris_write_cache_args;
+
+int iris_write_quantized_cache_launch(const iris_write_cache_args* args, void* stream);
+
+/*
+ * Cached tokens read back: rows [starts[i], starts[i + 1]) of k_out and v_out [tokens][heads][head_dim] (fp32, fp16 or bf16; rounded to
+ * nearest) take the tokens at the last positions of request i's lengths[i], which block_table[i] has the pages of.  Rows of no
+ * request stay as they are.  A row whose position is negative or past the table's room, or whose page lies outside the cache, is reported
+ * and not a number.
+ */
+typedef struct iris_read_cache_args {
+  const void* k_cache;
+  const void* v_cache;
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  const int32_t* block_table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  void* k_out;
+  void* v_out;
+  uint32_t* status;
+  int64_t stride_kt, stride_kh, stride_vt, stride_vh;
+  int64_t stride_kc_page, stride_kc_row, stride_kc_head, stride_vc_page, stride_vc_row, stride_vc_head;
+  int64_t stride_ks_page, stride_ks_block, stride_ks_head, stride_vs_page, stride_vs_block, stride_vs_head;
+  int64_t stride_table;
+  int32_t requests, tokens, heads, head_dim, page_size, table_width, num_pages, block, dtype, code;
+} iris_read_cache_args;
+
+int iris_read_quantized_cache_launch(const iris_read_cache_args* args, void* stream);
 
 /* Library version, bumped when a signature in this header changes. */
 int iris_amd_abi_version(void);

@@ -19,6 +19,7 @@ TESTING_LIB_PATH = os.path.join(_PKG_DIR, "libiris_amd_testing.so")
 
 # element types (IRIS_DTYPE_*)
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+DTYPE_E4M3, DTYPE_E5M2 = 6, 7  # codes of a quantised cache
 # epilogues (IRIS_EPI_*)
 EPI_ALL_SCATTER, EPI_ATOMIC_ADD, EPI_ONE_SHOT = 0, 1, 2
 # ONE_SHOT phases (IRIS_PHASE_*)
@@ -182,6 +183,40 @@ class AttentionPlanInfo(ctypes.Structure):
     _fields_ = _fields((ctypes.c_int64, "workspace_elems workgroups"), (ctypes.c_int32, "kernel parts"))
 
 
+class CacheScales(ctypes.Structure):
+    """``iris_cache_scales``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "k_scales v_scales"),
+        (ctypes.c_int64, "stride_ks_page stride_ks_block stride_ks_head stride_vs_page stride_vs_block stride_vs_head"),
+        (ctypes.c_int32, "block code"),
+    )
+
+
+class WriteCacheArgs(ctypes.Structure):
+    """``iris_write_cache_args``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "k v k_cache v_cache k_scales v_scales slots status"),
+        (ctypes.c_int64, "stride_kt stride_kh stride_vt stride_vh"),
+        (ctypes.c_int64, "stride_kc_page stride_kc_row stride_kc_head stride_vc_page stride_vc_row stride_vc_head"),
+        (ctypes.c_int64, "stride_ks_page stride_ks_block stride_ks_head stride_vs_page stride_vs_block stride_vs_head num_slots"),
+        (ctypes.c_int32, "tokens heads head_dim page_size block dtype code"),
+    )
+
+
+class ReadCacheArgs(ctypes.Structure):
+    """``iris_read_cache_args``."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "k_cache v_cache k_scales v_scales block_table lengths starts k_out v_out status"),
+        (ctypes.c_int64, "stride_kt stride_kh stride_vt stride_vh"),
+        (ctypes.c_int64, "stride_kc_page stride_kc_row stride_kc_head stride_vc_page stride_vc_row stride_vc_head"),
+        (ctypes.c_int64, "stride_ks_page stride_ks_block stride_ks_head stride_vs_page stride_vs_block stride_vs_head stride_table"),
+        (ctypes.c_int32, "requests tokens heads head_dim page_size table_width num_pages block dtype code"),
+    )
+
+
 ATTENTION_NOTHING, ATTENTION_DECODE, ATTENTION_PROMPT_TILES, ATTENTION_PROMPT_ROWS = 0, 1, 2, 3
 
 
@@ -227,6 +262,13 @@ SIGNATURES = {
     "iris_attention_workspace_elems": (ctypes.c_int64, [ctypes.c_int32]),
     "iris_attention_plan": (_I, [ctypes.POINTER(AttentionArgs), ctypes.c_int32, ctypes.POINTER(AttentionPlanInfo)]),
     "iris_attention_kernel_info": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),
+    "iris_quantized_attention_launch": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), _P]),
+    "iris_quantized_attention_plan": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), ctypes.c_int32,
+                                           ctypes.POINTER(AttentionPlanInfo)]),
+    "iris_quantized_attention_kernel_info": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), ctypes.POINTER(ctypes.c_int),
+                                                  ctypes.POINTER(ctypes.c_int)]),
+    "iris_write_quantized_cache_launch": (_I, [ctypes.POINTER(WriteCacheArgs), _P]),
+    "iris_read_quantized_cache_launch": (_I, [ctypes.POINTER(ReadCacheArgs), _P]),
     "iris_amd_abi_version": (_I, []),
 }
 ALLOCATOR_SYMBOLS = ("finegrained_hipMalloc", "finegrained_hipFree")

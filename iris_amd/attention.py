@@ -18,9 +18,17 @@ tensors they are given, and neither synchronise nor allocate.  What only the
 device can see (an index outside of what it indexes, a ring of free pages
 that runs out) is OR-ed into an optional ``status`` word, as ``STATUS_*`` bits.
 
+A cache may be kept in 8 bits instead:
+
+    write_quantized_cache  keys and values of new tokens into it (qk_norm_rope then writes none)
+    decode_attention, prompt_attention  over it, with ``k_scales`` and ``v_scales``
+    read_quantized_cache   cached tokens as 16-bit or fp32 heads again
+
 A cache is a tensor ``[pages, page_size, key heads, head size]`` in any order
 of memory whose head elements are contiguous; ``block_table[i, j]`` is the page of request i's
-tokens ``[j * page_size, (j + 1) * page_size)``.
+tokens ``[j * page_size, (j + 1) * page_size)``.  One in 8 bits holds codes (``torch.float8_e4m3fn`` or ``torch.float8_e5m2``) and beside them
+``k_scales`` and ``v_scales`` ``torch.float8_e8m0fnu`` [pages, blocks of a page, key heads], a power of two for every block of
+``page_size // blocks`` tokens (a multiple of 16) and head: an element is its code times its block's scale.
 """
 
 from __future__ import annotations
@@ -43,6 +51,9 @@ __all__ = [
     "QkNormRope",
     "decode_attention",
     "prompt_attention",
+    "make_quantized_cache",
+    "write_quantized_cache",
+    "read_quantized_cache",
     "make_workspace",
     "make_gradient_workspace",
     "STATUS_BAD_INDEX",
@@ -131,6 +142,61 @@ def _cache(name, t, device, dtype, heads, dim):
         raise ValueError(f"{name}: the elements of a head must be contiguous")
 
 
+_CODES = {torch.float8_e4m3fn: _native.DTYPE_E4M3, torch.float8_e5m2: _native.DTYPE_E5M2}
+
+
+def _quantized(a, scales, k_cache, v_cache, k_scales, v_scales, device, heads, dim):
+    """Checks a cache in 8 bits; its strides go to ``a``, those of its scales to ``scales``."""
+    _require_cuda("k_cache", k_cache, device)
+    if k_cache.dtype not in _CODES:
+        raise TypeError(f"k_cache: a cache with scales holds float8_e4m3fn or float8_e5m2, got {k_cache.dtype}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _cache(name, t, device, k_cache.dtype, heads, dim)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape")
+    if dim % 16 or not 0 < dim <= MAX_ATTENTION_HEAD_DIM:
+        raise ValueError(f"the head size of a cache in 8 bits must be a multiple of 16 and at most {MAX_ATTENTION_HEAD_DIM}, got {dim}")
+    pages, page_size = k_cache.shape[:2]
+    if k_scales is None or v_scales is None:
+        raise ValueError("k_scales and v_scales come together")
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        _require_cuda(name, t, device)
+        if t.dtype != torch.float8_e8m0fnu or t.dim() != 3:
+            raise TypeError(f"{name} must be float8_e8m0fnu [pages, blocks of a page, key heads], got {t.dtype} {tuple(t.shape)}")
+        if t.shape[0] != pages or t.shape[2] != heads:
+            raise ValueError(f"{name} is for {t.shape[0]} pages of {t.shape[2]} heads, the cache has {pages} of {heads}")
+        if t.shape[1] < 1 or page_size % t.shape[1] or page_size // t.shape[1] % 16:
+            raise ValueError(f"{name}: {t.shape[1]} blocks do not cut pages of {page_size} tokens into blocks of a multiple of 16")
+    if k_scales.shape != v_scales.shape:
+        raise ValueError("k_scales and v_scales must have the same shape")
+    a.stride_kc_page, a.stride_kc_row, a.stride_kc_head = _steps(k_cache, 3)
+    a.stride_vc_page, a.stride_vc_row, a.stride_vc_head = _steps(v_cache, 3)
+    a.k_cache, a.v_cache, a.page_size = _ptr(k_cache), _ptr(v_cache), page_size
+    scales.k_scales, scales.v_scales = _ptr(k_scales), _ptr(v_scales)
+    scales.stride_ks_page, scales.stride_ks_block, scales.stride_ks_head = _steps(k_scales, 3)
+    scales.stride_vs_page, scales.stride_vs_block, scales.stride_vs_head = _steps(v_scales, 3)
+    scales.block, scales.code = page_size // k_scales.shape[1], _CODES[k_cache.dtype]
+
+
+def _aligned(*operands):
+    for name, t in operands:
+        vec = 16 // t.element_size()
+        if t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+            raise ValueError(f"{name}: every head must begin at a multiple of 16 bytes")
+
+
+def _block_table(block_table, device, page_size):
+    _require_cuda("block_table", block_table, device)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise TypeError("block_table must be an int32 matrix with contiguous rows")
+    requests, width = block_table.shape
+    if requests > 1 and block_table.stride(0) < width:
+        raise ValueError("the rows of block_table must not overlap")
+    if width * page_size > INT32_MAX:
+        raise ValueError("block_table has room for more tokens than 31 bits count")
+    return requests, width
+
+
 def _tangent(t):
     return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
 
@@ -158,7 +224,8 @@ def _native_call(err):
 
 
 def _rest(err, name, args, device):
-    """Launches a call that the native code declined.  Any other status may have come from behind a launch, which is not made again."""
+    """Launches a call that the native code declined.  Any other status may have come from behind a launch, which is not made again.
+    ``args``: the call's struct, or a tuple of them."""
     if err != DECLINED:
         _rejected(name)
     _launch(name, args, device)
@@ -171,7 +238,7 @@ def _rejected(name):
 def _launch(name, args, device):
     stream = torch.cuda.current_stream(device).cuda_stream
     with torch.cuda.device(device):
-        err = getattr(_native.lib(), name)(ctypes.byref(args), stream)
+        err = getattr(_native.lib(), name)(*map(ctypes.byref, args if isinstance(args, tuple) else (args,)), stream)
     if err == _native.HIP_ERROR_INVALID_VALUE:
         _rejected(name)
     _native.hip_try(err)
@@ -552,9 +619,14 @@ def _without_a_page(out, lse, status, lengths, query_starts, room):
         status.view(torch.int32).as_strided((1,), (1,)).bitwise_or_(bits)
 
 
-def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status):
-    err = _native.host().attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale,
-                                   window, sinks)
+def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status, k_scales, v_scales):
+    quantized = k_scales is not None or v_scales is not None
+    if quantized:
+        err = _native.host().quantized_attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status,
+                                                 k_scales, v_scales, scale, window, sinks)
+    else:
+        err = _native.host().attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale,
+                                       window, sinks)
     if _native_call(err):
         return
     device, dtype = q.device, q.dtype
@@ -567,32 +639,27 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     if k_cache.dim() != 4:
         raise ValueError(f"k_cache must be [pages, page_size, key heads, head size], got {tuple(k_cache.shape)}")
     pages, page_size, hk, _ = k_cache.shape
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _cache(name, t, device, dtype, hk, dim)
-    if v_cache.shape != k_cache.shape:
-        raise ValueError("k_cache and v_cache must have the same shape")
+    a, cache_scales = _native.AttentionArgs(), _native.CacheScales()
+    if quantized:
+        _quantized(a, cache_scales, k_cache, v_cache, k_scales, v_scales, device, hk, dim)
+    else:
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            _cache(name, t, device, dtype, hk, dim)
+        if v_cache.shape != k_cache.shape:
+            raise ValueError("k_cache and v_cache must have the same shape")
     if hk == 0 or hq % hk:
         raise ValueError(f"{hq} query heads do not divide over {hk} key heads")
     vec = 16 // q.element_size()
     if dim % vec or not 0 < dim <= MAX_ATTENTION_HEAD_DIM:
         raise ValueError(f"the head size must be a multiple of {vec} and at most {MAX_ATTENTION_HEAD_DIM}, got {dim}")
-    for name, t in (("q", q), ("out", out), ("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
-            raise ValueError(f"{name}: every head must begin at a multiple of 16 bytes")
-    _require_cuda("block_table", block_table, device)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise TypeError("block_table must be an int32 matrix with contiguous rows")
-    requests, width = block_table.shape
-    if requests > 1 and block_table.stride(0) < width:
-        raise ValueError("the rows of block_table must not overlap")
+    _aligned(("q", q), ("out", out), ("k_cache", k_cache), ("v_cache", v_cache))
+    requests, width = _block_table(block_table, device, page_size)
     _ints("lengths", lengths, device, torch.int32, requests)
     if query_starts is None:
         if requests != tokens:
             raise ValueError(f"{tokens} queries for {requests} requests; decode_attention takes one each")
     else:
         _ints("query_starts", query_starts, device, torch.int32, requests + 1)
-    if width * page_size > INT32_MAX:
-        raise ValueError("block_table has room for more tokens than 31 bits count")
     if scale is None:
         scale = dim ** -0.5
     if not 0 < scale < math.inf:
@@ -602,7 +669,6 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     _no_gradient(q, k_cache, v_cache)
     _output("out", out)
     _status(status, device)
-    a = _native.AttentionArgs()
     if lse is not None:
         _require_cuda("lse", lse, device)
         if lse.dtype != torch.float32 or lse.shape != (tokens, hq) or (hq > 1 and lse.stride(1) != 1):
@@ -615,8 +681,8 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
             raise TypeError("workspace must be contiguous fp32 at a multiple of 16 bytes (make_workspace)")
         a.workspace, a.workspace_elems = _ptr(workspace), workspace.numel()
     _apart([("out", out), ("lse", lse), ("workspace", workspace)],
-           [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("lengths", lengths), ("query_starts", query_starts)],
-           [("out", "q")])
+           [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("lengths", lengths), ("query_starts", query_starts),
+            ("k_scales", k_scales), ("v_scales", v_scales)], [("out", "q")])
     if tokens == 0 or hq == 0:
         return
     if requests == 0:
@@ -635,7 +701,10 @@ def _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, sca
     a.page_size, a.table_width, a.num_pages = page_size, width, pages
     # (no context is longer than 31 bits count, so that the most they hold is all keys)
     a.window, a.sinks, a.dtype, a.scale = min(window, INT32_MAX), min(sinks, INT32_MAX), _DTYPES[dtype], scale
-    _rest(err, "iris_attention_launch", a, device)
+    if quantized:
+        _rest(err, "iris_quantized_attention_launch", (a, cache_scales), device)
+    else:
+        _rest(err, "iris_attention_launch", a, device)
 
 
 def _steps(t, n):
@@ -644,7 +713,7 @@ def _steps(t, n):
 
 
 def decode_attention(q, k_cache, v_cache, block_table, lengths, out, *, scale: Optional[float] = None, window=0, sinks=0, lse=None,
-                     workspace=None, status=None):
+                     workspace=None, status=None, k_scales=None, v_scales=None):
     """Attention of one new token a request over the paged cache.
 
     ``q`` and ``out`` [requests, query heads, head size] (fp16, bf16 or fp32);
@@ -658,12 +727,15 @@ def decode_attention(q, k_cache, v_cache, block_table, lengths, out, *, scale: O
     the sum of the rounded ones; sums are fp32 (and values times the number of keys have to stay in its range).  A
     table's entry need be no page where no query sees one of its keys: pages behind a window may be given back.
     ``out`` may be ``q``, and shares no other memory with an operand.
+
+    With ``k_scales`` and ``v_scales`` the cache is one in 8 bits (``write_quantized_cache``; head sizes that are multiples of 16): its elements,
+    codes times scales, are taken as numbers of the heads' type, which holds them without rounding as long as they are in its range.
     """
-    _attention(q, k_cache, v_cache, block_table, lengths, None, out, scale, window, sinks, lse, workspace, status)
+    _attention(q, k_cache, v_cache, block_table, lengths, None, out, scale, window, sinks, lse, workspace, status, k_scales, v_scales)
 
 
 def prompt_attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, *, scale: Optional[float] = None, window=0,
-                     sinks=0, lse=None, workspace=None, status=None):
+                     sinks=0, lse=None, workspace=None, status=None, k_scales=None, v_scales=None):
     """Causal attention of many new tokens a request over the paged cache.
 
     Request i's queries are the tokens ``query_starts[i] .. query_starts[i + 1]`` of ``q`` [tokens, query heads, head size] and stand at the last
@@ -671,4 +743,103 @@ def prompt_attention(q, k_cache, v_cache, block_table, lengths, query_starts, ou
     keys up to its own position.  With ``window`` > 0 it sees the last ``window`` of
     them and the request's first ``sinks``.  Rows of ``out`` past the last request's stay as they are.  The rest is as in ``decode_attention``.
     """
-    _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status)
+    _attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, scale, window, sinks, lse, workspace, status, k_scales, v_scales)
+
+
+# ---- a cache in 8 bits -------------------------------------------------------
+
+
+def make_quantized_cache(pages, page_size, heads, head_dim, *, block=None, dtype=torch.float8_e4m3fn, device="cuda"):
+    """(k_cache, v_cache, k_scales, v_scales) of a cache in 8 bits, zeros: ``dtype`` the codes', ``block`` tokens to a scale (a page's by default).
+    float8_e4m3fn keeps four significant bits over 15 powers of two below a block's largest element, float8_e5m2 three over 30."""
+    block = page_size if block is None else block
+    if dtype not in _CODES:
+        raise TypeError(f"codes are float8_e4m3fn or float8_e5m2, got {dtype}")
+    if pages < 0 or heads < 0 or block < 1 or block % 16 or page_size < 1 or page_size % block:
+        raise ValueError(f"pages of {page_size} tokens are not made of blocks of {block}, or those are no multiple of 16")
+    if head_dim % 16 or not 0 < head_dim <= MAX_ATTENTION_HEAD_DIM:
+        raise ValueError(f"the head size of a cache in 8 bits must be a multiple of 16 and at most {MAX_ATTENTION_HEAD_DIM}, got {head_dim}")
+    caches = (torch.zeros((pages, page_size, heads, head_dim), dtype=dtype, device=device) for _ in range(2))
+    scales = (torch.full((pages, page_size // block, heads), 127, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu) for _ in range(2))
+    return (*caches, *scales)
+
+
+def write_quantized_cache(k, v, k_cache, v_cache, k_scales, v_scales, slots, *, status=None):
+    """Keys and values of new tokens into a cache in 8 bits.
+
+    ``k`` and ``v`` [tokens, key heads, head size] (fp16, bf16 or fp32; views of a fused projection's output will do) go to
+    ``slots`` int64 [tokens], as ``build_block_tables`` makes them: a negative slot is skipped, and the new tokens of a block are neighbours, at
+    slots in a row.  (A token that follows one of its own block at any other slot is skipped and sets ``STATUS_BAD_INDEX``, as a slot outside of
+    the cache does; no block may be come back to further on in the same call.)
+
+    A block's rows before its first new one are its earlier tokens, and rows behind the last new one count as empty.  Its scale (for
+    each head, keys and values apart) becomes the smallest power of two, 2^-100 at least, by which the largest of the new elements does not
+    exceed the largest code (448 or 57344); a larger one that earlier tokens have stays.  Where it grows, the earlier tokens' codes are
+    rounded to it.  Roundings are to nearest, ties to even.  Elements that are not finite become NaN and have no part in a scale.
+    """
+    err = _native.host().write_quantized_cache(k, v, k_cache, v_cache, k_scales, v_scales, slots, status)
+    if _native_call(err):
+        return
+    device, dtype = k.device, k.dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"k: unsupported dtype {dtype}")
+    _heads("k", k, device)
+    tokens, heads, dim = k.shape
+    _heads("v", v, device, dtype, tokens, heads, dim)
+    a = _native.WriteCacheArgs()
+    _quantized(a, a, k_cache, v_cache, k_scales, v_scales, device, heads, dim)
+    _ints("slots", slots, device, torch.int64, tokens)
+    _aligned(("k", k), ("v", v), ("k_cache", k_cache), ("v_cache", v_cache))
+    _no_gradient(k, v)
+    _status(status, device)
+    outputs = [("k_cache", k_cache), ("v_cache", v_cache), ("k_scales", k_scales), ("v_scales", v_scales)]
+    for name, t in outputs:
+        _output(name, t)
+    _apart(outputs, [("k", k), ("v", v), ("slots", slots)])
+    a.num_slots = k_cache.shape[0] * k_cache.shape[1]
+    if a.num_slots > INT32_MAX:
+        raise ValueError("more slots than 31 bits count")
+    a.k, a.v, a.slots, a.status = _ptr(k), _ptr(v), _ptr(slots), _ptr(status)
+    _strides(a, "k", k)
+    _strides(a, "v", v)
+    a.tokens, a.heads, a.head_dim, a.dtype = tokens, heads, dim, _DTYPES[dtype]
+    _rest(err, "iris_write_quantized_cache_launch", a, device)
+
+
+def read_quantized_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, k_out, v_out, *, status=None):
+    """Cached tokens of a cache in 8 bits as heads again.
+
+    Rows ``starts[i] .. starts[i + 1]`` of ``k_out`` and ``v_out`` [tokens, key heads, head size] (fp16, bf16 or fp32) take request i's tokens at the
+    last positions of its ``lengths[i]`` (``starts`` int32 [requests + 1] the sums of ``lengths``: all of them; of new tokens: those).  Codes times
+    scales, rounded to the outputs' type.  Rows past the last request's stay as they are.  A row whose position is none of the
+    request's, or whose page is none of the cache's, is NaN and sets ``STATUS_BAD_INDEX``.
+    """
+    err = _native.host().read_quantized_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, k_out, v_out, status)
+    if _native_call(err):
+        return
+    device, dtype = k_out.device, k_out.dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"k_out: unsupported dtype {dtype}")
+    _heads("k_out", k_out, device)
+    tokens, heads, dim = k_out.shape
+    _heads("v_out", v_out, device, dtype, tokens, heads, dim)
+    a = _native.ReadCacheArgs()
+    _quantized(a, a, k_cache, v_cache, k_scales, v_scales, device, heads, dim)
+    requests, width = _block_table(block_table, device, k_cache.shape[1])
+    _ints("lengths", lengths, device, torch.int32, requests)
+    _ints("starts", starts, device, torch.int32, requests + 1)
+    _aligned(("k_out", k_out), ("v_out", v_out), ("k_cache", k_cache), ("v_cache", v_cache))
+    _no_gradient(k_cache, v_cache)
+    _status(status, device)
+    outputs = [("k_out", k_out), ("v_out", v_out)]
+    for name, t in outputs:
+        _output(name, t)
+    _apart(outputs, [("k_cache", k_cache), ("v_cache", v_cache), ("k_scales", k_scales), ("v_scales", v_scales), ("block_table", block_table),
+                     ("lengths", lengths), ("starts", starts)])
+    a.block_table, a.lengths, a.starts, a.k_out, a.v_out, a.status = (_ptr(t) for t in (block_table, lengths, starts, k_out, v_out, status))
+    _strides(a, "k", k_out)
+    _strides(a, "v", v_out)
+    a.stride_table = block_table.stride(0) if requests > 1 else width
+    a.requests, a.tokens, a.heads, a.head_dim, a.table_width = requests, tokens, heads, dim, width
+    a.num_pages, a.dtype = k_cache.shape[0], _DTYPES[dtype]
+    _rest(err, "iris_read_quantized_cache_launch", a, device)

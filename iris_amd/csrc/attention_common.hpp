@@ -1,7 +1,9 @@
 // What the attention kernels share: the paged cache's addresses, the keys that rows see, the parts of a split axis.
 #pragma once
 
-#include "heads_common.hpp"
+#include <type_traits>
+
+#include "cache_codes.hpp"
 
 namespace iris_amd {
 
@@ -16,6 +18,14 @@ struct AttentionKArgs {
   float* slots;       // partial results, `slot_elems` floats each
   int32_t* counters;  // arrivals at split units; zero between launches
 };
+
+// A cache in 8 bits has scales beside its codes.  CT: the codes' type, or 0 for a cache of the heads' own type.
+struct QuantizedKArgs : AttentionKArgs {
+  iris_cache_scales s;
+  PageDiv block;
+};
+template <int CT>
+using KArgs = std::conditional_t<CT == 0, AttentionKArgs, QuantizedKArgs>;
 
 // The keys that the queries at positions first .. last see, as tiles of BT keys: `front` tiles that hold the first tokens (sinks),
 // then tiles from `start` on; `count` in all.

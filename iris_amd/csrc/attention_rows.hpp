@@ -30,17 +30,21 @@ constexpr int REST = 2;                           // tiles that cost as much as 
                                                   // 8192 keys, us at 1 / 2 / 4: 21.3 / 20.7 / 22.0)
 constexpr int LATER = 1024, TOP = 2048;           // counters of fans but the first (by their first workgroup), and of a unit's fans
 
-template <int DT, int DP>
+template <int DT, int DP, int CT = 0>
 struct Cfg {
   static constexpr bool F32 = DT == IRIS_DTYPE_F32;
   static constexpr int ES = F32 ? 4 : 2;
-  static constexpr int SUBS = F32 ? 1 : 2;           // 16-key tiles of S^T a step
+  static constexpr int CS = CT ? 1 : ES;             // bytes of an element in the cache
+  static constexpr int SUBS = CT ? 4 : F32 ? 1 : 2;  // 16-key tiles of S^T a step: 16 bits' bytes in flight, whatever the type
   static constexpr int KS = 16 * SUBS;               // keys a wave takes a step
   static constexpr int BT = KS * WAVES;              // keys a workgroup takes a step
-  static constexpr int KC = DP * ES / 64;            // 16-byte pieces of a key that a lane loads
+  static constexpr int QC = DP * ES / 64;            // 16-byte pieces of a query that a lane loads
+  static constexpr int KC = DP * CS / 64;            // ... of a key
+  static constexpr int PER = QC / KC;                // pieces of a query to one of a key
   static constexpr int VE = DP / 16;                 // elements of a value that a lane loads
-  static constexpr int VB = VE * ES;                 // their bytes: 8, 16, 32 or 64
+  static constexpr int VB = VE * CS;                 // their bytes: 4 to 64
   static constexpr int VW = VB / 4;                  // their words
+  static constexpr int GROUPS = F32 ? SUBS : SUBS / 2;  // operands of weights: of 16 keys (fp32) or 32
   static constexpr int SLOT = ROWS * (DP + 4);       // floats of a partial result
   // Weights are 2^(score - maximum + LIFT): fp16 ones of keys far below the maximum stay normal numbers (to 2^-28 of the largest
   // weight), and the sum, lifted alike, takes it out again.
@@ -97,17 +101,20 @@ __device__ inline void store_out(const iris_attention_args& a, int64_t at, int d
 // PG: page sizes are multiples of 16, so that 16 keys lie in one page (its number is the wave's); otherwise each lane
 // looks its keys' pages up.
 // ONE: all of a unit's rows stand at one position (single tokens).
-template <int DT, int DP, bool PG, bool ONE>
+// CT: the codes of a cache in 8 bits (or 0).  A code is as good as the number that it and its scale stand for in the heads' type, so codes become
+// such numbers on their way into the matrix instructions, and the rest is the same.
+template <int DT, int DP, bool PG, bool ONE, int CT = 0>
 struct Unit {
-  using C = Cfg<DT, DP>;
-  const AttentionKArgs& g;
+  static_assert(PG || CT == 0, "scales are for 16 keys and more");
+  using C = Cfg<DT, DP, CT>;
+  const KArgs<CT>& g;
   const iris_attention_args& a;
   Lds<DT, DP>& lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;  // the lane's row, and which of its four shares of a key or of the keys
   bool bad_page;
 
-  __device__ inline Unit(const AttentionKArgs& g, Lds<DT, DP>& lds) : g(g), a(g.a), lds(lds) {}
+  __device__ inline Unit(const KArgs<CT>& g, Lds<DT, DP>& lds) : g(g), a(g.a), lds(lds) {}
 
   // The table's entries for a step's keys (for the wave, or for each of the lane's keys), and the keys and values themselves.
   struct Pages {
@@ -116,12 +123,13 @@ struct Unit {
   struct Step {
     u32x4 k[C::SUBS][C::KC];
     uint32_t v[C::SUBS][4][C::VW];
+    uint32_t k_scale[CT ? C::SUBS : 1], v_scale[CT ? C::SUBS : 1];
   };
   __device__ inline int step_base(const Piece& p, int j) { return p.tiles.tile(j) * C::BT + wave * C::KS; }
 
   // The state of the lane's row.  l: the sum of the weights as they are multiplied; lse_l: as they are, for the logarithm.
   struct Row {
-    u32x4 q[C::KC];
+    u32x4 q[C::QC];
     f32x4 o[C::VE];
     float m, l, lse_l;
     int at;                // the row's position
@@ -170,21 +178,28 @@ struct Unit {
       const int first_key = base + 16 * s, own = min(first_key + n, last);
       const int64_t page = PG ? checked(pages.k[s], row, first_key, first_key + 15) : checked(pages.k[s], row, first_key + n, first_key + n);
       const IRIS_GLOBAL char* kp = (const IRIS_GLOBAL char*)a.k_cache +
-                                   (page * a.stride_kc_page + (int64_t)in_page(own) * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::ES + quad * 16;
+                                   (page * a.stride_kc_page + (int64_t)in_page(own) * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::CS + quad * 16;
+      if constexpr (CT != 0) {
+        const int64_t block = page_div((uint32_t)in_page(min(first_key, last)), g.block);
+        x.k_scale[s] = scale_byte(g.s.k_scales + page * g.s.stride_ks_page + block * g.s.stride_ks_block + p.head * g.s.stride_ks_head);
+        x.v_scale[s] = scale_byte(g.s.v_scales + page * g.s.stride_vs_page + block * g.s.stride_vs_block + p.head * g.s.stride_vs_head);
+      }
 #pragma unroll
       for (int c = 0; c < C::KC; ++c) {
         x.k[s][c] = u32x4{0, 0, 0, 0};
-        if ((c * 64 + quad * 16) / C::ES < a.head_dim) x.k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + c * 64);
+        if ((c * 64 + quad * 16) / C::CS < a.head_dim) x.k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + c * 64);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int own_key = first_key + quad * 4 + r, key = min(own_key, last);
         const int64_t vpage = PG ? page : checked(pages.v[s][r], row, own_key, own_key);
         const IRIS_GLOBAL char* vp = (const IRIS_GLOBAL char*)a.v_cache +
-                                     (vpage * a.stride_vc_page + (int64_t)in_page(key) * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::ES + n * C::VB;
+                                     (vpage * a.stride_vc_page + (int64_t)in_page(key) * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::CS + n * C::VB;
 #pragma unroll
         for (int w = 0; w < C::VW; ++w) x.v[s][r][w] = 0;
-        if constexpr (C::VB == 8) {
+        if constexpr (C::VB == 4) {
+          if (n * C::VE < a.head_dim) x.v[s][r][0] = *(const IRIS_GLOBAL uint32_t*)vp;
+        } else if constexpr (C::VB == 8) {
           if (n * C::VE < a.head_dim) {
             const u32x2 y = *(const IRIS_GLOBAL u32x2*)vp;
             x.v[s][r][0] = y[0], x.v[s][r][1] = y[1];
@@ -192,7 +207,7 @@ struct Unit {
         } else {
 #pragma unroll
           for (int w = 0; w < C::VW; w += 4)
-            if (n * C::VE + w * 4 / C::ES < a.head_dim) {
+            if (n * C::VE + w * 4 / C::CS < a.head_dim) {
               const u32x4 y = *(const IRIS_GLOBAL u32x4*)(vp + w * 4);
 #pragma unroll
               for (int i = 0; i < 4; ++i) x.v[s][r][w + i] = y[i];
@@ -206,15 +221,44 @@ struct Unit {
     const int base = step_base(p, j);
     auto& v = x.v;
     f32x4 s[C::SUBS];
+    float v_scale[C::SUBS];
+    bool poisoned = false;  // a value that some row must not see is not a finite number
+    if constexpr (CT != 0) {
 #pragma unroll
-    for (int u = 0; u < C::SUBS; ++u) {
-      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < C::SUBS; ++u) {
+        // (a scale that is no number makes its codes such, and itself one)
+        int kb = __builtin_amdgcn_readfirstlane((int)x.k_scale[u]), vb = __builtin_amdgcn_readfirstlane((int)x.v_scale[u]);
+        if (kb == SCALE_NAN) {
 #pragma unroll
-      for (int c = 0; c < C::KC; ++c) s[u] = mfma<DT>(x.k[u][c], row.q[c], s[u]);
+          for (int c = 0; c < C::KC; ++c) x.k[u][c] = u32x4{NAN_CODES, NAN_CODES, NAN_CODES, NAN_CODES};
+          kb = SCALE_ONE;
+        }
+        if (vb == SCALE_NAN) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < C::VW; ++w) v[u][r][w] = NAN_CODES;
+          vb = SCALE_ONE;
+        }
+        v_scale[u] = scale_of(vb);
+        if (!ONE) poisoned |= vb > LARGEST_SCALE;  // (codes might leave the type's range)
+        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C::KC; ++c)
+#pragma unroll
+          for (int i = 0; i < C::PER; ++i) s[u] = mfma<DT>(decode_piece(x.k[u][c], i, scale_of(kb)), row.q[c * C::PER + i], s[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < C::SUBS; ++u) {
+        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C::KC; ++c) s[u] = mfma<DT>(x.k[u][c], row.q[c], s[u]);
+      }
     }
     // Some of the step's keys may be hidden from some of the rows?  (the last keys; the window's edge)
     const bool edge = base + C::KS - 1 > row.first_at || (a.window > 0 && row.last_at - base >= a.window && base + C::KS > a.sinks);
-    bool poisoned = false;  // a value that some row must not see is not a finite number
+    if (!edge) poisoned = false;
     if (edge) {
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u)
@@ -249,23 +293,27 @@ struct Unit {
     for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[u][r] = __builtin_amdgcn_exp2f(s[u][r] * g.scale_log2 - ref);
-    u32x4 weights;  // in the operand's type: for fp32 themselves
-    if constexpr (C::F32) {
-      weights = __builtin_bit_cast(u32x4, s[0]);
-      row.l += (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
-      row.lse_l = row.l;
-    } else {
-      weights = u32x4{pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]), pack2<DT>(s[1][2], s[1][3])};
+    u32x4 weights[C::GROUPS];  // in the operand's type: for fp32 themselves
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        row.l = add_weights<DT>(weights[e], row.l);
-        row.lse_l += s[0][e] + s[1][e];
+    for (int i = 0; i < C::GROUPS; ++i) {
+      if constexpr (C::F32) {
+        weights[i] = __builtin_bit_cast(u32x4, s[i]);
+        row.l += (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
+        row.lse_l = row.l;
+      } else {
+        const f32x4 lo = s[2 * i], hi = s[2 * i + 1];
+        weights[i] = u32x4{pack2<DT>(lo[0], lo[1]), pack2<DT>(lo[2], lo[3]), pack2<DT>(hi[0], hi[1]), pack2<DT>(hi[2], hi[3])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          row.l = add_weights<DT>(weights[i][e], row.l);
+          row.lse_l += lo[e] + hi[e];
+        }
       }
     }
 #pragma unroll
     for (int e = 0; e < C::VE; ++e) row.o[e] *= shrink;
     if (!poisoned) {
-      add_values(weights, v, row.o);
+      add_values(weights, v, v_scale, row.o);
     } else {
       // (0 times it would still be NaN: each row's keys apart, with what it does not see taken out)
       for (int y = 0; y < ROWS; ++y) {
@@ -282,7 +330,7 @@ struct Unit {
         f32x4 one[C::VE];
 #pragma unroll
         for (int e = 0; e < C::VE; ++e) one[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        add_values(weights, vy, one);
+        add_values(weights, vy, v_scale, one);
 #pragma unroll
         for (int e = 0; e < C::VE; ++e)
           if (n == y) row.o[e] += one[e];
@@ -305,11 +353,16 @@ struct Unit {
     Step x;
         {
       const IRIS_GLOBAL char* qp =
-          (const IRIS_GLOBAL char*)a.q + ((int64_t)(p.token0 + token) * a.stride_qt + (int64_t)head * a.stride_qh) * C::ES + quad * 16;
+          (const IRIS_GLOBAL char*)a.q + ((int64_t)(p.token0 + token) * a.stride_qt + (int64_t)head * a.stride_qh) * C::ES + (CT ? 0 : quad * 16);
 #pragma unroll
-      for (int c = 0; c < C::KC; ++c) {
+      for (int c = 0; c < C::QC; ++c) {
         row.q[c] = u32x4{0, 0, 0, 0};
-        if (have_row && (c * 64 + quad * 16) / C::ES < a.head_dim) row.q[c] = *(const IRIS_GLOBAL u32x4*)(qp + c * 64);
+        if constexpr (CT == 0) {
+          if (have_row && (c * 64 + quad * 16) / C::ES < a.head_dim) row.q[c] = *(const IRIS_GLOBAL u32x4*)(qp + c * 64);
+        } else {  // the elements of the lane's sixteen codes
+          const int d = c / C::PER * 64 + quad * 16 + c % C::PER * (16 / C::ES);
+          if (have_row && d < a.head_dim) row.q[c] = *(const IRIS_GLOBAL u32x4*)(qp + d * C::ES);
+        }
       }
     }
 #pragma unroll
@@ -337,32 +390,79 @@ struct Unit {
   }
 
   static __device__ inline bool not_finite(uint32_t w) {
+    if constexpr (CT != 0) {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= ((w >> (8 * i)) & 0x7F) >= Codes<CT>::NOT_FINITE;
+      return any;
+    }
     if constexpr (DT == IRIS_DTYPE_F32) return (w & 0x7F800000u) == 0x7F800000u;
     constexpr uint32_t E = DT == IRIS_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
     return (w & E) == E || ((w >> 16) & E) == E;
   }
 
+  // Scales from which on the largest code times them may be past the largest number of the heads' type.
+  static constexpr int LARGEST_SCALE = SCALE_ONE + (DT == IRIS_DTYPE_F16 ? 16 : 128) - Codes<CT ? CT : IRIS_DTYPE_E4M3>::TOP;
+
+  // Piece i of sixteen codes, scaled, in the heads' type.
+  static __device__ inline u32x4 decode_piece(u32x4 x, int i, float scale) {
+    if constexpr (C::F32)
+      return __builtin_bit_cast(u32x4, decode4_f32<CT>(x[i], scale));
+    else
+      return u32x4{decode2<CT, DT, false>(x[2 * i], scale), decode2<CT, DT, true>(x[2 * i], scale), decode2<CT, DT, false>(x[2 * i + 1], scale),
+                   decode2<CT, DT, true>(x[2 * i + 1], scale)};
+  }
+
   // O^T += V^T P^T
-  __device__ inline void add_values(u32x4 w, const uint32_t (&v)[C::SUBS][4][C::VW], f32x4 (&o)[C::VE]) {
+  __device__ inline void add_values(const u32x4 (&w)[C::GROUPS], const uint32_t (&v)[C::SUBS][4][C::VW], const float (&scale)[C::SUBS], f32x4 (&o)[C::VE]) {
     if constexpr (C::F32) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
-        for (int e = 0; e < C::VE; ++e)
-          o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[0][r][e]), __builtin_bit_cast(f32x4, w)[r], o[e], 0, 0, 0);
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < C::VE; ++e) {
+            float x;
+            if constexpr (CT == 0)
+              x = __builtin_bit_cast(float, v[u][r][e]);
+            else
+              x = (e & 2 ? decode2_f32<CT, true>(v[u][r][e / 4], scale[u]) : decode2_f32<CT, false>(v[u][r][e / 4], scale[u]))[e & 1];
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, __builtin_bit_cast(f32x4, w[u])[r], o[e], 0, 0, 0);
+          }
     } else {
       // The weights are in 16 bits, as the matrix instruction takes both its operands: off by half a last place of the values' own
       // type, which the output is rounded to as well.  (Errors against 64 bits 0.0015 to 0.0016 of the output where fp32 weights
       // have 0.0014 to 0.0015, fp16 4.9e-5 for 4.5e-5; a second product for the rest of each weight would double these instructions.)
 #pragma unroll
-      for (int e = 0; e < C::VE; ++e) {
-        u32x4 t;
+      for (int i = 0; i < C::GROUPS; ++i) {
+        if constexpr (CT == 0) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+          for (int e = 0; e < C::VE; ++e) {
+            u32x4 t;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            t[2 * u + h] = __builtin_amdgcn_perm(v[u][2 * h + 1][e / 2], v[u][2 * h][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
-        o[e] = mfma<DT>(t, w, o[e]);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                t[2 * u + h] = __builtin_amdgcn_perm(v[u][2 * h + 1][e / 2], v[u][2 * h][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+            o[e] = mfma<DT>(t, w[i], o[e]);
+          }
+        } else {
+          // two elements of two keys meet in a word by one byte permute, and become pairs of keys as they are converted
+#pragma unroll
+          for (int e = 0; e < C::VE; e += 2) {
+            u32x4 t[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t x = __builtin_amdgcn_perm(v[2 * i + u][2 * h + 1][e / 4], v[2 * i + u][2 * h][e / 4], e & 2 ? 0x07030602u : 0x05010400u);
+                t[0][2 * u + h] = decode2<CT, DT, false>(x, scale[2 * i + u]);
+                t[1][2 * u + h] = decode2<CT, DT, true>(x, scale[2 * i + u]);
+              }
+            o[e] = mfma<DT>(t[0], w[i], o[e]);
+            o[e + 1] = mfma<DT>(t[1], w[i], o[e + 1]);
+          }
+        }
       }
     }
   }
@@ -588,13 +688,13 @@ __device__ inline int keys_of(const AttentionKArgs& g, int request) {
 // Single tokens.  All units (request, key head, rows of 16) lie in one line, each as long as its key tiles and REST more for what a
 // unit costs beside them, and the workgroups cut the line into equal runs: requests of any lengths load every workgroup
 // alike.  A run's first and last unit may be shared with the workgroups beside it.
-template <int DT, int DP, bool PG>
-__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void decode_kernel(AttentionKArgs g) {
-  using C = Cfg<DT, DP>;
+template <int DT, int DP, bool PG, int CT = 0>
+__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void decode_kernel(KArgs<CT> g) {
+  using C = Cfg<DT, DP, CT>;
   __shared__ Lds<DT, DP> lds;
   __shared__ int wave_sum[WAVES];
   __shared__ int found_request, found_before, found_length;
-  touch_args<sizeof(AttentionKArgs)>();
+  touch_args<sizeof(KArgs<CT>)>();
   const iris_attention_args& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row_tiles = (g.group + ROWS - 1) / ROWS, units = a.k_heads * row_tiles;
@@ -648,7 +748,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void decode_kernel(A
     int request = __builtin_amdgcn_readfirstlane(found_request), next_length = __builtin_amdgcn_readfirstlane(found_length);
     uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane(found_before) * units;  // the request's place in the line
 
-    Unit<DT, DP, PG, true> unit(g, lds);
+    Unit<DT, DP, PG, true, CT> unit(g, lds);
     for (uint32_t at = begin; at < end; ++request) {
       Piece p;
       p.request = request;
@@ -697,9 +797,9 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void decode_kernel(A
 // Prompts: a workgroup for 16 rows of a request and key head, and a share of the keys they see.  Row tile x of the grid is the
 // (x - bound)-th of the last request whose bound, floor(query_starts * group / 16) + request, is not past x: bounds leave each
 // request room for its row tiles without a sum over the requests.
-template <int DT, int DP, bool PG>
-__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void prompt_rows_kernel(AttentionKArgs g) {
-  using C = Cfg<DT, DP>;
+template <int DT, int DP, bool PG, int CT = 0>
+__global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void prompt_rows_kernel(KArgs<CT> g) {
+  using C = Cfg<DT, DP, CT>;
   __shared__ Lds<DT, DP> lds;
   const iris_attention_args& a = g.a;
   const int x = blockIdx.x / g.splits, split = blockIdx.x - x * g.splits;
@@ -733,7 +833,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 256 ? 1 : 2) void prompt_rows_ker
   p.later_slot = p.first_slot;
   p.slot_step = 1;
   p.counter = index;
-  Unit<DT, DP, PG, false> unit(g, lds);
+  Unit<DT, DP, PG, false, CT> unit(g, lds);
   unit.run(p);
 }
 

@@ -45,6 +45,8 @@ struct Cfg {
   static constexpr int CHUNKS = ROW_BYTES / 16;        // 16-byte chunks of a key
   static constexpr int DMA_ROWS = 1024 / ROW_BYTES;    // keys that one LDS-DMA instruction of a wave moves
   static constexpr int DMAS = 16 / DMA_ROWS;           // ... and how many move a wave's 16 keys of a tile
+  static constexpr int CODE_CHUNKS = DP / 16;          // 16-byte chunks of a key in 8 bits
+  static constexpr int CODE_LOADS = CODE_CHUNKS / 4;   // loads of a wave that move its 16 keys of a tile
   static constexpr int KC = DP / 16;                   // matrix instructions over a head
   static constexpr int DTILES = DP / 32;               // 32-column tiles of the output
   static constexpr int SLOT = ROWS * DP + WAVES * 64 * 4;  // floats of a partial result
@@ -138,8 +140,10 @@ __device__ inline bool nth_longest(const AttentionKArgs& g, int k, int* request,
 }
 
 // LSE: the logarithms of the rows' sums are wanted.
-template <int DT, int DP, bool LSE>
-__global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu_waves_per_eu(waves_a_simd(DP), waves_a_simd(DP)))) void prompt_tiles_kernel(AttentionKArgs g) {
+// CT: the codes of a cache in 8 bits (or 0).  Codes come to registers a tile ahead, and to LDS as numbers of the heads' type: each wave
+// converts the keys that it fetches, once for all four.
+template <int DT, int DP, bool LSE, int CT = 0>
+__global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu_waves_per_eu(waves_a_simd(DP), waves_a_simd(DP)))) void prompt_tiles_kernel(KArgs<CT> g) {
   using C = Cfg<DT, DP>;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][C::TILE_BYTES];  // [stage][keys, values]
   const iris_attention_args& a = g.a;
@@ -207,7 +211,16 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
   }
 
   // What a wave fetches: 16 keys of each tile, DMA_ROWS an instruction.  Offsets of the lane's chunk from the first of the 16.
-  uint32_t k_off[C::DMAS], v_off[C::DMAS];
+  constexpr int LOADS = CT ? C::CODE_LOADS : C::DMAS, LOAD_ROWS = 16 / LOADS;
+  uint32_t k_off[LOADS], v_off[LOADS];
+  if constexpr (CT != 0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = i * LOAD_ROWS + lane / C::CODE_CHUNKS, p = lane % C::CODE_CHUNKS;
+      k_off[i] = p * 16 < a.head_dim ? (uint32_t)(r * a.stride_kc_row) + p * 16 : DEAD_OFFSET;
+      v_off[i] = p * 16 < a.head_dim ? (uint32_t)(r * a.stride_vc_row) + p * 16 : DEAD_OFFSET;
+    }
+  } else
 #pragma unroll
   for (int i = 0; i < C::DMAS; ++i) {
     const int r = i * C::DMA_ROWS + lane / C::CHUNKS, p = lane % C::CHUNKS;
@@ -220,6 +233,9 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
     const int key = list.tile(j) * BT + wave * 16;
     return key < length ? scalar_at(a.block_table, (int64_t)request * a.stride_table + page_div((uint32_t)key, g.page)) : 0;
   };
+  // codes on their way to LDS, and their scales
+  u32x4 k_codes[CT ? LOADS : 1], v_codes[CT ? LOADS : 1];
+  uint32_t k_scale = SCALE_ONE, v_scale = SCALE_ONE;
   auto fetch = [&](int j, int page, int stage) {
     const int key = list.tile(j) * BT + wave * 16;
     if ((uint32_t)page >= (uint32_t)a.num_pages) {
@@ -229,6 +245,24 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
     }
     const int in_page = key - (int)(page_div((uint32_t)key, g.page) * g.page.d);
     const int valid = length - key;  // of the 16 keys
+    if constexpr (CT != 0) {
+      const __amdgpu_buffer_rsrc_t kr = tile_rsrc((const IRIS_GLOBAL char*)a.k_cache + ((int64_t)page * a.stride_kc_page + (int64_t)head * a.stride_kc_head), 0x7FFFFFFF);
+      const __amdgpu_buffer_rsrc_t vr = tile_rsrc((const IRIS_GLOBAL char*)a.v_cache + ((int64_t)page * a.stride_vc_page + (int64_t)head * a.stride_vc_head), 0x7FFFFFFF);
+      const int k_at = in_page * (int)a.stride_kc_row, v_at = in_page * (int)a.stride_vc_row;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const bool there = i * LOAD_ROWS + lane / C::CODE_CHUNKS < valid;
+        k_codes[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(there ? k_off[i] : DEAD_OFFSET), k_at, 0);
+        v_codes[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, (int)(there ? v_off[i] : DEAD_OFFSET), v_at, 0);
+      }
+      k_scale = v_scale = SCALE_ONE;
+      if (valid > 0) {
+        const int64_t block = page_div((uint32_t)in_page, g.block);
+        k_scale = scale_byte(g.s.k_scales + (int64_t)page * g.s.stride_ks_page + block * g.s.stride_ks_block + head * g.s.stride_ks_head);
+        v_scale = scale_byte(g.s.v_scales + (int64_t)page * g.s.stride_vs_page + block * g.s.stride_vs_block + head * g.s.stride_vs_head);
+      }
+      return;
+    }
     const __amdgpu_buffer_rsrc_t kr = tile_rsrc((const IRIS_GLOBAL char*)a.k_cache + ((int64_t)page * a.stride_kc_page + (int64_t)head * a.stride_kc_head) * 2, 0x7FFFFFFF);
     const __amdgpu_buffer_rsrc_t vr = tile_rsrc((const IRIS_GLOBAL char*)a.v_cache + ((int64_t)page * a.stride_vc_page + (int64_t)head * a.stride_vc_head) * 2, 0x7FFFFFFF);
     const int k_at = in_page * (int)(a.stride_kc_row * 2), v_at = in_page * (int)(a.stride_vc_row * 2);
@@ -284,9 +318,55 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
     fetch(j0, fetch_page(j0), j0 & 1);
     if (j0 + 1 < j1) page = fetch_page(j0 + 1);
   }
+  // The wave's share of tile j becomes numbers of the heads' type in LDS; `look`: whether any of its values is no finite number.
+  auto convert = [&](int j, bool look) {
+    if constexpr (CT != 0) {
+      int kb = __builtin_amdgcn_readfirstlane((int)k_scale), vb = __builtin_amdgcn_readfirstlane((int)v_scale);
+      const bool k_none = kb == SCALE_NAN, v_none = vb == SCALE_NAN;  // (its codes are then no numbers either, for 0 times it might be one)
+      if (k_none) kb = SCALE_ONE;
+      if (v_none) vb = SCALE_ONE;
+      const float ks = scale_of(kb), vs = scale_of(vb);
+      char* const to = &lds[j & 1][0][wave * 16 * C::ROW_BYTES];
+      u32x4 bad = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int r = i * LOAD_ROWS + lane / C::CODE_CHUNKS, c = lane % C::CODE_CHUNKS * 2;
+        const IRIS_LDS char* const row = (const IRIS_LDS char*)to + r * C::ROW_BYTES;
+        if (k_none) k_codes[i] = u32x4{NAN_CODES, NAN_CODES, NAN_CODES, NAN_CODES};
+        if (v_none) v_codes[i] = u32x4{NAN_CODES, NAN_CODES, NAN_CODES, NAN_CODES};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          using Rows = rows::Unit<DT, DP, true, false, CT>;
+          const u32x4 k = Rows::decode_piece(k_codes[i], h, ks), v = Rows::decode_piece(v_codes[i], h, vs);
+          *(IRIS_LDS u32x4*)(row + swizzle_k<DP>(r, c + h) * 16) = k;
+          *(IRIS_LDS u32x4*)(row + C::TILE_BYTES + swizzle_v<DP>(r, c + h) * 16) = v;
+          if (look) {
+            typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+            const u32x4 magnitudes = v & 0x7FFF7FFFu;
+            bad = __builtin_bit_cast(u32x4, __builtin_elementwise_max(__builtin_bit_cast(u16x8, bad), __builtin_bit_cast(u16x8, magnitudes)));
+          }
+        }
+      }
+      if (look) {
+        constexpr uint32_t INF = DT == IRIS_DTYPE_BF16 ? 0x7F80 : 0x7C00;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) poisoned |= (bad[w] & 0xFFFFu) >= INF || (bad[w] >> 16) >= INF;
+      }
+      IRIS_WAIT_LGKMCNT0();
+    }
+  };
   auto next_stage = [&](int j) {
-    IRIS_WAIT_VMCNT(0);  // this wave's share of the tile has arrived; behind the barrier everyone's has
     const int base = list.tile(j) * BT;
+    if constexpr (CT != 0) {
+      convert(j, base + BT - 1 > rows_first || (a.window > 0 && rows_last - base >= a.window && base + BT > a.sinks));
+      block_barrier_raw();
+      if (j + 1 < j1) {
+        fetch(j + 1, page, (j + 1) & 1);
+        if (j + 2 < j1) page = fetch_page(j + 2);
+      }
+      return;
+    }
+    IRIS_WAIT_VMCNT(0);  // this wave's share of the tile has arrived; behind the barrier everyone's has
     if (base + BT - 1 > rows_first || (a.window > 0 && rows_last - base >= a.window && base + BT > a.sinks)) {
       // some rows must not see some of the tile's values: is any among the wave's share of them not a finite number?
       typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -485,7 +565,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
   // A weight of 0 times a value that is no number is NaN: then the rows are computed again by the kernel that takes hidden values out.
   if (redo) {
     static_assert(sizeof(rows::Lds<DT, DP>) <= sizeof(lds), "the tiles' room is given over");
-    rows::Unit<DT, DP, true, false> unit(g, *(rows::Lds<DT, DP>*)lds);
+    rows::Unit<DT, DP, true, false, CT> unit(g, *(rows::Lds<DT, DP>*)lds);
 #pragma unroll 1
     for (int r = 0; r < num_rows; r += rows::ROWS) {
       rows::Piece p{};
@@ -496,7 +576,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
       p.token0 = token0;
       p.length = length;
       p.first = first;
-      p.tiles = key_tiles<rows::Cfg<DT, DP>::BT>(a, first + p.row0 / g.group, first + (p.row0 + p.rows - 1) / g.group);
+      p.tiles = key_tiles<rows::Cfg<DT, DP, CT>::BT>(a, first + p.row0 / g.group, first + (p.row0 + p.rows - 1) / g.group);
       p.j1 = p.tiles.count;
       p.parts = 1;
       unit.run(p);

@@ -643,6 +643,26 @@ bool cache_of(const Operand& t, at::ScalarType type, int64_t heads, int64_t dim,
   return true;
 }
 
+// The codes of a cache in 8 bits; -1: of none.
+int code_of(const Operand& t) {
+  if (!t) return -1;
+  switch (t.t->scalar_type()) {
+    case at::ScalarType::Float8_e4m3fn: return IRIS_DTYPE_E4M3;
+    case at::ScalarType::Float8_e5m2: return IRIS_DTYPE_E5M2;
+    default: return -1;
+  }
+}
+// Scales [pages, blocks of a page, heads] of a cache; *block: tokens to a scale.
+bool scales_of(const Operand& t, const Operand& cache, CacheStrides* s, int32_t* block) {
+  if (!t || t.t->dim() != 3 || t.t->scalar_type() != at::ScalarType::Float8_e8m0fnu || t.t->size(0) != cache.t->size(0) || t.t->size(1) < 1 ||
+      t.t->size(2) != cache.t->size(2) || cache.t->size(1) % t.t->size(1) || cache.t->size(1) / t.t->size(1) % 16)
+    return false;
+  int64_t* const out[3] = {&s->page, &s->row, &s->head};
+  for (int i = 0; i < 3; ++i) *out[i] = t.t->size(i) > 1 ? t.t->stride(i) : 0;
+  *block = (int32_t)(cache.t->size(1) / t.t->size(1));
+  return true;
+}
+
 void strides_of(const Operand& t, int64_t* token, int64_t* head) {
   *token = t.t->size(0) > 1 ? t.t->stride(0) : 0;
   *head = t.t->size(1) > 1 ? t.t->stride(1) : 0;
@@ -770,38 +790,50 @@ PyObject* qk_norm_rope_backward(PyObject*, PyObject* const* x, Py_ssize_t n) {
   return PyLong_FromLong(unlocked([&] { return iris_qk_norm_rope_backward_launch(&a, stream); }));
 }
 
-// attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale, window, sinks)
-PyObject* attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
-  if (n != 13) {
-    PyErr_SetString(PyExc_TypeError, "attention takes 13 arguments");
-    return nullptr;
-  }
+// Both kinds of cache: `operands` tensors, then scale, window and sinks.
+PyObject* attention_over(PyObject* const* x, int operands) {
   const int device = launch_device(x[0]);
-  Operand t[10];
+  Operand t[12];
   iris_attention_args a{};
+  iris_cache_scales s{};
   double scale = 0;
-  bool ok = device >= 0 && (x[10] == Py_None || real(x[10], &scale)) && int32(x[11], &a.window) && int32(x[12], &a.sinks);
-  for (int i = 0; ok && i < 10; ++i) ok = operand(x[i], device, &t[i]);
+  PyObject* const* numbers = x + operands;
+  bool ok = device >= 0 && (numbers[0] == Py_None || real(numbers[0], &scale)) && int32(numbers[1], &a.window) && int32(numbers[2], &a.sinks);
+  for (int i = 0; ok && i < operands; ++i) ok = operand(x[i], device, &t[i]);
   PyErr_Clear();
-  enum { Q, K_CACHE, V_CACHE, TABLE, LENGTHS, STARTS, OUT, LSE, WORKSPACE, STATUS };
+  enum { Q, K_CACHE, V_CACHE, TABLE, LENGTHS, STARTS, OUT, LSE, WORKSPACE, STATUS, K_SCALES, V_SCALES };
+  const bool quantized = operands > K_SCALES;
   if (!ok || !t[Q] || t[Q].t->dim() != 3 || dtype_code(*t[Q].t) < 0 || !t[K_CACHE] || t[K_CACHE].t->dim() != 4 || !rows_contiguous(t[TABLE]))
     return PyLong_FromLong(DECLINED);
   const auto type = t[Q].t->scalar_type();
   const int64_t tokens = t[Q].t->size(0), hq = t[Q].t->size(1), dim = t[Q].t->size(2), hk = t[K_CACHE].t->size(2);
   const int64_t requests = t[TABLE].t->size(0), width = t[TABLE].t->size(1), pages = t[K_CACHE].t->size(0), page_size = t[K_CACHE].t->size(1);
-  const int64_t vec = 16 / (int64_t)t[Q].t->element_size();
+  const int64_t vec = quantized ? 16 : 16 / (int64_t)t[Q].t->element_size();
   CacheStrides k, v;
+  const auto cached = quantized ? t[K_CACHE].t->scalar_type() : type;
   // (calls with nothing to do, and those whose sizes are refused, are the Python code's)
   if (!tokens || !hq || !hk || !requests || !width || !pages || hq % hk || dim % vec || dim <= 0 || dim > MAX_ATTENTION_HEAD_DIM ||
       width > INT32_MAX || requests > INT32_MAX || width * page_size > INT32_MAX)
     return PyLong_FromLong(DECLINED);
-  if (!heads_of(t[Q], type, -1, -1, -1) || !heads_of(t[OUT], type, tokens, hq, dim) || !cache_of(t[K_CACHE], type, hk, dim, &k) ||
-      !cache_of(t[V_CACHE], type, hk, dim, &v) || t[K_CACHE].t->sizes() != t[V_CACHE].t->sizes() || t[TABLE].t->scalar_type() != at::kInt ||
+  if (!heads_of(t[Q], type, -1, -1, -1) || !heads_of(t[OUT], type, tokens, hq, dim) || !cache_of(t[K_CACHE], cached, hk, dim, &k) ||
+      !cache_of(t[V_CACHE], cached, hk, dim, &v) || t[K_CACHE].t->sizes() != t[V_CACHE].t->sizes() || t[TABLE].t->scalar_type() != at::kInt ||
       !vector_of(t[LENGTHS], at::kInt, requests) || (t[STARTS] ? !vector_of(t[STARTS], at::kInt, requests + 1) : requests != tokens) ||
       !output(t[OUT]) || !status_ok(t[STATUS]))
     return PyLong_FromLong(DECLINED);
   for (const int i : {Q, K_CACHE, V_CACHE})
     if (differentiates(t[i])) return PyLong_FromLong(DECLINED);
+  if (quantized) {
+    CacheStrides ks, vs;
+    int32_t blocks[2];
+    if ((s.code = code_of(t[K_CACHE])) < 0 || !scales_of(t[K_SCALES], t[K_CACHE], &ks, &blocks[0]) ||
+        !scales_of(t[V_SCALES], t[V_CACHE], &vs, &blocks[1]) || blocks[0] != blocks[1])
+      return PyLong_FromLong(DECLINED);
+    s.k_scales = (const uint8_t*)t[K_SCALES].ptr();
+    s.v_scales = (const uint8_t*)t[V_SCALES].ptr();
+    s.stride_ks_page = ks.page, s.stride_ks_block = ks.row, s.stride_ks_head = ks.head;
+    s.stride_vs_page = vs.page, s.stride_vs_block = vs.row, s.stride_vs_head = vs.head;
+    s.block = blocks[0];
+  }
   if (t[LSE]) {
     if (t[LSE].t->scalar_type() != at::kFloat || !rows_contiguous(t[LSE]) || t[LSE].t->size(0) != tokens || t[LSE].t->size(1) != hq || !output(t[LSE]))
       return PyLong_FromLong(DECLINED);
@@ -813,7 +845,7 @@ PyObject* attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.workspace = (float*)t[WORKSPACE].ptr();
     a.workspace_elems = t[WORKSPACE].t->numel();
   }
-  if (!apart(t, {OUT, LSE, WORKSPACE}, {Q, K_CACHE, V_CACHE, TABLE, LENGTHS, STARTS}, {{OUT, Q}})) return PyLong_FromLong(DECLINED);
+  if (!apart(t, {OUT, LSE, WORKSPACE}, {Q, K_CACHE, V_CACHE, TABLE, LENGTHS, STARTS, K_SCALES, V_SCALES}, {{OUT, Q}})) return PyLong_FromLong(DECLINED);
   a.q = t[Q].ptr();
   a.k_cache = t[K_CACHE].ptr();
   a.v_cache = t[V_CACHE].ptr();
@@ -837,9 +869,135 @@ PyObject* attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
   a.table_width = (int32_t)width;
   a.num_pages = (int32_t)pages;
   a.dtype = dtype_code(*t[Q].t);
-  a.scale = (float)(x[10] == Py_None ? 1.0 / std::sqrt((double)dim) : scale);
+  a.scale = (float)(numbers[0] == Py_None ? 1.0 / std::sqrt((double)dim) : scale);
   void* stream = current_stream(device);
-  return PyLong_FromLong(unlocked([&] { return iris_attention_launch(&a, stream); }));
+  return PyLong_FromLong(unlocked([&] {
+    return quantized ? iris_quantized_attention_launch(&a, &s, stream) : iris_attention_launch(&a, stream);
+  }));
+}
+
+// attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, scale, window, sinks)
+PyObject* attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 13) {
+    PyErr_SetString(PyExc_TypeError, "attention takes 13 arguments");
+    return nullptr;
+  }
+  return attention_over(x, 10);
+}
+
+// quantized_attention(q, k_cache, v_cache, block_table, lengths, query_starts, out, lse, workspace, status, k_scales, v_scales, scale,
+//                     window, sinks)
+PyObject* quantized_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 15) {
+    PyErr_SetString(PyExc_TypeError, "quantized_attention takes 15 arguments");
+    return nullptr;
+  }
+  return attention_over(x, 12);
+}
+
+// What a call that writes or reads a cache in 8 bits takes of it.
+template <class Args>
+bool quantized_cache(const Operand& k_cache, const Operand& v_cache, const Operand& k_scales, const Operand& v_scales, int64_t heads, int64_t dim, Args* a) {
+  CacheStrides k, v, ks, vs;
+  int32_t blocks[2];
+  if ((a->code = code_of(k_cache)) < 0 || dim <= 0 || dim % 16 || dim > MAX_ATTENTION_HEAD_DIM ||
+      !cache_of(k_cache, k_cache.t->scalar_type(), heads, dim, &k) || !cache_of(v_cache, k_cache.t->scalar_type(), heads, dim, &v) ||
+      k_cache.t->sizes() != v_cache.t->sizes() || !scales_of(k_scales, k_cache, &ks, &blocks[0]) || !scales_of(v_scales, v_cache, &vs, &blocks[1]) ||
+      blocks[0] != blocks[1])
+    return false;
+  a->stride_kc_page = k.page, a->stride_kc_row = k.row, a->stride_kc_head = k.head;
+  a->stride_vc_page = v.page, a->stride_vc_row = v.row, a->stride_vc_head = v.head;
+  a->stride_ks_page = ks.page, a->stride_ks_block = ks.row, a->stride_ks_head = ks.head;
+  a->stride_vs_page = vs.page, a->stride_vs_block = vs.row, a->stride_vs_head = vs.head;
+  a->page_size = (int32_t)k_cache.t->size(1);
+  a->block = blocks[0];
+  a->heads = (int32_t)heads;
+  a->head_dim = (int32_t)dim;
+  return true;
+}
+
+// write_quantized_cache(k, v, k_cache, v_cache, k_scales, v_scales, slots, status)
+PyObject* write_quantized_cache(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "write_quantized_cache takes 8 arguments");
+    return nullptr;
+  }
+  const int device = launch_device(x[0]);
+  Operand t[8];
+  iris_write_cache_args a{};
+  bool ok = device >= 0;
+  for (int i = 0; ok && i < 8; ++i) ok = operand(x[i], device, &t[i]);
+  enum { K, V, K_CACHE, V_CACHE, K_SCALES, V_SCALES, SLOTS, STATUS };
+  if (!ok || !t[K] || t[K].t->dim() != 3 || (a.dtype = dtype_code(*t[K].t)) < 0) return PyLong_FromLong(DECLINED);
+  const auto type = t[K].t->scalar_type();
+  const int64_t tokens = t[K].t->size(0), heads = t[K].t->size(1), dim = t[K].t->size(2);
+  if (!heads_of(t[K], type, -1, -1, -1) || !heads_of(t[V], type, tokens, heads, dim) || !vector_of(t[SLOTS], at::kLong, tokens) || !status_ok(t[STATUS]) ||
+      !quantized_cache(t[K_CACHE], t[V_CACHE], t[K_SCALES], t[V_SCALES], heads, dim, &a))
+    return PyLong_FromLong(DECLINED);
+  for (const int i : {K, V})
+    if (differentiates(t[i])) return PyLong_FromLong(DECLINED);
+  for (const int i : {K_CACHE, V_CACHE, K_SCALES, V_SCALES})
+    if (!output(t[i])) return PyLong_FromLong(DECLINED);
+  a.num_slots = t[K_CACHE].t->size(0) * t[K_CACHE].t->size(1);
+  if (a.num_slots > INT32_MAX || !apart(t, {K_CACHE, V_CACHE, K_SCALES, V_SCALES}, {K, V, SLOTS}, {})) return PyLong_FromLong(DECLINED);
+  a.k = t[K].ptr();
+  a.v = t[V].ptr();
+  a.k_cache = t[K_CACHE].ptr();
+  a.v_cache = t[V_CACHE].ptr();
+  a.k_scales = (uint8_t*)t[K_SCALES].ptr();
+  a.v_scales = (uint8_t*)t[V_SCALES].ptr();
+  a.slots = (const int64_t*)t[SLOTS].ptr();
+  a.status = (uint32_t*)t[STATUS].ptr();
+  strides_of(t[K], &a.stride_kt, &a.stride_kh);
+  strides_of(t[V], &a.stride_vt, &a.stride_vh);
+  a.tokens = (int32_t)tokens;
+  void* stream = current_stream(device);
+  return PyLong_FromLong(unlocked([&] { return iris_write_quantized_cache_launch(&a, stream); }));
+}
+
+// read_quantized_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, k_out, v_out, status)
+PyObject* read_quantized_cache(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  if (n != 10) {
+    PyErr_SetString(PyExc_TypeError, "read_quantized_cache takes 10 arguments");
+    return nullptr;
+  }
+  const int device = launch_device(x[0]);
+  Operand t[10];
+  iris_read_cache_args a{};
+  bool ok = device >= 0;
+  for (int i = 0; ok && i < 10; ++i) ok = operand(x[i], device, &t[i]);
+  enum { K_CACHE, V_CACHE, K_SCALES, V_SCALES, TABLE, LENGTHS, STARTS, K_OUT, V_OUT, STATUS };
+  if (!ok || !t[K_OUT] || t[K_OUT].t->dim() != 3 || (a.dtype = dtype_code(*t[K_OUT].t)) < 0 || !rows_contiguous(t[TABLE])) return PyLong_FromLong(DECLINED);
+  const auto type = t[K_OUT].t->scalar_type();
+  const int64_t tokens = t[K_OUT].t->size(0), heads = t[K_OUT].t->size(1), dim = t[K_OUT].t->size(2);
+  const int64_t requests = t[TABLE].t->size(0), width = t[TABLE].t->size(1);
+  if (!heads_of(t[K_OUT], type, -1, -1, -1) || !heads_of(t[V_OUT], type, tokens, heads, dim) || !output(t[K_OUT]) || !output(t[V_OUT]) ||
+      !status_ok(t[STATUS]) || !quantized_cache(t[K_CACHE], t[V_CACHE], t[K_SCALES], t[V_SCALES], heads, dim, &a) ||
+      t[TABLE].t->scalar_type() != at::kInt || requests < 1 || requests >= INT32_MAX || width > INT32_MAX || width * a.page_size > INT32_MAX ||
+      !vector_of(t[LENGTHS], at::kInt, requests) || !vector_of(t[STARTS], at::kInt, requests + 1) || (requests > 1 && t[TABLE].t->stride(0) < width))
+    return PyLong_FromLong(DECLINED);
+  for (const int i : {K_CACHE, V_CACHE})
+    if (differentiates(t[i])) return PyLong_FromLong(DECLINED);
+  if (!apart(t, {K_OUT, V_OUT}, {K_CACHE, V_CACHE, K_SCALES, V_SCALES, TABLE, LENGTHS, STARTS}, {})) return PyLong_FromLong(DECLINED);
+  a.k_cache = t[K_CACHE].ptr();
+  a.v_cache = t[V_CACHE].ptr();
+  a.k_scales = (const uint8_t*)t[K_SCALES].ptr();
+  a.v_scales = (const uint8_t*)t[V_SCALES].ptr();
+  a.block_table = (const int32_t*)t[TABLE].ptr();
+  a.lengths = (const int32_t*)t[LENGTHS].ptr();
+  a.starts = (const int32_t*)t[STARTS].ptr();
+  a.k_out = t[K_OUT].ptr();
+  a.v_out = t[V_OUT].ptr();
+  a.status = (uint32_t*)t[STATUS].ptr();
+  strides_of(t[K_OUT], &a.stride_kt, &a.stride_kh);
+  strides_of(t[V_OUT], &a.stride_vt, &a.stride_vh);
+  a.stride_table = requests > 1 ? t[TABLE].t->stride(0) : width;
+  a.requests = (int32_t)requests;
+  a.tokens = (int32_t)tokens;
+  a.table_width = (int32_t)width;
+  a.num_pages = (int32_t)t[K_CACHE].t->size(0);
+  void* stream = current_stream(device);
+  return PyLong_FromLong(unlocked([&] { return iris_read_quantized_cache_launch(&a, stream); }));
 }
 
 PyMethodDef methods[] = {
@@ -852,6 +1010,9 @@ PyMethodDef methods[] = {
     {"qk_norm_rope_backward", (PyCFunction)(void (*)(void))qk_norm_rope_backward, METH_FASTCALL, "launch their gradient; -1: declined"},
     {"overlap", (PyCFunction)(void (*)(void))overlap, METH_FASTCALL, "whether two tensors have memory in common"},
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "launch attention over a paged cache; -1: declined"},
+    {"quantized_attention", (PyCFunction)(void (*)(void))quantized_attention, METH_FASTCALL, "... over one in 8 bits; -1: declined"},
+    {"write_quantized_cache", (PyCFunction)(void (*)(void))write_quantized_cache, METH_FASTCALL, "launch the write of a cache in 8 bits; -1: declined"},
+    {"read_quantized_cache", (PyCFunction)(void (*)(void))read_quantized_cache, METH_FASTCALL, "launch its reading back; -1: declined"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", "launches through the C-ABI on torch's current stream", -1, methods,
