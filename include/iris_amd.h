@@ -564,7 +564,8 @@ int iris_attention_kernel_info(const iris_attention_args* args, int* n_regs, int
  * A paged cache in 8 bits: codes (8-bit floats, `code` IRIS_DTYPE_E4M3 or _E5M2) laid out as the 16-bit cache is, strides in elements,
  * and for every `block` tokens of a page (a multiple of 16 that divides the page size) and key head a scale: a power of two 2^(x - 127) held
  * as the byte x (255: not a number).  Element = code * scale.  Scales lie at k_scales / v_scales[page][row / block][head], strides
- * in bytes.  head_dim is a multiple of 16 up to 256, and every head begins at a multiple of 16 bytes.
+ * in bytes.  head_dim is a multiple of 16 up to 256, every head begins at a multiple of 16 bytes, and a page has 2^20 tokens at most.  (Attention
+ * takes pages less than 64 GiB, and their scales less than 4 GiB, apart.)
  */
 typedef struct iris_cache_scales {
   const uint8_t* k_scales;

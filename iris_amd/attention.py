@@ -64,6 +64,7 @@ __all__ = [
 MAX_REQUESTS = 8192  # of a call of build_block_tables (include/iris_amd.h)
 MAX_HEAD_DIM = 512  # of the norms and the rotation
 MAX_ATTENTION_HEAD_DIM = 256
+MAX_QUANTIZED_PAGE = 1 << 20  # tokens of a page of a cache in 8 bits
 INT32_MAX = (1 << 31) - 1
 
 
@@ -157,6 +158,8 @@ def _quantized(a, scales, k_cache, v_cache, k_scales, v_scales, device, heads, d
     if dim % 16 or not 0 < dim <= MAX_ATTENTION_HEAD_DIM:
         raise ValueError(f"the head size of a cache in 8 bits must be a multiple of 16 and at most {MAX_ATTENTION_HEAD_DIM}, got {dim}")
     pages, page_size = k_cache.shape[:2]
+    if page_size > MAX_QUANTIZED_PAGE:
+        raise ValueError(f"a page of a cache in 8 bits has at most {MAX_QUANTIZED_PAGE} tokens, got {page_size}")
     if k_scales is None or v_scales is None:
         raise ValueError("k_scales and v_scales come together")
     for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
@@ -755,7 +758,7 @@ def make_quantized_cache(pages, page_size, heads, head_dim, *, block=None, dtype
     block = page_size if block is None else block
     if dtype not in _CODES:
         raise TypeError(f"codes are float8_e4m3fn or float8_e5m2, got {dtype}")
-    if pages < 0 or heads < 0 or block < 1 or block % 16 or page_size < 1 or page_size % block:
+    if pages < 0 or heads < 0 or block < 1 or block % 16 or not 1 <= page_size <= MAX_QUANTIZED_PAGE or page_size % block:
         raise ValueError(f"pages of {page_size} tokens are not made of blocks of {block}, or those are no multiple of 16")
     if head_dim % 16 or not 0 < head_dim <= MAX_ATTENTION_HEAD_DIM:
         raise ValueError(f"the head size of a cache in 8 bits must be a multiple of 16 and at most {MAX_ATTENTION_HEAD_DIM}, got {head_dim}")

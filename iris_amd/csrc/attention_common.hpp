@@ -22,8 +22,24 @@ struct AttentionKArgs {
 // A cache in 8 bits has scales beside its codes.  CT: the codes' type, or 0 for a cache of the heads' own type.
 struct QuantizedKArgs : AttentionKArgs {
   iris_cache_scales s;
-  PageDiv block;
+  // Strides as 32 bits hold them (the launcher has seen to it), so that a product with a page's number is two scalar instructions.
+  uint32_t k_page16, v_page16;  // of pages of codes, in 16 bytes
+  uint32_t ks_page, vs_page, ks_block, vs_block;
+  uint32_t block16;             // (block_of)
 };
+// Where sixteen keys of a cache in 8 bits lie, `at` places into a page.
+struct CodesAt {
+  uint64_t k, v, k_scale, v_scale;  // bytes from a head's first codes and first scales
+};
+// at / block for places that are multiples of 16: with d = block / 16 and m = ceil(2^32 / d) - 1, floor((n + 1) m / 2^32) = floor(n / d)
+// for (n + 1) d <= 2^32, which pages of up to 2^20 tokens leave.
+__host__ inline uint32_t make_block16(uint32_t block) { return (uint32_t)(((1ull << 32) + block / 16 - 1) / (block / 16) - 1); }
+__device__ inline uint32_t block_of(const QuantizedKArgs& g, int at) { return __umulhi((uint32_t)at / 16 + 1, g.block16); }
+__device__ inline CodesAt codes_at(const QuantizedKArgs& g, int page, int at) {
+  const uint32_t block = block_of(g, at);
+  return {((uint64_t)(uint32_t)page * g.k_page16) * 16, ((uint64_t)(uint32_t)page * g.v_page16) * 16,
+          (uint64_t)(uint32_t)page * g.ks_page + (uint64_t)block * g.ks_block, (uint64_t)(uint32_t)page * g.vs_page + (uint64_t)block * g.vs_block};
+}
 template <int CT>
 using KArgs = std::conditional_t<CT == 0, AttentionKArgs, QuantizedKArgs>;
 

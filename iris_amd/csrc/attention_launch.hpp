@@ -31,12 +31,15 @@ hipError_t check(const iris_attention_args& a, const iris_cache_scales* s) {
   const int cache_vec = CT ? 16 : vec;  // elements of the cache in 16 bytes
   if (a.head_dim <= 0 || a.head_dim > MAX_HEAD_DIM || a.head_dim % cache_vec) return hipErrorInvalidValue;
   if constexpr (CT != 0)
-    if (s->block <= 0 || s->block % 16 || a.page_size % s->block) return hipErrorInvalidValue;
+    if (s->block <= 0 || s->block % 16 || a.page_size % s->block || a.page_size > MAX_CODES_PAGE) return hipErrorInvalidValue;
   if (a.tokens == 0 || a.q_heads == 0) return hipSuccess;
   if (a.k_heads == 0 || a.q_heads % a.k_heads || a.requests == 0 || a.table_width == 0 || a.num_pages == 0) return hipErrorInvalidValue;
   if (!a.query_starts && a.requests != a.tokens) return hipErrorInvalidValue;
-  if constexpr (CT != 0)
+  if constexpr (CT != 0) {
     if (!s->k_scales || !s->v_scales) return hipErrorInvalidValue;
+    for (const int64_t step : {a.stride_kc_page / 16, a.stride_vc_page / 16, s->stride_ks_page, s->stride_vs_page, s->stride_ks_block, s->stride_vs_block})
+      if (step < 0 || step > UINT32_MAX) return hipErrorInvalidValue;
+  }
   if (!a.q || !a.k_cache || !a.v_cache || !a.block_table || !a.lengths || !a.out || a.stride_table < a.table_width) return hipErrorInvalidValue;
   if ((int64_t)a.table_width * a.page_size > INT32_MAX) return hipErrorInvalidValue;
   for (const void* p : {a.q, a.k_cache, a.v_cache, (const void*)a.out, (const void*)a.workspace})
@@ -176,7 +179,10 @@ int launch_call(const iris_attention_args& a, const iris_cache_scales* s, void* 
   g.a = a;
   if constexpr (CT != 0) {
     g.s = *s;
-    g.block = make_page_div((uint32_t)s->block);
+    g.k_page16 = (uint32_t)(a.stride_kc_page / 16), g.v_page16 = (uint32_t)(a.stride_vc_page / 16);
+    g.ks_page = (uint32_t)s->stride_ks_page, g.vs_page = (uint32_t)s->stride_vs_page;
+    g.ks_block = (uint32_t)s->stride_ks_block, g.vs_block = (uint32_t)s->stride_vs_block;
+    g.block16 = make_block16((uint32_t)s->block);
   }
   g.page = make_page_div((uint32_t)a.page_size);
   g.scale_log2 = a.scale * 1.4426950408889634f;

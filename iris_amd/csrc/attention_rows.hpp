@@ -35,7 +35,9 @@ struct Cfg {
   static constexpr bool F32 = DT == IRIS_DTYPE_F32;
   static constexpr int ES = F32 ? 4 : 2;
   static constexpr int CS = CT ? 1 : ES;             // bytes of an element in the cache
-  static constexpr int SUBS = CT ? 4 : F32 ? 1 : 2;  // 16-key tiles of S^T a step: 16 bits' bytes in flight, whatever the type
+  // 16-key tiles of S^T a step.  (A cache in 8 bits, us with two / four of them: one request of 1999 keys, heads of 128, 9.8 / 11.4, 16 of up to
+  // 32000 25.9 / 26.9, of up to 131072 67 / 67; fp32, 16 of up to 32000 33 / 41; heads of 64, 128 that see 1028 keys 20.0 / 22.2.)
+  static constexpr int SUBS = CT == 0 && F32 ? 1 : 2;
   static constexpr int KS = 16 * SUBS;               // keys a wave takes a step
   static constexpr int BT = KS * WAVES;              // keys a workgroup takes a step
   static constexpr int QC = DP * ES / 64;            // 16-byte pieces of a query that a lane loads
@@ -170,36 +172,72 @@ struct Unit {
   }
   __device__ inline int in_page(int key) { return key - (int)(page_div((uint32_t)key, g.page) * g.page.d); }
 
+  // Of a cache in 8 bits sixteen keys lie in one page, with all sixteen places of it there to be read: their addresses are the wave's, and
+  // a lane adds its own part, the same for all of them.  Keys past `last` are what the page holds there, or the last ones' sixteen again.
+  // (As below, with every key's own address, 128 requests that see 1028 keys in heads of 64 took 27.4 us for 20.0.)
+  __device__ inline void load_codes(const Piece& p, const Row& row, int j, int last, const Pages& pages, Step& x) {
+    const int base = step_base(p, j);
+    const int64_t k_lane = (int64_t)n * a.stride_kc_row + quad * 16, v_lane = (int64_t)(quad * 4) * a.stride_vc_row + n * C::VE;
+#pragma unroll
+    for (int s = 0; s < C::SUBS; ++s) {
+      const int first_key = base + 16 * s;
+      const int64_t page = checked(pages.k[s], row, first_key, first_key + 15);
+      const int at = in_page(min(first_key, last & ~15));
+      const CodesAt w = codes_at(g, (int)page, at);
+      const IRIS_GLOBAL char* const kp = (const IRIS_GLOBAL char*)a.k_cache + (int64_t)p.head * a.stride_kc_head + w.k + (int64_t)at * a.stride_kc_row;
+      const IRIS_GLOBAL char* const vp = (const IRIS_GLOBAL char*)a.v_cache + (int64_t)p.head * a.stride_vc_head + w.v + (int64_t)at * a.stride_vc_row;
+      x.k_scale[s] = scale_byte(g.s.k_scales + p.head * g.s.stride_ks_head + w.k_scale);
+      x.v_scale[s] = scale_byte(g.s.v_scales + p.head * g.s.stride_vs_head + w.v_scale);
+#pragma unroll
+      for (int c = 0; c < C::KC; ++c) {
+        x.k[s][c] = u32x4{0, 0, 0, 0};
+        if (c * 64 + quad * 16 < a.head_dim) x.k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + k_lane + c * 64);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const IRIS_GLOBAL char* const at_r = vp + r * a.stride_vc_row + v_lane;
+#pragma unroll
+        for (int w = 0; w < C::VW; ++w) x.v[s][r][w] = 0;
+        if (n * C::VE < a.head_dim) {
+          if constexpr (C::VB == 4) {
+            x.v[s][r][0] = *(const IRIS_GLOBAL uint32_t*)at_r;
+          } else if constexpr (C::VB == 8) {
+            const u32x2 y = *(const IRIS_GLOBAL u32x2*)at_r;
+            x.v[s][r][0] = y[0], x.v[s][r][1] = y[1];
+          } else {
+            const u32x4 y = *(const IRIS_GLOBAL u32x4*)at_r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.v[s][r][i] = y[i];
+          }
+        }
+      }
+    }
+  }
+
   // Keys past `last` are read as that one, and hidden later.
   __device__ inline void load(const Piece& p, const Row& row, int j, int last, const Pages& pages, Step& x) {
+    if constexpr (CT != 0) return load_codes(p, row, j, last, pages, x);
     const int base = step_base(p, j);
 #pragma unroll
     for (int s = 0; s < C::SUBS; ++s) {
       const int first_key = base + 16 * s, own = min(first_key + n, last);
       const int64_t page = PG ? checked(pages.k[s], row, first_key, first_key + 15) : checked(pages.k[s], row, first_key + n, first_key + n);
       const IRIS_GLOBAL char* kp = (const IRIS_GLOBAL char*)a.k_cache +
-                                   (page * a.stride_kc_page + (int64_t)in_page(own) * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::CS + quad * 16;
-      if constexpr (CT != 0) {
-        const int64_t block = page_div((uint32_t)in_page(min(first_key, last)), g.block);
-        x.k_scale[s] = scale_byte(g.s.k_scales + page * g.s.stride_ks_page + block * g.s.stride_ks_block + p.head * g.s.stride_ks_head);
-        x.v_scale[s] = scale_byte(g.s.v_scales + page * g.s.stride_vs_page + block * g.s.stride_vs_block + p.head * g.s.stride_vs_head);
-      }
+                                   (page * a.stride_kc_page + (int64_t)in_page(own) * a.stride_kc_row + (int64_t)p.head * a.stride_kc_head) * C::ES + quad * 16;
 #pragma unroll
       for (int c = 0; c < C::KC; ++c) {
         x.k[s][c] = u32x4{0, 0, 0, 0};
-        if ((c * 64 + quad * 16) / C::CS < a.head_dim) x.k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + c * 64);
+        if ((c * 64 + quad * 16) / C::ES < a.head_dim) x.k[s][c] = *(const IRIS_GLOBAL u32x4*)(kp + c * 64);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int own_key = first_key + quad * 4 + r, key = min(own_key, last);
         const int64_t vpage = PG ? page : checked(pages.v[s][r], row, own_key, own_key);
         const IRIS_GLOBAL char* vp = (const IRIS_GLOBAL char*)a.v_cache +
-                                     (vpage * a.stride_vc_page + (int64_t)in_page(key) * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::CS + n * C::VB;
+                                     (vpage * a.stride_vc_page + (int64_t)in_page(key) * a.stride_vc_row + (int64_t)p.head * a.stride_vc_head) * C::ES + n * C::VB;
 #pragma unroll
         for (int w = 0; w < C::VW; ++w) x.v[s][r][w] = 0;
-        if constexpr (C::VB == 4) {
-          if (n * C::VE < a.head_dim) x.v[s][r][0] = *(const IRIS_GLOBAL uint32_t*)vp;
-        } else if constexpr (C::VB == 8) {
+        if constexpr (C::VB == 8) {
           if (n * C::VE < a.head_dim) {
             const u32x2 y = *(const IRIS_GLOBAL u32x2*)vp;
             x.v[s][r][0] = y[0], x.v[s][r][1] = y[1];
@@ -207,7 +245,7 @@ struct Unit {
         } else {
 #pragma unroll
           for (int w = 0; w < C::VW; w += 4)
-            if (n * C::VE + w * 4 / C::CS < a.head_dim) {
+            if (n * C::VE + w * 4 / C::ES < a.head_dim) {
               const u32x4 y = *(const IRIS_GLOBAL u32x4*)(vp + w * 4);
 #pragma unroll
               for (int i = 0; i < 4; ++i) x.v[s][r][w + i] = y[i];

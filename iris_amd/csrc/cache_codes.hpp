@@ -17,6 +17,7 @@ struct Codes {
   static constexpr int TOP = E4M3 ? 9 : 16;
   static constexpr uint32_t NOT_FINITE = E4M3 ? 0x7F : 0x7C;
 };
+constexpr int MAX_CODES_PAGE = 1 << 20;  // tokens of a page
 constexpr int SCALE_ONE = 127, SCALE_NAN = 255;  // a scale's byte x is 2^(x - 127)
 constexpr int SCALE_LEAST = SCALE_ONE - 100;     // of a block that is written: codes times it are ordinary fp32 numbers
 constexpr uint32_t NAN_CODES = 0x7F7F7F7Fu;      // (of both kinds)

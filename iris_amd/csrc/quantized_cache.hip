@@ -341,7 +341,7 @@ template <class Args>
 bool sizes_ok(const Args& a) {
   return (a.dtype == IRIS_DTYPE_F32 || a.dtype == IRIS_DTYPE_F16 || a.dtype == IRIS_DTYPE_BF16) &&
          (a.code == IRIS_DTYPE_E4M3 || a.code == IRIS_DTYPE_E5M2) && a.tokens >= 0 && a.heads >= 0 && a.head_dim > 0 && a.head_dim <= MAX_DIM &&
-         a.head_dim % 16 == 0 && a.page_size > 0 && a.block > 0 && a.block % 16 == 0 && a.page_size % a.block == 0;
+         a.head_dim % 16 == 0 && a.page_size > 0 && a.page_size <= MAX_CODES_PAGE && a.block > 0 && a.block % 16 == 0 && a.page_size % a.block == 0;
 }
 // (a cache without a slot has no memory)
 template <class Args>

@@ -283,9 +283,9 @@ def test_a_server_steps_in_a_captured_graph():
 
 @pytest.mark.parametrize("code", [E4M3, E5M2])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-@pytest.mark.parametrize("dim,most", [(64, 0), (128, 0), (256, 64)])
+@pytest.mark.parametrize("dim,most", [(64, 0), (128, 64), (256, 372)])
 def test_scratch_of_the_kernels(dtype, code, dim, most, monkeypatch):
-    """Scratch bytes a lane: none for heads of up to 128 in tiles of 16 rows, and no more than when they were measured elsewhere."""
+    """Scratch bytes a lane: none in tiles of 16 rows, and no more than when they were measured in those of 128."""
     for news, kernel in ((None, _native.ATTENTION_DECODE), ([3, 9], _native.ATTENTION_PROMPT_ROWS), ([900, 1300], _native.ATTENTION_PROMPT_TILES)):
         if dtype == F32 and kernel == _native.ATTENTION_PROMPT_TILES:
             continue
@@ -300,5 +300,4 @@ def test_scratch_of_the_kernels(dtype, code, dim, most, monkeypatch):
         assert _native.lib().iris_quantized_attention_plan(*args, 0, ctypes.byref(info)) == 0 and info.kernel == kernel
         assert _native.lib().iris_quantized_attention_kernel_info(*args, ctypes.byref(registers), ctypes.byref(spills)) == 0
         assert 0 < registers.value <= 512
-        if kernel != _native.ATTENTION_PROMPT_TILES:
-            assert spills.value <= most
+        assert spills.value <= (most if kernel == _native.ATTENTION_PROMPT_TILES else 0)

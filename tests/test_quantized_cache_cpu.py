@@ -62,7 +62,7 @@ def test_the_write_and_the_read_reject_bad_arguments_without_a_device():
         assert launch() == INVALID  # no tensors
         for name in names.split():  # (addresses that are never followed: every call here is refused before a launch)
             setattr(a, name, 4096)
-        common = [("dtype", 3), ("code", 5), ("code", 0), ("head_dim", 72), ("head_dim", 272), ("head_dim", 0), ("page_size", 0), ("page_size", 40), ("block", 8),
+        common = [("dtype", 3), ("code", 5), ("code", 0), ("head_dim", 72), ("head_dim", 272), ("head_dim", 0), ("page_size", 0), ("page_size", 40), ("page_size", 1 << 21), ("block", 8),
                   ("block", 0), ("block", 64), ("block", 24), ("tokens", -1), ("heads", -1), ("k_cache", 4104), ("v_cache", 4097), ("stride_kc_row", 72),
                   ("stride_vc_page", 8), ("stride_kt", 4), ("stride_vh", 7)] + [(name, 0) for name in names.split()]
         refused(launch, a, common)
@@ -86,7 +86,8 @@ def test_attention_rejects_bad_arguments_without_a_device():
     assert lib.iris_quantized_attention_launch(None, ctypes.byref(s), None) == INVALID
     assert lib.iris_quantized_attention_launch(ctypes.byref(a), None, None) == INVALID
     refused(launch, s, [("code", 2), ("code", 0), ("block", 0), ("block", 8), ("block", 64), ("block", 24), ("k_scales", 0), ("v_scales", 0)])
-    refused(launch, a, [("head_dim", 72), ("head_dim", 264), ("page_size", 20), ("stride_kc_row", 72), ("stride_vc_page", 8), ("q", 4104), ("k_cache", 4104),
+    refused(launch, s, [("stride_ks_page", 1 << 32), ("stride_vs_block", 1 << 32), ("stride_vs_page", -1)])
+    refused(launch, a, [("head_dim", 72), ("head_dim", 264), ("page_size", 20), ("page_size", 1 << 21), ("stride_kc_page", 1 << 36), ("stride_vc_page", -16), ("stride_kc_row", 72), ("stride_vc_page", 8), ("q", 4104), ("k_cache", 4104),
                         ("stride_qt", 4), ("scale", math.nan), ("k_heads", 3), ("dtype", 6), ("num_pages", 0), ("stride_table", 2)])
     info, n = _native.AttentionPlanInfo(), ctypes.c_int()
     assert lib.iris_quantized_attention_plan(ctypes.byref(a), None, CUS, ctypes.byref(info)) == INVALID
@@ -277,8 +278,13 @@ def test_make_quantized_cache():
     k, v, ks, vs = attention.make_quantized_cache(3, 64, 2, 80, device="cpu")
     assert k.shape == v.shape == (3, 64, 2, 80) and k.dtype == E4M3 and ks.shape == vs.shape == (3, 1, 2) and ks.dtype == E8M0
     assert not k.float().any() and bool((ks.float() == 1).all())
+    wide = cache(page=1, blocks=1)  # (expanded, so that it takes no memory)
+    o = dict(read_operands(), **{n: t.expand(6, 1 << 21, 2, 64) for n, t in wide.items() if "cache" in n}, k_scales=wide["k_scales"], v_scales=wide["v_scales"])
+    with pytest.raises(ValueError, match="at most 1048576"), pytest.MonkeyPatch.context() as m:
+        m.setattr(attention, "_require_cuda", lambda what, t, device: None)
+        read(**o)
     assert attention.make_quantized_cache(3, 64, 2, 80, block=16, dtype=E5M2, device="cpu")[3].shape == (3, 4, 2)
-    for bad in (dict(block=8), dict(block=48), dict(block=0), dict(page_size=24), dict(head_dim=72), dict(head_dim=512), dict(head_dim=0), dict(pages=-1)):
+    for bad in (dict(block=8), dict(block=48), dict(block=0), dict(page_size=24), dict(page_size=1 << 21), dict(head_dim=72), dict(head_dim=512), dict(head_dim=0), dict(pages=-1)):
         with pytest.raises(ValueError):
             attention.make_quantized_cache(**dict(dict(pages=3, page_size=64, heads=2, head_dim=80, device="cpu"), **bad))
     with pytest.raises(TypeError):
