@@ -3,11 +3,13 @@
 // Writing.  With M the largest code, a block of tokens of a head gets the smallest scale s = 2^e >= 2^-100 with max |x| <= M s over its
 // finite new elements, or keeps a larger one that its earlier tokens have; codes are x / s to nearest.  Earlier tokens' codes are rounded again
 // only where the scale grew, by a power of two, which moves their exponents and costs places only where they become subnormal.
-// One pass: a wave takes one block of one head (of K or of V), sixteen elements a lane, holds it in registers until the
-// maximum is known, which is an exchange within the wave, and nothing else is shared.  Blocks are found from the slots alone: a token
-// begins one where the token before it has no slot there.
+// One pass over the data: one wave (blocks of more than 16 tokens: four) takes one block of one head, of K or of V, 16 bytes a lane, and holds it
+// in registers until the maximum is known.  Blocks are found from the slots alone: a token begins one where the token
+// before it has no slot there.  bf16, 8 heads of 128, four prompts of up to 4096 tokens (50 MB) in 10.6 us, 4.7 TB/s, where a copy of 4 GB runs
+// at 4.9; 64 single tokens of one head in 2.9 us, a chain of slots, heads and scales, and stores.
 //
-// Reading.  A wave takes rows of one head of K or V, sixteen elements a lane; requests are found by bisection of their starts.
+// Reading.  A wave takes rows of one head of K or V, 16 bytes of them a lane; requests are found by bisection of their starts.  16 contexts of
+// up to 16384 tokens, 2 heads of 128 (160 MB), in 27.4 us; one of 1999 in 3.5.
 #include <initializer_list>
 #include <type_traits>
 
@@ -18,31 +20,18 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_DIM = 256;
+constexpr int NARROW = 8192;      // bytes of a block that a wave takes alone
+constexpr int MOST_UNITS = 2048;  // waves that look for blocks, at most where that leaves them 32 tokens each
 
 // ---- writing -------------------------------------------------------------------
 
 struct WriteKArgs {
   iris_write_cache_args a;
   PageDiv page, block;
-  int span;       // tokens whose blocks a wave looks after
-  int64_t units;  // waves with something to do
+  int span;       // tokens whose blocks a wave (or four) looks after
+  int64_t units;  // waves (or workgroups) with something to do
 };
 
-// Sixteen elements of type DT as they lie in memory.
-template <int DT>
-struct Sixteen {
-  static constexpr bool F32 = DT == IRIS_DTYPE_F32;
-  static constexpr int QUADS = F32 ? 4 : 2;
-  u32x4 x[QUADS];
-  __device__ inline void load(const IRIS_GLOBAL char* p) {
-#pragma unroll
-    for (int i = 0; i < QUADS; ++i) x[i] = *(const IRIS_GLOBAL u32x4*)(p + i * 16);
-  }
-  __device__ inline void clear() {
-#pragma unroll
-    for (int i = 0; i < QUADS; ++i) x[i] = u32x4{0, 0, 0, 0};
-  }
-};
 // Magnitudes of type DT as whole numbers grow as they do; from INF on they are not finite.
 template <int DT>
 struct Magnitude {
@@ -70,35 +59,56 @@ struct Magnitude {
   }
 };
 
-template <int DT, int CT>
-__device__ inline u32x4 encode16(const Sixteen<DT>& v, float scale) {
-  u32x4 y;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t w = 0;
-    if constexpr (DT == IRIS_DTYPE_F32) {
-      const f32x4 f = __builtin_bit_cast(f32x4, v.x[i]);
-      w = encode2_f32<CT, false>(w, f[0], f[1], scale);
-      w = encode2_f32<CT, true>(w, f[2], f[3], scale);
+// The codes of a lane's 16 bytes: eight, or of fp32 four.
+template <int DT>
+struct LaneCodes {
+  static constexpr int ELEMS = DT == IRIS_DTYPE_F32 ? 4 : 8, WORDS = ELEMS / 4;
+  uint32_t w[WORDS];
+  __device__ inline void load(const IRIS_GLOBAL char* p) {
+    if constexpr (WORDS == 1) {
+      w[0] = *(const IRIS_GLOBAL uint32_t*)p;
     } else {
-      w = encode2<CT, DT, false>(w, v.x[i / 2][2 * (i & 1)], scale);
-      w = encode2<CT, DT, true>(w, v.x[i / 2][2 * (i & 1) + 1], scale);
+      const u32x2 x = *(const IRIS_GLOBAL u32x2*)p;
+      w[0] = x[0], w[1] = x[1];
     }
-    y[i] = w;
   }
-  return y;
-}
+  __device__ inline void store(IRIS_GLOBAL char* p) const {
+    if constexpr (WORDS == 1)
+      *(IRIS_GLOBAL uint32_t*)p = w[0];
+    else
+      *(IRIS_GLOBAL u32x2*)p = u32x2{w[0], w[1]};
+  }
+  template <int CT>
+  __device__ inline void encode(u32x4 x, float scale) {
+    if constexpr (WORDS == 1) {
+      const f32x4 f = __builtin_bit_cast(f32x4, x);
+      w[0] = encode2_f32<CT, true>(encode2_f32<CT, false>(0, f[0], f[1], scale), f[2], f[3], scale);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) w[i] = encode2<CT, DT, true>(encode2<CT, DT, false>(0, x[2 * i], scale), x[2 * i + 1], scale);
+    }
+  }
+  template <int CT>
+  __device__ inline u32x4 decode(float scale) const {
+    if constexpr (WORDS == 1)
+      return __builtin_bit_cast(u32x4, decode4_f32<CT>(w[0], scale));
+    else
+      return u32x4{decode2<CT, DT, false>(w[0], scale), decode2<CT, DT, true>(w[0], scale), decode2<CT, DT, false>(w[1], scale),
+                   decode2<CT, DT, true>(w[1], scale)};
+  }
+};
 
-// LANES lanes hold a row.
-template <int DT, int CT, int LANES>
-__global__ __launch_bounds__(THREADS) void write_kernel(WriteKArgs g) {
+// LANES lanes hold a row, WIDE waves share a block, and each holds HOLD rows of it; MORE: blocks may have more, which are read twice.
+template <int DT, int CT, int LANES, int WIDE, int HOLD, bool MORE>
+__global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(WriteKArgs g) {
   using M = Magnitude<DT>;
-  constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, PASS = 64 / LANES;
-  constexpr int HOLD = DT == IRIS_DTYPE_F32 ? 4 : 8;  // passes of rows that stay in registers; more are read twice
+  using Codes8 = LaneCodes<DT>;
+  constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, PASS = 64 / LANES, HELD = HOLD / PASS, BATCH = 8;
+  __shared__ uint32_t wave_most[2][WIDE];
   const iris_write_cache_args& a = g.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t unit = (int64_t)blockIdx.x * WAVES + wave;
-  if (unit >= g.units) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part_of = WIDE > 1 ? wave : 0;
+  const int64_t unit = WIDE > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * WAVES + wave;
+  if (unit >= g.units) return;  // (with WIDE waves all of a workgroup's)
   // values and keys change fastest, then heads
   const bool values = unit & 1;
   const int chunk = (int)(unit / 2 / a.heads), head = (int)(unit / 2 - (int64_t)chunk * a.heads);
@@ -112,114 +122,125 @@ __global__ __launch_bounds__(THREADS) void write_kernel(WriteKArgs g) {
   const int64_t scale_page = values ? a.stride_vs_page : a.stride_ks_page, scale_block = values ? a.stride_vs_block : a.stride_ks_block;
   const int64_t scale_head = values ? a.stride_vs_head : a.stride_ks_head;
 
-  // the chunk's tokens that begin a block
+  // The chunk's tokens that begin a block.  Lanes behind the chunk hold the slots that its last block may go on with.
   const int first = chunk * g.span;
   int64_t slot = -1, before = -1;
-  if (lane < g.span && first + lane < a.tokens) {
+  if (first + lane < a.tokens) {
     slot = slots[first + lane];
     if (first + lane > 0) before = slots[first + lane - 1];
   }
   const bool inside = slot >= 0 && slot < a.num_slots;
   const bool goes_on = inside && before >= 0 && before < a.num_slots && page_div((uint32_t)before, g.block) == page_div((uint32_t)slot, g.block);
-  if (slot >= a.num_slots || (goes_on && slot != before + 1)) report(a.status, IRIS_STATUS_BAD_INDEX);
-  for (uint64_t begins = __ballot(inside && !goes_on); begins; begins &= begins - 1) {
+  if (lane < g.span && (slot >= a.num_slots || (goes_on && slot != before + 1))) report(a.status, IRIS_STATUS_BAD_INDEX);
+  const uint64_t in_a_row = __ballot(goes_on && slot == before + 1);
+  int parity = 0;
+  for (uint64_t begins = __ballot(inside && !goes_on && lane < g.span); begins; begins &= begins - 1) {
     const int at = __builtin_ctzll(begins), token = first + at;
     const uint32_t slot0 = __builtin_amdgcn_readlane((int)slot, at);
     const uint32_t page = page_div(slot0, g.page), row_in_page = slot0 - page * g.page.d;
     const uint32_t block = page_div(row_in_page, g.block);  // of the page
     const int older = (int)(row_in_page - block * g.block.d);
-    // the block's new tokens
-    int rows = 0;
-    for (int most = min((int)g.block.d - older, a.tokens - token); rows < most;) {
-      const int i = rows + lane;
-      const uint64_t others = ~__ballot(i < most && slots[token + min(i, most - 1)] == (int64_t)slot0 + i);
-      const int n = others ? __builtin_ctzll(others) : 64;
-      rows += n;
-      if (n < 64) break;
-    }
     IRIS_GLOBAL uint8_t* const scale_at = scales + page * scale_page + block * scale_block + head * scale_head;
     int old = 0;
     if (older) old = *scale_at;
-
-    const int row = lane / LANES, part = lane % LANES;
-    const bool live = part * 16 < a.head_dim;
-    const IRIS_GLOBAL char* const source = from + ((int64_t)(token + row) * stride_t + head * stride_h + part * 16) * ES;
-    IRIS_GLOBAL char* const target = to + page * to_page + (int64_t)row_in_page * to_row + head * to_head + part * 16;
-    Sixteen<DT> held[HOLD];
-    uint32_t most = 0;
-    auto load = [&](Sixteen<DT>& v, int i) {
-      v.clear();
-      if (live && i * PASS + row < rows) v.load(source + (int64_t)i * PASS * stride_t * ES);
-    };
-    auto measure = [&](const Sixteen<DT>& v) {
-#pragma unroll
-      for (int q = 0; q < Sixteen<DT>::QUADS; ++q)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) most = M::larger(most, v.x[q][w]);
-    };
-    auto replace = [&](Sixteen<DT>& v, uint32_t by) {
-#pragma unroll
-      for (int q = 0; q < Sixteen<DT>::QUADS; ++q)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) v.x[q][w] = M::replaced(v.x[q][w], by);
-    };
-#pragma unroll
-    for (int i = 0; i < HOLD; ++i)
-      if (i * PASS < rows) load(held[i], i);
-#pragma unroll
-    for (int i = 0; i < HOLD; ++i)
-      if (i * PASS < rows) measure(held[i]);
-    for (int i = HOLD; i * PASS < rows; ++i) {
-      Sixteen<DT> v;
-      load(v, i);
-      measure(v);
+    // the block's new tokens, those whose slots the lanes hold first
+    const uint64_t breaks = ~(in_a_row >> at) & ~1ull;  // (bits past the lanes' are breaks)
+    int rows = breaks ? __builtin_ctzll(breaks) : 64;
+    if (rows == 64 - at) {
+      for (int most = min((int)g.block.d - older, a.tokens - token); rows < most;) {
+        const int i = rows + lane;
+        const uint64_t others = ~__ballot(i < most && slots[token + min(i, most - 1)] == (int64_t)slot0 + i);
+        const int n = others ? __builtin_ctzll(others) : 64;
+        rows += n;
+        if (n < 64) break;
+      }
     }
+
+    const int row = part_of * PASS + lane / LANES, part = lane % LANES;  // (of the first pass)
+    const bool live = part * Codes8::ELEMS < a.head_dim;
+    const IRIS_GLOBAL char* const source = from + ((int64_t)(token + row) * stride_t + head * stride_h) * ES + part * 16;
+    IRIS_GLOBAL char* const target = to + page * to_page + (int64_t)row_in_page * to_row + head * to_head + part * Codes8::ELEMS;
+    u32x4 held[HELD];
+    uint32_t most = 0;
+    auto mine = [&](int i) { return live && i * (WIDE * PASS) + row < rows; };
+    auto load = [&](int i) { return mine(i) ? *(const IRIS_GLOBAL u32x4*)(source + (int64_t)i * (WIDE * PASS) * stride_t * ES) : u32x4{0, 0, 0, 0}; };
+    auto measure = [&](u32x4 v) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) most = M::larger(most, v[w]);
+    };
+    auto replace = [&](u32x4 v, uint32_t by) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v[w] = M::replaced(v[w], by);
+      return v;
+    };
+    // The largest of the block's, as a number; all waves that share it agree.
+    auto over_block = [&](uint32_t x) {
+      uint32_t all = __builtin_bit_cast(uint32_t, over_lanes<64>(M::number(M::only(x)), Larger{}));
+      if constexpr (WIDE > 1) {
+        if (lane == 0) wave_most[parity][wave] = all;
+        __syncthreads();  // (the other half is read before the next one's barrier, this one written behind it)
+#pragma unroll
+        for (int w = 0; w < WIDE; ++w) all = max(all, wave_most[parity][w]);
+        parity ^= 1;
+      }
+      return all;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) held[i] = load(i);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) measure(held[i]);
+    // f(passes that are not held, one at a time), BATCH of their loads in flight
+    auto rest = [&](auto f) {
+      if constexpr (!MORE) return;
+      for (int i0 = HELD; i0 * (WIDE * PASS) < rows; i0 += BATCH) {
+        u32x4 v[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) v[i] = load(i0 + i);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) f(i0 + i, v[i]);
+      }
+    };
+    rest([&](int, u32x4 v) { measure(v); });
     // what is not finite counts for nothing here, and is no number as a code
     const bool odd = __any(M::only(most) >= M::INF);
     if (odd) {
       most = 0;
-      for (int i = 0; i * PASS < rows; ++i) {
-        Sixteen<DT> v;
-        load(v, i);
-        replace(v, 0);
-        measure(v);
-      }
 #pragma unroll
-      for (int i = 0; i < HOLD; ++i)
-        if (i * PASS < rows) replace(held[i], M::NOT_A_NUMBER);
+      for (int i = 0; i < HELD; ++i) {
+        measure(replace(held[i], 0));
+        held[i] = replace(held[i], M::NOT_A_NUMBER);
+      }
+      rest([&](int, u32x4 v) { measure(replace(v, 0)); });
     }
-    const uint32_t largest = __builtin_bit_cast(uint32_t, over_lanes<64>(M::number(M::only(most)), Larger{}));
+    old = __builtin_amdgcn_readfirstlane(old);  // (read by all waves that share the block, before one of them writes it)
+    const uint32_t largest = over_block(most);
     // largest = 1.m * 2^(x - 127) and M = 1.75 * 2^(TOP - 1)
     int need = (int)(largest >> 23) - (Codes<CT>::TOP - 1) + ((largest & 0x7FFFFFu) > 0x600000u);
     need = __builtin_amdgcn_readfirstlane(max(need, SCALE_LEAST));
-    old = __builtin_amdgcn_readfirstlane(old);
     const int now = older ? max(need, old) : need;
     const float scale = scale_of(min(now, 254));
+    Codes8 y;
+    auto write = [&](int i, u32x4 v) {
+      if (!mine(i)) return;
+      y.template encode<CT>(v, scale);
+      y.store(target + (int64_t)(i * (WIDE * PASS) + row) * to_row);
+    };
 #pragma unroll
-    for (int i = 0; i < HOLD; ++i)
-      if (live && i * PASS + row < rows) *(IRIS_GLOBAL u32x4*)(target + (int64_t)(i * PASS + row) * to_row) = encode16<DT, CT>(held[i], scale);
-    for (int i = HOLD; i * PASS < rows; ++i) {
-      Sixteen<DT> v;
-      load(v, i);
-      if (odd) replace(v, M::NOT_A_NUMBER);
-      if (live && i * PASS + row < rows) *(IRIS_GLOBAL u32x4*)(target + (int64_t)(i * PASS + row) * to_row) = encode16<DT, CT>(v, scale);
-    }
+    for (int i = 0; i < HELD; ++i) write(i, held[i]);
+    rest([&](int i, u32x4 v) { write(i, odd ? replace(v, M::NOT_A_NUMBER) : v); });
     if (now == old && older) continue;
-    if (lane == 0) *scale_at = (uint8_t)now;
+    if (lane == 0 && part_of == 0) *scale_at = (uint8_t)now;
     if (older) {
       const float shrink = scale_of(max(old - now + SCALE_ONE, 1));
       IRIS_GLOBAL char* const there = target - (int64_t)older * to_row;
-      for (int r = row; r < older; r += PASS) {
-        if (!live) break;
-        IRIS_GLOBAL char* const p = there + (int64_t)r * to_row;
-        u32x4 y = *(const IRIS_GLOBAL u32x4*)p;
+      for (int r = row; r < older && live; r += WIDE * PASS) {
+        y.load(there + (int64_t)r * to_row);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const f32x4 f = decode4_f32<CT>(y[w], shrink);
-          uint32_t c = encode2_f32<CT, false>(0, f[0], f[1], 1.f);
-          y[w] = encode2_f32<CT, true>(c, f[2], f[3], 1.f);
+        for (int w = 0; w < Codes8::WORDS; ++w) {
+          const f32x4 f = decode4_f32<CT>(y.w[w], shrink);
+          y.w[w] = encode2_f32<CT, true>(encode2_f32<CT, false>(0, f[0], f[1], 1.f), f[2], f[3], 1.f);
         }
-        *(IRIS_GLOBAL u32x4*)p = y;
+        y.store(there + (int64_t)r * to_row);
       }
     }
   }
@@ -237,6 +258,7 @@ constexpr int STARTS = 2048;  // requests whose starts a workgroup holds; with m
 // LANES lanes hold a row; a wave takes PASSES times 64 / LANES rows.
 template <int DT, int CT, int LANES, int PASSES>
 __global__ __launch_bounds__(THREADS) void read_kernel(ReadKArgs g) {
+  using Codes8 = LaneCodes<DT>;
   constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, PASS = 64 / LANES;
   __shared__ int32_t starts[STARTS + 1];
   const iris_read_cache_args& a = g.a;
@@ -253,77 +275,84 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadKArgs g) {
   const int head = (int)(unit / 2 - chunk * a.heads);
   auto start = [&](int r) { return held ? starts[r] : a.starts[r]; };
   const int row = lane / LANES, part = lane % LANES;
-  const bool live = part * 16 < a.head_dim;
+  const bool live = part * Codes8::ELEMS < a.head_dim;
+  const IRIS_GLOBAL char* const cache = (const IRIS_GLOBAL char*)(values ? a.v_cache : a.k_cache) + head * (values ? a.stride_vc_head : a.stride_kc_head) +
+                                        part * Codes8::ELEMS;
+  const uint8_t* const scales = (values ? a.v_scales : a.k_scales) + head * (values ? a.stride_vs_head : a.stride_ks_head);
+  const int64_t from_page = values ? a.stride_vc_page : a.stride_kc_page, from_row = values ? a.stride_vc_row : a.stride_kc_row;
+  const int64_t scale_page = values ? a.stride_vs_page : a.stride_ks_page, scale_block = values ? a.stride_vs_block : a.stride_ks_block;
+  IRIS_GLOBAL char* const out = (IRIS_GLOBAL char*)(values ? a.v_out : a.k_out) + head * (values ? a.stride_vh : a.stride_kh) * ES + part * 16;
+  const int64_t out_row = (values ? a.stride_vt : a.stride_kt) * ES;
 
-  int64_t token[PASSES];
+  const int64_t first = chunk * (PASSES * PASS);
+  // the last request that does not start behind the wave's first row, and from there for each row
+  int lo = 0;
+  for (int hi = a.requests; hi - lo > 1;) {
+    const int mid = (lo + hi) / 2;
+    if (start(mid) <= first)
+      lo = mid;
+    else
+      hi = mid;
+  }
   int request[PASSES], position[PASSES], page[PASSES];
   bool mine[PASSES], there[PASSES];
+  int ends = start(lo + 1), begins = start(lo);
+  int64_t length = a.lengths[lo];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    token[i] = chunk * (PASSES * PASS) + i * PASS + row;
-    // the last request that does not start behind it
-    int lo = 0;
-    for (int hi = a.requests; hi - lo > 1;) {
-      const int mid = (lo + hi) / 2;
-      if (start(mid) <= token[i])
-        lo = mid;
-      else
-        hi = mid;
+    const int64_t token = first + i * PASS + row;
+    if (token >= ends && lo + 1 < a.requests) {
+      // (of a wave's rows in a middle request; bisection again, for there may be many that have none)
+      for (int hi = a.requests; hi - lo > 1;) {
+        const int mid = (lo + hi) / 2;
+        if (start(mid) <= token)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      begins = start(lo);
+      ends = start(lo + 1);
+      length = a.lengths[lo];
     }
     request[i] = lo;
-    mine[i] = token[i] < a.tokens && start(lo) <= token[i] && token[i] < start(lo + 1);
-    position[i] = 0;
-    there[i] = false;
-    if (mine[i]) {
-      const int64_t at = (int64_t)a.lengths[lo] - start(lo + 1) + token[i];
-      there[i] = at >= 0 && at < (int64_t)a.table_width * a.page_size;
-      position[i] = there[i] ? (int)at : 0;
-    }
+    mine[i] = token < a.tokens && begins <= token && token < ends;
+    const int64_t at = length - ends + token;
+    there[i] = mine[i] && at >= 0 && at < (int64_t)a.table_width * a.page_size;
+    position[i] = there[i] ? (int)at : 0;
   }
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    page[i] = 0;
+    page[i] = -1;
     if (there[i]) page[i] = a.block_table[request[i] * a.stride_table + page_div((uint32_t)position[i], g.page)];
-    there[i] = there[i] && (uint32_t)page[i] < (uint32_t)a.num_pages;
-    if (mine[i] && !there[i]) report(a.status, IRIS_STATUS_BAD_INDEX);
   }
-  u32x4 codes[PASSES];
+  Codes8 codes[PASSES];
   uint32_t byte[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    codes[i] = u32x4{NAN_CODES, NAN_CODES, NAN_CODES, NAN_CODES};
-    byte[i] = SCALE_ONE;
+    there[i] = there[i] && (uint32_t)page[i] < (uint32_t)a.num_pages;
+    byte[i] = SCALE_NAN;
     if (there[i] && live) {
       const int in_page = position[i] - (int)(page_div((uint32_t)position[i], g.page) * g.page.d);
-      const int block = (int)page_div((uint32_t)in_page, g.block);
-      const int64_t at = values ? page[i] * a.stride_vc_page + in_page * a.stride_vc_row + head * a.stride_vc_head
-                                : page[i] * a.stride_kc_page + in_page * a.stride_kc_row + head * a.stride_kc_head;
-      const int64_t scale_at = values ? page[i] * a.stride_vs_page + block * a.stride_vs_block + head * a.stride_vs_head
-                                      : page[i] * a.stride_ks_page + block * a.stride_ks_block + head * a.stride_ks_head;
-      codes[i] = *(const IRIS_GLOBAL u32x4*)((const IRIS_GLOBAL char*)(values ? a.v_cache : a.k_cache) + at + part * 16);
-      byte[i] = scale_byte((values ? a.v_scales : a.k_scales) + scale_at);
+      codes[i].load(cache + page[i] * from_page + in_page * from_row);
+      byte[i] = scale_byte(scales + page[i] * scale_page + page_div((uint32_t)in_page, g.block) * scale_block);
     }
   }
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     if (!mine[i] || !live) continue;
-    IRIS_GLOBAL char* out = values ? (IRIS_GLOBAL char*)a.v_out + (token[i] * a.stride_vt + head * a.stride_vh + part * 16) * ES
-                                   : (IRIS_GLOBAL char*)a.k_out + (token[i] * a.stride_kt + head * a.stride_kh + part * 16) * ES;
-    if (byte[i] == SCALE_NAN) codes[i] = u32x4{NAN_CODES, NAN_CODES, NAN_CODES, NAN_CODES}, byte[i] = SCALE_ONE;
-    const float scale = scale_of((int)byte[i]);
-    if constexpr (DT == IRIS_DTYPE_F32) {
+    if (!there[i] && part == 0) report(a.status, IRIS_STATUS_BAD_INDEX);
+    if (byte[i] == SCALE_NAN) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) *(IRIS_GLOBAL f32x4*)(out + w * 16) = decode4_f32<CT>(codes[i][w], scale);
-    } else {
-      u32x4 y[2];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        y[w / 2][2 * (w & 1)] = decode2<CT, DT, false>(codes[i][w], scale);
-        y[w / 2][2 * (w & 1) + 1] = decode2<CT, DT, true>(codes[i][w], scale);
-      }
-      *(IRIS_GLOBAL u32x4*)out = y[0];
-      *(IRIS_GLOBAL u32x4*)(out + 16) = y[1];
+      for (int w = 0; w < Codes8::WORDS; ++w) codes[i].w[w] = NAN_CODES;
+      byte[i] = SCALE_ONE;
     }
+    const u32x4 y = codes[i].template decode<CT>(scale_of((int)byte[i]));
+    IRIS_GLOBAL u32x4* const to = (IRIS_GLOBAL u32x4*)(out + (first + i * PASS + row) * out_row);
+    // (many rows pass the caches by: 160 MB, a third of them codes, 27.4 us for 39.8)
+    if constexpr (PASSES > 2)
+      __builtin_nontemporal_store(y, to);
+    else
+      *to = y;
   }
 }
 
@@ -359,9 +388,10 @@ template <class Args, class F>
 hipError_t with_types(const Args& a, F f) {
   using std::integral_constant;
   auto lanes = [&](auto dt, auto ct) {
-    if (a.head_dim <= 64) return f(dt, ct, integral_constant<int, 4>{});
-    if (a.head_dim <= 128) return f(dt, ct, integral_constant<int, 8>{});
-    return f(dt, ct, integral_constant<int, 16>{});
+    constexpr int ELEMS = LaneCodes<dt.value>::ELEMS;
+    if (a.head_dim <= 64) return f(dt, ct, integral_constant<int, 64 / ELEMS>{});
+    if (a.head_dim <= 128) return f(dt, ct, integral_constant<int, 128 / ELEMS>{});
+    return f(dt, ct, integral_constant<int, 256 / ELEMS>{});
   };
   auto codes = [&](auto dt) {
     return a.code == IRIS_DTYPE_E4M3 ? lanes(dt, integral_constant<int, IRIS_DTYPE_E4M3>{}) : lanes(dt, integral_constant<int, IRIS_DTYPE_E5M2>{});
@@ -385,15 +415,25 @@ extern "C" int iris_write_quantized_cache_launch(const iris_write_cache_args* ar
   g.a = a;
   g.page = make_page_div((uint32_t)a.page_size);
   g.block = make_page_div((uint32_t)a.block);
-  // Waves without a block cost their start only, waves with several take them one after another.
+  // A wave takes a short block alone, four share one of up to 128 tokens, sixteen a longer one.  (us with one / four, bf16: 32 tokens of 64
+  // elements 7.0 / 10.0, of 128 10.1 / 10.9; with four / sixteen: 64 tokens of 128 9.7 / 35, 128 10.4 / 25, 256 of 256 34 / 31, fp32 50 / 26.)
+  const int64_t bytes = (int64_t)a.block * (a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256) * dtype_size(a.dtype);
+  const int wide = a.block <= 32 && bytes <= NARROW ? 1 : a.block <= 128 ? 4 : 16;
+  // Units without a block cost their start, those with several take them one after another.  (us with 8192 / 2048 / 1024 units at most: prompts of
+  // up to 8192 tokens, one head, 5.8 / 4.7 / 5.4; 500 tokens in blocks of 64 5.4 / 3.4 / 3.1; 256 single tokens of 8 heads 3.9 / 4.0 / 4.8.)
   g.span = 1;
   auto units = [&] { return ((int64_t)a.tokens + g.span - 1) / g.span * a.heads * 2; };
-  while (g.span < 64 && units() > 16384) g.span *= 2;
+  while (g.span < (wide == 16 ? 64 : 32) && units() > MOST_UNITS / wide) g.span *= 2;
   g.units = units();
-  const int64_t groups = (g.units + WAVES - 1) / WAVES;
+  const int64_t groups = wide > 1 ? g.units : (g.units + WAVES - 1) / WAVES;
   if (groups > INT32_MAX) return hipErrorInvalidValue;
   return with_types(a, [&](auto dt, auto ct, auto lanes) {
-    return launch(write_kernel<dt.value, ct.value, lanes.value>, dim3((unsigned)groups), THREADS, 0, stream, g);
+    constexpr int DT = dt.value, CT = ct.value, LANES = lanes.value;
+    const auto kernel = wide == 1    ? (a.block <= 16 ? write_kernel<DT, CT, LANES, 1, 16, false> : write_kernel<DT, CT, LANES, 1, 32, false>)
+                        : wide == 4  ? (a.block <= 64 ? write_kernel<DT, CT, LANES, 4, 16, false> : write_kernel<DT, CT, LANES, 4, 32, false>)
+                        : a.block <= 256 ? write_kernel<DT, CT, LANES, 16, 16, false>
+                                         : write_kernel<DT, CT, LANES, 16, 16, true>;
+    return launch(kernel, dim3((unsigned)groups), wide > 1 ? wide * 64 : THREADS, 0, stream, g);
   });
 }
 
@@ -420,6 +460,6 @@ extern "C" int iris_read_quantized_cache_launch(const iris_read_cache_args* args
       return launch(read_kernel<DT, CT, LANES, passes.value>, dim3((unsigned)groups), THREADS, 0, stream, g);
     };
     using std::integral_constant;
-    return units(4) >= 8 * 4 * (int64_t)current_cu_count() ? run(integral_constant<int, 4>{}) : run(integral_constant<int, 1>{});
+    return units(8) >= 16 * (int64_t)current_cu_count() ? run(integral_constant<int, 8>{}) : run(integral_constant<int, 2>{});
   });
 }
