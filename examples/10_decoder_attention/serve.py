@@ -11,7 +11,8 @@ and its shards of both projections.  A step is
     prompt_attention      or decode_attention: the rank's heads over the cache
     one-shot all-reduce   y = sum over ranks of heads @ W_o, the rank's K-shard
 
-and requests that end give their pages back to the ring, from which later steps take them.
+With ``--cache_dtype e4m3`` (or ``e5m2``) the caches are in 8 bits: qk_norm_rope writes none, and write_quantized_cache stands behind it.
+Requests that end give their pages back to the ring, from which later steps take them.
 ``--validate`` compares every step's output with the layer computed densely in 64 bits on the CPU.
 """
 
@@ -30,6 +31,7 @@ from iris_amd.matmul import matmul_one_shot_all_reduce as all_reduce  # noqa: E4
 
 DATATYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 PROGRAMS, TILE_M, TILE_N = 256, 64, 64
+CODES = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 EPS = 1e-6
 
 
@@ -47,6 +49,7 @@ def parse_args(argv=None):
     p.add_argument("--window", type=int, default=0, help="Sliding window (0: none)")
     p.add_argument("--sinks", type=int, default=0, help="First tokens that stay visible outside of the window")
     p.add_argument("--datatype", choices=list(DATATYPES), default="bf16", help="Datatype of computation")
+    p.add_argument("--cache_dtype", choices=["same", *CODES], default="same", help="The caches' type: the datatype, or 8 bits with a scale a page and head")
     p.add_argument("-v", "--validate", action="store_true", help="Compare with the dense layer in 64 bits")
     return p.parse_args(argv)
 
@@ -73,8 +76,11 @@ class Layer:
         self.q_weight, self.k_weight = 1 + normal(d, std=0.1), 1 + normal(d, std=0.1)
         self.cos, self.sin = attention.rope_tables(args.pages * args.page_size, d)
         cache = (args.pages, args.page_size, self.hk, d)
-        self.caches = [(torch.zeros(cache, dtype=self.dtype, device="cuda"), torch.zeros(cache, dtype=self.dtype, device="cuda"))
-                       for _ in range(ranks)]
+        if args.cache_dtype == "same":
+            self.caches = [(torch.zeros(cache, dtype=self.dtype, device="cuda"), torch.zeros(cache, dtype=self.dtype, device="cuda"))
+                           for _ in range(ranks)]
+        else:
+            self.caches = [attention.make_quantized_cache(*cache, dtype=CODES[args.cache_dtype]) for _ in range(ranks)]
         self.workspace = attention.make_workspace(d)
         # what peers touch lies in the symmetric heap: partial sums, results, ready flags
         self.partial = self.shmem.zeros((self.most, args.hidden), dtype=torch.float32)
@@ -121,11 +127,16 @@ class Layer:
         ops.gemm_launch(x, self.w_qkv[r].T, None, qkv, None, None, 0, 1, PROGRAMS, TILE_M, TILE_N, 64, 4, ops.EPI_ALL_SCATTER, notify=False,
                         num_xcds=8)
         q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((self.hq * d, self.hk * d, self.hk * d), 1))
-        k_cache, v_cache = self.caches[r]
-        attention.qk_norm_rope(q, k, positions, self.cos, self.sin, q, None, q_weight=self.q_weight, k_weight=self.k_weight, eps=EPS, v=v,
-                               k_cache=k_cache, v_cache=v_cache, slots=slots, status=self.status)
+        k_cache, v_cache, *scales = self.caches[r]
+        norm = dict(q_weight=self.q_weight, k_weight=self.k_weight, eps=EPS, status=self.status)
         out = torch.empty((tokens, self.hq, d), dtype=self.dtype, device="cuda")
         options = dict(window=args.window, sinks=args.sinks, workspace=self.workspace, status=self.status)
+        if scales:
+            attention.qk_norm_rope(q, k, positions, self.cos, self.sin, q, k, **norm)
+            attention.write_quantized_cache(k, v, k_cache, v_cache, *scales, slots, status=self.status)
+            options.update(k_scales=scales[0], v_scales=scales[1])
+        else:
+            attention.qk_norm_rope(q, k, positions, self.cos, self.sin, q, None, v=v, k_cache=k_cache, v_cache=v_cache, slots=slots, **norm)
         if single:
             attention.decode_attention(q, k_cache, v_cache, self.table, self.lengths[0], out, **options)
         else:
@@ -189,6 +200,8 @@ def main(argv=None):
     if args.validate:
         # roundings to 16 bits on the way: projections, heads, weights, outputs, a few half places each
         bound = 8 * (2.0 ** -8 if layer.dtype == torch.bfloat16 else 2.0 ** -11)
+        # keys and values in 8 bits are off by half a place of theirs at most: each once
+        bound += {"same": 0, "e4m3": 2 * 2.0 ** -4, "e5m2": 2 * 2.0 ** -3}[args.cache_dtype]
         ok = worst <= bound and free == args.pages
         print(f"largest error of a step {worst:.2e} of its norm: {'passed' if ok else 'FAILED'}", flush=True)
         return 0 if ok else 1

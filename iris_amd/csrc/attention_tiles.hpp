@@ -269,7 +269,7 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
       bad_page |= none && key <= rows_last && (key + 15 >= list.lo || key < a.sinks);
       page = none ? 0 : page;
       const int in_page = key - (int)(page_div((uint32_t)key, g.page) * g.page.d);
-      coded = length - key;
+      coded = none ? 0 : length - key;
       const CodesAt w = codes_at(g, page, in_page);
       const __amdgpu_buffer_rsrc_t kr = tile_rsrc((const IRIS_GLOBAL char*)a.k_cache + (int64_t)head * a.stride_kc_head + w.k, 0x7FFFFFFF);
       const __amdgpu_buffer_rsrc_t vr = tile_rsrc((const IRIS_GLOBAL char*)a.v_cache + (int64_t)head * a.stride_vc_head + w.v, 0x7FFFFFFF);

@@ -103,7 +103,7 @@ template <int DT, int CT, int LANES, int WIDE, int HOLD, bool MORE>
 __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(WriteKArgs g) {
   using M = Magnitude<DT>;
   using Codes8 = LaneCodes<DT>;
-  constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, PASS = 64 / LANES, HELD = HOLD / PASS, BATCH = 8;
+  constexpr int ES = DT == IRIS_DTYPE_F32 ? 4 : 2, PASS = 64 / LANES, HELD = HOLD / PASS, BATCH = 4;
   __shared__ uint32_t wave_most[2][WIDE];
   const iris_write_cache_args& a = g.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part_of = WIDE > 1 ? wave : 0;
@@ -111,7 +111,8 @@ __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(W
   if (unit >= g.units) return;  // (with WIDE waves all of a workgroup's)
   // values and keys change fastest, then heads
   const bool values = unit & 1;
-  const int chunk = (int)(unit / 2 / a.heads), head = (int)(unit / 2 - (int64_t)chunk * a.heads);
+  const int64_t chunk = unit / 2 / a.heads;
+  const int head = (int)(unit / 2 - chunk * a.heads);
   const IRIS_GLOBAL int64_t* slots = (const IRIS_GLOBAL int64_t*)a.slots;
   const IRIS_GLOBAL char* from = (const IRIS_GLOBAL char*)(values ? a.v : a.k);
   const int64_t stride_t = values ? a.stride_vt : a.stride_kt, stride_h = values ? a.stride_vh : a.stride_kh;
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(W
   const int64_t scale_head = values ? a.stride_vs_head : a.stride_ks_head;
 
   // The chunk's tokens that begin a block.  Lanes behind the chunk hold the slots that its last block may go on with.
-  const int first = chunk * g.span;
+  const int64_t first = chunk * g.span;
   int64_t slot = -1, before = -1;
   if (first + lane < a.tokens) {
     slot = slots[first + lane];
@@ -135,7 +136,8 @@ __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(W
   const uint64_t in_a_row = __ballot(goes_on && slot == before + 1);
   int parity = 0;
   for (uint64_t begins = __ballot(inside && !goes_on && lane < g.span); begins; begins &= begins - 1) {
-    const int at = __builtin_ctzll(begins), token = first + at;
+    const int at = __builtin_ctzll(begins);
+    const int64_t token = first + at;
     const uint32_t slot0 = __builtin_amdgcn_readlane((int)slot, at);
     const uint32_t page = page_div(slot0, g.page), row_in_page = slot0 - page * g.page.d;
     const uint32_t block = page_div(row_in_page, g.block);  // of the page
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(W
     const uint64_t breaks = ~(in_a_row >> at) & ~1ull;  // (bits past the lanes' are breaks)
     int rows = breaks ? __builtin_ctzll(breaks) : 64;
     if (rows == 64 - at) {
-      for (int most = min((int)g.block.d - older, a.tokens - token); rows < most;) {
+      for (int most = (int)min((int64_t)g.block.d - older, a.tokens - token); rows < most;) {
         const int i = rows + lane;
         const uint64_t others = ~__ballot(i < most && slots[token + min(i, most - 1)] == (int64_t)slot0 + i);
         const int n = others ? __builtin_ctzll(others) : 64;
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(W
 
     const int row = part_of * PASS + lane / LANES, part = lane % LANES;  // (of the first pass)
     const bool live = part * Codes8::ELEMS < a.head_dim;
-    const IRIS_GLOBAL char* const source = from + ((int64_t)(token + row) * stride_t + head * stride_h) * ES + part * 16;
+    const IRIS_GLOBAL char* const source = from + ((token + row) * stride_t + head * stride_h) * ES + part * 16;
     IRIS_GLOBAL char* const target = to + page * to_page + (int64_t)row_in_page * to_row + head * to_head + part * Codes8::ELEMS;
     u32x4 held[HELD];
     uint32_t most = 0;
@@ -432,7 +434,7 @@ extern "C" int iris_write_quantized_cache_launch(const iris_write_cache_args* ar
     const auto kernel = wide == 1    ? (a.block <= 16 ? write_kernel<DT, CT, LANES, 1, 16, false> : write_kernel<DT, CT, LANES, 1, 32, false>)
                         : wide == 4  ? (a.block <= 64 ? write_kernel<DT, CT, LANES, 4, 16, false> : write_kernel<DT, CT, LANES, 4, 32, false>)
                         : a.block <= 256 ? write_kernel<DT, CT, LANES, 16, 16, false>
-                                         : write_kernel<DT, CT, LANES, 16, 16, true>;
+                                         : write_kernel<DT, CT, LANES, 16, 8, true>;
     return launch(kernel, dim3((unsigned)groups), wide > 1 ? wide * 64 : THREADS, 0, stream, g);
   });
 }

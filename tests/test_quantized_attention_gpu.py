@@ -281,6 +281,65 @@ def test_a_server_steps_in_a_captured_graph():
         state.copy_(state_out)
 
 
+@pytest.mark.parametrize("news", [None, [300], [9]])
+def test_addresses_past_32_bits(news):
+    """A cache of 6 GB of codes a side, whose last pages are a request's."""
+    p = Quantized([500], news, 4, 2, 128, BF16, 64, block=32)
+    pages, held = (6 << 30) // (64 * 2 * 128), p.k_cache.shape[0]
+    for name in ("k", "v"):
+        cache = torch.empty((pages, 64, 2, 128), dtype=E4M3, device="cuda")
+        scales = torch.empty((pages, 2, 2), dtype=torch.uint8, device="cuda")
+        cache.view(torch.uint8)[-held:] = getattr(p, name + "_cache").view(torch.uint8)
+        scales[-held:] = getattr(p, name + "_scales").view(torch.uint8)
+        setattr(p, name + "_cache", cache)
+        setattr(p, name + "_scales", scales.view(torch.float8_e8m0fnu))
+    count = R.cdiv(500, 64)
+    p.table[0, :count] += pages - held
+    p.launch()
+    p.check()
+
+
+@pytest.mark.parametrize("news", [None, [3, 2, 0]])
+def test_without_a_page(news):
+    """A cache or a table without a page: rows that would see a key are NaN and reported, the others zeros."""
+    p = Quantized([0, 5, 0], news, 4, 2, 64, BF16, 16)
+    caches = attention.make_quantized_cache(0, 16, 2, 64)
+    p.k_cache, p.v_cache, p.k_scales, p.v_scales = caches
+    p.table = torch.zeros((3, 4), dtype=torch.int32, device="cuda")
+    p.launch()
+    sees = [False, True, False] if news is None else [False] * 3 + [True] * 2
+    assert p.out.isnan().all(-1).all(-1).tolist() == sees and p.word.item() == attention.STATUS_BAD_INDEX
+    assert bool((p.out[~torch.tensor(sees, device="cuda")] == 0).all())
+
+
+@pytest.mark.parametrize("dtype,dim,news", [(BF16, 128, [300, 90]), (F16, 64, [300, 90]), (F32, 64, None), (BF16, 256, None)])
+def test_outputs_in_place_of_the_queries(dtype, dim, news):
+    p = run([400, 90], news, 8, 2, dim, dtype, 16)
+    want = p.out.clone()
+    p.out = p.q
+    p.launch()
+    assert torch.equal(p.q, want)
+
+
+def test_nothing_is_written_behind_a_workspace():
+    for news in (None, [40, 9]):
+        for behind in (1, 16 * 132 - 1, 2 * 16 * 132, 5 * 16 * 132 + 3):
+            p = Quantized([3000, 700], news, 8, 1, 128, BF16, 16)
+            room = torch.zeros(4096 + behind + 200 * 16 * 132, device="cuda")
+            room[4096 + behind:] = -7
+            for _ in range(2):
+                p.out.fill_(-7)
+                p.launch(room[:4096 + behind])
+                p.check()
+            assert bool((room[4096 + behind:] == -7).all()) and bool((room[:4096].view(torch.int32) == 0).all())
+
+
+@pytest.mark.parametrize("requests", [65, 150])
+def test_prompts_of_many_requests(requests):
+    lengths = [40 + 17 * (i % 23) for i in range(requests)]
+    run(lengths, [n - (11 * i) % 40 for i, n in enumerate(lengths)], 4, 2, 64, F16, 16)
+
+
 @pytest.mark.parametrize("code", [E4M3, E5M2])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("dim,most", [(64, 0), (128, 64), (256, 372)])

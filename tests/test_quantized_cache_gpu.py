@@ -13,7 +13,7 @@ from quantized_reference import E4M3, E5M2, LARGEST, Cache, same
 
 pytestmark = pytest.mark.gpu
 
-CODES = [E4M3, E5M2]
+CODES, E8M0 = [E4M3, E5M2], torch.float8_e8m0fnu
 
 
 class Written:
@@ -92,9 +92,38 @@ def test_blocks(page, block, dtype, dim):
     run(SPANS + [(0, 300), (70, 300), (127, 2), (255, 70)], 3, dim, dtype, E4M3, page, block, heads_first=page == 64, fused=page != 16)
 
 
-def test_many_tokens_of_many_heads():
-    """More tokens than waves: a wave looks after several."""
-    run([(7, 1)] * 700 + [(0, 901), (30, 1003)], 8, 64, BF16, E4M3, 32, 16, padding=29)
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F32, 256), (F16, 64)])
+@pytest.mark.parametrize("block", [192, 256, 512])
+def test_long_blocks(block, dtype, dim):
+    """Blocks that sixteen waves share; of 512 tokens some rows are read twice."""
+    run([(0, 1), (0, 700), (block - 3, 5), (100, block + 60), (block, 33), (block - 1, 1)], 2, dim, dtype, E5M2, block, block)
+
+
+@pytest.mark.parametrize("page,block,requests", [(32, 16, 700), (64, 64, 150), (256, 256, 40)])
+def test_many_tokens_of_many_heads(page, block, requests):
+    """More tokens than waves: a wave, or the waves that share blocks, look after several."""
+    run([(7, 1)] * requests + [(0, 901), (30, 1003), (0, 16), (0, 16), (17, 300)], 8, 64, BF16, E4M3, page, block, padding=29)
+
+
+def test_scales_as_views():
+    """Scales as every other byte of something wider, heads before blocks, whose other bytes stay."""
+    p = Written([(5, 40), (0, 17), (70, 3)], 2, 64, BF16, E4M3, 64, 16)
+    pages = p.caches["k"].shape[0]
+    wide = torch.full((2, pages, 2, 9), 77, dtype=torch.uint8, device="cuda")
+    for i, name in enumerate("kv"):
+        view = wide[i, :, :, 1::2].transpose(1, 2)
+        view.copy_(p.scales[name].view(torch.uint8))
+        p.scales[name] = view.view(E8M0)
+    want = p.want()
+    p.launch()
+    p.check(want)
+    assert bool((wide[..., ::2] == 77).all())
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    lengths, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([pages * 64], [0, pages * 64]))
+    outs, word = read((p.caches["k"], p.caches["v"], p.scales["k"], p.scales["v"]), table, lengths, starts, pages * 64, 2, 64, BF16)
+    assert word.item() == 0
+    for got, name in zip(outs, "kv"):
+        assert torch.equal(got.cpu(), Cache(p.caches[name], p.scales[name], 16, E4M3).elements().to(BF16))
 
 
 def test_padded_tokens_and_slots_outside():
