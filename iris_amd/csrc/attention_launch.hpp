@@ -115,7 +115,9 @@ hipError_t make_plan(const iris_attention_args& a, int cus, Plan* p) {
     // of 16, bf16, 8 + 1 heads of 128 unless stated.  By rows a request: 64 requests behind up to 4096 tokens, 19 rows each
     // 41 / 37, 27 each 41 / 46, 42 each 42 / 49.  By 16-row units and the most keys a row may see: 102 x 200 11.3 / 7.7,
     // 93 x 2004 20.5 / 17.2, 201 x 400 16.4 / 10.9, 460 x 500 17.1 / 13.4, 57 x 8001 31 / 26; 501 x 1000 20.2 / 20.5,
-    // 188 x 4113 29 / 39, 268 x 2001 (4 + 4 heads) 27 / 37, 55 x 46398 79 / 86; 537 x 180 12.6 / 14.1.
+    // 188 x 4113 29 / 39, 268 x 2001 (4 + 4 heads) 27 / 37, 55 x 46398 79 / 86; 537 x 180 12.6 / 14.1.  Over a cache in 8 bits the line
+    // lies there too: 64 requests behind up to 4096, up to 6 tokens each 37 / 31, 10 each 38 / 39, 16 each 40 / 41; one prompt of 300 tokens
+    // 14.4 / 9.5, 700 20.4 / 14.8, 1000 21.2 / 19.3; 8 of up to 60 behind 4000 25.3 / 18.1, 4 of up to 300 behind 2000 22.8 / 29.8.
     const bool few_rows = (int64_t)a.tokens * group <= 24 * (int64_t)a.requests ||
                           (few_units <= 2 * cus && few_units * most_keys <= (int64_t)1536 * cus);
     const int64_t row_tiles = (int64_t)a.tokens * group / tiles::ROWS + a.requests;

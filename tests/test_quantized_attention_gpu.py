@@ -334,6 +334,66 @@ def test_nothing_is_written_behind_a_workspace():
             assert bool((room[4096 + behind:] == -7).all()) and bool((room[:4096].view(torch.int32) == 0).all())
 
 
+@pytest.mark.parametrize("news,hq,hk,kernel", [([400, 130], 8, 1, _native.ATTENTION_PROMPT_TILES), ([9, 3], 8, 1, _native.ATTENTION_PROMPT_ROWS)])
+def test_prompts_in_a_captured_graph(news, hq, hk, kernel):
+    """Parts that join, replayed over other numbers and shorter contexts with eager work in between; rows past the last request's stay."""
+    p = Quantized([1500, 900], news, hq, hk, 128, BF16, 16)
+    tokens = sum(news)
+    q = torch.zeros((tokens + 7, hq, 128), dtype=BF16, device="cuda")
+    out = torch.full_like(q, -7.0)
+    q[:tokens] = p.q
+    p.q, p.out, p.lse = q, out, torch.full((tokens + 7, hq), -7.0, device="cuda")
+    if kernel == _native.ATTENTION_PROMPT_TILES:  # (a table this wide has many keys to see)
+        p.table = torch.cat((p.table, torch.full((2, 400), 1 << 30, dtype=torch.int32, device="cuda")), 1)
+    workspace = attention.make_workspace(128)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        p.launch(workspace)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            p.launch(workspace)
+    torch.cuda.current_stream().wait_stream(stream)
+    for shorter in (0, 100, 0, 333, 700):
+        p.lens.copy_(torch.tensor([1500 - shorter, 900 - shorter // 2], device="cuda"))
+        p.q[:tokens] = torch.randn_like(p.q[:tokens]) * 1.5
+        p.out.fill_(-7)
+        graph.replay()
+        got = p.out.clone()
+        p.out.fill_(-7)
+        p.launch(workspace)  # eager, the same
+        assert torch.equal(got, p.out) and p.word.item() == 0
+        assert bool((got[tokens:] == -7).all()) and bool((p.lse[tokens:] == -7).all())
+        at = 0
+        for i, (n, new) in enumerate(zip(p.lens.tolist(), news)):
+            rows = slice(at, at + 2), slice(at + new - 2, at + new)
+            for r, first in zip(rows, (n - new, n - 2)):
+                want, _, spread = R.attention(p.q[r], p.k[i][:n], p.v[i][:n], first, 128 ** -0.5)
+                assert bool(((got[r].double().cpu() - want).abs() <= R.attention_error(BF16, want, spread, 128)).all())
+            at += new
+
+
+def test_calls_on_two_streams_at_once():
+    """Single tokens, prompts and reads over one cache from two streams, each with its own workspace, while a third call writes another cache."""
+    p, q = Quantized([5000, 700, 3001], None, 8, 2, 128, BF16, 16), Quantized([900, 1200], [900, 300], 8, 2, 128, BF16, 16, seed=3)
+    spare = attention.make_quantized_cache(64, 16, 2, 128)
+    k = torch.randn((1000, 2, 128), device="cuda", dtype=BF16)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [attention.make_workspace(128) for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            p.launch(spaces[0])
+            attention.write_quantized_cache(k, k, *spare, torch.arange(1000, device="cuda"))
+        with torch.cuda.stream(streams[1]):
+            q.launch(spaces[1])
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    p.check()
+    q.check()
+
+
 @pytest.mark.parametrize("requests", [65, 150])
 def test_prompts_of_many_requests(requests):
     lengths = [40 + 17 * (i % 23) for i in range(requests)]
