@@ -418,9 +418,9 @@ extern "C" int iris_write_quantized_cache_launch(const iris_write_cache_args* ar
   g.page = make_page_div((uint32_t)a.page_size);
   g.block = make_page_div((uint32_t)a.block);
   // A wave takes a short block alone, four share one of up to 128 tokens, sixteen a longer one.  (us with one / four, bf16: 32 tokens of 64
-  // elements 7.0 / 10.0, of 128 10.1 / 10.9; with four / sixteen: 64 tokens of 128 9.7 / 35, 128 10.4 / 25, 256 of 256 34 / 31, fp32 50 / 26.)
-  const int64_t bytes = (int64_t)a.block * (a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256) * dtype_size(a.dtype);
-  const int wide = a.block <= 32 && bytes <= NARROW ? 1 : a.block <= 128 ? 4 : 16;
+  // elements 7.0 / 10.0, of 128 10.1 / 10.9; with four / sixteen: 64 tokens of 128 9.7 / 35, 128 10.4 / 25, 256 of 256 34 / 21, fp32 50 / 20.)
+  const int64_t row = (a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256) * dtype_size(a.dtype);  // as lanes hold it
+  const int wide = a.block <= 32 && a.block * row <= NARROW ? 1 : a.block <= 128 ? 4 : 16;
   // Units without a block cost their start, those with several take them one after another.  (us with 8192 / 2048 / 1024 units at most: prompts of
   // up to 8192 tokens, one head, 5.8 / 4.7 / 5.4; 500 tokens in blocks of 64 5.4 / 3.4 / 3.1; 256 single tokens of 8 heads 3.9 / 4.0 / 4.8.)
   g.span = 1;
@@ -431,10 +431,13 @@ extern "C" int iris_write_quantized_cache_launch(const iris_write_cache_args* ar
   if (groups > INT32_MAX) return hipErrorInvalidValue;
   return with_types(a, [&](auto dt, auto ct, auto lanes) {
     constexpr int DT = dt.value, CT = ct.value, LANES = lanes.value;
-    const auto kernel = wide == 1    ? (a.block <= 16 ? write_kernel<DT, CT, LANES, 1, 16, false> : write_kernel<DT, CT, LANES, 1, 32, false>)
-                        : wide == 4  ? (a.block <= 64 ? write_kernel<DT, CT, LANES, 4, 16, false> : write_kernel<DT, CT, LANES, 4, 32, false>)
-                        : a.block <= 256 ? write_kernel<DT, CT, LANES, 16, 16, false>
-                                         : write_kernel<DT, CT, LANES, 16, 8, true>;
+    void (*kernel)(WriteKArgs) = nullptr;
+    if constexpr (16 * LANES * 16 <= NARROW)
+      if (wide == 1) kernel = write_kernel<DT, CT, LANES, 1, 16, false>;
+    if constexpr (32 * LANES * 16 <= NARROW)
+      if (wide == 1 && a.block == 32) kernel = write_kernel<DT, CT, LANES, 1, 32, false>;
+    if (wide == 4) kernel = a.block <= 64 ? write_kernel<DT, CT, LANES, 4, 16, false> : write_kernel<DT, CT, LANES, 4, 32, false>;
+    if (wide == 16) kernel = a.block <= 256 ? write_kernel<DT, CT, LANES, 16, 16, false> : write_kernel<DT, CT, LANES, 16, 8, true>;
     return launch(kernel, dim3((unsigned)groups), wide > 1 ? wide * 64 : THREADS, 0, stream, g);
   });
 }
