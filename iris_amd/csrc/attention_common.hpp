@@ -26,6 +26,7 @@ struct QuantizedKArgs : AttentionKArgs {
   uint32_t k_page16, v_page16;  // of pages of codes, in 16 bytes
   uint32_t ks_page, vs_page, ks_block, vs_block;
   uint32_t block16;             // (block_of)
+  int dealt;                    // row tiles in the order of dealt() (prompts in tiles)
 };
 // Where sixteen keys of a cache in 8 bits lie, `at` places into a page.
 struct CodesAt {
@@ -42,6 +43,20 @@ __device__ inline CodesAt codes_at(const QuantizedKArgs& g, int page, int at) {
 }
 template <int CT>
 using KArgs = std::conditional_t<CT == 0, AttentionKArgs, QuantizedKArgs>;
+
+// A permutation of n items: 256 of them (and what is left, by powers of two) with their numbers' bits reversed.  Row tiles have room for each
+// request's without a sum over the requests, which leaves every so many-th of them empty, every other one where requests have one each;
+// and XCDs, and engines within them, get workgroups in turn, so that in the items' own order some of them would get all the empty ones.
+// (512 requests with 128 rows each behind 8192 keys, heads of 128: 558 us, dealt 363; behind 2048 158 and 93.)
+__device__ inline int dealt(int b, int n) {
+  int first = b & ~255, left = min(n - first, 256), bits = 31 - __builtin_clz(left);
+  while (b - first >= 1 << bits) {
+    first += 1 << bits;
+    left -= 1 << bits;
+    bits = 31 - __builtin_clz(left);
+  }
+  return bits ? first + (int)(__brev((uint32_t)(b - first)) >> (32 - bits)) : b;
+}
 
 // The keys that the queries at positions first .. last see, as tiles of BT keys: `front` tiles that hold the first tokens (sinks),
 // then tiles from `start` on; `count` in all.

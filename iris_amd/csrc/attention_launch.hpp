@@ -78,6 +78,7 @@ struct Plan {
   int64_t workgroups = 0;
   int64_t splits = 1;   // parts of a unit's keys (prompts)
   int by_length = 0;    // (AttentionKArgs)
+  int dealt = 0;        // (QuantizedKArgs)
   int64_t parted = 0;   // floats behind the workspace's counters that parts are left in; 0: no unit is split
 };
 
@@ -140,6 +141,8 @@ hipError_t make_plan(const iris_attention_args& a, int cus, Plan* p) {
       // Which starts first matters where places are taken twice: a CU's, or with a window (whose rows are nearly alike) all of them.  (us in the
       // requests' order / by length: window of 1024, 642 row tiles on 768 places 44.4 / 46.3; no window, 381 on 512 99.7 / 97.)
       if (p->splits == 1 && a.requests <= 64 && units > (a.window > 0 ? places : cus)) p->by_length = cus > a.k_heads ? cus / a.k_heads : 1;
+      // Where row tiles fill the places, how the empty ones among them are spread matters; where they do not, as they are is up to 3 us less.
+      p->dealt = p->splits == 1 && !p->by_length && units >= places;
       p->workgroups = units * p->splits;
       if (p->splits > 1) p->parted = units * p->splits * SLOT;
       return hipSuccess;
@@ -197,6 +200,7 @@ int launch_call(const iris_attention_args& a, const iris_cache_scales* s, void* 
     if (refused != hipSuccess) return refused;
     g.splits = (int)p.splits;
     g.by_length = p.by_length;
+    if constexpr (CT != 0) g.dealt = p.dealt;
     g.grid_units = (int)p.workgroups;
     if (p.parted) {
       g.counters = (int32_t*)a.workspace;

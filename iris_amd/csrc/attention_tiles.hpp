@@ -171,7 +171,11 @@ __global__ __launch_bounds__(WAVES * 64, waves_a_simd(DP)) __attribute__((amdgpu
   const int n = lane & 31, half = lane >> 5;
 
   // The workgroup's rows, and its share of their keys.  Key heads change fastest: with eight of them each XCD has one.
-  const int item = blockIdx.x / a.k_heads, head = blockIdx.x - item * a.k_heads, x = item / g.splits, split = item - x * g.splits;
+  const int place = blockIdx.x / a.k_heads, head = blockIdx.x - place * a.k_heads;
+  int item = place;
+  if constexpr (CT != 0)
+    if (g.dealt) item = dealt(place, gridDim.x / a.k_heads);
+  const int x = item / g.splits, split = item - x * g.splits;
   int request, row_tile;
   if (g.by_length) {
     // Of those that take one place a CU every other batch is turned round: beside the longest runs the shortest of the next.  (One prompt

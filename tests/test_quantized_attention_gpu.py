@@ -394,6 +394,13 @@ def test_calls_on_two_streams_at_once():
     q.check()
 
 
+@pytest.mark.parametrize("requests,new,hq,hk", [(140, 32, 8, 2), (270, 16, 8, 1)])
+def test_prompts_of_one_row_tile_each(requests, new, hq, hk):
+    """As many row tiles as places, every other one empty: they are dealt out in another order."""
+    lengths = [new + (7 * i) % 53 for i in range(requests)]
+    run(lengths, [new] * (requests - 1) + [new - 3], hq, hk, 64, BF16, 16)
+
+
 @pytest.mark.parametrize("requests", [65, 150])
 def test_prompts_of_many_requests(requests):
     lengths = [40 + 17 * (i % 23) for i in range(requests)]
