@@ -78,10 +78,10 @@ int iris_hip_arch_name(int device, char* buf, size_t len);
 #define IRIS_DTYPE_I8 3
 #define IRIS_DTYPE_I16 4
 #define IRIS_DTYPE_I32 5
-/* 8-bit floats, the codes of a quantised cache: 4 bits of exponent and 3 of fraction (no infinity), 5 and 2 */
-#define IRIS_DTYPE_E4M3 6
-#define IRIS_DTYPE_E5M2 7
 #define IRIS_DTYPE_I64 6
+/* 8-bit floats, the codes of a quantised cache: 4 bits of exponent and 3 of fraction (no infinity), 5 and 2 */
+#define IRIS_DTYPE_E4M3 7
+#define IRIS_DTYPE_E5M2 8
 
 /* epilogues of the persistent shard GEMM */
 #define IRIS_EPI_ALL_SCATTER 0 /* examples/07_gemm_all_scatter/gemm_all_scatter.py:209-251 */

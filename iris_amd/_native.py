@@ -19,7 +19,7 @@ TESTING_LIB_PATH = os.path.join(_PKG_DIR, "libiris_amd_testing.so")
 
 # element types (IRIS_DTYPE_*)
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
-DTYPE_E4M3, DTYPE_E5M2 = 6, 7  # codes of a quantised cache
+DTYPE_E4M3, DTYPE_E5M2 = 7, 8  # codes of a quantised cache
 # epilogues (IRIS_EPI_*)
 EPI_ALL_SCATTER, EPI_ATOMIC_ADD, EPI_ONE_SHOT = 0, 1, 2
 # ONE_SHOT phases (IRIS_PHASE_*)
