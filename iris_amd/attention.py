@@ -772,10 +772,11 @@ def write_quantized_cache(k, v, k_cache, v_cache, k_scales, v_scales, slots, *, 
 
     ``k`` and ``v`` [tokens, key heads, head size] (fp16, bf16 or fp32; views of a fused projection's output will do) go to
     ``slots`` int64 [tokens], as ``build_block_tables`` makes them: a negative slot is skipped, and the new tokens of a block are neighbours, at
-    slots in a row.  (A token that follows one of its own block at any other slot is skipped and sets ``STATUS_BAD_INDEX``, as a slot outside of
-    the cache does; no block may be come back to further on in the same call.)
+    slots in a row.  (A token that follows one of its own block at any other slot sets ``STATUS_BAD_INDEX``, as a slot outside of the cache does, and
+    is skipped with all tokens of that block that follow it: of slots 0, 1, 5, 6, 7 the first two are written.  No block may be come back
+    to further on in the same call.)
 
-    A block's rows before its first new one are its earlier tokens, and rows behind the last new one count as empty.  Its scale (for
+    A block's rows before its first new one are its earlier tokens, and rows behind the last one that is written count as empty.  Its scale (for
     each head, keys and values apart) becomes the smallest power of two, 2^-100 at least, by which the largest of the new elements does not
     exceed the largest code (448 or 57344); a larger one that earlier tokens have stays.  Where it grows, the earlier tokens' codes are
     rounded to it.  Roundings are to nearest, ties to even.  Elements that are not finite become NaN and have no part in a scale.
