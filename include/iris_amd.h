@@ -585,8 +585,9 @@ int iris_quantized_attention_kernel_info(const iris_attention_args* args, const 
 /*
  * Keys and values of new tokens into such a cache.  Token t goes to slots[t] (a negative slot is skipped; one past num_slots is
  * reported and skipped).  The new tokens of a block are neighbours in k and v with slots in a row; one that follows a token of
- * its own block at any other slot is reported, and it and the tokens of that block that follow it are skipped, at whatever slots (of
- * slots 0 1 5 6 7 the first two are written).  No block may come up again further on.  Rows of a block before its first new one are earlier
+ * its own block in any other way, at another slot or with skipped tokens between them, is reported, and it and the tokens of that block that
+ * follow it are skipped (of slots 0 1 5 6 7, and of 0 1 -1 2 3, the first two are written).  No block may come up again behind tokens of
+ * others: that is not seen, and leaves that block with numbers of no meaning.  Rows of a block before its first new one are earlier
  * tokens and stay, rows behind the last new one that is written are left as they are and count as empty.
  * A block's scale becomes the smallest power of two, 2^-100 at least, by which the largest finite new element does not exceed the largest code
  * (448 or 57344), or stays as it is where earlier tokens have a larger one; earlier tokens' codes are rounded to a scale

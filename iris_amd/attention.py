@@ -772,9 +772,10 @@ def write_quantized_cache(k, v, k_cache, v_cache, k_scales, v_scales, slots, *, 
 
     ``k`` and ``v`` [tokens, key heads, head size] (fp16, bf16 or fp32; views of a fused projection's output will do) go to
     ``slots`` int64 [tokens], as ``build_block_tables`` makes them: a negative slot is skipped, and the new tokens of a block are neighbours, at
-    slots in a row.  (A token that follows one of its own block at any other slot sets ``STATUS_BAD_INDEX``, as a slot outside of the cache does, and
-    is skipped with all tokens of that block that follow it: of slots 0, 1, 5, 6, 7 the first two are written.  No block may be come back
-    to further on in the same call.)
+    slots in a row.  (A token that follows one of its own block in any other way, at another slot or with skipped tokens between them, sets
+    ``STATUS_BAD_INDEX``, as a slot outside of the cache does, and is skipped with all tokens of that block that follow it: of slots 0, 1, 5, 6, 7, and
+    of 0, 1, -1, 2, 3, the first two are written.  No block may be come back to behind tokens of others in the same call: that is not
+    seen, and leaves the block with numbers of no meaning.)
 
     A block's rows before its first new one are its earlier tokens, and rows behind the last one that is written count as empty.  Its scale (for
     each head, keys and values apart) becomes the smallest power of two, 2^-100 at least, by which the largest of the new elements does not

@@ -4,8 +4,8 @@
 // finite new elements, or keeps a larger one that its earlier tokens have; codes are x / s to nearest.  Earlier tokens' codes are rounded again
 // only where the scale grew, by a power of two, which moves their exponents and costs places only where they become subnormal.
 // One pass over the data: one wave (blocks of more than 16 tokens: four) takes one block of one head, of K or of V, 16 bytes a lane, and holds it
-// in registers until the maximum is known.  Blocks are found from the slots alone: a token begins one where the token
-// before it has no slot there.  bf16, 8 heads of 128, four prompts of up to 4096 tokens (50 MB) in 10.6 us, 4.7 TB/s, where a copy of 4 GB runs
+// in registers until the maximum is known.  Blocks are found from the slots alone: a token begins one where the last
+// token before it that has a slot has none there.  bf16, 8 heads of 128, four prompts of up to 4096 tokens (50 MB) in 10.6 us, 4.7 TB/s, where a copy of 4 GB runs
 // at 4.9; 64 single tokens of one head in 2.9 us, a chain of slots, heads and scales, and stores.
 //
 // Reading.  A wave takes rows of one head of K or V, 16 bytes of them a lane; requests are found by bisection of their starts.  16 contexts of
@@ -22,6 +22,7 @@ constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int MAX_DIM = 256;
 constexpr int NARROW = 8192;      // bytes of a block that a wave takes alone
 constexpr int MOST_UNITS = 2048;  // waves that look for blocks, at most where that leaves them 32 tokens each
+constexpr int FAR = 512;          // tokens in front of a wave's own, but for the last 64, that are looked at at once for one with a slot
 
 // ---- writing -------------------------------------------------------------------
 
@@ -130,10 +131,39 @@ __global__ __launch_bounds__(WIDE > 1 ? WIDE * 64 : THREADS) void write_kernel(W
     slot = slots[first + lane];
     if (first + lane > 0) before = slots[first + lane - 1];
   }
-  const bool inside = slot >= 0 && slot < a.num_slots;
-  const bool goes_on = inside && before >= 0 && before < a.num_slots && page_div((uint32_t)before, g.block) == page_div((uint32_t)slot, g.block);
-  if (lane < g.span && (slot >= a.num_slots || (goes_on && slot != before + 1))) report(a.status, IRIS_STATUS_BAD_INDEX);
-  const uint64_t in_a_row = __ballot(goes_on && slot == before + 1);
+  auto have = [&](int64_t s) { return s >= 0 && s < a.num_slots; };
+  const bool inside = have(slot), beside = have(before);
+  // The last slot in front of a token: its neighbour's, or where that one is skipped another's, for the block may have begun there, and two
+  // waves that both took it to begin with them would race on its scale and its older codes.  (us with / without: 64 single tokens, every
+  // other one padding, 3.0 / 2.7; prompts of up to 4096, each padded to the longest, 27.9 / 22.8; without padding the same.)
+  int last = beside ? (int)before : -1;
+  if (__any(inside && !beside && lane < g.span)) {
+    const uint64_t held = __ballot(inside);
+    int in_front = -1;  // of the chunk
+    if (__builtin_amdgcn_readlane((int)!beside, __builtin_ctzll(held))) {
+      // (the nearest first; padding in front of a chunk may be long)
+      const int64_t close = first > lane ? slots[first - 1 - lane] : -1;
+      const uint64_t near = __ballot(have(close));
+      if (near) in_front = __builtin_amdgcn_readlane((int)close, __builtin_ctzll(near));
+      for (int64_t at = first - 64; in_front < 0 && at > 0; at -= FAR) {
+        int64_t far[FAR / 64];
+#pragma unroll
+        for (int i = 0; i < FAR / 64; ++i) far[i] = at > i * 64 + lane ? slots[at - 1 - i * 64 - lane] : -1;
+#pragma unroll
+        for (int i = 0; i < FAR / 64; ++i) {
+          const uint64_t any = __ballot(have(far[i]));
+          if (in_front < 0 && any) in_front = __builtin_amdgcn_readlane((int)far[i], __builtin_ctzll(any));
+        }
+      }
+    }
+    const uint64_t below = held & ((1ull << lane) - 1);
+    const int nearest = __shfl((int)slot, below ? 63 - __builtin_clzll(below) : 0);
+    if (!beside) last = below ? nearest : in_front;
+  }
+  const bool goes_on = inside && last >= 0 && page_div((uint32_t)last, g.block) == page_div((uint32_t)slot, g.block);
+  const bool in_order = goes_on && beside && slot == before + 1;
+  if (lane < g.span && (slot >= a.num_slots || (goes_on && !in_order))) report(a.status, IRIS_STATUS_BAD_INDEX);
+  const uint64_t in_a_row = __ballot(in_order);
   int parity = 0;
   for (uint64_t begins = __ballot(inside && !goes_on && lane < g.span); begins; begins &= begins - 1) {
     const int at = __builtin_ctzll(begins);

@@ -62,3 +62,44 @@ def test_the_rest_of_a_block_is_skipped_behind_a_slot_that_is_not_the_next(slots
 def test_the_same_in_blocks_that_waves_share(block):
     slots = [*range(40, 60), 61, 62, 63, *range(block, block + 20), block + 19, *range(block + 20, block + 30)]
     Slots(slots, page=block, block=block, pages=3).check([*range(20), *range(23, 43)], attention.STATUS_BAD_INDEX)
+
+
+@pytest.mark.parametrize("dtype,dim,code", TYPES)
+@pytest.mark.parametrize("slots,written", [
+    ([0, 1, -1, 2, 3], [0, 1]),                              # padding inside a block
+    ([5, -1, 7], [0]),
+    ([-1, 5, -1, 5, -1, 16], [1, 5]),
+    ([0, 1, 1 << 40, 2, 3, 20, -7, 21], [0, 1, 5]),          # what lies outside of the cache is skipped, too
+    ([3, 256, 4], [0]),
+    ([3, 5, -1, 6, -1, -1, 7, 33, -1, 48], [0, 7, 9]),       # behind a token that is skipped itself
+])
+def test_no_block_goes_on_behind_skipped_tokens(slots, written, dtype, dim, code):
+    Slots(slots, dtype=dtype, dim=dim, code=code).check(written, attention.STATUS_BAD_INDEX)
+
+
+@pytest.mark.parametrize("dtype,dim,code", TYPES)
+def test_padding_between_blocks_is_no_mistake(dtype, dim, code):
+    slots = [14, 15, -1, -1, 16, 17, -1, 32, -1, 67, 68, -1]
+    Slots(slots, dtype=dtype, dim=dim, code=code).check([i for i, s in enumerate(slots) if s >= 0], 0)
+
+
+@pytest.mark.parametrize("page,block", [(16, 16), (64, 64), (256, 256), (512, 512)])
+@pytest.mark.parametrize("gap", [1, 30, 31, 32, 33, 62, 63, 64, 65, 127, 128, 129, 700, 1086, 1087, 1088, 1089, 2112, 5000])
+def test_skipped_tokens_of_any_number_between_two_of_a_block(gap, page, block):
+    """At every place of the waves' chunks, and before other blocks, which are written."""
+    for ahead in (0, 3, 29, 64):
+        front = [block * 20 + i for i in range(min(ahead, block))]  # another block's tokens
+        slots = [*front, 2, 3, *[SKIPPED] * gap, 4, 5, block, block + 1, *[SKIPPED] * gap, 2 * block + 9]
+        n = len(front)
+        Slots(slots, page=page, block=block, pages=24, heads=1).check([*range(n + 2), n + gap + 4, n + gap + 5, len(slots) - 1], attention.STATUS_BAD_INDEX)
+
+
+@pytest.mark.parametrize("page,block", [(16, 16), (64, 64), (256, 256)])
+def test_a_padded_batch(page, block):
+    """Every request padded to the longest: many begin far behind the last slot."""
+    longest, lengths = 2500, [3, 2500, 1, 17, 900]
+    slots = []
+    for i, n in enumerate(lengths):
+        start = i * 2560 + (7 if n < 20 else 0)
+        slots += [*range(start, start + n), *[SKIPPED] * (longest - n)]
+    Slots(slots, page=page, block=block, pages=5 * 2560 // page, heads=1).check([i for i, s in enumerate(slots) if s >= 0], 0)
