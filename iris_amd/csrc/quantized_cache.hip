@@ -320,7 +320,7 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadKArgs g) {
   // the last request that does not start behind the wave's first row, and from there for each row
   int lo = 0;
   for (int hi = a.requests; hi - lo > 1;) {
-    const int mid = (lo + hi) / 2;
+    const int mid = lo + (hi - lo) / 2;
     if (start(mid) <= first)
       lo = mid;
     else
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadKArgs g) {
     if (token >= ends && lo + 1 < a.requests) {
       // (of a wave's rows in a middle request; bisection again, for there may be many that have none)
       for (int hi = a.requests; hi - lo > 1;) {
-        const int mid = (lo + hi) / 2;
+        const int mid = lo + (hi - lo) / 2;
         if (start(mid) <= token)
           lo = mid;
         else

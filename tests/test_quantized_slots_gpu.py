@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from iris_amd import attention
-from quantized_reference import E4M3, E5M2
+from quantized_reference import E4M3, E5M2, Cache
 
 pytestmark = pytest.mark.gpu
 
@@ -103,3 +103,25 @@ def test_a_padded_batch(page, block):
         start = i * 2560 + (7 if n < 20 else 0)
         slots += [*range(start, start + n), *[SKIPPED] * (longest - n)]
     Slots(slots, page=page, block=block, pages=5 * 2560 // page, heads=1).check([i for i, s in enumerate(slots) if s >= 0], 0)
+
+
+def test_reading_more_requests_than_half_of_what_31_bits_count():
+    """Most of them without a token."""
+    requests, page, some = (1 << 30) + 9, 16, 7
+    caches = attention.make_quantized_cache(some, page, 1, 64)
+    x = torch.randn((some * page, 1, 64), device="cuda", dtype=BF16)
+    attention.write_quantized_cache(x, x, *caches, torch.arange(some * page, device="cuda"))
+    table, lengths = (torch.zeros((requests, 1) if wide else requests, dtype=torch.int32, device="cuda") for wide in (True, False))
+    starts = torch.zeros(requests + 1, dtype=torch.int32, device="cuda")
+    news = torch.tensor([1, 16, 0, 3, 9, 16, 2], dtype=torch.int32, device="cuda")
+    table[-some:, 0] = torch.arange(some, dtype=torch.int32, device="cuda").flip(0)
+    lengths[-some:] = news
+    starts[-some:] = news.cumsum(0).int()
+    tokens = int(news.sum())
+    outs, word = [torch.zeros((tokens, 1, 64), dtype=F32, device="cuda") for _ in range(2)], torch.zeros(1, dtype=torch.int32, device="cuda")
+    attention.read_quantized_cache(*caches, table, lengths, starts, *outs, status=word)
+    assert word.item() == 0
+    numbers = Cache(caches[0], caches[2], page, E4M3).elements().float().unflatten(0, (some, page)).flip(0)
+    want = torch.cat([numbers[i, :n] for i, n in enumerate(news.tolist())])
+    for got in outs:
+        assert torch.equal(got.cpu(), want)
