@@ -265,6 +265,8 @@ SIGNATURES = {
     "iris_quantized_attention_launch": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), _P]),
     "iris_quantized_attention_plan": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), ctypes.c_int32,
                                            ctypes.POINTER(AttentionPlanInfo)]),
+    "iris_quantized_attention_item": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), ctypes.c_int32, ctypes.c_int64,
+                                           ctypes.POINTER(ctypes.c_int64)]),
     "iris_quantized_attention_kernel_info": (_I, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(CacheScales), ctypes.POINTER(ctypes.c_int),
                                                   ctypes.POINTER(ctypes.c_int)]),
     "iris_write_quantized_cache_launch": (_I, [ctypes.POINTER(WriteCacheArgs), _P]),

@@ -48,14 +48,14 @@ using KArgs = std::conditional_t<CT == 0, AttentionKArgs, QuantizedKArgs>;
 // request's without a sum over the requests, which leaves every so many-th of them empty, every other one where requests have one each;
 // and XCDs, and engines within them, get workgroups in turn, so that in the items' own order some of them would get all the empty ones.
 // (512 requests with 128 rows each behind 8192 keys, heads of 128: 558 us, dealt 363; behind 2048 158 and 93.)
-__device__ inline int dealt(int b, int n) {
-  int first = b & ~255, left = min(n - first, 256), bits = 31 - __builtin_clz(left);
+__host__ __device__ inline int dealt(int b, int n) {
+  int first = b & ~255, left = n - first < 256 ? n - first : 256, bits = 31 - __builtin_clz(left);
   while (b - first >= 1 << bits) {
     first += 1 << bits;
     left -= 1 << bits;
     bits = 31 - __builtin_clz(left);
   }
-  return bits ? first + (int)(__brev((uint32_t)(b - first)) >> (32 - bits)) : b;
+  return bits ? first + (int)(__builtin_bitreverse32((uint32_t)(b - first)) >> (32 - bits)) : b;
 }
 
 // The keys that the queries at positions first .. last see, as tiles of BT keys: `front` tiles that hold the first tokens (sinks),

@@ -46,6 +46,10 @@ extern "C" int iris_quantized_attention_plan(const iris_attention_args* args, co
   if (!args || !plan || num_cus < 0) return hipErrorInvalidValue;
   return with_codes(scales, [&](auto ct) { return plan_call<ct.value>(*args, scales, num_cus, plan); });
 }
+extern "C" int iris_quantized_attention_item(const iris_attention_args* args, const iris_cache_scales* scales, int32_t num_cus, int64_t place, int64_t* item) {
+  if (!args || !item || num_cus < 0) return hipErrorInvalidValue;
+  return with_codes(scales, [&](auto ct) { return item_call<ct.value>(*args, scales, num_cus, place, item); });
+}
 extern "C" int iris_quantized_attention_kernel_info(const iris_attention_args* args, const iris_cache_scales* scales, int* n_regs, int* n_spills) {
   if (!args || !n_regs || !n_spills) return hipErrorInvalidValue;
   return with_codes(scales, [&](auto ct) { return info_call<ct.value>(*args, scales, n_regs, n_spills); });

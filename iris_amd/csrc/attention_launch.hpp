@@ -226,6 +226,23 @@ int plan_call(const iris_attention_args& a, const iris_cache_scales* s, int32_t 
   });
 }
 
+// The work that the workgroups at a place take, by its number in its own order (kernels that take it by lengths: as if they did not).
+template <int CT>
+int item_call(const iris_attention_args& a, const iris_cache_scales* s, int32_t num_cus, int64_t place, int64_t* item) {
+  const hipError_t bad = check<CT>(a, s);
+  if (bad != hipSuccess) return bad;
+  if (a.tokens == 0 || a.q_heads == 0) return hipErrorInvalidValue;
+  return with_types<CT>(a, [&](auto dt, auto dp, auto pg) {
+    Plan p;
+    const hipError_t refused = make_plan<dt.value, dp.value, pg.value, CT>(a, num_cus ? num_cus : current_cu_count(), &p);
+    if (refused != hipSuccess) return refused;
+    const int64_t places = p.kernel == IRIS_ATTENTION_DECODE ? p.workgroups : p.workgroups / a.k_heads;
+    if (place < 0 || place >= places) return hipErrorInvalidValue;
+    *item = CT != 0 && p.dealt ? dealt((int)place, (int)places) : place;
+    return hipSuccess;
+  });
+}
+
 template <int CT>
 int info_call(const iris_attention_args& a, const iris_cache_scales* s, int* n_regs, int* n_spills) {
   const hipError_t bad = check<CT>(a, s);
@@ -248,6 +265,7 @@ int info_call(const iris_attention_args& a, const iris_cache_scales* s, int* n_r
 #define IRIS_ATTENTION_CALLS(extern_, CT)                                                                                                \
   extern_ template int launch_call<CT>(const iris_attention_args&, const iris_cache_scales*, void*);                                     \
   extern_ template int plan_call<CT>(const iris_attention_args&, const iris_cache_scales*, int32_t, iris_attention_plan_info*);          \
+  extern_ template int item_call<CT>(const iris_attention_args&, const iris_cache_scales*, int32_t, int64_t, int64_t*);                  \
   extern_ template int info_call<CT>(const iris_attention_args&, const iris_cache_scales*, int*, int*);
 
 }  // namespace calls
