@@ -5,11 +5,13 @@
 // only where the scale grew, by a power of two, which moves their exponents and costs places only where they become subnormal.
 // One pass over the data: one wave (blocks of more than 16 tokens: four) takes one block of one head, of K or of V, 16 bytes a lane, and holds it
 // in registers until the maximum is known.  Blocks are found from the slots alone: a token begins one where the last
-// token before it that has a slot has none there.  bf16, 8 heads of 128, four prompts of up to 4096 tokens (50 MB) in 10.6 us, 4.7 TB/s, where a copy of 4 GB runs
-// at 4.9; 64 single tokens of one head in 2.9 us, a chain of slots, heads and scales, and stores.
+// token before it that has a slot has none there.  bf16, 8 heads of 128, four prompts of up to 4096 tokens (50 MB): 12 us from cold caches, 18 behind 512 MB of
+// dirty lines, 10.6 where the last-level cache holds some of it (four sets of operands in turn); a copy of 4 GiB takes 10.8 for as many bytes, at 4.58
+// TB/s on the same card.  64 single tokens of one head in 2.9 us, a chain of slots, heads and scales, and stores.
 //
 // Reading.  A wave takes rows of one head of K or V, 16 bytes of them a lane; requests are found by bisection of their starts.  16 contexts of
-// up to 16384 tokens, 2 heads of 128 (160 MB), in 27.4 us; one of 1999 in 3.5.
+// up to 16384 tokens, 2 heads of 128 (160 MB, of which 53 are codes): 36 us from cold caches, 45 behind dirty lines, 27.4 where the codes are in the
+// last-level cache; one of 1999 in 3.5.
 #include <initializer_list>
 #include <type_traits>
 
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(THREADS) void read_kernel(ReadKArgs g) {
     }
     const u32x4 y = codes[i].template decode<CT>(scale_of((int)byte[i]));
     IRIS_GLOBAL u32x4* const to = (IRIS_GLOBAL u32x4*)(out + (first + i * PASS + row) * out_row);
-    // (many rows pass the caches by: 160 MB, a third of them codes, 27.4 us for 39.8)
+    // (many rows pass the caches by, so that these keep codes from pass to pass: 160 MB, a third of them codes, 27.4 us for 39.8)
     if constexpr (PASSES > 2)
       __builtin_nontemporal_store(y, to);
     else
@@ -452,7 +454,9 @@ extern "C" int iris_write_quantized_cache_launch(const iris_write_cache_args* ar
   const int64_t row = (a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256) * dtype_size(a.dtype);  // as lanes hold it
   const int wide = a.block <= 32 && a.block * row <= NARROW ? 1 : a.block <= 128 ? 4 : 16;
   // Units without a block cost their start, those with several take them one after another.  (us with 8192 / 2048 / 1024 units at most: prompts of
-  // up to 8192 tokens, one head, 5.8 / 4.7 / 5.4; 500 tokens in blocks of 64 5.4 / 3.4 / 3.1; 256 single tokens of 8 heads 3.9 / 4.0 / 4.8.)
+  // up to 8192 tokens, one head, 5.8 / 4.7 / 5.4; 500 tokens in blocks of 64 5.4 / 3.4 / 3.1; 256 single tokens of 8 heads 3.9 / 4.0 / 4.8.
+  // That is in blocks of 16.  Of longer blocks waves that share one take as many in turn, whatever a block gets: the same single tokens in blocks of 64
+  // 8.9 us, of 128 11.0, of 256 41, where only one of sixteen waves has a token.)
   g.span = 1;
   auto units = [&] { return ((int64_t)a.tokens + g.span - 1) / g.span * a.heads * 2; };
   while (g.span < (wide == 16 ? 64 : 32) && units() > MOST_UNITS / wide) g.span *= 2;
