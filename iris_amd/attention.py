@@ -83,6 +83,8 @@ def _heads(name, t, device, dtype=None, tokens=None, heads=None, dim=None):
             raise ValueError(f"{name} has {got} {what}, expected {want}")
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
+    if max(t.shape[:2]) > INT32_MAX:
+        raise ValueError(f"{name} has more tokens or heads than 31 bits count")
     return t
 
 
@@ -139,6 +141,8 @@ def _cache(name, t, device, dtype, heads, dim):
         raise ValueError(f"{name} holds {t.shape[2]} heads of {t.shape[3]}, expected {heads} of {dim}")
     if t.shape[1] < 1:
         raise ValueError(f"{name} has empty pages")
+    if max(t.shape[:2]) > INT32_MAX:
+        raise ValueError(f"{name} has more pages, or longer ones, than 31 bits count")
     if t.shape[3] > 1 and t.stride(3) != 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
 
@@ -193,6 +197,8 @@ def _block_table(block_table, device, page_size):
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise TypeError("block_table must be an int32 matrix with contiguous rows")
     requests, width = block_table.shape
+    if requests > INT32_MAX:
+        raise ValueError("block_table is for more requests than 31 bits count")
     if requests > 1 and block_table.stride(0) < width:
         raise ValueError("the rows of block_table must not overlap")
     if width * page_size > INT32_MAX:
