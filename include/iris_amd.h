@@ -582,7 +582,7 @@ int iris_quantized_attention_launch(const iris_attention_args* args, const iris_
 int iris_quantized_attention_plan(const iris_attention_args* args, const iris_cache_scales* scales, int32_t num_cus, iris_attention_plan_info* plan);
 /*
  * The order in which a launch's workgroups take its work: those at `place` (of each key head's workgroups; of single tokens of all) take item *item, the
- * `place`-th but where row tiles of prompts are dealt out so that empty ones are spread.
+ * `place`-th but where row tiles of prompts are dealt out so that empty ones are spread.  (What the device orders by lengths counts in that order.)
  */
 int iris_quantized_attention_item(const iris_attention_args* args, const iris_cache_scales* scales, int32_t num_cus, int64_t place, int64_t* item);
 int iris_quantized_attention_kernel_info(const iris_attention_args* args, const iris_cache_scales* scales, int* n_regs, int* n_spills);
